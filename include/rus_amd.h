@@ -23,10 +23,15 @@
 extern "C" {
 #endif
 
-#define RUS_ABI_VERSION 19
+#define RUS_ABI_VERSION 20
 
 #define RUS_DTYPE_F16 0
 #define RUS_DTYPE_F32 1
+#define RUS_DTYPE_BF16 2 /* microscaled entry points only */
+
+/* Element formats of microscaled blocks. */
+#define RUS_MX_FP4 0 /* e2m1, two to a byte, the even element in the low half */
+#define RUS_MX_FP8 1 /* e4m3 */
 
 #define RUS_OK 0
 #define RUS_ERR_INVALID 1     /* bad pointer, size, stride, alignment or dtype */
@@ -817,6 +822,70 @@ int rus_lora_cast_t(const float* flat, int64_t n_layers, int32_t n_seg, const in
 int rus_adamw_step(float* param, const float* grad, float* exp_avg, float* exp_avg_sq, int64_t n,
                    double lr, double beta1, double beta2, double eps, double weight_decay,
                    int64_t step, void* stream);
+
+/*
+ * Microscaled operands: blocks of 32 elements along a row, each with a power-of-two scale byte b
+ * (E8M0: 2^(b-127), 255 = NaN). A matrix [rows, cols] is codes [rows, nb * 16] (fp4) or
+ * [rows, nb * 32] (fp8) and scales [rows, nb], nb = 4 * ceil(cols / 128), contiguous, codes 16-byte
+ * and scales 4-byte aligned; elements and scales behind `cols` are zero (the products read them).
+ * None of these has a counterpart in the reference, whose 4-bit weights are NF4 only
+ * (solution/kernels.py:27-118); they stand beside rus_nf4_dequant and rus_nf4_gemm.
+ *
+ * rus_mx_quantize: per block b = E - emax (at least 0), E the biased fp32 exponent of max|x| and
+ * emax = 2 (fp4) / 8 (fp8); element = nearest-even of x 2^(127-b), clamped to +-6 / +-448. A block
+ * with an infinity or NaN gets scale 255. x: fp16, fp32 or bf16, row stride stride_row.
+ */
+int rus_mx_quantize(const void* x, int32_t dtype, int64_t n_rows, int64_t n_cols,
+                    int64_t stride_row, int32_t fmt, void* codes, void* scales, void* stream);
+
+/* The values the blocks stand for, rounded once to out's type (fp16, fp32 or bf16). */
+int rus_mx_dequantize(const void* codes, const void* scales, int32_t fmt, int64_t n_rows,
+                      int64_t n_cols, void* out, int32_t dtype, int64_t stride_row, void* stream);
+
+/*
+ * rus_rmsnorm_fwd with the output as fp8 blocks: h = T(x + residual) (sum_out, both or neither),
+ * rstd = 1/sqrt(mean(h^2) + eps), blocks of (h rstd) weight formed in fp64 and rounded once to the
+ * element. x, residual and sum_out share dtype (fp16 / fp32) and stride_row; weight has w_dtype.
+ * rus_rmsnorm_bwd takes (h, rstd) as saved here.
+ */
+int rus_rmsnorm_mx_fwd(const void* x, const void* residual, const void* weight, int32_t w_dtype,
+                       void* sum_out, void* codes, void* scales, float* rstd, int64_t n_rows,
+                       int64_t n_cols, int64_t stride_row, float eps, int32_t dtype, void* stream);
+
+/*
+ * y[m, n] = T(sum_k X[m, k] W[n, k] + bias[n]); X [m, k] and W [n, k] in either format, T fp16 or
+ * bf16 (dtype), bias in T or NULL; fp32 sums.
+ */
+int rus_mx_gemm(const void* x_codes, const void* x_scales, int32_t x_fmt, const void* w_codes,
+                const void* w_scales, int32_t w_fmt, int64_t m, int64_t n, int64_t k,
+                const void* bias, void* y, int64_t stride_y, int32_t dtype, void* stream);
+
+/*
+ * The input gradient of rus_mx_gemm: dx[m, k] = T(sum_n dy[m, n] T(W[n, k])), dy and dx in T = fp16
+ * or bf16 (dtype), W decoded to T inside the product (an fp16 decode of |W| > 65504 is infinite;
+ * bf16 holds every value); fp32 sums.
+ */
+int rus_mx_gemm_t(const void* dy, int64_t stride_dy, int32_t dtype, const void* w_codes,
+                  const void* w_scales, int32_t w_fmt, int64_t m, int64_t n, int64_t k, void* dx,
+                  int64_t stride_dx, void* stream);
+
+/*
+ * Gated feed-forward, first half, in one kernel: G = X W[0:n]^T, U = X W[n:2n]^T (W [2n, k]: gate
+ * rows, then up rows), h[m, n] = T(silu(G) U); G and U stay in registers.
+ */
+int rus_mx_glu_fwd(const void* x_codes, const void* x_scales, int32_t x_fmt, const void* w_codes,
+                   const void* w_scales, int32_t w_fmt, int64_t m, int64_t n, int64_t k, void* h,
+                   int64_t stride_h, int32_t dtype, void* stream);
+
+/*
+ * Its backward up to the two projections' outputs: G and U formed again from X and W,
+ *   d_gu[m, 0:n] = T((dh U) silu'(G)),  d_gu[m, n:2n] = T(dh silu(G)),
+ * silu' = s + silu(G) (1 - s), s = sigmoid(G). rus_mx_gemm_t(d_gu, W) is the gradient of X.
+ */
+int rus_mx_glu_bwd(const void* dh, int64_t stride_dh, const void* x_codes, const void* x_scales,
+                   int32_t x_fmt, const void* w_codes, const void* w_scales, int32_t w_fmt,
+                   int64_t m, int64_t n, int64_t k, void* d_gu, int64_t stride_d_gu, int32_t dtype,
+                   void* stream);
 
 #ifdef __cplusplus
 }

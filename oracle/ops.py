@@ -528,5 +528,74 @@ def fp16_ulp(x: torch.Tensor) -> torch.Tensor:
     e = torch.floor(torch.log2(a))
     return torch.pow(2.0, e - 10)
 
+# ---------------------------------------------------------------------------------------------
+# Microscaled blocks (no reference counterpart): definitions in float64
+# ---------------------------------------------------------------------------------------------
+
+MX_GRID = {
+    "fp4": np.array([0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0]),
+    "fp8": np.array([m * 2.0**-9 for m in range(8)]
+                    + [2.0 ** (e - 7) * (1 + m / 8) for e in range(1, 16) for m in range(8)][:-1]),
+}
+MX_EMAX = {"fp4": 2, "fp8": 8}
+
+
+def mx_blocks(cols: int) -> int:
+    """Stored blocks of a row: whole groups of four."""
+    return -(-cols // 128) * 4
+
+
+def mx_quantize(x, fmt: str):
+    """(code numbers uint8 [rows, 32 nb], scale bytes uint8 [rows, nb]) of x [rows, cols]."""
+    x = np.asarray(x, dtype=np.float64)
+    rows, cols = x.shape
+    nb = mx_blocks(cols)
+    full = np.zeros((rows, nb * 32))
+    full[:, :cols] = x
+    full = full.reshape(rows, nb, 32)
+    bad = ~np.isfinite(full).all(axis=2)
+    full = np.where(bad[:, :, None], 0.0, full)
+    top = np.abs(full).max(axis=2)
+    _, e = np.frexp(top)  # top = m 2^e, 0.5 <= m < 1
+    s = np.where(top > 0, np.clip(e - 1 - MX_EMAX[fmt], -127, 127), -127)
+    v = full * np.exp2(-s.astype(np.float64))[:, :, None]
+    grid = MX_GRID[fmt]
+    a = np.minimum(np.abs(v), grid[-1])
+    hi = np.clip(np.searchsorted(grid, a), 1, len(grid) - 1)
+    lo = hi - 1
+    to_lo = (a - grid[lo] < grid[hi] - a) | ((a - grid[lo] == grid[hi] - a) & (lo % 2 == 0))
+    code = np.where(to_lo, lo, hi) + np.where(np.signbit(v), len(grid) if fmt == "fp4" else 128, 0)
+    code = np.where(bad[:, :, None], 0 if fmt == "fp4" else 127, code)
+    return (code.reshape(rows, nb * 32).astype(np.uint8),
+            np.where(bad, 255, s + 127).astype(np.uint8))
+
+
+def mx_pack(code: np.ndarray, fmt: str) -> np.ndarray:
+    """Code numbers as stored: fp4 two to a byte, the even element in the low half."""
+    return code if fmt == "fp8" else (code[:, 0::2] | (code[:, 1::2] << 4)).astype(np.uint8)
+
+
+def mx_values(packed: np.ndarray, scales: np.ndarray, cols: int, fmt: str) -> np.ndarray:
+    """float64 values [rows, cols] of stored blocks."""
+    rows, nb = scales.shape
+    if fmt == "fp4":
+        code = np.stack([packed & 15, packed >> 4], axis=2).reshape(rows, nb * 32)
+        el = np.where(code > 7, -1.0, 1.0) * MX_GRID["fp4"][code & 7]
+    else:
+        grid = np.concatenate([MX_GRID["fp8"], [np.nan]])
+        el = np.where(packed > 127, -1.0, 1.0) * grid[packed & 127]
+    scale = np.where(scales == 255, np.nan, np.exp2(scales.astype(np.float64) - 127))
+    return (el.reshape(rows, nb, 32) * scale[:, :, None]).reshape(rows, nb * 32)[:, :cols]
+
+
+def mx_glu(g: np.ndarray, u: np.ndarray) -> np.ndarray:
+    return g / (1.0 + np.exp(-g)) * u
+
+
+def mx_glu_bwd(dh: np.ndarray, g: np.ndarray, u: np.ndarray) -> np.ndarray:
+    """[d_gate | d_up] before rounding."""
+    s = 1.0 / (1.0 + np.exp(-g))
+    return np.concatenate([dh * u * (s + g * s * (1.0 - s)), dh * g * s], axis=1)
+
 
 __all__ = [name for name in dir() if not name.startswith("_") and name not in ("math", "np", "torch")]

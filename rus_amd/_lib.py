@@ -11,10 +11,12 @@ import threading
 from pathlib import Path
 
 LIB_PATH = Path(__file__).resolve().parent / "librus_amd.so"
-ABI_VERSION = 19
+ABI_VERSION = 20
 
 DTYPE_F16 = 0
 DTYPE_F32 = 1
+DTYPE_BF16 = 2  # microscaled entry points only
+MX_FP4, MX_FP8 = 0, 1
 
 _vp = ctypes.c_void_p
 _i64 = ctypes.c_int64
@@ -148,6 +150,15 @@ SIGNATURES: dict[str, list] = {
                                 _f32, _vp, _vp, _i32, _vp],
     "rus_lmhead_ce_dh_finish_probs": [_vp, _i32, _i64, _i64, _vp, _vp, _vp, _vp, _i64, _i64, _i32,
                                       _vp, _f32, _vp, _vp, _vp, _vp, _vp, _i32, _vp],
+    "rus_mx_quantize": [_vp, _i32, _i64, _i64, _i64, _i32, _vp, _vp, _vp],
+    "rus_mx_dequantize": [_vp, _vp, _i32, _i64, _i64, _vp, _i32, _i64, _vp],
+    "rus_rmsnorm_mx_fwd": [_vp, _vp, _vp, _i32, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _f32, _i32,
+                           _vp],
+    "rus_mx_gemm": [_vp, _vp, _i32, _vp, _vp, _i32, _i64, _i64, _i64, _vp, _vp, _i64, _i32, _vp],
+    "rus_mx_gemm_t": [_vp, _i64, _i32, _vp, _vp, _i32, _i64, _i64, _i64, _vp, _i64, _vp],
+    "rus_mx_glu_fwd": [_vp, _vp, _i32, _vp, _vp, _i32, _i64, _i64, _i64, _vp, _i64, _i32, _vp],
+    "rus_mx_glu_bwd": [_vp, _i64, _vp, _vp, _i32, _vp, _vp, _i32, _i64, _i64, _i64, _vp, _i64,
+                       _i32, _vp],
 }
 
 _lock = threading.Lock()

@@ -75,6 +75,13 @@ __all__ = [
     "attn_varlen_bwd_parts",
     "gemm_parts",
     "gemm_parts_count",
+    "MXTensor",
+    "mx_quantize",
+    "mx_dequantize",
+    "mx_gemm",
+    "rms_norm_mx_fwd",
+    "mx_mlp_glu_fwd",
+    "mx_mlp_glu_bwd",
 ]
 
 
@@ -2283,3 +2290,332 @@ def lora_cast_t(flat: torch.Tensor, n_layers: int, shapes, out: torch.Tensor,
     _launch("lora_cast_t", n * (4 + 2 + (2 if out_t is not None else 0)), 0, "rus_lora_cast_t",
             flat.data_ptr(), int(n_layers), len(shapes), rows, cols, out.data_ptr(), _ptr(out_t),
             _stream(flat))
+
+
+# ---------------------------------------------------------------------------------------------
+# Microscaled operands: blocks of 32 elements in 4 or 8 bits with a power-of-two scale, which the
+# matrix cores read directly (no counterpart in the reference, whose 4-bit weights are NF4 only)
+# ---------------------------------------------------------------------------------------------
+
+MX_BLOCK = 32
+_MX_FMT = {"fp4": (_lib.MX_FP4, 16), "fp8": (_lib.MX_FP8, 32)}  # code, bytes of a block
+_MX_DTYPE = {torch.float16: DTYPE_F16, torch.float32: DTYPE_F32, torch.bfloat16: _lib.DTYPE_BF16}
+
+
+def _mx_fmt(fn: str, fmt: str) -> tuple[int, int]:
+    got = _MX_FMT.get(fmt)
+    if got is None:
+        raise ValueError(f"{fn}: unknown block format {fmt!r} (fp4 or fp8)")
+    return got
+
+
+def _mx_blocks(cols: int) -> int:
+    return 4 * -(-cols // 128)
+
+
+def _mx_dtype(fn: str, dtype: torch.dtype, wide: bool = True) -> int:
+    """``wide``: fp32 too (rows that are read or decoded; products give 16-bit results)."""
+    got = _MX_DTYPE.get(dtype)
+    if got is None or (got == DTYPE_F32 and not wide):
+        raise TypeError(f"{fn}: unsupported dtype {dtype} (fp16{', fp32' if wide else ''} or bf16)")
+    return got
+
+
+class MXTensor:
+    """A matrix [rows, cols] in microscaled blocks of 32 along its rows: ``fmt`` "fp4" (e2m1, two
+    codes to a byte, the even element in the low half) or "fp8" (e4m3), one E8M0 scale byte per
+    block (2^(b - 127), 255 = NaN). Rows are stored padded to whole groups of four blocks:
+    ``codes`` uint8 [rows, nb * 16 or 32] and ``scales`` uint8 [rows, nb], nb = 4 ceil(cols / 128),
+    contiguous, zero behind ``cols`` (the products rely on that; ``from_blocks`` pads)."""
+
+    __slots__ = ("codes", "scales", "shape", "fmt")
+
+    def __init__(self, codes: torch.Tensor, scales: torch.Tensor, shape: tuple[int, int], fmt: str):
+        fn = "MXTensor"
+        _, nbytes = _mx_fmt(fn, fmt)
+        rows, cols = int(shape[0]), int(shape[1])
+        if rows < 0 or cols <= 0:
+            raise ValueError(f"{fn}: bad shape {tuple(shape)}")
+        nb = _mx_blocks(cols)
+        if codes.dtype != torch.uint8 or scales.dtype != torch.uint8:
+            raise TypeError(f"{fn}: codes and scales must be uint8")
+        if codes.shape != (rows, nb * nbytes) or scales.shape != (rows, nb):
+            raise ValueError(f"{fn}: {fmt} blocks of {rows} x {cols} are codes [{rows}, {nb * nbytes}] and "
+                             f"scales [{rows}, {nb}], got {tuple(codes.shape)} and {tuple(scales.shape)}")
+        if not codes.is_contiguous() or not scales.is_contiguous():
+            raise ValueError(f"{fn}: codes and scales must be contiguous")
+        if codes.device != scales.device:
+            raise ValueError(f"{fn}: codes on {codes.device}, scales on {scales.device}")
+        self.codes, self.scales, self.shape, self.fmt = codes, scales, (rows, cols), fmt
+
+    @property
+    def device(self) -> torch.device:
+        return self.codes.device
+
+    def to(self, device) -> "MXTensor":
+        return MXTensor(self.codes.to(device), self.scales.to(device), self.shape, self.fmt)
+
+    @classmethod
+    def from_blocks(cls, codes: torch.Tensor, scales: torch.Tensor, shape: tuple[int, int],
+                    fmt: str) -> "MXTensor":
+        """From codes [rows, ceil(cols / 32) * 16 or 32] and scales [rows, ceil(cols / 32)] without
+        row padding, as other programs store them (elements of the last block behind ``cols`` are
+        cleared)."""
+        fn = "MXTensor.from_blocks"
+        _, nbytes = _mx_fmt(fn, fmt)
+        rows, cols = int(shape[0]), int(shape[1])
+        n = -(-cols // MX_BLOCK)
+        if codes.dtype != torch.uint8 or scales.dtype != torch.uint8:
+            raise TypeError(f"{fn}: codes and scales must be uint8")
+        if codes.shape != (rows, n * nbytes) or scales.shape != (rows, n):
+            raise ValueError(f"{fn}: {fmt} blocks of {rows} x {cols} are codes [{rows}, {n * nbytes}] and "
+                             f"scales [{rows}, {n}], got {tuple(codes.shape)} and {tuple(scales.shape)}")
+        nb = _mx_blocks(cols)
+        c = codes.new_zeros(rows, nb * nbytes)
+        c[:, : n * nbytes] = codes
+        if fmt == "fp8":
+            c[:, cols:] = 0
+        else:
+            c[:, (cols + 1) // 2:] = 0
+            if cols % 2:
+                c[:, cols // 2] &= 15
+        s = scales.new_zeros(rows, nb)
+        s[:, :n] = scales
+        return cls(c, s, (rows, cols), fmt)
+
+
+def _mx_check(fn: str, t: MXTensor, name: str, like: torch.Tensor) -> None:
+    if not isinstance(t, MXTensor):
+        raise TypeError(f"{fn}: {name} must be an MXTensor, got {type(t).__name__}")
+    if t.codes.device != like.device:
+        raise ValueError(f"{fn}: {name} is on {t.codes.device}, other operands on {like.device}")
+
+
+def _same_device(fn: str, like: torch.Tensor, *tensors: torch.Tensor | None) -> None:
+    _require_device(fn, like, *tensors)
+    for t in tensors:
+        if t is not None and t.device != like.device:
+            raise ValueError(f"{fn}: operands on {t.device} and {like.device}")
+
+
+def _mx_rows(fn: str, x: torch.Tensor, width: int | None, name: str) -> torch.Tensor:
+    """x as rows the kernels address: 2-D, unit column stride, rows that do not overlap."""
+    if x.dim() != 2 or (width is not None and x.shape[1] != width):
+        raise ValueError(f"{fn}: {name} must be 2-D{'' if width is None else f' with {width} columns'}, "
+                         f"got {tuple(x.shape)}")
+    if x.shape[1] > 1 and x.stride(1) != 1 or x.shape[0] > 1 and x.stride(0) < x.shape[1]:
+        return x.contiguous()
+    return x
+
+
+def _mx_out(fn: str, out: torch.Tensor | None, m: int, n: int, dtype: torch.dtype,
+            like: torch.Tensor) -> torch.Tensor:
+    if out is None:
+        return torch.empty((m, n), dtype=dtype, device=like.device)
+    if out.dtype != dtype or tuple(out.shape) != (m, n) or (n > 1 and out.stride(1) != 1) or \
+            (m > 1 and out.stride(0) < n):
+        raise ValueError(f"{fn}: out must be {dtype} [{m}, {n}] with unit column stride")
+    return out
+
+
+def _ld(t: torch.Tensor) -> int:
+    return max(t.stride(0), t.shape[1])  # a single row's stride may be anything
+
+
+def _mx_launch(kernel: str, nbytes: float, flops: float, like: torch.Tensor, fn: str, *args) -> None:
+    """``_launch`` on ``like``'s device and that device's current stream (the last argument)."""
+    index = like.get_device()
+    if index == torch.cuda.current_device():
+        _launch(kernel, nbytes, flops, fn, *args, _raw_stream(index))
+    else:
+        with torch.cuda.device(index):
+            _launch(kernel, nbytes, flops, fn, *args, _raw_stream(index))
+
+
+def mx_quantize(x: torch.Tensor, fmt: str = "fp4") -> MXTensor:
+    """x [rows, cols] (fp16, bf16 or fp32) in blocks of 32 along its rows. Per block the scale is
+    2^(floor(log2 max|x|) - 2) (fp4) or ... - 8 (fp8), at least 2^-127; elements are rounded to
+    nearest even and saturate (at 6 / 448 times the scale). A block with an infinity or a NaN is NaN
+    as a whole."""
+    fn = "mx_quantize"
+    code, nbytes = _mx_fmt(fn, fmt)
+    _require_device(fn, x)
+    dt = _mx_dtype(fn, x.dtype)
+    x2 = _mx_rows(fn, x, None, "x")
+    rows, cols = x2.shape
+    if cols == 0:
+        raise ValueError(f"{fn}: rows without columns")
+    nb = _mx_blocks(cols)
+    codes = torch.empty((rows, nb * nbytes), dtype=torch.uint8, device=x2.device)
+    scales = torch.empty((rows, nb), dtype=torch.uint8, device=x2.device)
+    _mx_launch("mx_quantize", rows * (cols * x2.element_size() + nb * (nbytes + 1)), 0, x2,
+               "rus_mx_quantize", x2.data_ptr(), dt, rows, cols, _ld(x2), code, codes.data_ptr(),
+               scales.data_ptr())
+    return MXTensor(codes, scales, (rows, cols), fmt)
+
+
+def mx_dequantize(t: MXTensor, dtype: torch.dtype = torch.float16,
+                  out: torch.Tensor | None = None) -> torch.Tensor:
+    """The values ``t`` stands for, [rows, cols], rounded once to ``dtype`` (fp16, bf16, fp32)."""
+    fn = "mx_dequantize"
+    if not isinstance(t, MXTensor):
+        raise TypeError(f"{fn}: an MXTensor, got {type(t).__name__}")
+    _same_device(fn, t.codes, out)
+    dt = _mx_dtype(fn, dtype)
+    code, nbytes = _MX_FMT[t.fmt]
+    rows, cols = t.shape
+    out = _mx_out(fn, out, rows, cols, dtype, t.codes)
+    _mx_launch("mx_dequantize", rows * (_mx_blocks(cols) * (nbytes + 1) + cols * out.element_size()),
+               0, t.codes, "rus_mx_dequantize", t.codes.data_ptr(), t.scales.data_ptr(), code, rows,
+               cols, out.data_ptr(), dt, _ld(out))
+    return out
+
+
+def rms_norm_mx_fwd(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6,
+                    residual: torch.Tensor | None = None):
+    """``rms_norm_fwd`` whose output is fp8 blocks: returns (MXTensor [rows, cols], sum_out or x,
+    rstd). h = x + residual rounded to x's type, the blocks those of h * rstd * weight, formed in
+    fp64 and rounded once. Leading axes of x become rows. ``rms_norm_bwd(dy, h, weight, rstd)`` is
+    the gradient."""
+    fn = "rms_norm_mx_fwd"
+    _same_device(fn, x, weight, residual)
+    dt, wdt = _dtype_code(fn, x.dtype), _dtype_code(fn, weight.dtype)
+    n_cols = x.shape[-1]
+    if n_cols == 0:
+        raise ValueError(f"{fn}: rows without columns")
+    x_2d = x.contiguous().view(-1, n_cols)
+    n_rows = x_2d.shape[0]
+    w = weight.contiguous()
+    if w.numel() != n_cols:
+        raise ValueError(f"{fn}: weight has {w.numel()} entries, rows have {n_cols}")
+    res_2d = sum_out = None
+    if residual is not None:
+        if residual.dtype != x.dtype or residual.shape != x.shape:
+            raise ValueError(f"{fn}: residual must match x in shape and dtype")
+        res_2d = residual.contiguous().view(-1, n_cols)
+        sum_out = torch.empty_like(x_2d)
+    nb = _mx_blocks(n_cols)
+    codes = torch.empty((n_rows, nb * 32), dtype=torch.uint8, device=x.device)
+    scales = torch.empty((n_rows, nb), dtype=torch.uint8, device=x.device)
+    rstd = torch.empty((n_rows,), dtype=torch.float32, device=x.device)
+    nbytes = n_rows * ((1 if res_2d is None else 3) * n_cols * x_2d.element_size() + nb * 33 + 4) + \
+        w.numel() * w.element_size()
+    _mx_launch("rmsnorm_mx_fwd", nbytes, 0, x_2d, "rus_rmsnorm_mx_fwd", x_2d.data_ptr(), _ptr(res_2d),
+               w.data_ptr(), wdt, _ptr(sum_out), codes.data_ptr(), scales.data_ptr(), rstd.data_ptr(),
+               n_rows, n_cols, n_cols, float(eps), dt)
+    return (MXTensor(codes, scales, (n_rows, n_cols), "fp8"),
+            x if sum_out is None else sum_out.view(x.shape), rstd)
+
+
+def _mx_operand(fn: str, x, act: str, k: int, dtype: torch.dtype | None):
+    """(blocks of x, result type): x as it is, or quantised to ``act``."""
+    if not isinstance(x, MXTensor):
+        dtype = x.dtype if dtype is None else dtype
+        _require_device(fn, x)
+        x = mx_quantize(_mx_rows(fn, x, k, "x"), act)
+    elif x.shape[1] != k:
+        raise ValueError(f"{fn}: x has {x.shape[1]} columns, W {k}")
+    return x, torch.float16 if dtype is None else dtype
+
+
+def _mx_bytes(t: MXTensor) -> int:
+    return t.codes.numel() + t.scales.numel()
+
+
+def mx_gemm(x, w: MXTensor, trans: bool = False, bias: torch.Tensor | None = None,
+            out: torch.Tensor | None = None, act: str = "fp8",
+            dtype: torch.dtype | None = None) -> torch.Tensor:
+    """trans=False: x [m, in] @ W^T (+ bias) -> [m, out] with W [out, in] in blocks and x in blocks
+    too: an ``MXTensor`` or a tensor, quantised here to ``act`` ("fp8" or "fp4"). The result has
+    ``dtype`` (fp16 or bf16; default x's own, fp16 for blocks), fp32 sums rounded once.
+    trans=True: x [m, out] (a 16-bit tensor) @ W -> [m, in], the input gradient, with W decoded to
+    x's type inside the product (fp16: infinite above 65504)."""
+    fn = "mx_gemm"
+    if not isinstance(w, MXTensor):
+        raise TypeError(f"{fn}: w must be an MXTensor, got {type(w).__name__}")
+    wf = _MX_FMT[w.fmt][0]
+    n, k = w.shape
+    if trans:
+        if isinstance(x, MXTensor):
+            raise TypeError(f"{fn}: the gradient product takes a tensor, not blocks")
+        if bias is not None:
+            raise ValueError(f"{fn}: bias belongs to the forward product")
+        if dtype is not None and dtype != x.dtype:
+            raise ValueError(f"{fn}: the gradient has its operand's dtype")
+        _same_device(fn, w.codes, x, out)
+        dt = _mx_dtype(fn, x.dtype, wide=False)
+        x2 = _mx_rows(fn, x, n, "x")
+        m = x2.shape[0]
+        out = _mx_out(fn, out, m, k, x2.dtype, x2)
+        if n == 0:
+            return out.zero_()
+        _mx_launch("mx_gemm_t", 2 * m * (n + k) + _mx_bytes(w), 2 * m * n * k, x2, "rus_mx_gemm_t",
+                   x2.data_ptr(), _ld(x2), dt, w.codes.data_ptr(), w.scales.data_ptr(), wf, m, n, k,
+                   out.data_ptr(), _ld(out))
+        return out
+    _same_device(fn, w.codes, x.codes if isinstance(x, MXTensor) else x, bias, out)
+    x, dtype = _mx_operand(fn, x, act, k, dtype)
+    dt = _mx_dtype(fn, dtype, wide=False)
+    if bias is not None:
+        if bias.dtype != dtype or bias.numel() != n:
+            raise ValueError(f"{fn}: bias must be {dtype} [{n}]")
+        bias = bias.reshape(-1).contiguous()
+    m = x.shape[0]
+    out = _mx_out(fn, out, m, n, dtype, x.codes)
+    if n == 0:
+        return out
+    _mx_launch("mx_gemm", _mx_bytes(x) + _mx_bytes(w) + 2 * m * n, 2 * m * n * k, x.codes,
+               "rus_mx_gemm", x.codes.data_ptr(), x.scales.data_ptr(), _MX_FMT[x.fmt][0],
+               w.codes.data_ptr(), w.scales.data_ptr(), wf, m, n, k, _ptr(bias), out.data_ptr(),
+               _ld(out), dt)
+    return out
+
+
+def _mx_glu_weight(fn: str, w: MXTensor) -> int:
+    if not isinstance(w, MXTensor):
+        raise TypeError(f"{fn}: w must be an MXTensor, got {type(w).__name__}")
+    if w.shape[0] % 2 or w.shape[0] == 0:
+        raise ValueError(f"{fn}: [gate | up] needs an even number of rows, got {w.shape[0]}")
+    return w.shape[0] // 2
+
+
+def mx_mlp_glu_fwd(x, w: MXTensor, act: str = "fp8", out: torch.Tensor | None = None,
+                   dtype: torch.dtype | None = None) -> torch.Tensor:
+    """silu(x Wg^T) * (x Wu^T) -> [m, inner] in one kernel, W = [gate rows | up rows] [2 inner, in]
+    in blocks, x as in ``mx_gemm``. The two projections stay in fp32 registers."""
+    fn = "mx_mlp_glu_fwd"
+    n = _mx_glu_weight(fn, w)
+    k = w.shape[1]
+    _same_device(fn, w.codes, x.codes if isinstance(x, MXTensor) else x, out)
+    x, dtype = _mx_operand(fn, x, act, k, dtype)
+    dt = _mx_dtype(fn, dtype, wide=False)
+    m = x.shape[0]
+    out = _mx_out(fn, out, m, n, dtype, x.codes)
+    _mx_launch("mx_glu_fwd", _mx_bytes(x) + _mx_bytes(w) + 2 * m * n, 4 * m * n * k, x.codes,
+               "rus_mx_glu_fwd", x.codes.data_ptr(), x.scales.data_ptr(), _MX_FMT[x.fmt][0],
+               w.codes.data_ptr(), w.scales.data_ptr(), _MX_FMT[w.fmt][0], m, n, k, out.data_ptr(),
+               _ld(out), dt)
+    return out
+
+
+def mx_mlp_glu_bwd(dh: torch.Tensor, x, w: MXTensor, act: str = "fp8",
+                   out: torch.Tensor | None = None) -> torch.Tensor:
+    """[d_gate | d_up] [m, 2 inner] of ``mx_mlp_glu_fwd`` for dh [m, inner] (fp16 or bf16, also the
+    result's type): the projections are formed again from x (as passed to the forward) and W.
+    ``mx_gemm(d_gu, w, trans=True)`` is the gradient of x."""
+    fn = "mx_mlp_glu_bwd"
+    n = _mx_glu_weight(fn, w)
+    k = w.shape[1]
+    _same_device(fn, w.codes, x.codes if isinstance(x, MXTensor) else x, dh, out)
+    dt = _mx_dtype(fn, dh.dtype, wide=False)
+    x, _ = _mx_operand(fn, x, act, k, dh.dtype)
+    dh2 = _mx_rows(fn, dh, n, "dh")
+    m = x.shape[0]
+    if dh2.shape[0] != m:
+        raise ValueError(f"{fn}: dh has {dh2.shape[0]} rows, x {m}")
+    out = _mx_out(fn, out, m, 2 * n, dh.dtype, dh2)
+    _mx_launch("mx_glu_bwd", _mx_bytes(x) + _mx_bytes(w) + 6 * m * n, 4 * m * n * k, dh2,
+               "rus_mx_glu_bwd", dh2.data_ptr(), _ld(dh2), x.codes.data_ptr(), x.scales.data_ptr(),
+               _MX_FMT[x.fmt][0], w.codes.data_ptr(), w.scales.data_ptr(), _MX_FMT[w.fmt][0], m, n, k,
+               out.data_ptr(), _ld(out), dt)
+    return out

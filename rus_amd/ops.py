@@ -112,6 +112,99 @@ def qkv_lora_rope(qkv, cos, sin, pos_ids, q_lora=None, v_lora=None, scale_q=2.0,
 
 
 # ---------------------------------------------------------------------------------------------
+# Layers over microscaled weights (frozen, as the NF4 ones): gradients of the activations only,
+# straight through their quantisation
+# ---------------------------------------------------------------------------------------------
+
+
+def _no_weight_grad(fn: str, **tensors) -> None:
+    for name, t in tensors.items():
+        if t is not None and t.requires_grad:
+            raise RuntimeError(f"{fn}: {name} is frozen here: no gradient is formed for it")
+
+
+class FusedMXLinearFn(torch.autograd.Function):
+    """y = x W^T + bias with W (``kernels.MXTensor``) and x in blocks; dx = dy W."""
+
+    @staticmethod
+    def forward(ctx, x, w, bias=None, act="fp8"):
+        ctx.w = w
+        y = K.mx_gemm(x.reshape(-1, x.shape[-1]), w, bias=bias, act=act)
+        return y.view(*x.shape[:-1], w.shape[0])
+
+    @staticmethod
+    def backward(ctx, dy):
+        dx = K.mx_gemm(dy.reshape(-1, dy.shape[-1]), ctx.w, trans=True)
+        return dx.view(*dy.shape[:-1], ctx.w.shape[1]), None, None, None
+
+
+def mx_linear(x, w, bias=None, act: str = "fp8"):
+    """``F.linear`` over a microscaled weight: x [..., in] (fp16 or bf16) quantised to ``act``."""
+    _no_weight_grad("mx_linear", bias=bias)
+    return FusedMXLinearFn.apply(x, w, bias, act)
+
+
+class FusedMXMLPGLUFn(torch.autograd.Function):
+    """silu(x Wg^T) * (x Wu^T), W = [gate | up] rows in blocks. Keeps x's blocks only; the backward
+    forms the projections again."""
+
+    @staticmethod
+    def forward(ctx, x, w, act="fp8"):
+        q = K.mx_quantize(x.reshape(-1, x.shape[-1]), act)
+        ctx.w, ctx.act, ctx.rows = w, act, q.shape
+        ctx.save_for_backward(q.codes, q.scales)
+        h = K.mx_mlp_glu_fwd(q, w, dtype=x.dtype)
+        return h.view(*x.shape[:-1], w.shape[0] // 2)
+
+    @staticmethod
+    def backward(ctx, dh):
+        q = K.MXTensor(*ctx.saved_tensors, ctx.rows, ctx.act)
+        d_gu = K.mx_mlp_glu_bwd(dh.reshape(-1, dh.shape[-1]), q, ctx.w)
+        dx = K.mx_gemm(d_gu, ctx.w, trans=True)
+        return dx.view(*dh.shape[:-1], ctx.w.shape[1]), None, None
+
+
+def mx_mlp_glu(x, w_gate_up, act: str = "fp8"):
+    """The gated half of a feed-forward block over microscaled weights, x [..., in] fp16 or bf16."""
+    return FusedMXMLPGLUFn.apply(x, w_gate_up, act)
+
+
+class FusedMXNormMLPFn(torch.autograd.Function):
+    """A feed-forward block from the residual sum on: RMSNorm into fp8 blocks, gate / up / SiLU in
+    one kernel, down projection. Keeps h, rstd and the norm's blocks (1.03 bytes per element)."""
+
+    @staticmethod
+    def forward(ctx, x, weight, w_gate_up, w_down, eps=1e-6, residual=None):
+        q, h, rstd = K.rms_norm_mx_fwd(x, weight, eps=eps, residual=residual)
+        a = K.mx_mlp_glu_fwd(q, w_gate_up, dtype=x.dtype)
+        y = K.mx_gemm(a, w_down).view(*x.shape[:-1], w_down.shape[0])
+        ctx.weights = w_gate_up, w_down
+        ctx.with_residual, ctx.rows = residual is not None, q.shape
+        ctx.save_for_backward(h, weight, rstd, q.codes, q.scales)
+        return (y, h) if ctx.with_residual else y
+
+    @staticmethod
+    def backward(ctx, dy, *d_h):
+        h, weight, rstd, codes, scales = ctx.saved_tensors
+        w_gate_up, w_down = ctx.weights
+        q = K.MXTensor(codes, scales, ctx.rows, "fp8")
+        d_a = K.mx_gemm(dy.reshape(-1, dy.shape[-1]), w_down, trans=True)
+        d_gu = K.mx_mlp_glu_bwd(d_a, q, w_gate_up)
+        d_n = K.mx_gemm(d_gu, w_gate_up, trans=True).view(h.shape)
+        dx = K.rms_norm_bwd(d_n, h, weight, rstd, dresidual=d_h[0] if ctx.with_residual else None)
+        return dx, None, None, None, None, (dx if ctx.with_residual else None)
+
+
+def mx_norm_mlp(x, weight, w_gate_up, w_down, eps: float = 1e-6, residual=None):
+    """down(silu(gate(n)) * up(n)), n = RMSNorm(x + residual), over microscaled weights; fp16.
+    Returns the output, with a residual also the sum (as ``rms_norm``)."""
+    _no_weight_grad("mx_norm_mlp", weight=weight)
+    if x.dtype != torch.float16:
+        raise TypeError(f"mx_norm_mlp: fp16 activations, got {x.dtype}")
+    return FusedMXNormMLPFn.apply(x, weight, w_gate_up, w_down, eps, residual)
+
+
+# ---------------------------------------------------------------------------------------------
 # Chunked lm_head cross-entropy (solution/ops.py:174-349)
 # ---------------------------------------------------------------------------------------------
 
