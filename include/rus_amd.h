@@ -863,11 +863,14 @@ int rus_mx_gemm(const void* x_codes, const void* x_scales, int32_t x_fmt, const 
 /*
  * The input gradient of rus_mx_gemm: dx[m, k] = T(sum_n dy[m, n] T(W[n, k])), dy and dx in T = fp16
  * or bf16 (dtype), W decoded to T inside the product (an fp16 decode of |W| > 65504 is infinite;
- * bf16 holds every value); fp32 sums.
+ * bf16 holds every value); fp32 sums. workspace: the fp32 elements rus_mx_gemm_t_workspace names
+ * (0: none; 16-byte aligned), the sums of a contraction that few tiles split among them; not
+ * shared by calls that overlap.
  */
+int rus_mx_gemm_t_workspace(int64_t m, int64_t n, int64_t k, int64_t* floats);
 int rus_mx_gemm_t(const void* dy, int64_t stride_dy, int32_t dtype, const void* w_codes,
                   const void* w_scales, int32_t w_fmt, int64_t m, int64_t n, int64_t k, void* dx,
-                  int64_t stride_dx, void* stream);
+                  int64_t stride_dx, float* workspace, int64_t n_workspace, void* stream);
 
 /*
  * Gated feed-forward, first half, in one kernel: G = X W[0:n]^T, U = X W[n:2n]^T (W [2n, k]: gate

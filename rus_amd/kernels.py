@@ -2522,6 +2522,20 @@ def _mx_bytes(t: MXTensor) -> int:
     return t.codes.numel() + t.scales.numel()
 
 
+_mx_grad_floats: dict[tuple[int, int, int], int] = {}
+
+
+def _mx_grad_workspace(m: int, n: int, k: int) -> int:
+    """fp32 elements of scratch that the gradient product of this shape takes."""
+    key = (m, n, k)
+    got = _mx_grad_floats.get(key)
+    if got is None:
+        floats = ctypes.c_int64()
+        _lib.call("rus_mx_gemm_t_workspace", m, n, k, ctypes.byref(floats))
+        got = _mx_grad_floats[key] = floats.value
+    return got
+
+
 def mx_gemm(x, w: MXTensor, trans: bool = False, bias: torch.Tensor | None = None,
             out: torch.Tensor | None = None, act: str = "fp8",
             dtype: torch.dtype | None = None) -> torch.Tensor:
@@ -2549,9 +2563,11 @@ def mx_gemm(x, w: MXTensor, trans: bool = False, bias: torch.Tensor | None = Non
         out = _mx_out(fn, out, m, k, x2.dtype, x2)
         if n == 0:
             return out.zero_()
+        floats = _mx_grad_workspace(m, n, k)
+        ws = torch.empty(floats, dtype=torch.float32, device=x2.device) if floats else None
         _mx_launch("mx_gemm_t", 2 * m * (n + k) + _mx_bytes(w), 2 * m * n * k, x2, "rus_mx_gemm_t",
                    x2.data_ptr(), _ld(x2), dt, w.codes.data_ptr(), w.scales.data_ptr(), wf, m, n, k,
-                   out.data_ptr(), _ld(out))
+                   out.data_ptr(), _ld(out), _ptr(ws), floats)
         return out
     _same_device(fn, w.codes, x.codes if isinstance(x, MXTensor) else x, bias, out)
     x, dtype = _mx_operand(fn, x, act, k, dtype)

@@ -168,10 +168,12 @@ F16, F32, BF16, FP4, FP8 = 0, 1, 2, 0, 1
     ("rus_mx_glu_bwd", (16, 64, 16, 16, FP8, 16, 16, FP4, 4, 64, 64, 16, 127, F16, None), "stride"),
     ("rus_mx_glu_bwd", (16, 63, 16, 16, FP8, 16, 16, FP4, 4, 64, 64, 16, 128, F16, None), "stride_dh"),
     ("rus_mx_glu_bwd", (None, 64, 16, 16, FP8, 16, 16, FP4, 4, 64, 64, 16, 128, F16, None), "dh is null"),
-    ("rus_mx_gemm_t", (16, 63, F16, 16, 16, FP4, 4, 64, 64, 16, 64, None), "strides"),
-    ("rus_mx_gemm_t", (16, 64, F32, 16, 16, FP4, 4, 64, 64, 16, 64, None), "fp16 or bf16"),
-    ("rus_mx_gemm_t", (16, 64, F16, 16, 16, 3, 4, 64, 64, 16, 64, None), "format"),
-    ("rus_mx_gemm_t", (16, 64, F16, 16, 16, FP4, 4, 64, 64, None, 64, None), "null"),
+    ("rus_mx_gemm_t", (16, 63, F16, 16, 16, FP4, 4, 64, 64, 16, 64, None, 0, None), "strides"),
+    ("rus_mx_gemm_t", (16, 64, F32, 16, 16, FP4, 4, 64, 64, 16, 64, None, 0, None), "fp16 or bf16"),
+    ("rus_mx_gemm_t", (16, 64, F16, 16, 16, 3, 4, 64, 64, 16, 64, None, 0, None), "format"),
+    ("rus_mx_gemm_t", (16, 64, F16, 16, 16, FP4, 4, 64, 64, None, 64, None, 0, None), "null"),
+    ("rus_mx_gemm_t", (16, 17920, F16, 16, 16, FP4, 4, 17920, 1536, 16, 1536, 16, 8, None), "workspace holds"),
+    ("rus_mx_gemm_t_workspace", (4, 0, 64, None), "null result"),
 ])
 def test_entry_points_refuse(name, args, msg):
     with pytest.raises(RuntimeError, match=msg):
@@ -181,4 +183,4 @@ def test_entry_points_refuse(name, args, msg):
 def test_empty_batches_launch_nothing():
     _lib.call("rus_mx_quantize", None, F16, 0, 64, 64, FP4, None, None, None)
     _lib.call("rus_mx_gemm", None, None, FP8, None, None, FP4, 0, 64, 64, None, None, 64, F16, None)
-    _lib.call("rus_mx_gemm_t", None, 64, F16, None, None, FP4, 0, 64, 64, None, 64, None)
+    _lib.call("rus_mx_gemm_t", None, 64, F16, None, None, FP4, 0, 64, 64, None, 64, None, 0, None)
