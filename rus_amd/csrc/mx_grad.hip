@@ -22,6 +22,8 @@ typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) char* lds_ptr;
 
+typedef u32x4s u32x4u __attribute__((aligned(2)));  // a 16-byte access at any alignment of elements
+
 constexpr int kGradN = 256, kGradK = 64, kGradThreads = 512;
 constexpr int kWRow = kGradN * 2;  // bytes of one contraction row of the W stage
 
@@ -33,7 +35,6 @@ struct GradArgs {
   int tiles_m, tiles_k, splits, stages;  // stages of 64 rows of W, dealt evenly to the splits
   void* dx;          // [m, k], or the splits' fp32 sums [splits, m, k]
   int64_t ld_dx;
-  bool vec;          // dy's rows allow 16-byte loads
 };
 
 template <typename T>
@@ -72,7 +73,7 @@ __device__ __forceinline__ u32x4s decode8(uint32_t lo, uint32_t hi, float s) {
   return o;
 }
 
-template <typename T, int FMT, int TM, bool SPLIT>
+template <typename T, int FMT, int TM>
 __global__ __launch_bounds__(kGradThreads) __attribute__((amdgpu_waves_per_eu(2, 2))) void
 mx_grad_kernel(GradArgs g) {
   constexpr int WM = TM >= 128 ? 2 : 1, WN = 8 / WM;           // waves along tokens and columns
@@ -116,15 +117,18 @@ mx_grad_kernel(GradArgs g) {
   const uint32_t bat = brow * kWRow + (((4 * bblk) ^ ((brow & 3) << 2)) << 4);
 
   u32x4s ra[AC > 0 ? AC : 1], rb[WV];
-  float rs = 0.0f;
+  uint32_t rs = 0;
+  const int ragged = g.n & 7;
   auto load = [&](int s) {
     const int n0 = s * kGradK, n = n0 + 8 * (t & 7);
     if (has_a) {
+      if (n0 + kGradK <= g.n || !ragged) {  // whole pieces, at any alignment (those past the end: `store`)
 #pragma unroll
-      for (int i = 0; i < (AC > 0 ? AC : 1); ++i) {
-        if (g.vec && n + 8 <= g.n) {
-          ra[i] = *reinterpret_cast<const u32x4s*>(dy + arow[i] + n);
-        } else {
+        for (int i = 0; i < (AC > 0 ? AC : 1); ++i)
+          ra[i] = *reinterpret_cast<const u32x4u*>(dy + arow[i] + (n < g.n ? n : 0));
+      } else {
+#pragma unroll
+        for (int i = 0; i < (AC > 0 ? AC : 1); ++i) {
           Pack<T, 8> p;
 #pragma unroll
           for (int j = 0; j < 8; ++j) p.v[j] = n + j < g.n ? dy[arow[i] + n + j] : static_cast<T>(0.0f);
@@ -132,19 +136,23 @@ mx_grad_kernel(GradArgs g) {
         }
       }
     }
-    const int wrow = n0 + brow;
-    const int64_t at = static_cast<int64_t>(min(wrow, g.n - 1)) * g.nb + blk;
+    const int64_t at = static_cast<int64_t>(min(n0 + brow, g.n - 1)) * g.nb + blk;
     const u32x4s* src = reinterpret_cast<const u32x4s*>(g.wc + at * kCodeBytes<FMT>);
 #pragma unroll
-    for (int v = 0; v < WV; ++v) rb[v] = wrow < g.n ? src[v] : u32x4s{0, 0, 0, 0};
-    rs = wrow < g.n ? mx_scale(g.ws[at]) : 1.0f;
+    for (int v = 0; v < WV; ++v) rb[v] = src[v];
+    rs = g.ws[at];
   };
-  auto store = [&](int buf) {
+  auto store = [&](int s, int buf) {  // stage s, in registers, to LDS; zeros past the contraction's end
     char* base = smem + buf * (kABytes + kBBytes);
+    const bool a_in = s * kGradK + 8 * (t & 7) < g.n, b_in = s * kGradK + brow < g.n;
     if (has_a) {
 #pragma unroll
-      for (int i = 0; i < (AC > 0 ? AC : 1); ++i) *reinterpret_cast<u32x4s*>(base + aat[i]) = ra[i];
+      for (int i = 0; i < (AC > 0 ? AC : 1); ++i)
+        *reinterpret_cast<u32x4s*>(base + aat[i]) = a_in ? ra[i] : u32x4s{0, 0, 0, 0};
     }
+    const float scale = b_in ? mx_scale(rs) : 1.0f;
+#pragma unroll
+    for (int v = 0; v < WV; ++v) rb[v] = b_in ? rb[v] : u32x4s{0, 0, 0, 0};
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const int q = j ^ spread;
@@ -156,7 +164,7 @@ mx_grad_kernel(GradArgs g) {
         lo = q & 1 ? w.z : w.x;
         hi = q & 1 ? w.w : w.y;
       }
-      *reinterpret_cast<u32x4s*>(base + kABytes + bat + q * 16) = decode8<T, FMT>(lo, hi, rs);
+      *reinterpret_cast<u32x4s*>(base + kABytes + bat + q * 16) = decode8<T, FMT>(lo, hi, scale);
     }
   };
 
@@ -178,12 +186,15 @@ mx_grad_kernel(GradArgs g) {
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) acc[mt][nt] = f32x16{};
 
-  auto step = [&](int buf, int kk) {
+  // Two sets of fragments: one step's are read while the other's products run.
+  struct Frags {
+    u32x4s a[MT], b[NT];
+  };
+  auto read = [&](Frags& f, int buf, int kk) {
     const char* base = smem + buf * (kABytes + kBBytes);
-    u32x4s fa[MT], fb[NT];
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt)
-      fa[mt] = *reinterpret_cast<const u32x4s*>(base + af + mt * 4096 + (((2 * kk + half) ^ asw) << 4));
+      f.a[mt] = *reinterpret_cast<const u32x4s*>(base + af + mt * 4096 + (((2 * kk + half) ^ asw) << 4));
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       lds_ptr p = (lds_ptr)(base + kABytes) + bf[nt] + kk * 16 * kWRow;
@@ -191,48 +202,60 @@ mx_grad_kernel(GradArgs g) {
       const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((vec_ptr)p);
       const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((vec_ptr)(p + 4 * kWRow));
       const u32x2s l2 = __builtin_bit_cast(u32x2s, lo), h2 = __builtin_bit_cast(u32x2s, hi);
-      fb[nt] = u32x4s{l2.x, l2.y, h2.x, h2.y};
+      f.b[nt] = u32x4s{l2.x, l2.y, h2.x, h2.y};
     }
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  auto mma = [&](const Frags& f) {
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) acc[mt][nt] = mma16<T>(fa[mt], fb[nt], acc[mt][nt]);
+      for (int nt = 0; nt < NT; ++nt) acc[mt][nt] = mma16<T>(f.a[mt], f.b[nt], acc[mt][nt]);
+    __builtin_amdgcn_sched_barrier(0);
   };
 
-  if (s0 < s1) {
-    load(s0);
-    store(0);
-    if (s0 + 1 < s1) load(s0 + 1);
+  load(s0);
+  store(s0, 0);
+  if (s0 + 1 < s1) load(s0 + 1);
+  __syncthreads();
+  Frags f0, f1;
+  read(f0, 0, 0);
+  for (int s = s0; s < s1; ++s) {
+    const int buf = (s - s0) & 1;
+    read(f1, buf, 1);
+    mma(f0);
+    read(f0, buf, 2);
+    // Stage s + 1 goes into the buffer whose last reads the barrier of stage s - 1 ended.
+    if (s + 1 < s1) store(s + 1, buf ^ 1);
+    if (s + 2 < s1) load(s + 2);
+    mma(f1);
+    read(f1, buf, 3);
+    mma(f0);
     __syncthreads();
-    for (int s = s0; s < s1; ++s) {
-      const int buf = (s - s0) & 1;
-      step(buf, 0);
-      step(buf, 1);
-      // Stage s + 1 goes into the buffer whose last reads the barrier of stage s - 1 ended.
-      if (s + 1 < s1) store(buf ^ 1);
-      if (s + 2 < s1) load(s + 2);
-      step(buf, 2);
-      step(buf, 3);
-      __syncthreads();
-    }
+    if (s + 1 < s1) read(f0, buf ^ 1, 0);
+    mma(f1);
   }
 
+  auto write = [&](auto put) {
 #pragma unroll
-  for (int nt = 0; nt < NT; ++nt) {
-    const int col = c0 + wn * (kGradN / WN) + nt * 32 + (lane & 31);
-    if (col >= g.k) continue;
+    for (int nt = 0; nt < NT; ++nt) {
+      const int col = c0 + wn * (kGradN / WN) + nt * 32 + (lane & 31);
+      if (col >= g.k) continue;
 #pragma unroll
-    for (int mt = 0; mt < MT; ++mt)
+      for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const int row = m0 + wm * (TM / WM) + mt * 32 + 8 * (r >> 2) + 4 * half + (r & 3);
-        if (row >= g.m) continue;
-        if constexpr (SPLIT)
-          static_cast<float*>(g.dx)[(static_cast<int64_t>(split) * g.m + row) * g.k + col] =
-              acc[mt][nt][r];
-        else
-          static_cast<T*>(g.dx)[row * g.ld_dx + col] = from_f32<T>(acc[mt][nt][r]);
-      }
+        for (int r = 0; r < 16; ++r) {
+          const int row = m0 + wm * (TM / WM) + mt * 32 + 8 * (r >> 2) + 4 * half + (r & 3);
+          if (row < g.m) put(row, col, acc[mt][nt][r]);
+        }
+    }
+  };
+  if (g.splits > 1) {
+    float* parts = static_cast<float*>(g.dx) + static_cast<int64_t>(split) * g.m * g.k;
+    write([&](int row, int col, float v) { parts[static_cast<int64_t>(row) * g.k + col] = v; });
+  } else {
+    T* dx = static_cast<T*>(g.dx);
+    write([&](int row, int col, float v) { dx[row * g.ld_dx + col] = from_f32<T>(v); });
   }
 }
 
@@ -341,7 +364,6 @@ extern "C" int rus_mx_gemm_t(const void* dy, int64_t stride_dy, int32_t dtype, c
   g.stages = static_cast<int>((n + kGradK - 1) / kGradK);
   g.dx = split ? static_cast<void*>(workspace) : dx;
   g.ld_dx = stride_dx;
-  g.vec = aligned(dy, 16) && stride_dy % 8 == 0;
   hipStream_t st = static_cast<hipStream_t>(stream);
   const dim3 grid(static_cast<unsigned>(8 * ((tiles * plan.splits + 7) / 8)));
   auto go = [&](auto kern) { hipLaunchKernelGGL(kern, grid, dim3(kGradThreads), 0, st, g); };
@@ -350,13 +372,13 @@ extern "C" int rus_mx_gemm_t(const void* dy, int64_t stride_dy, int32_t dtype, c
     constexpr int F = decltype(fmt)::value;
     switch (plan.tm) {
       case 256:
-        return split ? go(mx_grad_kernel<T, F, 256, true>) : go(mx_grad_kernel<T, F, 256, false>);
+        return go(mx_grad_kernel<T, F, 256>);
       case 128:
-        return split ? go(mx_grad_kernel<T, F, 128, true>) : go(mx_grad_kernel<T, F, 128, false>);
+        return go(mx_grad_kernel<T, F, 128>);
       case 64:
-        return split ? go(mx_grad_kernel<T, F, 64, true>) : go(mx_grad_kernel<T, F, 64, false>);
+        return go(mx_grad_kernel<T, F, 64>);
       default:
-        return split ? go(mx_grad_kernel<T, F, 32, true>) : go(mx_grad_kernel<T, F, 32, false>);
+        return go(mx_grad_kernel<T, F, 32>);
     }
   };
   auto types = [&](auto t) {
