@@ -854,11 +854,16 @@ int rus_rmsnorm_mx_fwd(const void* x, const void* residual, const void* weight, 
 
 /*
  * y[m, n] = T(sum_k X[m, k] W[n, k] + bias[n]); X [m, k] and W [n, k] in either format, T fp16 or
- * bf16 (dtype), bias in T or NULL; fp32 sums.
+ * bf16 (dtype), bias in T or NULL; fp32 sums; k at most 2^22. workspace: the fp32 elements
+ * rus_mx_gemm_workspace names (0: none; 16-byte aligned), for a contraction that few tiles split
+ * among them; not shared by calls that overlap.
  */
+int rus_mx_gemm_workspace(int64_t m, int64_t n, int64_t k, int32_t x_fmt, int32_t w_fmt,
+                          int64_t* floats);
 int rus_mx_gemm(const void* x_codes, const void* x_scales, int32_t x_fmt, const void* w_codes,
                 const void* w_scales, int32_t w_fmt, int64_t m, int64_t n, int64_t k,
-                const void* bias, void* y, int64_t stride_y, int32_t dtype, void* stream);
+                const void* bias, void* y, int64_t stride_y, int32_t dtype, float* workspace,
+                int64_t n_workspace, void* stream);
 
 /*
  * The input gradient of rus_mx_gemm: dx[m, k] = T(sum_n dy[m, n] T(W[n, k])), dy and dx in T = fp16

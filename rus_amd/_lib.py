@@ -154,7 +154,9 @@ SIGNATURES: dict[str, list] = {
     "rus_mx_dequantize": [_vp, _vp, _i32, _i64, _i64, _vp, _i32, _i64, _vp],
     "rus_rmsnorm_mx_fwd": [_vp, _vp, _vp, _i32, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _f32, _i32,
                            _vp],
-    "rus_mx_gemm": [_vp, _vp, _i32, _vp, _vp, _i32, _i64, _i64, _i64, _vp, _vp, _i64, _i32, _vp],
+    "rus_mx_gemm_workspace": [_i64, _i64, _i64, _i32, _i32, ctypes.POINTER(_i64)],
+    "rus_mx_gemm": [_vp, _vp, _i32, _vp, _vp, _i32, _i64, _i64, _i64, _vp, _vp, _i64, _i32, _vp,
+                    _i64, _vp],
     "rus_mx_gemm_t_workspace": [_i64, _i64, _i64, ctypes.POINTER(_i64)],
     "rus_mx_gemm_t": [_vp, _i64, _i32, _vp, _vp, _i32, _i64, _i64, _i64, _vp, _i64, _vp, _i64,
                       _vp],

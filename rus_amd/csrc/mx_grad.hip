@@ -271,6 +271,7 @@ __global__ __launch_bounds__(256) void mx_grad_sum_kernel(const float* __restric
   const float* p = parts + row * k + c;
   float v[V];
   load_f32<float, V>(p, v);
+#pragma unroll 8
   for (int s = 1; s < splits; ++s) {
     float u[V];
     load_f32<float, V>(p + s * m * k, u);

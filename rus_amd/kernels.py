@@ -2522,18 +2522,19 @@ def _mx_bytes(t: MXTensor) -> int:
     return t.codes.numel() + t.scales.numel()
 
 
-_mx_grad_floats: dict[tuple[int, int, int], int] = {}
+_mx_floats: dict[tuple, int] = {}
 
 
-def _mx_grad_workspace(m: int, n: int, k: int) -> int:
-    """fp32 elements of scratch that the gradient product of this shape takes."""
-    key = (m, n, k)
-    got = _mx_grad_floats.get(key)
-    if got is None:
-        floats = ctypes.c_int64()
-        _lib.call("rus_mx_gemm_t_workspace", m, n, k, ctypes.byref(floats))
-        got = _mx_grad_floats[key] = floats.value
-    return got
+def _mx_scratch(fn: str, like: torch.Tensor, *sizes: int) -> tuple[torch.Tensor | None, int]:
+    """The fp32 scratch (and its length) that a product of these sizes takes, by ``fn``'s answer."""
+    floats = _mx_floats.get((fn, sizes))
+    if floats is None:
+        got = ctypes.c_int64()
+        _lib.call(fn, *sizes, ctypes.byref(got))
+        if len(_mx_floats) >= 65536:
+            _mx_floats.clear()
+        floats = _mx_floats[(fn, sizes)] = got.value
+    return (torch.empty(floats, dtype=torch.float32, device=like.device) if floats else None), floats
 
 
 def mx_gemm(x, w: MXTensor, trans: bool = False, bias: torch.Tensor | None = None,
@@ -2563,8 +2564,7 @@ def mx_gemm(x, w: MXTensor, trans: bool = False, bias: torch.Tensor | None = Non
         out = _mx_out(fn, out, m, k, x2.dtype, x2)
         if n == 0:
             return out.zero_()
-        floats = _mx_grad_workspace(m, n, k)
-        ws = torch.empty(floats, dtype=torch.float32, device=x2.device) if floats else None
+        ws, floats = _mx_scratch("rus_mx_gemm_t_workspace", x2, m, n, k)
         _mx_launch("mx_gemm_t", 2 * m * (n + k) + _mx_bytes(w), 2 * m * n * k, x2, "rus_mx_gemm_t",
                    x2.data_ptr(), _ld(x2), dt, w.codes.data_ptr(), w.scales.data_ptr(), wf, m, n, k,
                    out.data_ptr(), _ld(out), _ptr(ws), floats)
@@ -2580,10 +2580,12 @@ def mx_gemm(x, w: MXTensor, trans: bool = False, bias: torch.Tensor | None = Non
     out = _mx_out(fn, out, m, n, dtype, x.codes)
     if n == 0:
         return out
+    xf = _MX_FMT[x.fmt][0]
+    ws, floats = _mx_scratch("rus_mx_gemm_workspace", x.codes, m, n, k, xf, wf)
     _mx_launch("mx_gemm", _mx_bytes(x) + _mx_bytes(w) + 2 * m * n, 2 * m * n * k, x.codes,
-               "rus_mx_gemm", x.codes.data_ptr(), x.scales.data_ptr(), _MX_FMT[x.fmt][0],
-               w.codes.data_ptr(), w.scales.data_ptr(), wf, m, n, k, _ptr(bias), out.data_ptr(),
-               _ld(out), dt)
+               "rus_mx_gemm", x.codes.data_ptr(), x.scales.data_ptr(), xf, w.codes.data_ptr(),
+               w.scales.data_ptr(), wf, m, n, k, _ptr(bias), out.data_ptr(), _ld(out), dt, _ptr(ws),
+               floats)
     return out
 
 

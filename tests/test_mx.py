@@ -157,13 +157,16 @@ F16, F32, BF16, FP4, FP8 = 0, 1, 2, 0, 1
     ("rus_rmsnorm_mx_fwd", (16, 16, 16, F16, None, 16, 16, 16, 4, 64, 64, 1e-6, F16, None), "together"),
     ("rus_rmsnorm_mx_fwd", (16, None, 16, F16, None, 16, 16, 16, 4, 64, 64, 1e-6, BF16, None), "fp16 or fp32"),
     ("rus_rmsnorm_mx_fwd", (16, None, None, F16, None, 16, 16, 16, 4, 64, 64, 1e-6, F16, None), "null"),
-    ("rus_mx_gemm", (16, 16, FP8, 16, 16, FP4, 4, 0, 64, None, 16, 64, F16, None), "bad sizes"),
-    ("rus_mx_gemm", (16, 16, FP8, 16, 16, FP4, 4, 64, 64, None, 16, 63, F16, None), "stride"),
-    ("rus_mx_gemm", (16, 16, FP8, 16, 16, FP4, 4, 64, 64, None, 16, 64, F32, None), "fp16 or bf16"),
-    ("rus_mx_gemm", (16, 16, 7, 16, 16, FP4, 4, 64, 64, None, 16, 64, F16, None), "x has unknown"),
-    ("rus_mx_gemm", (16, 16, FP8, 16, 18, FP4, 4, 64, 64, None, 16, 64, F16, None), "w codes"),
-    ("rus_mx_gemm", (16, 16, FP8, 16, 16, FP4, 4, 64, 64, None, None, 64, F16, None), "output"),
-    ("rus_mx_gemm", (16, 16, FP8, 16, 16, FP4, 4, 64, 64, 17, 16, 64, F16, None), "bias"),
+    ("rus_mx_gemm", (16, 16, FP8, 16, 16, FP4, 4, 0, 64, None, 16, 64, F16, None, 0, None), "bad sizes"),
+    ("rus_mx_gemm", (16, 16, FP8, 16, 16, FP4, 4, 64, 64, None, 16, 63, F16, None, 0, None), "stride"),
+    ("rus_mx_gemm", (16, 16, FP8, 16, 16, FP4, 4, 64, 64, None, 16, 64, F32, None, 0, None), "fp16 or bf16"),
+    ("rus_mx_gemm", (16, 16, 7, 16, 16, FP4, 4, 64, 64, None, 16, 64, F16, None, 0, None), "x has unknown"),
+    ("rus_mx_gemm", (16, 16, FP8, 16, 18, FP4, 4, 64, 64, None, 16, 64, F16, None, 0, None), "w codes"),
+    ("rus_mx_gemm", (16, 16, FP8, 16, 16, FP4, 4, 64, 64, None, None, 64, F16, None, 0, None), "output"),
+    ("rus_mx_gemm", (16, 16, FP8, 16, 16, FP4, 4, 64, 64, 17, 16, 64, F16, None, 0, None), "bias"),
+    ("rus_mx_gemm", (16, 16, FP8, 16, 16, FP4, 1, 1536, 8960, None, 16, 1536, F16, 16, 8, None), "workspace holds"),
+    ("rus_mx_gemm", (16, 16, FP8, 16, 16, FP4, 1, 64, 1 << 23, None, 16, 64, F16, None, 0, None), "bad sizes"),
+    ("rus_mx_gemm_workspace", (1, 64, 0, FP8, FP4, None), "null result"),
     ("rus_mx_glu_fwd", (16, 16, FP8, 16, 16, FP4, 4, 64, 64, 16, 63, F16, None), "stride"),
     ("rus_mx_glu_bwd", (16, 64, 16, 16, FP8, 16, 16, FP4, 4, 64, 64, 16, 127, F16, None), "stride"),
     ("rus_mx_glu_bwd", (16, 63, 16, 16, FP8, 16, 16, FP4, 4, 64, 64, 16, 128, F16, None), "stride_dh"),
@@ -182,5 +185,5 @@ def test_entry_points_refuse(name, args, msg):
 
 def test_empty_batches_launch_nothing():
     _lib.call("rus_mx_quantize", None, F16, 0, 64, 64, FP4, None, None, None)
-    _lib.call("rus_mx_gemm", None, None, FP8, None, None, FP4, 0, 64, 64, None, None, 64, F16, None)
+    _lib.call("rus_mx_gemm", None, None, FP8, None, None, FP4, 0, 64, 64, None, None, 64, F16, None, 0, None)
     _lib.call("rus_mx_gemm_t", None, 64, F16, None, None, FP4, 0, 64, 64, None, 64, None, 0, None)
