@@ -866,6 +866,18 @@ int rus_mx_gemm(const void* x_codes, const void* x_scales, int32_t x_fmt, const 
                 int64_t n_workspace, void* stream);
 
 /*
+ * rus_mx_gemm of activations that are not in blocks yet: x [m, k] in T, quantised to `act` first
+ * (rus_mx_quantize). scratch: the bytes rus_mx_rows_scratch names (glu = 0; 16-byte aligned), not
+ * shared by calls that overlap.
+ */
+int rus_mx_rows_scratch(int64_t m, int64_t n, int64_t k, int32_t act, int32_t w_fmt, int32_t glu,
+                        int64_t* bytes);
+int rus_mx_gemm_rows(const void* x, int64_t stride_x, int32_t act, const void* w_codes,
+                     const void* w_scales, int32_t w_fmt, int64_t m, int64_t n, int64_t k,
+                     const void* bias, void* y, int64_t stride_y, int32_t dtype, void* scratch,
+                     int64_t n_scratch, void* stream);
+
+/*
  * The input gradient of rus_mx_gemm: dx[m, k] = T(sum_n dy[m, n] T(W[n, k])), dy and dx in T = fp16
  * or bf16 (dtype), W decoded to T inside the product (an fp16 decode of |W| > 65504 is infinite;
  * bf16 holds every value); fp32 sums. workspace: the fp32 elements rus_mx_gemm_t_workspace names
@@ -884,6 +896,11 @@ int rus_mx_gemm_t(const void* dy, int64_t stride_dy, int32_t dtype, const void* 
 int rus_mx_glu_fwd(const void* x_codes, const void* x_scales, int32_t x_fmt, const void* w_codes,
                    const void* w_scales, int32_t w_fmt, int64_t m, int64_t n, int64_t k, void* h,
                    int64_t stride_h, int32_t dtype, void* stream);
+
+/* rus_mx_glu_fwd of activations not in blocks yet, as rus_mx_gemm_rows (scratch with glu = 1). */
+int rus_mx_glu_fwd_rows(const void* x, int64_t stride_x, int32_t act, const void* w_codes,
+                        const void* w_scales, int32_t w_fmt, int64_t m, int64_t n, int64_t k, void* h,
+                        int64_t stride_h, int32_t dtype, void* scratch, int64_t n_scratch, void* stream);
 
 /*
  * Its backward up to the two projections' outputs: G and U formed again from X and W,

@@ -160,6 +160,11 @@ SIGNATURES: dict[str, list] = {
     "rus_mx_gemm_t_workspace": [_i64, _i64, _i64, ctypes.POINTER(_i64)],
     "rus_mx_gemm_t": [_vp, _i64, _i32, _vp, _vp, _i32, _i64, _i64, _i64, _vp, _i64, _vp, _i64,
                       _vp],
+    "rus_mx_rows_scratch": [_i64, _i64, _i64, _i32, _i32, _i32, ctypes.POINTER(_i64)],
+    "rus_mx_gemm_rows": [_vp, _i64, _i32, _vp, _vp, _i32, _i64, _i64, _i64, _vp, _vp, _i64, _i32, _vp,
+                         _i64, _vp],
+    "rus_mx_glu_fwd_rows": [_vp, _i64, _i32, _vp, _vp, _i32, _i64, _i64, _i64, _vp, _i64, _i32, _vp,
+                            _i64, _vp],
     "rus_mx_glu_fwd": [_vp, _vp, _i32, _vp, _vp, _i32, _i64, _i64, _i64, _vp, _i64, _i32, _vp],
     "rus_mx_glu_bwd": [_vp, _i64, _vp, _vp, _i32, _vp, _vp, _i32, _i64, _i64, _i64, _vp, _i64,
                        _i32, _vp],

@@ -13,6 +13,11 @@
 #include "common.h"
 
 namespace rus {
+
+// rus_mx_quantize, for entry points that quantise what they are given.
+int quantize_rows(const char* fn, const void* x, int32_t dtype, int64_t n_rows, int64_t n_cols,
+                  int64_t stride_row, int32_t fmt, void* codes, void* scales, hipStream_t stream);
+
 namespace {
 
 constexpr int kFp4 = RUS_MX_FP4, kFp8 = RUS_MX_FP8;

@@ -906,15 +906,43 @@ extern "C" int rus_mx_gemm_workspace(int64_t m, int64_t n, int64_t k, int32_t x_
   return RUS_OK;
 }
 
-extern "C" int rus_mx_gemm(const void* x_codes, const void* x_scales, int32_t x_fmt,
-                           const void* w_codes, const void* w_scales, int32_t w_fmt, int64_t m,
-                           int64_t n, int64_t k, const void* bias, void* y, int64_t stride_y,
-                           int32_t dtype, float* workspace, int64_t n_workspace, void* stream) {
-  const char* fn = "rus_mx_gemm";
+// Scratch of a call that quantises its activations: codes, scales, sums, each 16-byte aligned.
+namespace rus {
+namespace {
+struct RowsScratch {
+  int64_t codes, scales, sums;
+  int64_t bytes() const { return codes + scales + 4 * sums; }
+};
+RowsScratch rows_scratch(int64_t m, int64_t n, int64_t k, int32_t act, int32_t w_fmt, bool glu) {
+  const int64_t nb = mx_blocks(k);
+  const GemmPlan p = gemm_plan(m, n, nb, act, w_fmt, glu);
+  return {m * nb * (act == RUS_MX_FP4 ? 16 : 32), (m * nb + 15) / 16 * 16, p.splits > 1 ? p.splits * m * n : 0};
+}
+int check_sizes(const char* fn, int64_t m, int64_t n, int64_t k) {
+  if (m < 0 || n <= 0 || k <= 0 || m >= (1 << 30) || n >= (1 << 28) || k > (1 << 22))
+    return fail(RUS_ERR_INVALID, "%s: bad sizes m=%lld n=%lld k=%lld", fn, (long long)m, (long long)n,
+                (long long)k);
+  return RUS_OK;
+}
+// The scratch's parts, or a refusal.
+int place(const char* fn, const RowsScratch& need, void* scratch, int64_t n_scratch, char*& codes, char*& scales,
+          float*& sums) {
+  if (!scratch || !aligned(scratch, 16) || n_scratch < need.bytes())
+    return fail(RUS_ERR_INVALID, "%s: scratch holds %lld bytes (16-byte aligned), needs %lld", fn,
+                (long long)n_scratch, (long long)need.bytes());
+  codes = static_cast<char*>(scratch);
+  scales = codes + need.codes;
+  sums = need.sums ? reinterpret_cast<float*>(scales + need.scales) : nullptr;
+  return RUS_OK;
+}
+
+// rus_mx_gemm and rus_mx_glu_fwd; `first` runs once nothing is left to refuse.
+template <typename F>
+int run_gemm(const char* fn, const void* xc, const void* xs, int32_t x_fmt, const void* wc, const void* ws,
+             int32_t w_fmt, int64_t m, int64_t n, int64_t k, const void* bias, void* y, int64_t ldy,
+             int32_t dtype, float* workspace, int64_t n_workspace, void* stream, F first) {
   MxArgs g;
-  if (int e = prepare(fn, g, x_codes, x_scales, x_fmt, w_codes, w_scales, w_fmt, m, n, k, y, stride_y,
-                      n, dtype))
-    return e;
+  if (int e = prepare(fn, g, xc, xs, x_fmt, wc, ws, w_fmt, m, n, k, y, ldy, n, dtype)) return e;
   if (m == 0) return RUS_OK;
   if (bias && !aligned(bias, 2)) return fail(RUS_ERR_INVALID, "%s: misaligned bias", fn);
   const GemmPlan plan = gemm_plan(m, n, g.nb, x_fmt, w_fmt, false);
@@ -923,22 +951,83 @@ extern "C" int rus_mx_gemm(const void* x_codes, const void* x_scales, int32_t x_
                 (long long)n_workspace, (long long)(plan.splits * m * n));
   g.bias = bias;
   g.vec = g.vec && (!bias || aligned(bias, 16));
+  if (int e = first()) return e;
   const hipStream_t st = static_cast<hipStream_t>(stream);
   return dtype == RUS_DTYPE_BF16 ? product<bf16>(fn, g, plan, x_fmt, w_fmt, workspace, st)
                                  : product<f16>(fn, g, plan, x_fmt, w_fmt, workspace, st);
+}
+
+template <typename F>
+int run_glu(const char* fn, const void* xc, const void* xs, int32_t x_fmt, const void* wc, const void* ws,
+            int32_t w_fmt, int64_t m, int64_t n, int64_t k, void* h, int64_t ldh, int32_t dtype, void* stream,
+            F first) {
+  MxArgs g;
+  if (int e = prepare(fn, g, xc, xs, x_fmt, wc, ws, w_fmt, m, n, k, h, ldh, n, dtype)) return e;
+  if (m == 0) return RUS_OK;
+  if (int e = first()) return e;
+  return dispatch<kGluFwd>(fn, g, x_fmt, w_fmt, dtype, static_cast<hipStream_t>(stream));
+}
+
+}  // namespace
+}  // namespace rus
+
+extern "C" int rus_mx_gemm(const void* x_codes, const void* x_scales, int32_t x_fmt,
+                           const void* w_codes, const void* w_scales, int32_t w_fmt, int64_t m,
+                           int64_t n, int64_t k, const void* bias, void* y, int64_t stride_y,
+                           int32_t dtype, float* workspace, int64_t n_workspace, void* stream) {
+  return run_gemm("rus_mx_gemm", x_codes, x_scales, x_fmt, w_codes, w_scales, w_fmt, m, n, k, bias, y,
+                  stride_y, dtype, workspace, n_workspace, stream, [] { return RUS_OK; });
+}
+
+extern "C" int rus_mx_rows_scratch(int64_t m, int64_t n, int64_t k, int32_t act, int32_t w_fmt, int32_t glu,
+                                   int64_t* bytes) {
+  const char* fn = "rus_mx_rows_scratch";
+  if (!bytes) return fail(RUS_ERR_INVALID, "%s: null result", fn);
+  if (int e = check_sizes(fn, m, n, k)) return e;
+  *bytes = m > 0 ? rows_scratch(m, n, k, act, w_fmt, glu != 0).bytes() : 0;
+  return RUS_OK;
+}
+
+extern "C" int rus_mx_gemm_rows(const void* x, int64_t stride_x, int32_t act, const void* w_codes,
+                                const void* w_scales, int32_t w_fmt, int64_t m, int64_t n, int64_t k,
+                                const void* bias, void* y, int64_t stride_y, int32_t dtype,
+                                void* scratch, int64_t n_scratch, void* stream) {
+  const char* fn = "rus_mx_gemm_rows";
+  if (int e = check_sizes(fn, m, n, k)) return e;
+  if (m == 0) return RUS_OK;
+  const RowsScratch need = rows_scratch(m, n, k, act, w_fmt, false);
+  char *codes, *scales;
+  float* sums;
+  if (int e = place(fn, need, scratch, n_scratch, codes, scales, sums)) return e;
+  return run_gemm(fn, codes, scales, act, w_codes, w_scales, w_fmt, m, n, k, bias, y, stride_y, dtype, sums,
+                  need.sums, stream, [&] {
+                    return quantize_rows(fn, x, dtype, m, k, stride_x, act, codes, scales,
+                                         static_cast<hipStream_t>(stream));
+                  });
+}
+
+extern "C" int rus_mx_glu_fwd_rows(const void* x, int64_t stride_x, int32_t act, const void* w_codes,
+                                   const void* w_scales, int32_t w_fmt, int64_t m, int64_t n, int64_t k,
+                                   void* h, int64_t stride_h, int32_t dtype, void* scratch,
+                                   int64_t n_scratch, void* stream) {
+  const char* fn = "rus_mx_glu_fwd_rows";
+  if (int e = check_sizes(fn, m, n, k)) return e;
+  if (m == 0) return RUS_OK;
+  char *codes, *scales;
+  float* sums;
+  if (int e = place(fn, rows_scratch(m, n, k, act, w_fmt, true), scratch, n_scratch, codes, scales, sums))
+    return e;
+  return run_glu(fn, codes, scales, act, w_codes, w_scales, w_fmt, m, n, k, h, stride_h, dtype, stream, [&] {
+    return quantize_rows(fn, x, dtype, m, k, stride_x, act, codes, scales, static_cast<hipStream_t>(stream));
+  });
 }
 
 extern "C" int rus_mx_glu_fwd(const void* x_codes, const void* x_scales, int32_t x_fmt,
                               const void* w_codes, const void* w_scales, int32_t w_fmt, int64_t m,
                               int64_t n, int64_t k, void* h, int64_t stride_h, int32_t dtype,
                               void* stream) {
-  const char* fn = "rus_mx_glu_fwd";
-  MxArgs g;
-  if (int e = prepare(fn, g, x_codes, x_scales, x_fmt, w_codes, w_scales, w_fmt, m, n, k, h, stride_h,
-                      n, dtype))
-    return e;
-  if (m == 0) return RUS_OK;
-  return dispatch<kGluFwd>(fn, g, x_fmt, w_fmt, dtype, static_cast<hipStream_t>(stream));
+  return run_glu("rus_mx_glu_fwd", x_codes, x_scales, x_fmt, w_codes, w_scales, w_fmt, m, n, k, h, stride_h,
+                 dtype, stream, [] { return RUS_OK; });
 }
 
 extern "C" int rus_mx_glu_bwd(const void* dh, int64_t stride_dh, const void* x_codes,

@@ -204,14 +204,9 @@ int check_rows(const char* fn, int64_t rows, int64_t cols) {
 }
 
 }  // namespace
-}  // namespace rus
 
-using namespace rus;
-
-extern "C" int rus_mx_quantize(const void* x, int32_t dtype, int64_t n_rows, int64_t n_cols,
-                               int64_t stride_row, int32_t fmt, void* codes, void* scales,
-                               void* stream) {
-  const char* fn = "rus_mx_quantize";
+int quantize_rows(const char* fn, const void* x, int32_t dtype, int64_t n_rows, int64_t n_cols,
+                  int64_t stride_row, int32_t fmt, void* codes, void* scales, hipStream_t stream) {
   if (int e = check_rows(fn, n_rows, n_cols)) return e;
   if (stride_row < n_cols && n_rows > 1)
     return fail(RUS_ERR_INVALID, "%s: stride_row=%lld smaller than a row", fn, (long long)stride_row);
@@ -225,9 +220,8 @@ extern "C" int rus_mx_quantize(const void* x, int32_t dtype, int64_t n_rows, int
     const bool vec = aligned(x, 16) && (stride_row * sizeof(T)) % 16 == 0;
     const dim3 grid(static_cast<unsigned>((total + 255) / 256));
     auto go = [&](auto k) {
-      hipLaunchKernelGGL(k, grid, dim3(256), 0, static_cast<hipStream_t>(stream),
-                         static_cast<const T*>(x), stride_row, static_cast<int>(n_cols), nb, total,
-                         vec, static_cast<uint8_t*>(codes), static_cast<uint8_t*>(scales));
+      hipLaunchKernelGGL(k, grid, dim3(256), 0, stream, static_cast<const T*>(x), stride_row,
+                         static_cast<int>(n_cols), nb, total, vec, static_cast<uint8_t*>(codes), static_cast<uint8_t*>(scales));
     };
     if (fmt == RUS_MX_FP4)
       go(mx_quantize_kernel<T, kFp4>);
@@ -235,6 +229,17 @@ extern "C" int rus_mx_quantize(const void* x, int32_t dtype, int64_t n_rows, int
       go(mx_quantize_kernel<T, kFp8>);
     return check_launch(fn);
   });
+}
+
+}  // namespace rus
+
+using namespace rus;
+
+extern "C" int rus_mx_quantize(const void* x, int32_t dtype, int64_t n_rows, int64_t n_cols,
+                               int64_t stride_row, int32_t fmt, void* codes, void* scales,
+                               void* stream) {
+  return quantize_rows("rus_mx_quantize", x, dtype, n_rows, n_cols, stride_row, fmt, codes, scales,
+                       static_cast<hipStream_t>(stream));
 }
 
 extern "C" int rus_mx_dequantize(const void* codes, const void* scales, int32_t fmt, int64_t n_rows,

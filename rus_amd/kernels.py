@@ -101,6 +101,7 @@ def _dtype_code(fn: str, dtype: torch.dtype) -> int:
 
 # The current stream's handle by device index, without a Stream object: 0.2 us instead of 3 us on
 # each of the launches, five to nine of which make up one LoRA branch or one lm_head pass.
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
     lambda index: torch.cuda.current_stream(index).cuda_stream)
 
@@ -2348,6 +2349,13 @@ class MXTensor:
             raise ValueError(f"{fn}: codes on {codes.device}, scales on {scales.device}")
         self.codes, self.scales, self.shape, self.fmt = codes, scales, (rows, cols), fmt
 
+    @classmethod
+    def _of(cls, codes, scales, shape, fmt) -> "MXTensor":
+        """Of a kernel's own outputs (nothing to check)."""
+        t = object.__new__(cls)
+        t.codes, t.scales, t.shape, t.fmt = codes, scales, shape, fmt
+        return t
+
     @property
     def device(self) -> torch.device:
         return self.codes.device
@@ -2384,18 +2392,14 @@ class MXTensor:
         return cls(c, s, (rows, cols), fmt)
 
 
-def _mx_check(fn: str, t: MXTensor, name: str, like: torch.Tensor) -> None:
-    if not isinstance(t, MXTensor):
-        raise TypeError(f"{fn}: {name} must be an MXTensor, got {type(t).__name__}")
-    if t.codes.device != like.device:
-        raise ValueError(f"{fn}: {name} is on {t.codes.device}, other operands on {like.device}")
-
-
 def _same_device(fn: str, like: torch.Tensor, *tensors: torch.Tensor | None) -> None:
-    _require_device(fn, like, *tensors)
+    index = like.get_device()  # -1: not on a device
     for t in tensors:
-        if t is not None and t.device != like.device:
+        if t is not None and t.get_device() != index:
+            _require_device(fn, like, t)
             raise ValueError(f"{fn}: operands on {t.device} and {like.device}")
+    if index < 0:
+        _require_device(fn, like)
 
 
 def _mx_rows(fn: str, x: torch.Tensor, width: int | None, name: str) -> torch.Tensor:
@@ -2422,14 +2426,18 @@ def _ld(t: torch.Tensor) -> int:
     return max(t.stride(0), t.shape[1])  # a single row's stride may be anything
 
 
-def _mx_launch(kernel: str, nbytes: float, flops: float, like: torch.Tensor, fn: str, *args) -> None:
-    """``_launch`` on ``like``'s device and that device's current stream (the last argument)."""
+def _mx_launch(kernel: str, cost, like: torch.Tensor, fn: str, *args) -> None:
+    """``_launch`` on ``like``'s device and that device's current stream (the last argument);
+    ``cost()``: (bytes, FLOPs), asked for only under a KernelTimer."""
     index = like.get_device()
-    if index == torch.cuda.current_device():
-        _launch(kernel, nbytes, flops, fn, *args, _raw_stream(index))
+    if index == _current_device():
+        if KernelTimer.active is None:
+            _lib.call(fn, *args, _raw_stream(index))
+        else:
+            _launch(kernel, *cost(), fn, *args, _raw_stream(index))
     else:
         with torch.cuda.device(index):
-            _launch(kernel, nbytes, flops, fn, *args, _raw_stream(index))
+            _launch(kernel, *cost(), fn, *args, _raw_stream(index))
 
 
 def mx_quantize(x: torch.Tensor, fmt: str = "fp4") -> MXTensor:
@@ -2448,10 +2456,10 @@ def mx_quantize(x: torch.Tensor, fmt: str = "fp4") -> MXTensor:
     nb = _mx_blocks(cols)
     codes = torch.empty((rows, nb * nbytes), dtype=torch.uint8, device=x2.device)
     scales = torch.empty((rows, nb), dtype=torch.uint8, device=x2.device)
-    _mx_launch("mx_quantize", rows * (cols * x2.element_size() + nb * (nbytes + 1)), 0, x2,
+    _mx_launch("mx_quantize", lambda: (rows * (cols * x2.element_size() + nb * (nbytes + 1)), 0), x2,
                "rus_mx_quantize", x2.data_ptr(), dt, rows, cols, _ld(x2), code, codes.data_ptr(),
                scales.data_ptr())
-    return MXTensor(codes, scales, (rows, cols), fmt)
+    return MXTensor._of(codes, scales, (rows, cols), fmt)
 
 
 def mx_dequantize(t: MXTensor, dtype: torch.dtype = torch.float16,
@@ -2465,8 +2473,9 @@ def mx_dequantize(t: MXTensor, dtype: torch.dtype = torch.float16,
     code, nbytes = _MX_FMT[t.fmt]
     rows, cols = t.shape
     out = _mx_out(fn, out, rows, cols, dtype, t.codes)
-    _mx_launch("mx_dequantize", rows * (_mx_blocks(cols) * (nbytes + 1) + cols * out.element_size()),
-               0, t.codes, "rus_mx_dequantize", t.codes.data_ptr(), t.scales.data_ptr(), code, rows,
+    _mx_launch("mx_dequantize",
+               lambda: (rows * (_mx_blocks(cols) * (nbytes + 1) + cols * out.element_size()), 0), t.codes,
+               "rus_mx_dequantize", t.codes.data_ptr(), t.scales.data_ptr(), code, rows,
                cols, out.data_ptr(), dt, _ld(out))
     return out
 
@@ -2483,8 +2492,8 @@ def rms_norm_mx_fwd(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6,
     n_cols = x.shape[-1]
     if n_cols == 0:
         raise ValueError(f"{fn}: rows without columns")
-    x_2d = x.contiguous().view(-1, n_cols)
-    n_rows = x_2d.shape[0]
+    x_2d = x.contiguous()
+    n_rows = x_2d.numel() // n_cols
     w = weight.contiguous()
     if w.numel() != n_cols:
         raise ValueError(f"{fn}: weight has {w.numel()} entries, rows have {n_cols}")
@@ -2492,49 +2501,51 @@ def rms_norm_mx_fwd(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6,
     if residual is not None:
         if residual.dtype != x.dtype or residual.shape != x.shape:
             raise ValueError(f"{fn}: residual must match x in shape and dtype")
-        res_2d = residual.contiguous().view(-1, n_cols)
+        res_2d = residual.contiguous()
         sum_out = torch.empty_like(x_2d)
     nb = _mx_blocks(n_cols)
     codes = torch.empty((n_rows, nb * 32), dtype=torch.uint8, device=x.device)
     scales = torch.empty((n_rows, nb), dtype=torch.uint8, device=x.device)
     rstd = torch.empty((n_rows,), dtype=torch.float32, device=x.device)
-    nbytes = n_rows * ((1 if res_2d is None else 3) * n_cols * x_2d.element_size() + nb * 33 + 4) + \
-        w.numel() * w.element_size()
-    _mx_launch("rmsnorm_mx_fwd", nbytes, 0, x_2d, "rus_rmsnorm_mx_fwd", x_2d.data_ptr(), _ptr(res_2d),
+    def cost():
+        streams = 1 if res_2d is None else 3
+        return n_rows * (streams * n_cols * x_2d.element_size() + nb * 33 + 4) + n_cols * w.element_size(), 0
+    _mx_launch("rmsnorm_mx_fwd", cost, x_2d, "rus_rmsnorm_mx_fwd", x_2d.data_ptr(), _ptr(res_2d),
                w.data_ptr(), wdt, _ptr(sum_out), codes.data_ptr(), scales.data_ptr(), rstd.data_ptr(),
                n_rows, n_cols, n_cols, float(eps), dt)
-    return (MXTensor(codes, scales, (n_rows, n_cols), "fp8"),
-            x if sum_out is None else sum_out.view(x.shape), rstd)
+    return MXTensor._of(codes, scales, (n_rows, n_cols), "fp8"), x if sum_out is None else sum_out, rstd
 
 
-def _mx_operand(fn: str, x, act: str, k: int, dtype: torch.dtype | None):
-    """(blocks of x, result type): x as it is, or quantised to ``act``."""
+def _mx_operand(fn: str, x, act: str, k: int) -> MXTensor:
+    """x in blocks: as it is, or quantised to ``act``."""
     if not isinstance(x, MXTensor):
-        dtype = x.dtype if dtype is None else dtype
-        _require_device(fn, x)
-        x = mx_quantize(_mx_rows(fn, x, k, "x"), act)
-    elif x.shape[1] != k:
+        return mx_quantize(_mx_rows(fn, x, k, "x"), act)
+    if x.shape[1] != k:
         raise ValueError(f"{fn}: x has {x.shape[1]} columns, W {k}")
-    return x, torch.float16 if dtype is None else dtype
+    return x
 
 
 def _mx_bytes(t: MXTensor) -> int:
     return t.codes.numel() + t.scales.numel()
 
 
-_mx_floats: dict[tuple, int] = {}
+_mx_sizes: dict[tuple, int] = {}
 
 
-def _mx_scratch(fn: str, like: torch.Tensor, *sizes: int) -> tuple[torch.Tensor | None, int]:
-    """The fp32 scratch (and its length) that a product of these sizes takes, by ``fn``'s answer."""
-    floats = _mx_floats.get((fn, sizes))
-    if floats is None:
+def _mx_scratch(fn: str, *sizes: int) -> int:
+    """How much scratch a call of these sizes takes, by the library function ``fn``."""
+    need = _mx_sizes.get((fn, sizes))
+    if need is None:
         got = ctypes.c_int64()
         _lib.call(fn, *sizes, ctypes.byref(got))
-        if len(_mx_floats) >= 65536:
-            _mx_floats.clear()
-        floats = _mx_floats[(fn, sizes)] = got.value
-    return (torch.empty(floats, dtype=torch.float32, device=like.device) if floats else None), floats
+        if len(_mx_sizes) >= 65536:
+            _mx_sizes.clear()
+        need = _mx_sizes[(fn, sizes)] = got.value
+    return need
+
+
+def _floats(n: int, like: torch.Tensor) -> torch.Tensor | None:
+    return torch.empty(n, dtype=torch.float32, device=like.device) if n else None
 
 
 def mx_gemm(x, w: MXTensor, trans: bool = False, bias: torch.Tensor | None = None,
@@ -2564,25 +2575,42 @@ def mx_gemm(x, w: MXTensor, trans: bool = False, bias: torch.Tensor | None = Non
         out = _mx_out(fn, out, m, k, x2.dtype, x2)
         if n == 0:
             return out.zero_()
-        ws, floats = _mx_scratch("rus_mx_gemm_t_workspace", x2, m, n, k)
-        _mx_launch("mx_gemm_t", 2 * m * (n + k) + _mx_bytes(w), 2 * m * n * k, x2, "rus_mx_gemm_t",
+        floats = _mx_scratch("rus_mx_gemm_t_workspace", m, n, k)
+        ws = _floats(floats, x2)
+        _mx_launch("mx_gemm_t", lambda: (2 * m * (n + k) + _mx_bytes(w), 2 * m * n * k), x2, "rus_mx_gemm_t",
                    x2.data_ptr(), _ld(x2), dt, w.codes.data_ptr(), w.scales.data_ptr(), wf, m, n, k,
                    out.data_ptr(), _ld(out), _ptr(ws), floats)
         return out
-    _same_device(fn, w.codes, x.codes if isinstance(x, MXTensor) else x, bias, out)
-    x, dtype = _mx_operand(fn, x, act, k, dtype)
+    blocks = isinstance(x, MXTensor)
+    _same_device(fn, w.codes, x.codes if blocks else x, bias, out)
+    if dtype is None:
+        dtype = torch.float16 if blocks else x.dtype
     dt = _mx_dtype(fn, dtype, wide=False)
     if bias is not None:
         if bias.dtype != dtype or bias.numel() != n:
             raise ValueError(f"{fn}: bias must be {dtype} [{n}]")
         bias = bias.reshape(-1).contiguous()
+    if not blocks and x.dtype == dtype:  # quantised on the way
+        xf, x = _mx_fmt(fn, act)[0], _mx_rows(fn, x, k, "x")
+        m = x.shape[0]
+        out = _mx_out(fn, out, m, n, dtype, x)
+        if n == 0:
+            return out
+        need = _mx_scratch("rus_mx_rows_scratch", m, n, k, xf, wf, 0)
+        scratch = torch.empty(need, dtype=torch.uint8, device=x.device)
+        _mx_launch("mx_gemm", lambda: (2 * m * (n + k) + _mx_bytes(w), 2 * m * n * k), x, "rus_mx_gemm_rows",
+                   x.data_ptr(), _ld(x), xf, w.codes.data_ptr(), w.scales.data_ptr(), wf, m, n, k, _ptr(bias),
+                   out.data_ptr(), _ld(out), dt, scratch.data_ptr(), need)
+        return out
+    x = _mx_operand(fn, x, act, k)
     m = x.shape[0]
     out = _mx_out(fn, out, m, n, dtype, x.codes)
     if n == 0:
         return out
     xf = _MX_FMT[x.fmt][0]
-    ws, floats = _mx_scratch("rus_mx_gemm_workspace", x.codes, m, n, k, xf, wf)
-    _mx_launch("mx_gemm", _mx_bytes(x) + _mx_bytes(w) + 2 * m * n, 2 * m * n * k, x.codes,
+    floats = _mx_scratch("rus_mx_gemm_workspace", m, n, k, xf, wf)
+    ws = _floats(floats, x.codes)
+    _mx_launch("mx_gemm", lambda: (_mx_bytes(x) + _mx_bytes(w) + 2 * m * n, 2 * m * n * k), x.codes,
                "rus_mx_gemm", x.codes.data_ptr(), x.scales.data_ptr(), xf, w.codes.data_ptr(),
                w.scales.data_ptr(), wf, m, n, k, _ptr(bias), out.data_ptr(), _ld(out), dt, _ptr(ws),
                floats)
@@ -2603,16 +2631,28 @@ def mx_mlp_glu_fwd(x, w: MXTensor, act: str = "fp8", out: torch.Tensor | None = 
     in blocks, x as in ``mx_gemm``. The two projections stay in fp32 registers."""
     fn = "mx_mlp_glu_fwd"
     n = _mx_glu_weight(fn, w)
-    k = w.shape[1]
-    _same_device(fn, w.codes, x.codes if isinstance(x, MXTensor) else x, out)
-    x, dtype = _mx_operand(fn, x, act, k, dtype)
+    k, wf = w.shape[1], _MX_FMT[w.fmt][0]
+    blocks = isinstance(x, MXTensor)
+    _same_device(fn, w.codes, x.codes if blocks else x, out)
+    if dtype is None:
+        dtype = torch.float16 if blocks else x.dtype
     dt = _mx_dtype(fn, dtype, wide=False)
+    if not blocks and x.dtype == dtype:  # quantised on the way
+        xf, x = _mx_fmt(fn, act)[0], _mx_rows(fn, x, k, "x")
+        m = x.shape[0]
+        out = _mx_out(fn, out, m, n, dtype, x)
+        need = _mx_scratch("rus_mx_rows_scratch", m, n, k, xf, wf, 1)
+        scratch = torch.empty(need, dtype=torch.uint8, device=x.device)
+        _mx_launch("mx_glu_fwd", lambda: (2 * m * (n + k) + _mx_bytes(w), 4 * m * n * k), x,
+                   "rus_mx_glu_fwd_rows", x.data_ptr(), _ld(x), xf, w.codes.data_ptr(), w.scales.data_ptr(),
+                   wf, m, n, k, out.data_ptr(), _ld(out), dt, scratch.data_ptr(), need)
+        return out
+    x = _mx_operand(fn, x, act, k)
     m = x.shape[0]
     out = _mx_out(fn, out, m, n, dtype, x.codes)
-    _mx_launch("mx_glu_fwd", _mx_bytes(x) + _mx_bytes(w) + 2 * m * n, 4 * m * n * k, x.codes,
+    _mx_launch("mx_glu_fwd", lambda: (_mx_bytes(x) + _mx_bytes(w) + 2 * m * n, 4 * m * n * k), x.codes,
                "rus_mx_glu_fwd", x.codes.data_ptr(), x.scales.data_ptr(), _MX_FMT[x.fmt][0],
-               w.codes.data_ptr(), w.scales.data_ptr(), _MX_FMT[w.fmt][0], m, n, k, out.data_ptr(),
-               _ld(out), dt)
+               w.codes.data_ptr(), w.scales.data_ptr(), wf, m, n, k, out.data_ptr(), _ld(out), dt)
     return out
 
 
@@ -2626,13 +2666,13 @@ def mx_mlp_glu_bwd(dh: torch.Tensor, x, w: MXTensor, act: str = "fp8",
     k = w.shape[1]
     _same_device(fn, w.codes, x.codes if isinstance(x, MXTensor) else x, dh, out)
     dt = _mx_dtype(fn, dh.dtype, wide=False)
-    x, _ = _mx_operand(fn, x, act, k, dh.dtype)
+    x = _mx_operand(fn, x, act, k)
     dh2 = _mx_rows(fn, dh, n, "dh")
     m = x.shape[0]
     if dh2.shape[0] != m:
         raise ValueError(f"{fn}: dh has {dh2.shape[0]} rows, x {m}")
     out = _mx_out(fn, out, m, 2 * n, dh.dtype, dh2)
-    _mx_launch("mx_glu_bwd", _mx_bytes(x) + _mx_bytes(w) + 6 * m * n, 4 * m * n * k, dh2,
+    _mx_launch("mx_glu_bwd", lambda: (_mx_bytes(x) + _mx_bytes(w) + 6 * m * n, 4 * m * n * k), dh2,
                "rus_mx_glu_bwd", dh2.data_ptr(), _ld(dh2), x.codes.data_ptr(), x.scales.data_ptr(),
                _MX_FMT[x.fmt][0], w.codes.data_ptr(), w.scales.data_ptr(), _MX_FMT[w.fmt][0], m, n, k,
                out.data_ptr(), _ld(out), dt)

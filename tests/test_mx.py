@@ -167,6 +167,15 @@ F16, F32, BF16, FP4, FP8 = 0, 1, 2, 0, 1
     ("rus_mx_gemm", (16, 16, FP8, 16, 16, FP4, 1, 1536, 8960, None, 16, 1536, F16, 16, 8, None), "workspace holds"),
     ("rus_mx_gemm", (16, 16, FP8, 16, 16, FP4, 1, 64, 1 << 23, None, 16, 64, F16, None, 0, None), "bad sizes"),
     ("rus_mx_gemm_workspace", (1, 64, 0, FP8, FP4, None), "null result"),
+    ("rus_mx_gemm_rows", (16, 64, FP8, 16, 16, FP4, 4, 64, 64, None, 16, 64, F16, 16, 8, None), "scratch holds"),
+    ("rus_mx_gemm_rows", (16, 64, FP8, 16, 16, FP4, 4, 64, 64, None, 16, 64, F16, None, 1 << 20, None), "scratch holds"),
+    ("rus_mx_gemm_rows", (16, 64, FP8, 16, 16, FP4, 4, 0, 64, None, 16, 64, F16, 16, 1 << 20, None), "bad sizes"),
+    ("rus_mx_gemm_rows", (16, 64, FP8, 16, 18, FP4, 4, 64, 64, None, 16, 64, F16, 16, 1 << 20, None), "w codes"),
+    ("rus_mx_gemm_rows", (16, 63, FP8, 16, 16, FP4, 4, 64, 64, None, 16, 64, F16, 16, 1 << 20, None), "stride_row"),
+    ("rus_mx_gemm_rows", (16, 64, 9, 16, 16, FP4, 4, 64, 64, None, 16, 64, F16, 16, 1 << 20, None), "format"),
+    ("rus_mx_glu_fwd_rows", (16, 64, FP8, 16, 16, FP4, 4, 64, 64, 16, 64, F16, 16, 8, None), "scratch holds"),
+    ("rus_mx_glu_fwd_rows", (16, 64, FP8, 16, 16, 5, 4, 64, 64, 16, 64, F16, 16, 1 << 20, None), "w has unknown"),
+    ("rus_mx_rows_scratch", (1, 64, 64, FP8, FP4, 0, None), "null result"),
     ("rus_mx_glu_fwd", (16, 16, FP8, 16, 16, FP4, 4, 64, 64, 16, 63, F16, None), "stride"),
     ("rus_mx_glu_bwd", (16, 64, 16, 16, FP8, 16, 16, FP4, 4, 64, 64, 16, 127, F16, None), "stride"),
     ("rus_mx_glu_bwd", (16, 63, 16, 16, FP8, 16, 16, FP4, 4, 64, 64, 16, 128, F16, None), "stride_dh"),
