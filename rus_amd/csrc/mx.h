@@ -10,6 +10,9 @@
 // A block that holds an infinity or a NaN is NaN as a whole (scale 255).
 #pragma once
 
+#include <type_traits>
+#include <utility>
+
 #include "common.h"
 
 namespace rus {
@@ -102,6 +105,42 @@ __device__ __forceinline__ void from_fp4(uint32_t w, float s, float (&v)[8]) {
 #pragma unroll
   for (int i = 0; i < 8; ++i) v[i] = e[i] * s;
 }
+
+// f(0), f(1), .. f(N - 1) as compile-time constants.
+template <typename F, int... I>
+__device__ __forceinline__ void each_of(F f, std::integer_sequence<int, I...>) {
+  (f(std::integral_constant<int, I>{}), ...);
+}
+template <int N, typename F>
+__device__ __forceinline__ void each(F f) {
+  each_of(f, std::make_integer_sequence<int, N>{});
+}
+
+// A thread's last plans by the sizes they are for: finding one goes over all choices, a few us.
+template <typename Plan>
+class PlanMemo {
+ public:
+  struct Key {
+    int64_t a, b, c, d;
+  };
+  template <typename F>
+  Plan get(const Key& k, F find) {
+    const uint64_t h = (static_cast<uint64_t>(k.a) * 0x9e3779b97f4a7c15u + static_cast<uint64_t>(k.b)) *
+                           0x9e3779b97f4a7c15u + static_cast<uint64_t>(k.c) * 31u + static_cast<uint64_t>(k.d);
+    Slot& s = slots_[(h >> 32) % kSlots];
+    if (!s.used || s.key.a != k.a || s.key.b != k.b || s.key.c != k.c || s.key.d != k.d)
+      s = {true, k, find()};
+    return s.plan;
+  }
+
+ private:
+  static constexpr int kSlots = 64;
+  struct Slot {
+    bool used = false;
+    Key key{};
+    Plan plan{};
+  } slots_[kSlots];
+};
 
 // The checks every entry point makes of a block operand.
 inline int check_mx(const char* fn, const void* codes, const void* scales, int32_t fmt,

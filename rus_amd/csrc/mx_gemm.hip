@@ -9,9 +9,6 @@
 // 4 (i / 8) + i % 4, so that a lane's 16 registers are 16 neighbouring features.
 // The instruction's sums are fp32; within the 16 products of an fp8 operand that it adds first it
 // keeps about 13 bits below the largest (fp4 by fp4 loses nothing), so results are 16-bit types.
-#include <type_traits>
-#include <utility>
-
 #include "mx.h"
 #include "swiglu_math.h"
 
@@ -235,16 +232,6 @@ __global__ __launch_bounds__(kRowsWaves* kWave) void mx_rows_kernel(MxArgs g) {
 constexpr int kTileThreads = 256;
 typedef u32x4s u32x4w __attribute__((aligned(4)));  // a 16-byte access at any word
 typedef __attribute__((address_space(3))) void* lds_void;
-
-// f(0), f(1), .. f(N - 1) as compile-time constants.
-template <typename F, int... I>
-__device__ __forceinline__ void each_of(F f, std::integer_sequence<int, I...>) {
-  (f(std::integral_constant<int, I>{}), ...);
-}
-template <int N, typename F>
-__device__ __forceinline__ void each(F f) {
-  each_of(f, std::make_integer_sequence<int, N>{});
-}
 
 template <int FMT, int GROUPS>
 constexpr int kStageRow = (FMT == kFp4 ? 64 : 128) * GROUPS;
@@ -759,7 +746,7 @@ struct GemmPlan {
   int bf, bt, splits;  // bt 32: the few-token kernel
 };
 
-GemmPlan gemm_plan(int64_t m, int64_t n, int64_t nb, int x_fmt, int w_fmt, bool glu) {
+GemmPlan find_gemm_plan(int64_t m, int64_t n, int64_t nb, int x_fmt, int w_fmt, bool glu) {
   const bool both4 = x_fmt == RUS_MX_FP4 && w_fmt == RUS_MX_FP4;
   const double few = (0.1 + 0.0027 * static_cast<double>(m < 32 ? m : 32)) * (glu ? 1.6 : 1.0);
   const struct {
@@ -788,6 +775,12 @@ GemmPlan gemm_plan(int64_t m, int64_t n, int64_t nb, int x_fmt, int w_fmt, bool 
     }
   }
   return best;
+}
+
+GemmPlan gemm_plan(int64_t m, int64_t n, int64_t nb, int x_fmt, int w_fmt, bool glu) {
+  static thread_local PlanMemo<GemmPlan> memo;
+  return memo.get({m, n, nb, x_fmt * 4 + w_fmt * 2 + glu},
+                  [&] { return find_gemm_plan(m, n, nb, x_fmt, w_fmt, glu); });
 }
 
 template <int EPI, typename T, int FX, int FW>

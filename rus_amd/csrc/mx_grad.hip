@@ -6,13 +6,13 @@
 // Eight waves form a tile of TM tokens x 256 columns, the contraction staged 64 at a time through two
 // LDS buffers. A stage's dy rows and W codes travel through registers one stage ahead: each of the 512
 // threads loads one block of W (32 codes, its scale), decodes it with 16 of gfx950's scaled
-// conversions and writes it transposed-readable; rows without alignment, and the contraction's end,
-// are filled element by element on the same way. W's rows lie along the contraction, so its fragments
-// leave LDS through the transposing ds_read_b64_tr_b16.
+// conversions and writes it transposed-readable; rows of any alignment, and the contraction's end, come
+// in on the same way. W's rows lie along the contraction, so its fragments leave LDS through the
+// transposing ds_read_b64_tr_b16. Reads, decoding, writes and loads go out between the products: bound by
+// the matrix pipe and its clock (2,048 x 17,920 x 1,536 bf16: 105 us and 11 for the sums, 1,073 TFLOP/s,
+// where a library product of 8192^3 reaches 1,197; in groups between bursts of products 113 us).
 // A tile count below the chip's 256 CUs splits the contraction; the splits' fp32 sums are added in
 // split order by a second launch.
-#include <type_traits>
-
 #include "mx.h"
 
 namespace rus {
@@ -101,7 +101,7 @@ mx_grad_kernel(GradArgs g) {
   const T* dy = static_cast<const T*>(g.dy);
   int64_t arow[AC > 0 ? AC : 1];
   uint32_t aat[AC > 0 ? AC : 1];
-  const bool has_a = AC > 0 || t < TM * 8;
+  const bool has_a = AC > 0 || t < TM * 8;  // (uniform over a wave)
 #pragma unroll
   for (int i = 0; i < (AC > 0 ? AC : 1); ++i) {
     const int row = (512 * i + t) >> 3;
@@ -116,19 +116,30 @@ mx_grad_kernel(GradArgs g) {
   const int spread = (bblk >> 2) | ((brow & 1) << 1);
   const uint32_t bat = brow * kWRow + (((4 * bblk) ^ ((brow & 3) << 2)) << 4);
 
-  u32x4s ra[AC > 0 ? AC : 1], rb[WV];
+  constexpr int AP = AC > 0 ? AC : 1;  // pieces of dy per thread (a tile of 32 rows: half the threads have one)
+  u32x4s ra[AP], rb[WV];
   uint32_t rs = 0;
-  const int ragged = g.n & 7;
+  // What a thread has of stage s: its pieces of dy (I < AP; columns past the end: `put`), its block of W.
+  auto load_piece = [&](int s, int i) {
+    const int n = s * kGradK + 8 * (t & 7);
+    ra[i] = *reinterpret_cast<const u32x4u*>(dy + arow[i] + (n + 8 <= g.n ? n : 0));
+  };
+  auto load_block = [&](int s) {
+    const int64_t at = static_cast<int64_t>(min(s * kGradK + brow, g.n - 1)) * g.nb + blk;
+    const u32x4s* src = reinterpret_cast<const u32x4s*>(g.wc + at * kCodeBytes<FMT>);
+#pragma unroll
+    for (int v = 0; v < WV; ++v) rb[v] = src[v];
+    rs = g.ws[at];
+  };
   auto load = [&](int s) {
-    const int n0 = s * kGradK, n = n0 + 8 * (t & 7);
     if (has_a) {
-      if (n0 + kGradK <= g.n || !ragged) {  // whole pieces, at any alignment (those past the end: `store`)
+      if ((s + 1) * kGradK <= g.n) {
 #pragma unroll
-        for (int i = 0; i < (AC > 0 ? AC : 1); ++i)
-          ra[i] = *reinterpret_cast<const u32x4u*>(dy + arow[i] + (n < g.n ? n : 0));
-      } else {
+        for (int i = 0; i < AP; ++i) load_piece(s, i);
+      } else {  // the contraction's end inside the stage: element by element
+        const int n = s * kGradK + 8 * (t & 7);
 #pragma unroll
-        for (int i = 0; i < (AC > 0 ? AC : 1); ++i) {
+        for (int i = 0; i < AP; ++i) {
           Pack<T, 8> p;
 #pragma unroll
           for (int j = 0; j < 8; ++j) p.v[j] = n + j < g.n ? dy[arow[i] + n + j] : static_cast<T>(0.0f);
@@ -136,25 +147,19 @@ mx_grad_kernel(GradArgs g) {
         }
       }
     }
-    const int64_t at = static_cast<int64_t>(min(n0 + brow, g.n - 1)) * g.nb + blk;
-    const u32x4s* src = reinterpret_cast<const u32x4s*>(g.wc + at * kCodeBytes<FMT>);
-#pragma unroll
-    for (int v = 0; v < WV; ++v) rb[v] = src[v];
-    rs = g.ws[at];
+    load_block(s);
   };
-  auto store = [&](int s, int buf) {  // stage s, in registers, to LDS; zeros past the contraction's end
+  // Piece I of stage s, in registers, to LDS: dy's, then the block's four chunks, decoded. WHOLE: the stage
+  // does not reach past the contraction's end (else zeros there, on both sides: no value of W matters).
+  auto put = [&](int s, int buf, auto I, auto WHOLE) {
+    constexpr int i = decltype(I)::value;
     char* base = smem + buf * (kABytes + kBBytes);
-    const bool a_in = s * kGradK + 8 * (t & 7) < g.n, b_in = s * kGradK + brow < g.n;
-    if (has_a) {
-#pragma unroll
-      for (int i = 0; i < (AC > 0 ? AC : 1); ++i)
-        *reinterpret_cast<u32x4s*>(base + aat[i]) = a_in ? ra[i] : u32x4s{0, 0, 0, 0};
-    }
-    const float scale = b_in ? mx_scale(rs) : 1.0f;
-#pragma unroll
-    for (int v = 0; v < WV; ++v) rb[v] = b_in ? rb[v] : u32x4s{0, 0, 0, 0};
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
+    if constexpr (i < AP) {
+      if (has_a) *reinterpret_cast<u32x4s*>(base + aat[i]) = ra[i];
+    } else {
+      constexpr int j = i - AP;
+      const bool in = decltype(WHOLE)::value || s * kGradK + brow < g.n;
+      const float scale = in ? mx_scale(rs) : 1.0f;
       const int q = j ^ spread;
       uint32_t lo, hi = 0;
       if constexpr (FMT == kFp4) {
@@ -164,9 +169,11 @@ mx_grad_kernel(GradArgs g) {
         lo = q & 1 ? w.z : w.x;
         hi = q & 1 ? w.w : w.y;
       }
+      if (!in) lo = hi = 0;
       *reinterpret_cast<u32x4s*>(base + kABytes + bat + q * 16) = decode8<T, FMT>(lo, hi, scale);
     }
   };
+  constexpr int kPieces = AP + 4;
 
   // Fragments. dy: row wm * (TM / WM) + 32 mt + l % 32, chunk 2 kk + l / 32. W: lane l (j = l % 16)
   // points at row 16 kk + 8 (l / 32) + j / 4 (+ 4 for the upper half), columns 16 ((l / 16) % 2) +
@@ -190,51 +197,96 @@ mx_grad_kernel(GradArgs g) {
   struct Frags {
     u32x4s a[MT], b[NT];
   };
-  auto read = [&](Frags& f, int buf, int kk) {
+  constexpr int kMma = MT * NT, kReads = MT + NT;
+  auto read_one = [&](Frags& f, int buf, int kk, auto R) {
+    constexpr int r = decltype(R)::value;
     const char* base = smem + buf * (kABytes + kBBytes);
-#pragma unroll
-    for (int mt = 0; mt < MT; ++mt)
-      f.a[mt] = *reinterpret_cast<const u32x4s*>(base + af + mt * 4096 + (((2 * kk + half) ^ asw) << 4));
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-      lds_ptr p = (lds_ptr)(base + kABytes) + bf[nt] + kk * 16 * kWRow;
+    if constexpr (r < MT) {
+      f.a[r] = *reinterpret_cast<const u32x4s*>(base + af + r * 4096 + (((2 * kk + half) ^ asw) << 4));
+    } else {
+      lds_ptr p = (lds_ptr)(base + kABytes) + bf[r - MT] + kk * 16 * kWRow;
       typedef __attribute__((address_space(3))) s16x4* vec_ptr;
       const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((vec_ptr)p);
       const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((vec_ptr)(p + 4 * kWRow));
       const u32x2s l2 = __builtin_bit_cast(u32x2s, lo), h2 = __builtin_bit_cast(u32x2s, hi);
-      f.b[nt] = u32x4s{l2.x, l2.y, h2.x, h2.y};
+      f.b[r - MT] = u32x4s{l2.x, l2.y, h2.x, h2.y};
     }
-    __builtin_amdgcn_sched_barrier(0);
   };
-  auto mma = [&](const Frags& f) {
-#pragma unroll
-    for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt) acc[mt][nt] = mma16<T>(f.a[mt], f.b[nt], acc[mt][nt]);
-    __builtin_amdgcn_sched_barrier(0);
+  // One step's products; after product j, then(j).
+  auto mma = [&](const Frags& f, auto then) {
+    each<kMma>([&](auto J) {
+      constexpr int m = decltype(J)::value / NT, n = decltype(J)::value % NT;
+      acc[m][n] = mma16<T>(f.a[m], f.b[n], acc[m][n]);
+      __builtin_amdgcn_sched_barrier(0);
+      then(J);
+      __builtin_amdgcn_sched_barrier(0);
+    });
+  };
+  // Part J of kMma of the reads of step kk.
+  auto read_part = [&](Frags& f, int buf, int kk, auto J) {
+    constexpr int per = (kReads + kMma - 1) / kMma;
+    each<per>([&](auto P) {
+      constexpr int r = decltype(J)::value * per + decltype(P)::value;
+      if constexpr (r < kReads) read_one(f, buf, kk, std::integral_constant<int, r>{});
+    });
   };
 
   load(s0);
-  store(s0, 0);
+  each<kPieces>([&](auto I) { put(s0, 0, I, std::false_type{}); });
   if (s0 + 1 < s1) load(s0 + 1);
   __syncthreads();
   Frags f0, f1;
-  read(f0, 0, 0);
-  for (int s = s0; s < s1; ++s) {
+  each<kReads>([&](auto R) { read_one(f0, 0, 0, R); });
+  // Everything but the products goes out between them: a step's fragments after the products of the step
+  // before, stage s + 1's pieces (into the buffer whose last reads the barrier of stage s - 1 ended) after
+  // those of the second and third step, stage s + 2's loads after the last's. The barrier falls before the
+  // last step, whose fragments are in registers by then. FAR: stages s + 1 and s + 2 are whole and there.
+  auto stage = [&](int s, auto FAR) {
+    constexpr bool far = decltype(FAR)::value;
     const int buf = (s - s0) & 1;
-    read(f1, buf, 1);
-    mma(f0);
-    read(f0, buf, 2);
-    // Stage s + 1 goes into the buffer whose last reads the barrier of stage s - 1 ended.
-    if (s + 1 < s1) store(s + 1, buf ^ 1);
-    if (s + 2 < s1) load(s + 2);
-    mma(f1);
-    read(f1, buf, 3);
-    mma(f0);
+    const bool more = far || s + 1 < s1;
+    constexpr int kPer = (kPieces + 2 * kMma - 1) / (2 * kMma);
+    auto pieces = [&](auto J, auto FROM) {
+      each<kPer>([&](auto P) {
+        constexpr int i = (decltype(FROM)::value + decltype(J)::value) * kPer + decltype(P)::value;
+        if constexpr (i < kPieces) put(s + 1, buf ^ 1, std::integral_constant<int, i>{}, FAR);
+      });
+    };
+    mma(f0, [&](auto J) { read_part(f1, buf, 1, J); });
+    if constexpr (far) {
+      mma(f1, [&](auto J) {
+        read_part(f0, buf, 2, J);
+        pieces(J, std::integral_constant<int, 0>{});
+      });
+      mma(f0, [&](auto J) {
+        read_part(f1, buf, 3, J);
+        pieces(J, std::integral_constant<int, kMma>{});
+      });
+    } else {
+      mma(f1, [&](auto J) { read_part(f0, buf, 2, J); });
+      if (more) each<kPieces>([&](auto I) { put(s + 1, buf ^ 1, I, std::false_type{}); });
+      mma(f0, [&](auto J) { read_part(f1, buf, 3, J); });
+      if (s + 2 < s1) load(s + 2);
+    }
     __syncthreads();
-    if (s + 1 < s1) read(f0, buf ^ 1, 0);
-    mma(f1);
-  }
+    mma(f1, [&](auto J) {
+      read_part(f0, buf ^ 1, 0, J);  // (past the last stage: what no product takes)
+      if constexpr (far) {
+        constexpr int j = decltype(J)::value, per = (AP + 1 + kMma - 1) / kMma;
+        each<per>([&](auto P) {
+          constexpr int i = j * per + decltype(P)::value;
+          if constexpr (i < AP) {
+            if (has_a) load_piece(s + 2, i);
+          } else if constexpr (i == AP) {
+            load_block(s + 2);
+          }
+        });
+      }
+    });
+  };
+  int s = s0;
+  for (; s + 2 < s1 && (s + 3) * kGradK <= g.n; ++s) stage(s, std::true_type{});
+  for (; s < s1; ++s) stage(s, std::false_type{});
 
   auto write = [&](auto put) {
 #pragma unroll
@@ -281,24 +333,27 @@ __global__ __launch_bounds__(256) void mx_grad_sum_kernel(const float* __restric
   store_from_f32<T, V>(dx + row * ld_dx + c, v);
 }
 
-// The tile height and the number of splits for a shape. A stage of a 256-token tile takes about 2 us on
-// a CU, of a lower tile in proportion to its tokens but at least 0.5 (the decode); a split's sums cost
-// 8 bytes per value written and read again.
+// The tile height and the number of splits for a shape, by what a launch is estimated to take: rounds of
+// 256 workgroups, each 3 us (5 of 256 tokens) and its stages (1.7, 1.05, 0.9 or 0.65 us of 256, 128, 64 or 32 tokens); a
+// split contraction pays for the second launch and 8 bytes a sum, which stay in the caches (10 TB/s).
+// Measured over 1 to 4,096 tokens: 4,096 x 17,920 x 1,536 in 256-token tiles and 5 splits 232 us (2: 238;
+// 128-token tiles unsplit 272, in 4 splits 307); 707 tokens 53; 256 tokens in 128-token tiles 29 (256:
+// 34, 64: 34); 16 tokens in 32-token tiles and 28 splits 14.5.
 struct GradPlan {
   int tm, splits;
 };
 
-GradPlan grad_plan(int64_t m, int64_t n, int64_t k) {
+GradPlan find_grad_plan(int64_t m, int64_t n, int64_t k) {
   const int64_t stages = (n + kGradK - 1) / kGradK, tk = (k + kGradN - 1) / kGradN;
   GradPlan best{256, 1};
   double least = 1e30;
   for (int tm : {256, 128, 64, 32}) {
     const int64_t tiles = (m + tm - 1) / tm * tk;
-    const double stage = tm == 256 ? 2.0 : tm == 128 ? 1.1 : tm == 64 ? 0.7 : 0.5;
+    const double stage = tm == 256 ? 1.7 : tm == 128 ? 1.05 : tm == 64 ? 0.9 : 0.65;
     for (int64_t s = 1; s <= 64 && s <= stages; ++s) {
       const double rounds = static_cast<double>((tiles * s + 255) / 256);
-      const double us = rounds * (static_cast<double>((stages + s - 1) / s) * stage + 3.0) +
-                        (s > 1 ? 4.0 + 8e-6 * static_cast<double>(s * m * k) / 4.0 : 0.0);
+      const double us = rounds * (static_cast<double>((stages + s - 1) / s) * stage + (tm == 256 ? 5.0 : 3.0)) +
+                        (s > 1 ? 4.0 + 8e-7 * static_cast<double>(s) * static_cast<double>(m * k) : 0.0);
       if (us < least) {
         least = us;
         best = {tm, static_cast<int>(s)};
@@ -306,6 +361,11 @@ GradPlan grad_plan(int64_t m, int64_t n, int64_t k) {
     }
   }
   return best;
+}
+
+GradPlan grad_plan(int64_t m, int64_t n, int64_t k) {
+  static thread_local PlanMemo<GradPlan> memo;
+  return memo.get({m, n, k, 0}, [&] { return find_grad_plan(m, n, k); });
 }
 
 }  // namespace
