@@ -210,15 +210,20 @@ __global__ __launch_bounds__(kRowsWaves* kWave) void mx_rows_kernel(MxArgs g) {
 
 // ---- tiles -----------------------------------------------------------------------------------------
 //
-// BF rows of W x BT tokens per workgroup of four waves (2 x 2 of BF/2 x BT/2), the contraction staged
+// BF rows of W x BT tokens per workgroup of four waves (2 x 2 of BF/2 x BT/2; eight, 2 x 4, for 256
+// tokens), the contraction staged
 // GROUPS x 128 at a time (a group of four blocks is two MFMA steps) through two LDS buffers that memory
 // is copied into directly (global_load_lds: 64 lanes' 16 bytes land one after the other), a stage ahead
-// of its products. Two workgroups share a CU: one's waits and epilogue run under the other's products.
+// of its products. Two workgroups of four waves share a CU: one's waits and epilogue run under the other's
+// products. One of eight has it to itself.
 //
 // What bounds it is the copies: a CU takes a line from its L2 in about 2.3 cycles whether it needs 128
 // bytes of it or 64 (55 or 28 bytes per cycle, measured with nothing else running). Where both operands
-// are fp4, a stage is therefore two groups, so that rows are whole lines; with an fp8 operand the
-// products take twice as long and a taller tile of one group covers the copies. They go out between the
+// are fp4, a stage is therefore two groups, so that rows are whole lines, and where there are tiles enough
+// a tile is 256 x 256, which copies half as much a product (8,161 x 17,920 x 1,536: 139 us, 3.2 PFLOP/s,
+// against 165 with 128 x 128; 8,161 x 8,960 x 8,960: 341 and 412); with an fp8 operand the products take
+// twice as long and a taller tile of one group covers the copies (8,161 x 17,920 x 1,536: 194 us with
+// 256 x 128, 195 with 256 x 256, 225 with 128 x 128). They go out between the
 // products, since a wave that issues them in a row waits for each.
 //
 // LDS rows of W are in MFMA order (row 32 q + i holds feature 32 q + feature_of(i)); with a gate, the
@@ -229,7 +234,9 @@ __global__ __launch_bounds__(kRowsWaves* kWave) void mx_rows_kernel(MxArgs g) {
 // banks once. Scales come four groups at a time, 16 bytes of a row in one request.
 // LDS is read by explicit instructions and waits: the compiler would wait for the copies in flight
 // before any LDS read. A register read this way is tied to the wait before its first use.
-constexpr int kTileThreads = 256;
+// Four waves, 2 x 2; eight, 2 x 4, for 256 tokens.
+template <int BT>
+constexpr int kTileThreads = BT == 256 ? 512 : 256;
 typedef u32x4s u32x4w __attribute__((aligned(4)));  // a 16-byte access at any word
 typedef __attribute__((address_space(3))) void* lds_void;
 
@@ -266,11 +273,11 @@ __device__ __forceinline__ void tie(u32x4s& v) { asm volatile("" : "+v"(v)); }
 __device__ __forceinline__ void tie(uint32_t& v) { asm volatile("" : "+v"(v)); }
 
 // The codes of ROWS rows of one operand on their way into LDS. Copy i of wave w fills bytes
-// 1024 (4 i + w) .. +1024 of the operand's stage.
-template <int FMT, int ROWS, int GROUPS, int PARTS>
+// 1024 (waves i + w) .. +1024 of the operand's stage.
+template <int FMT, int ROWS, int GROUPS, int PARTS, int THREADS>
 struct Copier {
   static constexpr int kRow = kStageRow<FMT, GROUPS>, kPer = kRow / 16;  // bytes and chunks per row
-  static constexpr int kCopies = ROWS * kPer / kTileThreads;             // copies per wave
+  static constexpr int kCopies = ROWS * kPer / THREADS;             // copies per wave
   static constexpr int kBytes = ROWS * kRow;
   static_assert(kCopies % PARTS == 0, "whole copies per part");
   // LDS row r holds the operand's row part(r * PARTS / ROWS) + in(r), in below 256: the gate's rows, then
@@ -284,7 +291,7 @@ struct Copier {
     for (int i = 0; i < PARTS; ++i) base[i] = codes + part(i) * bytes;
 #pragma unroll
     for (int i = 0; i < kCopies; ++i) {
-      const int q = i * kTileThreads + threadIdx.x, r = q / kPer;
+      const int q = i * THREADS + threadIdx.x, r = q / kPer;
       off[i] = static_cast<uint32_t>(in(r) * bytes + ((q % kPer) ^ swizzle<kRow>(r)) * 16);
     }
   }
@@ -293,11 +300,11 @@ struct Copier {
   __device__ __forceinline__ void copy(int s, bool last, char* stage, int wave) const {
     uint32_t o = off[I];
     if constexpr (GROUPS == 2) {
-      const int q = I * kTileThreads + threadIdx.x;
+      const int q = I * THREADS + threadIdx.x;
       if (last && ((q % kPer) ^ swizzle<kRow>(q / kPer)) >= kPer / 2) o -= kRow / 2;
     }
     const uint8_t* p = base[I * PARTS / kCopies] + static_cast<int64_t>(s) * kRow;
-    __builtin_amdgcn_global_load_lds(p + o, (lds_void)(stage + (4 * I + wave) * 1024), 16, 0, 0);
+    __builtin_amdgcn_global_load_lds(p + o, (lds_void)(stage + (THREADS / kWave * I + wave) * 1024), 16, 0, 0);
   }
 };
 
@@ -464,11 +471,12 @@ __device__ __forceinline__ void write_tile(const MxArgs& g, int fw, int tw0, cha
 
 template <int FX, int FW, int EPI, typename T, int BF, int BT, int GROUPS>
 __device__ __forceinline__ void mx_tile(const MxArgs& g, const TilePlace& tp, char* smem) {
-  constexpr int FT = BF / 64, TT = BT / 64;        // 32 x 32 results of a wave
+  constexpr int THREADS = kTileThreads<BT>, WT = THREADS / kWave / 2;  // waves along the tokens
+  constexpr int FT = BF / 64, TT = BT / 32 / WT;   // 32 x 32 results of a wave
   constexpr int NF = BF / outs_of(EPI);            // output features of a tile
   constexpr int PARTS = outs_of(EPI), kWaveRows = BF / 2 / PARTS;  // rows of W per wave and part
-  typedef Copier<FW, BF, GROUPS, PARTS> CW;
-  typedef Copier<FX, BT, GROUPS, 1> CX;
+  typedef Copier<FW, BF, GROUPS, PARTS, THREADS> CW;
+  typedef Copier<FX, BT, GROUPS, 1, THREADS> CX;
   typedef StepFrags<FW, FT, GROUPS, PARTS == 1 ? 0 : BF / 2> WF;
   typedef StepFrags<FX, TT, GROUPS, 0> XF;
   constexpr int kStage = CW::kBytes + CX::kBytes, kScales = (BF + BT) * 16;
@@ -476,7 +484,7 @@ __device__ __forceinline__ void mx_tile(const MxArgs& g, const TilePlace& tp, ch
   const int f0 = tp.f0, t0 = tp.t0;
   const int lane = threadIdx.x & 63, half = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int wf = wave >> 1, wt = wave & 1;
+  const int wf = wave / WT, wt = wave % WT;
   const bool edge = t0 + BT > g.m || f0 + NF > g.n;
 
   // rows past the edge re-read the last one; what they give is not stored
@@ -508,8 +516,8 @@ __device__ __forceinline__ void mx_tile(const MxArgs& g, const TilePlace& tp, ch
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       uint32_t* word = p + ((start + j) & 3) * (BF + BT);
-      if (BF >= kTileThreads || sr < BF) word[sr] = sw.v[j];
-      if (BT >= kTileThreads || sr < BT) word[BF + sr] = sx.v[j];
+      if (BF >= THREADS || sr < BF) word[sr] = sw.v[j];
+      if (BT >= THREADS || sr < BT) word[BF + sr] = sx.v[j];
     }
   };
   constexpr int kCopies = CW::kCopies + CX::kCopies;
@@ -522,7 +530,7 @@ __device__ __forceinline__ void mx_tile(const MxArgs& g, const TilePlace& tp, ch
     else if constexpr (i < kCopies)
       cx.template copy<i - CW::kCopies>(s, last, st + CW::kBytes, wave);
   };
-  const int wr = wf * kWaveRows + (lane & 31), xr = wt * (BT / 2) + (lane & 31);
+  const int wr = wf * kWaveRows + (lane & 31), xr = wt * (BT / WT) + (lane & 31);
   const uint32_t wat = lds_addr(smem) + wr * CW::kRow, xat = lds_addr(smem) + CW::kBytes + xr * CX::kRow;
   const int wsw = swizzle<CW::kRow>(wr), xsw = swizzle<CX::kRow>(xr);
   const uint32_t wsat = lds_addr(scales) + wr * 4 + 2 * half, xsat = lds_addr(scales) + (BF + xr) * 4 + 2 * half;
@@ -690,18 +698,18 @@ __device__ __forceinline__ void mx_tile(const MxArgs& g, const TilePlace& tp, ch
   __syncthreads();  // every wave has read the last stage: results go over it
 
   constexpr int kCols = NF / 2, kMine = (EPI == kGluBwd ? 2 : 1) * 32 * (kCols * 2 + 16);
-  static_assert(EPI == kParts || 4 * kMine <= 2 * kStage + 2 * kScales, "the results fit");
+  static_assert(EPI == kParts || THREADS / kWave * kMine <= 2 * kStage + 2 * kScales, "the results fit");
   if (edge)
-    write_tile<EPI, T, kCols, true>(g, f0 + wf * kCols, t0 + wt * (BT / 2), smem + wave * kMine, lane, acc);
+    write_tile<EPI, T, kCols, true>(g, f0 + wf * kCols, t0 + wt * (BT / WT), smem + wave * kMine, lane, acc);
   else
-    write_tile<EPI, T, kCols, false>(g, f0 + wf * kCols, t0 + wt * (BT / 2), smem + wave * kMine, lane, acc);
+    write_tile<EPI, T, kCols, false>(g, f0 + wf * kCols, t0 + wt * (BT / WT), smem + wave * kMine, lane, acc);
 }
 
 template <int FX, int FW, int EPI, typename T, int BF, int BT, int GROUPS>
-__global__ __launch_bounds__(kTileThreads) __attribute__((amdgpu_waves_per_eu(2))) void
+__global__ __launch_bounds__(kTileThreads<BT>) __attribute__((amdgpu_waves_per_eu(2))) void
 mx_tile_kernel(MxArgs g, int tiles_f, int tiles_t) {
   constexpr int kBytes =
-      2 * (Copier<FW, BF, GROUPS, 1>::kBytes + Copier<FX, BT, GROUPS, 1>::kBytes + (BF + BT) * 16);
+      2 * (BF * kStageRow<FW, GROUPS> + BT * kStageRow<FX, GROUPS> + (BF + BT) * 16);
   __shared__ __attribute__((aligned(16))) char smem[kBytes];
   TilePlace tp;
   if (!tile_place(tiles_f, tiles_t, BF / outs_of(EPI), BT, tp)) return;
@@ -736,12 +744,13 @@ __global__ __launch_bounds__(256) void mx_sum_kernel(const float* __restrict__ p
 // ---- which kernel --------------------------------------------------------------------------------
 //
 // The one whose launch is estimated shortest. A launch takes a + groups (b + r (rounds - 1)) us, groups of
-// four blocks of the contraction per workgroup, rounds of 256 workgroups; a contraction cut into parts
+// four blocks of the contraction per workgroup, rounds of 256 workgroups (and c a round); a contraction cut into parts
 // pays for a second launch and 8 bytes a value and part. Measured at 12 and 70 groups (k = 1536, 8960),
 // 1 to 8,161 tokens, 1,536 to 17,920 features: one round of 256 x 128 tiles 10.5 / 42 us, of 128 x 128
 // 7.4 / 28.5, of 128 x 64 6.4 / 25, of the few-token kernel 3.7 / 9.3 (one token) and 4.7 / 15.3 (32).
 // 707 tokens x 17,920: 22.9, 25.4, 28.4 and (few-token) 121; 192 tokens 12.5, 12.1, 9.9; 2,048 features at
-// 33 tokens 10.3, 7.1, 6.4 and 4.6. With both operands fp4 the taller tile has nothing to gain.
+// 33 tokens 10.3, 7.1, 6.4 and 4.6. With both operands fp4, 256 x 256 takes the taller tile's place: one
+// round 12 to 17 / 43 to 61 us, a further one 16 / 64, against 128 x 128's 6.5 / 21 to 33 and 4.8 / 28.
 struct GemmPlan {
   int bf, bt, splits;  // bt 32: the few-token kernel
 };
@@ -751,22 +760,23 @@ GemmPlan find_gemm_plan(int64_t m, int64_t n, int64_t nb, int x_fmt, int w_fmt, 
   const double few = (0.1 + 0.0027 * static_cast<double>(m < 32 ? m : 32)) * (glu ? 1.6 : 1.0);
   const struct {
     int bf, bt;
-    double a, b, r;
-  } kinds[] = {{32, 32, 2.5, few, few},
-               {128, 64, both4 ? 2.75 : 2.5, both4 ? 0.25 : 0.32, both4 ? 0.35 : 0.375},
-               {128, 128, 3.0, both4 ? 0.25 : 0.364, both4 ? 0.35 : 0.6},
-               {256, 128, 4.0, 0.54, 0.875}};
+    double a, b, r, c;
+  } kinds[] = {{32, 32, 2.5, few, few, 0.0},
+               {128, 64, both4 ? 2.75 : 2.5, both4 ? 0.25 : 0.32, both4 ? 0.35 : 0.375, 0.0},
+               {128, 128, 3.0, both4 ? 0.25 : 0.364, both4 ? 0.4 : 0.6, 0.0},
+               {256, 128, 4.0, 0.54, 0.875, 0.0},
+               {256, 256, 4.0, 0.75, 0.83, 6.0}};
   const int64_t groups = nb / 4;
   GemmPlan best{32, 32, 1};
   double least = 1e300;
   for (const auto& k : kinds) {
-    if (k.bf == 256 && (x_fmt != RUS_MX_FP8 || w_fmt != RUS_MX_FP4)) continue;
+    if (k.bf == 256 && (k.bt == 256 ? !both4 : x_fmt != RUS_MX_FP8 || w_fmt != RUS_MX_FP4)) continue;
     if (k.bt == 32 && m > 256) continue;
     const int64_t nf = k.bt == 32 || !glu ? k.bf : k.bf / 2;
     const int64_t tiles = ((n + nf - 1) / nf) * ((m + k.bt - 1) / k.bt);
     for (int64_t s = 1; s <= (glu ? 1 : 32) && 2 * s <= groups + 1; ++s) {
       const double rounds = static_cast<double>((tiles * s + 255) / 256 - 1);
-      const double us = k.a + static_cast<double>((groups + s - 1) / s) * (k.b + k.r * rounds) +
+      const double us = k.a + static_cast<double>((groups + s - 1) / s) * (k.b + k.r * rounds) + k.c * rounds +
                         (s > 1 ? 3.0 + 2e-6 * static_cast<double>(s) * static_cast<double>(m * n) : 0.0);
       if (us < least) {
         least = us;
@@ -792,7 +802,7 @@ void launch(const MxArgs& g, const GemmPlan& plan, hipStream_t st) {
     const int tiles_f = (g.n + nf - 1) / nf, tiles_t = (g.m + bt - 1) / bt;
     const int64_t total = static_cast<int64_t>(tiles_f) * tiles_t;
     hipLaunchKernelGGL(kern, dim3(static_cast<unsigned>(8 * ((total + 7) / 8)), 1, parts),
-                       dim3(kTileThreads), 0, st, g, tiles_f, tiles_t);
+                       dim3(bt == 256 ? 512 : 256), 0, st, g, tiles_f, tiles_t);
   };
   if (plan.bt == 32)
     hipLaunchKernelGGL((mx_rows_kernel<FX, FW, EPI, T>), dim3((g.n + 31) / 32, (g.m + 31) / 32, parts),
@@ -801,6 +811,8 @@ void launch(const MxArgs& g, const GemmPlan& plan, hipStream_t st) {
     tile(mx_tile_kernel<FX, FW, EPI, T, 128, 64, G>, 128, 64);
   else if (plan.bf == 128)
     tile(mx_tile_kernel<FX, FW, EPI, T, 128, 128, G>, 128, 128);
+  else if constexpr (FX == kFp4 && FW == kFp4)
+    tile(mx_tile_kernel<FX, FW, EPI, T, 256, 256, G>, 256, 256);
   else if constexpr (FX == kFp8 && FW == kFp4)
     tile(mx_tile_kernel<FX, FW, EPI, T, 256, 128, G>, 256, 128);
 }
