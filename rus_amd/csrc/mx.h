@@ -21,6 +21,21 @@ namespace rus {
 int quantize_rows(const char* fn, const void* x, int32_t dtype, int64_t n_rows, int64_t n_cols,
                   int64_t stride_row, int32_t fmt, void* codes, void* scales, hipStream_t stream);
 
+// The products' kernel for a few tokens, x in blocks (xc, xs) or rounded to them (x, rows of the result's
+// type). few_tokens: whether it takes these sizes; nothing else is checked here.
+struct TokenArgs {
+  const void* x;
+  int64_t ldx;
+  const uint8_t *xc, *xs, *wc, *ws;
+  int x_fmt, m, n, k, nb;
+  const void* bias;
+  void* y;
+  int64_t ldy;
+};
+enum { kTokenPlain = 0, kTokenGlu = 1 };
+bool few_tokens(int64_t m, int64_t n, int64_t nb);
+int token_product(const char* fn, const TokenArgs& g, int w_fmt, bool glu, bool bf, hipStream_t st);
+
 namespace {
 
 constexpr int kFp4 = RUS_MX_FP4, kFp8 = RUS_MX_FP8;
@@ -57,6 +72,12 @@ __device__ __forceinline__ uint32_t scale_byte(uint32_t top) {
 // 2^(127 - b) for a finite block (b <= 252).
 __device__ __forceinline__ float inv_scale(uint32_t b) {
   return __builtin_bit_cast(float, (254u - b) << 23);
+}
+
+// The largest of the four lanes that share a block.
+__device__ __forceinline__ uint32_t quad_max(uint32_t m) {
+  m = max(m, static_cast<uint32_t>(__shfl_xor(static_cast<int>(m), 1, kWave)));
+  return max(m, static_cast<uint32_t>(__shfl_xor(static_cast<int>(m), 2, kWave)));
 }
 
 // N (a multiple of 4 / 8) scaled elements to codes, in order; `nan`: the block is not finite.

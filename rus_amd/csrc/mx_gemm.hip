@@ -864,7 +864,7 @@ int product(const char* fn, MxArgs g, const GemmPlan& plan, int32_t x_fmt, int32
 // Checks shared by the three entry points; fills what they share.
 int prepare(const char* fn, MxArgs& g, const void* xc, const void* xs, int32_t x_fmt, const void* wc,
             const void* ws, int32_t w_fmt, int64_t m, int64_t n, int64_t k, void* y,
-            int64_t ldy, int64_t y_cols, int32_t dtype) {
+            int64_t ldy, int64_t y_cols, int32_t dtype, bool raw = false) {
   if (m < 0 || n <= 0 || k <= 0 || m >= (1 << 30) || n >= (1 << 28) || k > (1 << 22))
     return fail(RUS_ERR_INVALID, "%s: bad sizes m=%lld n=%lld k=%lld", fn, (long long)m,
                 (long long)n, (long long)k);
@@ -874,7 +874,8 @@ int prepare(const char* fn, MxArgs& g, const void* xc, const void* xs, int32_t x
     return fail(RUS_ERR_INVALID, "%s: output row stride %lld smaller than %lld columns", fn,
                 (long long)ldy, (long long)y_cols);
   if (m == 0) return RUS_OK;
-  if (int e = check_mx(fn, xc, xs, x_fmt, "x")) return e;
+  if (!raw)
+    if (int e = check_mx(fn, xc, xs, x_fmt, "x")) return e;
   if (int e = check_mx(fn, wc, ws, w_fmt, "w")) return e;
   if (!y || !aligned(y, 2)) return fail(RUS_ERR_INVALID, "%s: output is null or misaligned", fn);
   if (((m + 63) / 64) * ((n + 63) / 64) >= (int64_t(1) << 28))
@@ -907,7 +908,7 @@ extern "C" int rus_mx_gemm_workspace(int64_t m, int64_t n, int64_t k, int32_t x_
     return fail(RUS_ERR_INVALID, "%s: bad sizes m=%lld n=%lld k=%lld", fn, (long long)m, (long long)n,
                 (long long)k);
   const GemmPlan p = gemm_plan(m, n, mx_blocks(k), x_fmt, w_fmt, false);
-  *floats = m > 0 && p.splits > 1 ? p.splits * m * n : 0;
+  *floats = m > 0 && !few_tokens(m, n, mx_blocks(k)) && p.splits > 1 ? p.splits * m * n : 0;
   return RUS_OK;
 }
 
@@ -920,6 +921,7 @@ struct RowsScratch {
 };
 RowsScratch rows_scratch(int64_t m, int64_t n, int64_t k, int32_t act, int32_t w_fmt, bool glu) {
   const int64_t nb = mx_blocks(k);
+  if (few_tokens(m, n, nb)) return {0, 0, 0};
   const GemmPlan p = gemm_plan(m, n, nb, act, w_fmt, glu);
   return {m * nb * (act == RUS_MX_FP4 ? 16 : 32), (m * nb + 15) / 16 * 16, p.splits > 1 ? p.splits * m * n : 0};
 }
@@ -941,6 +943,10 @@ int place(const char* fn, const RowsScratch& need, void* scratch, int64_t n_scra
   return RUS_OK;
 }
 
+TokenArgs token_args(const MxArgs& g, int x_fmt, int64_t k, const void* bias) {
+  return {nullptr, 0, g.xc, g.xs, g.wc, g.ws, x_fmt, g.m, g.n, static_cast<int>(k), g.nb, bias, g.y, g.ldy};
+}
+
 // rus_mx_gemm and rus_mx_glu_fwd; `first` runs once nothing is left to refuse.
 template <typename F>
 int run_gemm(const char* fn, const void* xc, const void* xs, int32_t x_fmt, const void* wc, const void* ws,
@@ -950,6 +956,9 @@ int run_gemm(const char* fn, const void* xc, const void* xs, int32_t x_fmt, cons
   if (int e = prepare(fn, g, xc, xs, x_fmt, wc, ws, w_fmt, m, n, k, y, ldy, n, dtype)) return e;
   if (m == 0) return RUS_OK;
   if (bias && !aligned(bias, 2)) return fail(RUS_ERR_INVALID, "%s: misaligned bias", fn);
+  const hipStream_t st = static_cast<hipStream_t>(stream);
+  if (few_tokens(m, n, g.nb))
+    return token_product(fn, token_args(g, x_fmt, k, bias), w_fmt, false, dtype == RUS_DTYPE_BF16, st);
   const GemmPlan plan = gemm_plan(m, n, g.nb, x_fmt, w_fmt, false);
   if (plan.splits > 1 && (n_workspace < plan.splits * m * n || !workspace || !aligned(workspace, 16)))
     return fail(RUS_ERR_INVALID, "%s: workspace holds %lld floats (16-byte aligned), needs %lld", fn,
@@ -957,7 +966,6 @@ int run_gemm(const char* fn, const void* xc, const void* xs, int32_t x_fmt, cons
   g.bias = bias;
   g.vec = g.vec && (!bias || aligned(bias, 16));
   if (int e = first()) return e;
-  const hipStream_t st = static_cast<hipStream_t>(stream);
   return dtype == RUS_DTYPE_BF16 ? product<bf16>(fn, g, plan, x_fmt, w_fmt, workspace, st)
                                  : product<f16>(fn, g, plan, x_fmt, w_fmt, workspace, st);
 }
@@ -969,8 +977,28 @@ int run_glu(const char* fn, const void* xc, const void* xs, int32_t x_fmt, const
   MxArgs g;
   if (int e = prepare(fn, g, xc, xs, x_fmt, wc, ws, w_fmt, m, n, k, h, ldh, n, dtype)) return e;
   if (m == 0) return RUS_OK;
+  const hipStream_t st = static_cast<hipStream_t>(stream);
+  if (few_tokens(m, n, g.nb))
+    return token_product(fn, token_args(g, x_fmt, k, nullptr), w_fmt, true, dtype == RUS_DTYPE_BF16, st);
   if (int e = first()) return e;
-  return dispatch<kGluFwd>(fn, g, x_fmt, w_fmt, dtype, static_cast<hipStream_t>(stream));
+  return dispatch<kGluFwd>(fn, g, x_fmt, w_fmt, dtype, st);
+}
+
+// A few tokens that are rounded to blocks inside the product.
+int run_tokens(const char* fn, const void* x, int64_t ldx, int32_t act, const void* wc, const void* ws,
+               int32_t w_fmt, int64_t m, int64_t n, int64_t k, const void* bias, void* y, int64_t ldy,
+               int32_t dtype, bool glu, void* stream) {
+  MxArgs g;
+  if (int e = prepare(fn, g, nullptr, nullptr, act, wc, ws, w_fmt, m, n, k, y, ldy, n, dtype, true)) return e;
+  if (act != RUS_MX_FP4 && act != RUS_MX_FP8)
+    return fail(RUS_ERR_INVALID, "%s: unknown activation format %d", fn, (int)act);
+  if (ldx < k && m > 1) return fail(RUS_ERR_INVALID, "%s: stride_x=%lld smaller than a row", fn, (long long)ldx);
+  if (!x || !aligned(x, 2)) return fail(RUS_ERR_INVALID, "%s: x is null or misaligned", fn);
+  if (bias && !aligned(bias, 2)) return fail(RUS_ERR_INVALID, "%s: misaligned bias", fn);
+  TokenArgs t = token_args(g, act, k, bias);
+  t.x = x;
+  t.ldx = ldx;
+  return token_product(fn, t, w_fmt, glu, dtype == RUS_DTYPE_BF16, static_cast<hipStream_t>(stream));
 }
 
 }  // namespace
@@ -1000,6 +1028,8 @@ extern "C" int rus_mx_gemm_rows(const void* x, int64_t stride_x, int32_t act, co
   const char* fn = "rus_mx_gemm_rows";
   if (int e = check_sizes(fn, m, n, k)) return e;
   if (m == 0) return RUS_OK;
+  if (few_tokens(m, n, mx_blocks(k)))
+    return run_tokens(fn, x, stride_x, act, w_codes, w_scales, w_fmt, m, n, k, bias, y, stride_y, dtype, false, stream);
   const RowsScratch need = rows_scratch(m, n, k, act, w_fmt, false);
   char *codes, *scales;
   float* sums;
@@ -1018,6 +1048,8 @@ extern "C" int rus_mx_glu_fwd_rows(const void* x, int64_t stride_x, int32_t act,
   const char* fn = "rus_mx_glu_fwd_rows";
   if (int e = check_sizes(fn, m, n, k)) return e;
   if (m == 0) return RUS_OK;
+  if (few_tokens(m, n, mx_blocks(k)))
+    return run_tokens(fn, x, stride_x, act, w_codes, w_scales, w_fmt, m, n, k, nullptr, h, stride_h, dtype, true, stream);
   char *codes, *scales;
   float* sums;
   if (int e = place(fn, rows_scratch(m, n, k, act, w_fmt, true), scratch, n_scratch, codes, scales, sums))

@@ -41,12 +41,6 @@ __device__ __forceinline__ void store8(T* __restrict__ row, int c, int cols, con
   }
 }
 
-// The largest of the four lanes that share a block.
-__device__ __forceinline__ uint32_t quad_max(uint32_t m) {
-  m = max(m, static_cast<uint32_t>(__shfl_xor(static_cast<int>(m), 1, kWave)));
-  return max(m, static_cast<uint32_t>(__shfl_xor(static_cast<int>(m), 2, kWave)));
-}
-
 // A thread's eight scaled elements leave as one 4- or 8-byte store.
 template <int FMT>
 __device__ __forceinline__ void store_codes(uint8_t* p, const float (&v)[8], bool nan) {

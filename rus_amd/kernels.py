@@ -2597,10 +2597,10 @@ def mx_gemm(x, w: MXTensor, trans: bool = False, bias: torch.Tensor | None = Non
         if n == 0:
             return out
         need = _mx_scratch("rus_mx_rows_scratch", m, n, k, xf, wf, 0)
-        scratch = torch.empty(need, dtype=torch.uint8, device=x.device)
+        scratch = torch.empty(need, dtype=torch.uint8, device=x.device) if need else None
         _mx_launch("mx_gemm", lambda: (2 * m * (n + k) + _mx_bytes(w), 2 * m * n * k), x, "rus_mx_gemm_rows",
                    x.data_ptr(), _ld(x), xf, w.codes.data_ptr(), w.scales.data_ptr(), wf, m, n, k, _ptr(bias),
-                   out.data_ptr(), _ld(out), dt, scratch.data_ptr(), need)
+                   out.data_ptr(), _ld(out), dt, _ptr(scratch), need)
         return out
     x = _mx_operand(fn, x, act, k)
     m = x.shape[0]
@@ -2642,10 +2642,10 @@ def mx_mlp_glu_fwd(x, w: MXTensor, act: str = "fp8", out: torch.Tensor | None = 
         m = x.shape[0]
         out = _mx_out(fn, out, m, n, dtype, x)
         need = _mx_scratch("rus_mx_rows_scratch", m, n, k, xf, wf, 1)
-        scratch = torch.empty(need, dtype=torch.uint8, device=x.device)
+        scratch = torch.empty(need, dtype=torch.uint8, device=x.device) if need else None
         _mx_launch("mx_glu_fwd", lambda: (2 * m * (n + k) + _mx_bytes(w), 4 * m * n * k), x,
                    "rus_mx_glu_fwd_rows", x.data_ptr(), _ld(x), xf, w.codes.data_ptr(), w.scales.data_ptr(),
-                   wf, m, n, k, out.data_ptr(), _ld(out), dt, scratch.data_ptr(), need)
+                   wf, m, n, k, out.data_ptr(), _ld(out), dt, _ptr(scratch), need)
         return out
     x = _mx_operand(fn, x, act, k)
     m = x.shape[0]
