@@ -137,6 +137,37 @@ __device__ __forceinline__ void each(F f) {
   each_of(f, std::make_integer_sequence<int, N>{});
 }
 
+// The sum of `parts` groups of V floats, `step` apart, added in order. DEEP: sixteen loads at a time, for
+// few sums of many parts, which take a few rounds of the latency from other XCDs' caches (28 parts of
+// 16 x 1,536: 5.4 us by eights, 3.7 by sixteens); many sums are better served by more waves with fewer
+// registers (5 parts of 4,096 x 1,536: 22 us, by sixteens 27).
+template <bool DEEP, int V>
+__device__ __forceinline__ void sum_parts(const float* __restrict__ p, int64_t step, int parts, float (&v)[V]) {
+  load_f32<float, V>(p, v);
+  if constexpr (DEEP) {
+    constexpr int N = 16;
+    for (int s = 1; s < parts; s += N) {
+      float u[N][V];
+#pragma unroll
+      for (int i = 0; i < N; ++i) load_f32<float, V>(p + min(s + i, parts - 1) * step, u[i]);
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+#pragma unroll
+        for (int j = 0; j < V; ++j) v[j] = s + i < parts ? v[j] + u[i][j] : v[j];
+    }
+  } else {
+#pragma unroll 8
+    for (int s = 1; s < parts; ++s) {
+      float u[V];
+      load_f32<float, V>(p + s * step, u);
+#pragma unroll
+      for (int j = 0; j < V; ++j) v[j] += u[j];
+    }
+  }
+}
+// Whether a sum of that many threads is of the first kind.
+inline bool deep_sum(int64_t threads, int64_t parts) { return threads <= 32768 && parts > 8; }
+
 // A thread's last plans by the sizes they are for: finding one goes over all choices, a few us.
 template <typename Plan>
 class PlanMemo {

@@ -717,7 +717,7 @@ mx_tile_kernel(MxArgs g, int tiles_f, int tiles_t) {
 }
 
 // y = T(the parts' sums, added in order, + bias), V features per thread.
-template <typename T, int V>
+template <typename T, int V, bool DEEP>
 __global__ __launch_bounds__(256) void mx_sum_kernel(const float* __restrict__ parts, int splits,
                                                      int64_t m, int packs, int n,
                                                      const T* __restrict__ bias, T* __restrict__ y,
@@ -728,14 +728,7 @@ __global__ __launch_bounds__(256) void mx_sum_kernel(const float* __restrict__ p
   const int f = static_cast<int>(i - row * packs) * V;
   const float* p = parts + row * n + f;
   float v[V];
-  load_f32<float, V>(p, v);
-#pragma unroll 8
-  for (int s = 1; s < splits; ++s) {
-    float u[V];
-    load_f32<float, V>(p + s * m * n, u);
-#pragma unroll
-    for (int j = 0; j < V; ++j) v[j] += u[j];
-  }
+  sum_parts<DEEP, V>(p, m * n, splits, v);
 #pragma unroll
   for (int j = 0; j < V; ++j) v[j] += bias ? static_cast<float>(bias[f + j]) : 0.0f;
   store_from_f32<T, V>(y + row * ldy + f, v);
@@ -852,12 +845,14 @@ int product(const char* fn, MxArgs g, const GemmPlan& plan, int32_t x_fmt, int32
   g.y = parts;
   by_format<kParts, f16>(g, plan, x_fmt, w_fmt, st);
   const dim3 grid(static_cast<unsigned>((static_cast<int64_t>(g.m) * packs + 255) / 256));
-  if (wide)
-    hipLaunchKernelGGL((mx_sum_kernel<T, 4>), grid, dim3(256), 0, st, parts, plan.splits,
-                       static_cast<int64_t>(g.m), packs, g.n, bias, y, g.ldy);
+  auto add = [&](auto k) {
+    hipLaunchKernelGGL(k, grid, dim3(256), 0, st, parts, plan.splits, static_cast<int64_t>(g.m), packs, g.n, bias, y,
+                       g.ldy);
+  };
+  if (deep_sum(static_cast<int64_t>(g.m) * packs, plan.splits))
+    wide ? add(mx_sum_kernel<T, 4, true>) : add(mx_sum_kernel<T, 1, true>);
   else
-    hipLaunchKernelGGL((mx_sum_kernel<T, 1>), grid, dim3(256), 0, st, parts, plan.splits,
-                       static_cast<int64_t>(g.m), packs, g.n, bias, y, g.ldy);
+    wide ? add(mx_sum_kernel<T, 4, false>) : add(mx_sum_kernel<T, 1, false>);
   return check_launch(fn);
 }
 

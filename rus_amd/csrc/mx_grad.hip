@@ -312,7 +312,7 @@ mx_grad_kernel(GradArgs g) {
 }
 
 // dx = T(the splits' sums, added in order), V columns per thread.
-template <typename T, int V>
+template <typename T, int V, bool DEEP>
 __global__ __launch_bounds__(256) void mx_grad_sum_kernel(const float* __restrict__ parts, int splits,
                                                           int64_t m, int packs, int k,
                                                           T* __restrict__ dx, int64_t ld_dx) {
@@ -322,14 +322,7 @@ __global__ __launch_bounds__(256) void mx_grad_sum_kernel(const float* __restric
   const int c = static_cast<int>(i - row * packs) * V;
   const float* p = parts + row * k + c;
   float v[V];
-  load_f32<float, V>(p, v);
-#pragma unroll 8
-  for (int s = 1; s < splits; ++s) {
-    float u[V];
-    load_f32<float, V>(p + s * m * k, u);
-#pragma unroll
-    for (int j = 0; j < V; ++j) v[j] += u[j];
-  }
+  sum_parts<DEEP, V>(p, m * k, splits, v);
   store_from_f32<T, V>(dx + row * ld_dx + c, v);
 }
 
@@ -452,12 +445,14 @@ extern "C" int rus_mx_gemm_t(const void* dy, int64_t stride_dy, int32_t dtype, c
     const bool wide = k % 4 == 0 && stride_dx % 4 == 0 && aligned(dx, 8);
     const int packs = static_cast<int>(wide ? k / 4 : k);
     const dim3 sum(static_cast<unsigned>((m * packs + 255) / 256));
-    if (wide)
-      hipLaunchKernelGGL((mx_grad_sum_kernel<T, 4>), sum, dim3(256), 0, st, workspace, plan.splits, m,
-                         packs, g.k, static_cast<T*>(dx), stride_dx);
+    auto add = [&](auto k) {
+      hipLaunchKernelGGL(k, sum, dim3(256), 0, st, workspace, plan.splits, m, packs, g.k, static_cast<T*>(dx),
+                         stride_dx);
+    };
+    if (deep_sum(m * packs, plan.splits))
+      wide ? add(mx_grad_sum_kernel<T, 4, true>) : add(mx_grad_sum_kernel<T, 1, true>);
     else
-      hipLaunchKernelGGL((mx_grad_sum_kernel<T, 1>), sum, dim3(256), 0, st, workspace, plan.splits, m,
-                         packs, g.k, static_cast<T*>(dx), stride_dx);
+      wide ? add(mx_grad_sum_kernel<T, 4, false>) : add(mx_grad_sum_kernel<T, 1, false>);
   };
   if (dtype == RUS_DTYPE_F16)
     types(f16{});
