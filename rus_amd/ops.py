@@ -123,6 +123,26 @@ def _no_weight_grad(fn: str, **tensors) -> None:
             raise RuntimeError(f"{fn}: {name} is frozen here: no gradient is formed for it")
 
 
+def _note_stream(fn: str, leaf: torch.Tensor, stream: int, capturing: bool):
+    """Notes on ``leaf``'s gradient accumulator, which it returns, the first stream it is seen on. An
+    accumulator lives as long as some graph over the leaf does, and keeps to the stream it was made on; a
+    captured backward would wait for that stream, and ending the capture then ends the process: refused."""
+    node = torch.autograd.graph.get_gradient_edge(leaf).node
+    if node.metadata.setdefault("rus_stream", stream) != stream and capturing:
+        raise RuntimeError(f"{fn}: a graph recorded on another stream still holds this input, which requires "
+                           "gradients: drop that graph's outputs before capturing")
+    return node
+
+
+def _leaf_streams(fn: str, *tensors):
+    """``_note_stream`` of each leaf that is to have a gradient. Keep the result until the new graph
+    holds the accumulators itself."""
+    return [_note_stream(fn, t, torch.cuda.current_stream(t.device).cuda_stream,
+                         torch.cuda.is_current_stream_capturing())
+            for t in tensors
+            if t is not None and t.requires_grad and t.is_leaf and t.is_cuda and torch.is_grad_enabled()]
+
+
 class FusedMXLinearFn(torch.autograd.Function):
     """y = x W^T + bias with W (``kernels.MXTensor``) and x in blocks; dx = dy W."""
 
@@ -141,7 +161,10 @@ class FusedMXLinearFn(torch.autograd.Function):
 def mx_linear(x, w, bias=None, act: str = "fp8"):
     """``F.linear`` over a microscaled weight: x [..., in] (fp16 or bf16) quantised to ``act``."""
     _no_weight_grad("mx_linear", bias=bias)
-    return FusedMXLinearFn.apply(x, w, bias, act)
+    kept = _leaf_streams("mx_linear", x)
+    y = FusedMXLinearFn.apply(x, w, bias, act)
+    del kept
+    return y
 
 
 class FusedMXMLPGLUFn(torch.autograd.Function):
@@ -166,7 +189,10 @@ class FusedMXMLPGLUFn(torch.autograd.Function):
 
 def mx_mlp_glu(x, w_gate_up, act: str = "fp8"):
     """The gated half of a feed-forward block over microscaled weights, x [..., in] fp16 or bf16."""
-    return FusedMXMLPGLUFn.apply(x, w_gate_up, act)
+    kept = _leaf_streams("mx_mlp_glu", x)
+    y = FusedMXMLPGLUFn.apply(x, w_gate_up, act)
+    del kept
+    return y
 
 
 class FusedMXNormMLPFn(torch.autograd.Function):
@@ -201,7 +227,10 @@ def mx_norm_mlp(x, weight, w_gate_up, w_down, eps: float = 1e-6, residual=None):
     _no_weight_grad("mx_norm_mlp", weight=weight)
     if x.dtype != torch.float16:
         raise TypeError(f"mx_norm_mlp: fp16 activations, got {x.dtype}")
-    return FusedMXNormMLPFn.apply(x, weight, w_gate_up, w_down, eps, residual)
+    kept = _leaf_streams("mx_norm_mlp", x, residual)
+    y = FusedMXNormMLPFn.apply(x, weight, w_gate_up, w_down, eps, residual)
+    del kept
+    return y
 
 
 # ---------------------------------------------------------------------------------------------

@@ -3,6 +3,8 @@ differences, and every refusal of the host layer and the C entry points."""
 
 from __future__ import annotations
 
+import ctypes
+
 import numpy as np
 import pytest
 import torch
@@ -164,17 +166,29 @@ F16, F32, BF16, FP4, FP8 = 0, 1, 2, 0, 1
     ("rus_mx_gemm", (16, 16, FP8, 16, 18, FP4, 4, 64, 64, None, 16, 64, F16, None, 0, None), "w codes"),
     ("rus_mx_gemm", (16, 16, FP8, 16, 16, FP4, 4, 64, 64, None, None, 64, F16, None, 0, None), "output"),
     ("rus_mx_gemm", (16, 16, FP8, 16, 16, FP4, 4, 64, 64, 17, 16, 64, F16, None, 0, None), "bias"),
-    ("rus_mx_gemm", (16, 16, FP8, 16, 16, FP4, 1, 1536, 8960, None, 16, 1536, F16, 16, 8, None), "workspace holds"),
+    ("rus_mx_gemm", (16, 16, FP8, 16, 16, FP4, 5, 1536, 8960, None, 16, 1536, F16, 16, 8, None), "workspace holds"),
     ("rus_mx_gemm", (16, 16, FP8, 16, 16, FP4, 1, 64, 1 << 23, None, 16, 64, F16, None, 0, None), "bad sizes"),
     ("rus_mx_gemm_workspace", (1, 64, 0, FP8, FP4, None), "null result"),
-    ("rus_mx_gemm_rows", (16, 64, FP8, 16, 16, FP4, 4, 64, 64, None, 16, 64, F16, 16, 8, None), "scratch holds"),
-    ("rus_mx_gemm_rows", (16, 64, FP8, 16, 16, FP4, 4, 64, 64, None, 16, 64, F16, None, 1 << 20, None), "scratch holds"),
+    ("rus_mx_gemm_rows", (16, 64, FP8, 16, 16, FP4, 5, 64, 64, None, 16, 64, F16, 16, 8, None), "scratch holds"),
+    ("rus_mx_gemm_rows", (16, 64, FP8, 16, 16, FP4, 5, 64, 64, None, 16, 64, F16, None, 1 << 20, None), "scratch holds"),
     ("rus_mx_gemm_rows", (16, 64, FP8, 16, 16, FP4, 4, 0, 64, None, 16, 64, F16, 16, 1 << 20, None), "bad sizes"),
     ("rus_mx_gemm_rows", (16, 64, FP8, 16, 18, FP4, 4, 64, 64, None, 16, 64, F16, 16, 1 << 20, None), "w codes"),
-    ("rus_mx_gemm_rows", (16, 63, FP8, 16, 16, FP4, 4, 64, 64, None, 16, 64, F16, 16, 1 << 20, None), "stride_row"),
+    ("rus_mx_gemm_rows", (16, 63, FP8, 16, 16, FP4, 5, 64, 64, None, 16, 64, F16, 16, 1 << 20, None), "stride_row"),
     ("rus_mx_gemm_rows", (16, 64, 9, 16, 16, FP4, 4, 64, 64, None, 16, 64, F16, 16, 1 << 20, None), "format"),
-    ("rus_mx_glu_fwd_rows", (16, 64, FP8, 16, 16, FP4, 4, 64, 64, 16, 64, F16, 16, 8, None), "scratch holds"),
+    ("rus_mx_glu_fwd_rows", (16, 64, FP8, 16, 16, FP4, 5, 64, 64, 16, 64, F16, 16, 8, None), "scratch holds"),
     ("rus_mx_glu_fwd_rows", (16, 64, FP8, 16, 16, 5, 4, 64, 64, 16, 64, F16, 16, 1 << 20, None), "w has unknown"),
+    # a few tokens: no scratch, the same refusals
+    ("rus_mx_gemm_rows", (16, 63, FP8, 16, 16, FP4, 2, 64, 64, None, 16, 64, F16, None, 0, None), "stride_x"),
+    ("rus_mx_gemm_rows", (None, 64, FP8, 16, 16, FP4, 2, 64, 64, None, 16, 64, F16, None, 0, None), "x is null"),
+    ("rus_mx_gemm_rows", (17, 64, FP8, 16, 16, FP4, 2, 64, 64, None, 16, 64, F16, None, 0, None), "misaligned"),
+    ("rus_mx_gemm_rows", (16, 64, 9, 16, 16, FP4, 2, 64, 64, None, 16, 64, F16, None, 0, None), "format"),
+    ("rus_mx_gemm_rows", (16, 64, FP8, 16, 16, FP4, 2, 64, 64, 17, 16, 64, F16, None, 0, None), "bias"),
+    ("rus_mx_gemm_rows", (16, 64, FP8, 8, 16, FP4, 2, 64, 64, None, 16, 64, F16, None, 0, None), "w codes"),
+    ("rus_mx_gemm_rows", (16, 64, FP8, 16, 16, FP4, 2, 64, 64, None, 16, 63, F16, None, 0, None), "stride"),
+    ("rus_mx_gemm_rows", (16, 64, FP8, 16, 16, FP4, 2, 64, 64, None, 16, 64, F32, None, 0, None), "fp16 or bf16"),
+    ("rus_mx_gemm", (None, 16, FP8, 16, 16, FP4, 2, 64, 64, None, 16, 64, F16, None, 0, None), "x codes"),
+    ("rus_mx_glu_fwd_rows", (None, 64, FP8, 16, 16, FP4, 2, 64, 64, 16, 64, F16, None, 0, None), "x is null"),
+    ("rus_mx_glu_fwd_rows", (16, 64, FP8, 16, 16, FP4, 2, 64, 64, None, 64, F16, None, 0, None), "output"),
     ("rus_mx_rows_scratch", (1, 64, 64, FP8, FP4, 0, None), "null result"),
     ("rus_mx_glu_fwd", (16, 16, FP8, 16, 16, FP4, 4, 64, 64, 16, 63, F16, None), "stride"),
     ("rus_mx_glu_bwd", (16, 64, 16, 16, FP8, 16, 16, FP4, 4, 64, 64, 16, 127, F16, None), "stride"),
@@ -196,3 +210,46 @@ def test_empty_batches_launch_nothing():
     _lib.call("rus_mx_quantize", None, F16, 0, 64, 64, FP4, None, None, None)
     _lib.call("rus_mx_gemm", None, None, FP8, None, None, FP4, 0, 64, 64, None, None, 64, F16, None, 0, None)
     _lib.call("rus_mx_gemm_t", None, 64, F16, None, None, FP4, 0, 64, 64, None, 64, None, 0, None)
+
+
+def test_scratch_sizes():
+    """A few tokens take none, as long as they fit; others the codes, the scales and the sums of a split
+    contraction."""
+    def scratch(m, n, k, glu=0):
+        got = ctypes.c_int64()
+        _lib.call("rus_mx_rows_scratch", m, n, k, FP8, FP4, glu, ctypes.byref(got))
+        return got.value
+    assert scratch(0, 64, 64) == scratch(1, 1536, 8960) == scratch(2, 17920, 1536) == scratch(4, 2048, 1536) == 0
+    assert scratch(2, 8960, 1536, 1) == 0
+    assert scratch(5, 64, 64) >= 5 * 4 * 33 and scratch(3, 17920, 1536) >= 3 * 48 * 33
+    assert scratch(1, 64, 1 << 20) >= (1 << 15) * 33
+    got = ctypes.c_int64()
+    _lib.call("rus_mx_gemm_workspace", 1, 1536, 8960, FP8, FP4, ctypes.byref(got))
+    assert got.value == 0
+    _lib.call("rus_mx_gemm_workspace", 8, 1536, 8960, FP8, FP4, ctypes.byref(got))
+    assert got.value > 0 and got.value % (8 * 1536) == 0
+
+
+def test_capture_beside_a_living_graph_is_refused():
+    """The stream of a leaf's first graph is known while some graph over the leaf lives, and no longer."""
+    x = torch.zeros(3, requires_grad=True)
+
+    def record(stream, capturing):
+        kept = ops._note_stream("op", x, stream, capturing)
+        y = x.exp()
+        del kept
+        return y
+
+    alive = record(1, False)
+    record(2, False)  # another stream, not capturing: autograd's own synchronisation
+    record(1, True)
+    with pytest.raises(RuntimeError, match="op: a graph recorded on another stream"):
+        record(2, True)
+    del alive
+    captured = record(2, True)
+    record(1, False)
+    record(2, True)
+    with pytest.raises(RuntimeError, match="still holds"):
+        record(3, True)
+    del captured
+    record(3, True)
