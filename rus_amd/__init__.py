@@ -58,6 +58,12 @@ def _warm_up(device) -> None:
     head = torch.zeros(1024, 1536, dtype=torch.float16, device=dev)
     lab = torch.zeros(4, dtype=torch.int64, device=dev)
     K.lm_head_ce(hid, head, lab)
+    # microscaled blocks: round and decode, the norm into blocks, products and the gated feed-forward
+    wq = K.mx_quantize(torch.zeros(256, 1536, dtype=torch.float16, device=dev), "fp4")
+    K.mx_dequantize(wq)
+    q, _, _ = K.rms_norm_mx_fwd(x, w, residual=x)
+    K.mx_gemm(K.mx_gemm(x, wq), wq, trans=True)
+    K.mx_mlp_glu_bwd(K.mx_mlp_glu_fwd(q, wq), q, wq)
     torch.cuda.synchronize(dev)
 
 
