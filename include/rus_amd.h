@@ -844,8 +844,8 @@ int rus_mx_dequantize(const void* codes, const void* scales, int32_t fmt, int64_
 
 /*
  * rus_rmsnorm_fwd with the output as fp8 blocks: h = T(x + residual) (sum_out, both or neither),
- * rstd = 1/sqrt(mean(h^2) + eps), blocks of (h rstd) weight formed in fp64 and rounded once to the
- * element. x, residual and sum_out share dtype (fp16 / fp32) and stride_row; weight has w_dtype.
+ * rstd = 1/sqrt(mean(h^2) + eps), blocks of (h rstd) weight as if formed in fp64 and rounded once to
+ * the element. x, residual and sum_out share dtype (fp16 / fp32) and stride_row; weight has w_dtype.
  * rus_rmsnorm_bwd takes (h, rstd) as saved here.
  */
 int rus_rmsnorm_mx_fwd(const void* x, const void* residual, const void* weight, int32_t w_dtype,
@@ -854,9 +854,10 @@ int rus_rmsnorm_mx_fwd(const void* x, const void* residual, const void* weight, 
 
 /*
  * y[m, n] = T(sum_k X[m, k] W[n, k] + bias[n]); X [m, k] and W [n, k] in either format, T fp16 or
- * bf16 (dtype), bias in T or NULL; fp32 sums; k at most 2^22. workspace: the fp32 elements
- * rus_mx_gemm_workspace names (0: none; 16-byte aligned), for a contraction that few tiles split
- * among them; not shared by calls that overlap.
+ * bf16 (dtype), bias in T or NULL; fp32 sums; k at most 2^22. Beyond a few tokens the sums come from
+ * the scaled matrix instructions, which with an 8-bit operand keep about 13 bits below the largest of
+ * 16 products that they add first. workspace: the fp32 elements rus_mx_gemm_workspace names (0: none;
+ * 16-byte aligned), for a contraction that few tiles split among them; not shared by calls that overlap.
  */
 int rus_mx_gemm_workspace(int64_t m, int64_t n, int64_t k, int32_t x_fmt, int32_t w_fmt,
                           int64_t* floats);
@@ -867,8 +868,8 @@ int rus_mx_gemm(const void* x_codes, const void* x_scales, int32_t x_fmt, const 
 
 /*
  * rus_mx_gemm of activations that are not in blocks yet: x [m, k] in T, quantised to `act` first
- * (rus_mx_quantize). scratch: the bytes rus_mx_rows_scratch names (glu = 0; 16-byte aligned), not
- * shared by calls that overlap.
+ * (rus_mx_quantize; the same bits), a few tokens inside the product's own launch. scratch: the bytes
+ * rus_mx_rows_scratch names (glu = 0; 0: none; 16-byte aligned), not shared by calls that overlap.
  */
 int rus_mx_rows_scratch(int64_t m, int64_t n, int64_t k, int32_t act, int32_t w_fmt, int32_t glu,
                         int64_t* bytes);
