@@ -2412,13 +2412,34 @@ def _mx_rows(fn: str, x: torch.Tensor, width: int | None, name: str) -> torch.Te
     return x
 
 
+def _row_bytes(t: torch.Tensor) -> tuple[int, int, int]:
+    """(first byte, distance of two rows, bytes of a row) of 2-D rows with unit column stride."""
+    width = t.shape[1] * t.element_size()
+    return t.data_ptr(), (t.stride(0) * t.element_size() if t.shape[0] > 1 else width), width
+
+
+def _apart(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether no byte belongs to both: apart as a whole, or columns of one wider matrix."""
+    if a.numel() == 0 or b.numel() == 0 or a.untyped_storage().data_ptr() != b.untyped_storage().data_ptr():
+        return True
+    (pa, da, wa), (pb, db, wb) = _row_bytes(a), _row_bytes(b)
+    if pa + (a.shape[0] - 1) * da + wa <= pb or pb + (b.shape[0] - 1) * db + wb <= pa:
+        return True
+    at = (pb - pa) % da
+    return da == db and wa <= at and at + wb <= da
+
+
 def _mx_out(fn: str, out: torch.Tensor | None, m: int, n: int, dtype: torch.dtype,
-            like: torch.Tensor) -> torch.Tensor:
+            like: torch.Tensor, *operands: torch.Tensor) -> torch.Tensor:
+    """``out``, or a new one; it may not share memory with the rows it is formed from."""
     if out is None:
         return torch.empty((m, n), dtype=dtype, device=like.device)
     if out.dtype != dtype or tuple(out.shape) != (m, n) or (n > 1 and out.stride(1) != 1) or \
             (m > 1 and out.stride(0) < n):
         raise ValueError(f"{fn}: out must be {dtype} [{m}, {n}] with unit column stride")
+    for t in (like, *operands):
+        if not _apart(out, t):
+            raise ValueError(f"{fn}: out shares memory with an operand")
     return out
 
 
@@ -2472,7 +2493,7 @@ def mx_dequantize(t: MXTensor, dtype: torch.dtype = torch.float16,
     dt = _mx_dtype(fn, dtype)
     code, nbytes = _MX_FMT[t.fmt]
     rows, cols = t.shape
-    out = _mx_out(fn, out, rows, cols, dtype, t.codes)
+    out = _mx_out(fn, out, rows, cols, dtype, t.codes, t.scales)
     _mx_launch("mx_dequantize",
                lambda: (rows * (_mx_blocks(cols) * (nbytes + 1) + cols * out.element_size()), 0), t.codes,
                "rus_mx_dequantize", t.codes.data_ptr(), t.scales.data_ptr(), code, rows,
@@ -2572,7 +2593,7 @@ def mx_gemm(x, w: MXTensor, trans: bool = False, bias: torch.Tensor | None = Non
         dt = _mx_dtype(fn, x.dtype, wide=False)
         x2 = _mx_rows(fn, x, n, "x")
         m = x2.shape[0]
-        out = _mx_out(fn, out, m, k, x2.dtype, x2)
+        out = _mx_out(fn, out, m, k, x2.dtype, x2, w.codes, w.scales)
         if n == 0:
             return out.zero_()
         floats = _mx_scratch("rus_mx_gemm_t_workspace", m, n, k)
@@ -2590,10 +2611,12 @@ def mx_gemm(x, w: MXTensor, trans: bool = False, bias: torch.Tensor | None = Non
         if bias.dtype != dtype or bias.numel() != n:
             raise ValueError(f"{fn}: bias must be {dtype} [{n}]")
         bias = bias.reshape(-1).contiguous()
+        if out is not None and out.dim() == 2 and not _apart(out, bias.view(1, -1)):
+            raise ValueError(f"{fn}: out shares memory with the bias")
     if not blocks and x.dtype == dtype:  # quantised on the way
         xf, x = _mx_fmt(fn, act)[0], _mx_rows(fn, x, k, "x")
         m = x.shape[0]
-        out = _mx_out(fn, out, m, n, dtype, x)
+        out = _mx_out(fn, out, m, n, dtype, x, w.codes, w.scales)
         if n == 0:
             return out
         need = _mx_scratch("rus_mx_rows_scratch", m, n, k, xf, wf, 0)
@@ -2604,7 +2627,7 @@ def mx_gemm(x, w: MXTensor, trans: bool = False, bias: torch.Tensor | None = Non
         return out
     x = _mx_operand(fn, x, act, k)
     m = x.shape[0]
-    out = _mx_out(fn, out, m, n, dtype, x.codes)
+    out = _mx_out(fn, out, m, n, dtype, x.codes, x.scales, w.codes, w.scales)
     if n == 0:
         return out
     xf = _MX_FMT[x.fmt][0]
@@ -2640,7 +2663,7 @@ def mx_mlp_glu_fwd(x, w: MXTensor, act: str = "fp8", out: torch.Tensor | None = 
     if not blocks and x.dtype == dtype:  # quantised on the way
         xf, x = _mx_fmt(fn, act)[0], _mx_rows(fn, x, k, "x")
         m = x.shape[0]
-        out = _mx_out(fn, out, m, n, dtype, x)
+        out = _mx_out(fn, out, m, n, dtype, x, w.codes, w.scales)
         need = _mx_scratch("rus_mx_rows_scratch", m, n, k, xf, wf, 1)
         scratch = torch.empty(need, dtype=torch.uint8, device=x.device) if need else None
         _mx_launch("mx_glu_fwd", lambda: (2 * m * (n + k) + _mx_bytes(w), 4 * m * n * k), x,
@@ -2649,7 +2672,7 @@ def mx_mlp_glu_fwd(x, w: MXTensor, act: str = "fp8", out: torch.Tensor | None = 
         return out
     x = _mx_operand(fn, x, act, k)
     m = x.shape[0]
-    out = _mx_out(fn, out, m, n, dtype, x.codes)
+    out = _mx_out(fn, out, m, n, dtype, x.codes, x.scales, w.codes, w.scales)
     _mx_launch("mx_glu_fwd", lambda: (_mx_bytes(x) + _mx_bytes(w) + 2 * m * n, 4 * m * n * k), x.codes,
                "rus_mx_glu_fwd", x.codes.data_ptr(), x.scales.data_ptr(), _MX_FMT[x.fmt][0],
                w.codes.data_ptr(), w.scales.data_ptr(), wf, m, n, k, out.data_ptr(), _ld(out), dt)
@@ -2671,7 +2694,7 @@ def mx_mlp_glu_bwd(dh: torch.Tensor, x, w: MXTensor, act: str = "fp8",
     m = x.shape[0]
     if dh2.shape[0] != m:
         raise ValueError(f"{fn}: dh has {dh2.shape[0]} rows, x {m}")
-    out = _mx_out(fn, out, m, 2 * n, dh.dtype, dh2)
+    out = _mx_out(fn, out, m, 2 * n, dh.dtype, dh2, x.codes, x.scales, w.codes, w.scales)
     _mx_launch("mx_glu_bwd", lambda: (_mx_bytes(x) + _mx_bytes(w) + 6 * m * n, 4 * m * n * k), dh2,
                "rus_mx_glu_bwd", dh2.data_ptr(), _ld(dh2), x.codes.data_ptr(), x.scales.data_ptr(),
                _MX_FMT[x.fmt][0], w.codes.data_ptr(), w.scales.data_ptr(), _MX_FMT[w.fmt][0], m, n, k,

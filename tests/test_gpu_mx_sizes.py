@@ -428,6 +428,25 @@ def test_every_launch_is_timed():
     assert all(r[3] > 0 for r in t.records)
 
 
+def test_results_over_operands_are_refused():
+    w = K.mx_quantize(torch.ones(64, 64, device=DEV), "fp4")
+    for m in (1, 3, 50):
+        wide = torch.ones(m, 200, dtype=F16, device=DEV)
+        x, dh = wide[:, :64], wide[:, :32]
+        for call in (lambda o: K.mx_gemm(x, w, out=o), lambda o: K.mx_gemm(x, w, trans=True, out=o),
+                     lambda o: K.mx_mlp_glu_bwd(dh, w2, w, out=o)):
+            w2 = K.mx_quantize(x, "fp8")
+            with pytest.raises(ValueError, match="shares memory"):
+                call(wide[:, 20:84])
+            call(wide[:, 64:128])  # beside it
+        assert (wide[:, :64] == 1).all() and (wide[:, 128:] == 1).all()
+        with pytest.raises(ValueError, match="shares memory"):
+            K.mx_mlp_glu_fwd(x, w, out=wide[:, 63:95])
+        K.mx_mlp_glu_fwd(x, w, out=wide[:, 64:96])
+        with pytest.raises(ValueError, match="the bias"):
+            K.mx_gemm(x, w, bias=wide[m - 1, 130:194], out=wide[:, 136:200])
+
+
 def test_refusals_leave_nothing_behind():
     """A refused call, then a good one."""
     w = K.mx_quantize(torch.ones(64, 256, device=DEV), "fp4")

@@ -116,6 +116,20 @@ def test_cpu_tensors_are_refused():
             call()
 
 
+def test_results_apart_from_operands():
+    """Rows that share bytes against rows that only share a matrix."""
+    flat = torch.zeros(6, 40, dtype=torch.float16)
+    whole, left, right = flat, flat[:, :20], flat[:, 20:]
+    assert K._apart(left, right) and K._apart(right, left) and K._apart(flat[:3], flat[3:])
+    assert K._apart(flat[:, :10], flat[:, 10:12]) and K._apart(flat[1:, :10], flat[:, 30:])
+    assert K._apart(left, torch.zeros(6, 40)) and K._apart(whole[:0], whole)
+    for a, b in ((whole, whole), (left, whole), (flat[:4], flat[3:]), (flat[:, :21], right), (flat[:, 19:], left),
+                 (flat[1:, :21], right), (flat.view(12, 20), left), (flat.view(-1)[7:127].view(3, 40), left),
+                 (flat[2:3, 5:], flat[:, :6])):
+        assert not K._apart(a, b) and not K._apart(b, a)
+    assert K._apart(flat[2:3, 6:], flat[:2]) and K._apart(flat[2:3, 20:], flat[3:])
+
+
 def test_wrong_operands_are_refused():
     x, w = torch.zeros(2, 64, dtype=torch.float16), _mx(8, 64)
     for call, err in (
