@@ -2407,6 +2407,8 @@ def _mx_rows(fn: str, x: torch.Tensor, width: int | None, name: str) -> torch.Te
     if x.dim() != 2 or (width is not None and x.shape[1] != width):
         raise ValueError(f"{fn}: {name} must be 2-D{'' if width is None else f' with {width} columns'}, "
                          f"got {tuple(x.shape)}")
+    if x.is_contiguous():
+        return x
     if x.shape[1] > 1 and x.stride(1) != 1 or x.shape[0] > 1 and x.stride(0) < x.shape[1]:
         return x.contiguous()
     return x
@@ -2433,7 +2435,7 @@ def _mx_out(fn: str, out: torch.Tensor | None, m: int, n: int, dtype: torch.dtyp
             like: torch.Tensor, *operands: torch.Tensor) -> torch.Tensor:
     """``out``, or a new one; it may not share memory with the rows it is formed from."""
     if out is None:
-        return torch.empty((m, n), dtype=dtype, device=like.device)
+        return torch.empty(m, n, dtype=dtype, device=like.device)
     if out.dtype != dtype or tuple(out.shape) != (m, n) or (n > 1 and out.stride(1) != 1) or \
             (m > 1 and out.stride(0) < n):
         raise ValueError(f"{fn}: out must be {dtype} [{m}, {n}] with unit column stride")
@@ -2475,8 +2477,8 @@ def mx_quantize(x: torch.Tensor, fmt: str = "fp4") -> MXTensor:
     if cols == 0:
         raise ValueError(f"{fn}: rows without columns")
     nb = _mx_blocks(cols)
-    codes = torch.empty((rows, nb * nbytes), dtype=torch.uint8, device=x2.device)
-    scales = torch.empty((rows, nb), dtype=torch.uint8, device=x2.device)
+    codes = torch.empty(rows, nb * nbytes, dtype=torch.uint8, device=x2.device)
+    scales = torch.empty(rows, nb, dtype=torch.uint8, device=x2.device)
     _mx_launch("mx_quantize", lambda: (rows * (cols * x2.element_size() + nb * (nbytes + 1)), 0), x2,
                "rus_mx_quantize", x2.data_ptr(), dt, rows, cols, _ld(x2), code, codes.data_ptr(),
                scales.data_ptr())
@@ -2525,9 +2527,9 @@ def rms_norm_mx_fwd(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6,
         res_2d = residual.contiguous()
         sum_out = torch.empty_like(x_2d)
     nb = _mx_blocks(n_cols)
-    codes = torch.empty((n_rows, nb * 32), dtype=torch.uint8, device=x.device)
-    scales = torch.empty((n_rows, nb), dtype=torch.uint8, device=x.device)
-    rstd = torch.empty((n_rows,), dtype=torch.float32, device=x.device)
+    codes = torch.empty(n_rows, nb * 32, dtype=torch.uint8, device=x.device)
+    scales = torch.empty(n_rows, nb, dtype=torch.uint8, device=x.device)
+    rstd = torch.empty(n_rows, dtype=torch.float32, device=x.device)
     def cost():
         streams = 1 if res_2d is None else 3
         return n_rows * (streams * n_cols * x_2d.element_size() + nb * 33 + 4) + n_cols * w.element_size(), 0
