@@ -144,7 +144,7 @@ __device__ __forceinline__ void finish(const MxArgs& g, int t, int f, const floa
   }
 }
 
-// ---- few tokens ------------------------------------------------------------------------------------
+// ---- tens of tokens --------------------------------------------------------------------------------
 //
 // 32 features x 32 tokens per workgroup of four waves, the contraction's groups of four blocks dealt to
 // the waves, operands straight from memory to registers, two groups' loads in flight at a time; the
@@ -211,29 +211,29 @@ __global__ __launch_bounds__(kRowsWaves* kWave) void mx_rows_kernel(MxArgs g) {
 // ---- tiles -----------------------------------------------------------------------------------------
 //
 // BF rows of W x BT tokens per workgroup of four waves (2 x 2 of BF/2 x BT/2; eight, 2 x 4, for 256
-// tokens), the contraction staged
-// GROUPS x 128 at a time (a group of four blocks is two MFMA steps) through two LDS buffers that memory
-// is copied into directly (global_load_lds: 64 lanes' 16 bytes land one after the other), a stage ahead
-// of its products. Two workgroups of four waves share a CU: one's waits and epilogue run under the other's
-// products. One of eight has it to itself.
+// tokens), the contraction staged GROUPS x 128 at a time (a group of four blocks is two MFMA steps)
+// through two LDS buffers that memory is copied into directly (global_load_lds: 64 lanes' 16 bytes land
+// one after the other), a stage ahead of its products. Two workgroups of four waves share a CU: one's
+// waits and epilogue run under the other's products. One of eight has it to itself.
 //
 // What bounds it is the copies: a CU takes a line from its L2 in about 2.3 cycles whether it needs 128
 // bytes of it or 64 (55 or 28 bytes per cycle, measured with nothing else running). Where both operands
-// are fp4, a stage is therefore two groups, so that rows are whole lines, and where there are tiles enough
-// a tile is 256 x 256, which copies half as much a product (8,161 x 17,920 x 1,536: 139 us, 3.2 PFLOP/s,
-// against 165 with 128 x 128; 8,161 x 8,960 x 8,960: 341 and 412); with an fp8 operand the products take
-// twice as long and a taller tile of one group covers the copies (8,161 x 17,920 x 1,536: 194 us with
-// 256 x 128, 195 with 256 x 256, 225 with 128 x 128). They go out between the
-// products, since a wave that issues them in a row waits for each.
+// are fp4, a stage is therefore two groups, so that rows are whole lines, and where there are tiles
+// enough a tile is 256 x 256, which copies half as much a product (8,161 x 17,920 x 1,536: 139 us, 3.2
+// PFLOP/s, against 165 with 128 x 128; 8,161 x 8,960 x 8,960: 341 and 412); with an fp8 operand the
+// products take twice as long and a taller tile of one group covers the copies (8,161 x 17,920 x 1,536:
+// 194 us with 256 x 128, 195 with 256 x 256, 225 with 128 x 128). They go out between the products, since
+// a wave that issues them in a row waits for each.
 //
 // LDS rows of W are in MFMA order (row 32 q + i holds feature 32 q + feature_of(i)); with a gate, the
 // lower half is gate, the upper half up rows of the same features, and a wave takes the same part of
-// both, so that a lane holds both. The 16-byte chunk
-// c of row r lies at c ^ ((r / 4) % 4) of a 64-byte row, c ^ ((r / 2) % 8) of a 128-byte one, by each
-// lane fetching the chunk that belongs at its place: 16 neighbouring rows read at one chunk cover all
-// banks once. Scales come four groups at a time, 16 bytes of a row in one request.
-// LDS is read by explicit instructions and waits: the compiler would wait for the copies in flight
-// before any LDS read. A register read this way is tied to the wait before its first use.
+// both, so that a lane holds both. The 16-byte chunk c of row r lies at c ^ ((r / 4) % 4) of a 64-byte
+// row, c ^ ((r / 2) % 8) of a 128-byte one, by each lane fetching the chunk that belongs at its place: 16
+// neighbouring rows read at one chunk cover all banks once. Scales come four groups at a time, 16 bytes
+// of a row in one request. LDS is read by explicit instructions and waits: the compiler would wait for
+// the copies in flight before any LDS read. A register read this way is tied to the wait before its first
+// use.
+
 // Four waves, 2 x 2; eight, 2 x 4, for 256 tokens.
 template <int BT>
 constexpr int kTileThreads = BT == 256 ? 512 : 256;
@@ -736,16 +736,17 @@ __global__ __launch_bounds__(256) void mx_sum_kernel(const float* __restrict__ p
 
 // ---- which kernel --------------------------------------------------------------------------------
 //
-// The one whose launch is estimated shortest. A launch takes a + groups (b + r (rounds - 1)) us, groups of
-// four blocks of the contraction per workgroup, rounds of 256 workgroups (and c a round); a contraction cut into parts
-// pays for a second launch and 8 bytes a value and part. Measured at 12 and 70 groups (k = 1536, 8960),
-// 1 to 8,161 tokens, 1,536 to 17,920 features: one round of 256 x 128 tiles 10.5 / 42 us, of 128 x 128
-// 7.4 / 28.5, of 128 x 64 6.4 / 25, of the few-token kernel 3.7 / 9.3 (one token) and 4.7 / 15.3 (32).
-// 707 tokens x 17,920: 22.9, 25.4, 28.4 and (few-token) 121; 192 tokens 12.5, 12.1, 9.9; 2,048 features at
-// 33 tokens 10.3, 7.1, 6.4 and 4.6. With both operands fp4, 256 x 256 takes the taller tile's place: one
-// round 12 to 17 / 43 to 61 us, a further one 16 / 64, against 128 x 128's 6.5 / 21 to 33 and 4.8 / 28.
+// The one whose launch is estimated shortest. A launch takes a + groups (b + r (rounds - 1)) us, groups
+// of four blocks of the contraction per workgroup, rounds of 256 workgroups (and c for each after the
+// first); a contraction cut into parts pays for a second launch and 8 bytes a value and part. Measured at
+// 12 and 70 groups (k = 1536, 8960), 1 to 8,161 tokens, 1,536 to 17,920 features: one round of 256 x 128
+// tiles 10.5 / 42 us, of 128 x 128 7.4 / 28.5, of 128 x 64 6.4 / 25, of the 32 x 32 kernel 3.7 / 9.3
+// (one token) and 4.7 / 15.3 (32). 707 tokens x 17,920: 22.9, 25.4, 28.4 and (32 x 32) 121; 192 tokens
+// 12.5, 12.1, 9.9; 2,048 features at 33 tokens 10.3, 7.1, 6.4 and 4.6. With both operands fp4, 256 x 256
+// takes the taller tile's place: one round 12 to 17 / 43 to 61 us, a further one 16 / 64, against 128 x
+// 128's 6.5 / 21 to 33 and 4.8 / 28.
 struct GemmPlan {
-  int bf, bt, splits;  // bt 32: the few-token kernel
+  int bf, bt, splits;  // bt 32: the 32 x 32 kernel
 };
 
 GemmPlan find_gemm_plan(int64_t m, int64_t n, int64_t nb, int x_fmt, int w_fmt, bool glu) {
@@ -1024,7 +1025,8 @@ extern "C" int rus_mx_gemm_rows(const void* x, int64_t stride_x, int32_t act, co
   if (int e = check_sizes(fn, m, n, k)) return e;
   if (m == 0) return RUS_OK;
   if (few_tokens(m, n, mx_blocks(k)))
-    return run_tokens(fn, x, stride_x, act, w_codes, w_scales, w_fmt, m, n, k, bias, y, stride_y, dtype, false, stream);
+    return run_tokens(fn, x, stride_x, act, w_codes, w_scales, w_fmt, m, n, k, bias, y, stride_y, dtype, false,
+                      stream);
   const RowsScratch need = rows_scratch(m, n, k, act, w_fmt, false);
   char *codes, *scales;
   float* sums;
@@ -1044,7 +1046,8 @@ extern "C" int rus_mx_glu_fwd_rows(const void* x, int64_t stride_x, int32_t act,
   if (int e = check_sizes(fn, m, n, k)) return e;
   if (m == 0) return RUS_OK;
   if (few_tokens(m, n, mx_blocks(k)))
-    return run_tokens(fn, x, stride_x, act, w_codes, w_scales, w_fmt, m, n, k, nullptr, h, stride_h, dtype, true, stream);
+    return run_tokens(fn, x, stride_x, act, w_codes, w_scales, w_fmt, m, n, k, nullptr, h, stride_h, dtype, true,
+                      stream);
   char *codes, *scales;
   float* sums;
   if (int e = place(fn, rows_scratch(m, n, k, act, w_fmt, true), scratch, n_scratch, codes, scales, sums))

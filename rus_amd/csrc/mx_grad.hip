@@ -327,11 +327,11 @@ __global__ __launch_bounds__(256) void mx_grad_sum_kernel(const float* __restric
 }
 
 // The tile height and the number of splits for a shape, by what a launch is estimated to take: rounds of
-// 256 workgroups, each 3 us (5 of 256 tokens) and its stages (1.7, 1.05, 0.9 or 0.65 us of 256, 128, 64 or 32 tokens); a
-// split contraction pays for the second launch and 8 bytes a sum, which stay in the caches (10 TB/s).
-// Measured over 1 to 4,096 tokens: 4,096 x 17,920 x 1,536 in 256-token tiles and 5 splits 232 us (2: 238;
-// 128-token tiles unsplit 272, in 4 splits 307); 707 tokens 53; 256 tokens in 128-token tiles 29 (256:
-// 34, 64: 34); 16 tokens in 32-token tiles and 28 splits 14.5.
+// 256 workgroups, each 3 us (5 of 256 tokens) and its stages (1.7, 1.05, 0.9 or 0.65 us of 256, 128, 64
+// or 32 tokens); a split contraction pays for the second launch and 8 bytes a sum, which stay in the
+// caches (10 TB/s). Measured over 1 to 4,096 tokens: 4,096 x 17,920 x 1,536 in 256-token tiles and 5
+// splits 232 us (2: 238; 128-token tiles unsplit 272, in 4 splits 307); 707 tokens 53; 256 tokens in
+// 128-token tiles 29 (256: 34, 64: 34); 16 tokens in 32-token tiles and 28 splits 14.5.
 struct GradPlan {
   int tm, splits;
 };

@@ -167,9 +167,10 @@ __device__ __forceinline__ void exact_blocks(const float (&h)[8], const float (&
   *scale = b;
 }
 
-// The same from fp32 products; false (for the whole wave) where they do not settle it. `plain`: rstd
-// is far from fp32's limits; `inside`: the block holds some of the row's elements (else it is zeros). With the block's largest y in [2^-60, 2^100] and |w| up to 2^40, every product that is
-// not far below the smallest code is a normal number.
+// The same from fp32 products; false (for the whole wave) where they do not settle it. `plain`: rstd is
+// far from fp32's limits; `inside`: the block holds some of the row's elements (else it is zeros). With
+// the block's largest y in [2^-60, 2^100] and |w| up to 2^40, every product that is not far below the
+// smallest code is a normal number.
 __device__ __forceinline__ bool fast_blocks(const float (&h)[8], const float (&w)[8], float r,
                                             bool plain, bool inside, uint32_t (&code)[2], int* scale) {
   float y[8], wide = 0.0f;

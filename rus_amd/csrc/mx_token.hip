@@ -24,7 +24,8 @@ namespace {
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef u32x4s u32x4u __attribute__((aligned(2)));
 
-constexpr int kPitch = 80;  // bytes of a block of x in LDS: 64 and a gap, so that eight blocks' reads miss each other's banks
+// Bytes of a block of x in LDS: 64 and a gap, so that eight blocks' reads miss each other's banks.
+constexpr int kPitch = 80;
 
 // A block's 32 elements, two at a time, as fp16.
 template <int FMT>
