@@ -118,6 +118,9 @@ def qkv_lora_rope(qkv, cos, sin, pos_ids, q_lora=None, v_lora=None, scale_q=2.0,
 
 
 def _no_weight_grad(fn: str, **tensors) -> None:
+    """Refuses a tensor that autograd would expect a gradient for; where none is recorded any will do."""
+    if not torch.is_grad_enabled():
+        return
     for name, t in tensors.items():
         if t is not None and t.requires_grad:
             raise RuntimeError(f"{fn}: {name} is frozen here: no gradient is formed for it")
