@@ -113,7 +113,7 @@ def qkv_lora_rope(qkv, cos, sin, pos_ids, q_lora=None, v_lora=None, scale_q=2.0,
 
 # ---------------------------------------------------------------------------------------------
 # Layers over microscaled weights (frozen, as the NF4 ones): gradients of the activations only,
-# straight through their quantisation
+# straight through their quantisation; a gradient of such a gradient is refused
 # ---------------------------------------------------------------------------------------------
 
 
@@ -146,6 +146,23 @@ def _leaf_streams(fn: str, *tensors):
             if t is not None and t.requires_grad and t.is_leaf and t.is_cuda and torch.is_grad_enabled()]
 
 
+class _FirstOrderFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, g, fn):
+        ctx.fn = fn
+        return g.view_as(g)
+
+    @staticmethod
+    def backward(ctx, dg):
+        raise RuntimeError(f"{ctx.fn}: no second derivative is formed")
+
+
+def _first_order(fn: str, g: torch.Tensor) -> torch.Tensor:
+    """A gradient as a backward returns it. Its kernels are not recorded, so under create_graph it would
+    pass for a constant: a gradient of it raises instead."""
+    return _FirstOrderFn.apply(g.requires_grad_(), fn) if torch.is_grad_enabled() else g
+
+
 class FusedMXLinearFn(torch.autograd.Function):
     """y = x W^T + bias with W (``kernels.MXTensor``) and x in blocks; dx = dy W."""
 
@@ -158,7 +175,8 @@ class FusedMXLinearFn(torch.autograd.Function):
     @staticmethod
     def backward(ctx, dy):
         dx = K.mx_gemm(dy.reshape(-1, dy.shape[-1]), ctx.w, trans=True)
-        return dx.view(*dy.shape[:-1], ctx.w.shape[1]), None, None, None
+        dx = dx.view(*dy.shape[:-1], ctx.w.shape[1])
+        return _first_order("mx_linear", dx) if dy.requires_grad else dx, None, None, None
 
 
 def mx_linear(x, w, bias=None, act: str = "fp8"):
@@ -187,7 +205,7 @@ class FusedMXMLPGLUFn(torch.autograd.Function):
         q = K.MXTensor(*ctx.saved_tensors, ctx.rows, ctx.act)
         d_gu = K.mx_mlp_glu_bwd(dh.reshape(-1, dh.shape[-1]), q, ctx.w)
         dx = K.mx_gemm(d_gu, ctx.w, trans=True)
-        return dx.view(*dh.shape[:-1], ctx.w.shape[1]), None, None
+        return _first_order("mx_mlp_glu", dx.view(*dh.shape[:-1], ctx.w.shape[1])), None, None
 
 
 def mx_mlp_glu(x, w_gate_up, act: str = "fp8"):
@@ -221,6 +239,7 @@ class FusedMXNormMLPFn(torch.autograd.Function):
         d_gu = K.mx_mlp_glu_bwd(d_a, q, w_gate_up)
         d_n = K.mx_gemm(d_gu, w_gate_up, trans=True).view(h.shape)
         dx = K.rms_norm_bwd(d_n, h, weight, rstd, dresidual=d_h[0] if ctx.with_residual else None)
+        dx = _first_order("mx_norm_mlp", dx)
         return dx, None, None, None, None, (dx if ctx.with_residual else None)
 
 

@@ -31,3 +31,47 @@ def test_parameters_are_taken_where_no_gradient_is_recorded():
         for off in (torch.no_grad, torch.inference_mode):
             with off(), pytest.raises(RuntimeError, match="HIP device tensors"):
                 call()
+
+
+# ---- second derivatives --------------------------------------------------------------------------
+
+
+@pytest.fixture
+def plain_kernels(monkeypatch):
+    """Stand-ins of the launchers that return zeros of the right shape on the CPU."""
+    zeros = lambda m, n: torch.zeros(m, n, dtype=torch.float16)
+    monkeypatch.setattr(K, "mx_quantize", lambda x, fmt="fp4": _mx(*x.shape, fmt))
+    monkeypatch.setattr(K, "mx_gemm", lambda x, w, trans=False, **_: zeros(x.shape[0], w.shape[1 if trans else 0]))
+    monkeypatch.setattr(K, "mx_mlp_glu_fwd", lambda x, w, **_: zeros(x.shape[0], w.shape[0] // 2))
+    monkeypatch.setattr(K, "mx_mlp_glu_bwd", lambda dh, x, w, **_: zeros(dh.shape[0], w.shape[0]))
+    monkeypatch.setattr(K, "rms_norm_mx_fwd", lambda x, w, eps, residual: (
+        _mx(x.numel() // x.shape[-1], x.shape[-1], "fp8"), x if residual is None else x + residual, torch.zeros(2)))
+    monkeypatch.setattr(K, "rms_norm_bwd", lambda dy, h, w, rstd, dresidual=None: torch.zeros_like(dy))
+
+
+@pytest.mark.parametrize("layer", ["linear", "glu", "norm_mlp", "norm_mlp_residual"])
+def test_gradients_of_gradients_are_refused(layer, plain_kernels):
+    """The backward runs kernels that autograd does not see: what it returns may not pass for a constant."""
+    x = torch.ones(2, 64, dtype=torch.float16, requires_grad=True)
+    w, down, norm = _mx(16, 64), _mx(64, 8), torch.ones(64, dtype=torch.float16)
+    res = torch.ones_like(x, requires_grad=True)
+    y = {"linear": lambda: ops.mx_linear(x, w),
+         "glu": lambda: ops.mx_mlp_glu(x, w),
+         "norm_mlp": lambda: ops.mx_norm_mlp(x, norm, w, down),
+         "norm_mlp_residual": lambda: ops.mx_norm_mlp(x, norm, w, down, residual=res)[0]}[layer]()
+    for dy in (torch.ones_like(y), torch.ones_like(y, requires_grad=True)):
+        (dx,) = torch.autograd.grad(y, x, dy, create_graph=True)
+        if layer == "linear" and not dy.requires_grad:
+            assert not dx.requires_grad  # dy W is one
+            continue
+        with pytest.raises(RuntimeError, match="no second derivative"):
+            (dx.sum() + x.sum()).backward()
+    assert not torch.autograd.grad(y, x, torch.ones_like(y))[0].requires_grad
+
+
+def test_first_derivatives_under_create_graph(plain_kernels):
+    """A graph of the gradient that nothing differentiates costs nothing."""
+    x = torch.ones(2, 64, dtype=torch.float16, requires_grad=True)
+    z = ops.mx_mlp_glu(x, _mx(16, 64)).sum() + (x * x).sum()
+    (dx,) = torch.autograd.grad(z, x, create_graph=True)
+    assert torch.equal(dx, 2 * x)
