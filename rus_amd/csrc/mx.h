@@ -194,11 +194,15 @@ class PlanMemo {
   } slots_[kSlots];
 };
 
+inline int check_format(const char* fn, int32_t fmt, const char* name) {
+  if (fmt == RUS_MX_FP4 || fmt == RUS_MX_FP8) return RUS_OK;
+  return fail(RUS_ERR_INVALID, "%s: %s has unknown format %d", fn, name, (int)fmt);
+}
+
 // The checks every entry point makes of a block operand.
 inline int check_mx(const char* fn, const void* codes, const void* scales, int32_t fmt,
                     const char* name) {
-  if (fmt != RUS_MX_FP4 && fmt != RUS_MX_FP8)
-    return fail(RUS_ERR_INVALID, "%s: %s has unknown format %d", fn, name, (int)fmt);
+  if (int e = check_format(fn, fmt, name)) return e;
   if (!codes || !scales || !aligned(codes, 16) || !aligned(scales, 4))
     return fail(RUS_ERR_INVALID, "%s: %s codes / scales null or misaligned (16 / 4 bytes)", fn, name);
   return RUS_OK;

@@ -857,13 +857,25 @@ int product(const char* fn, MxArgs g, const GemmPlan& plan, int32_t x_fmt, int32
   return check_launch(fn);
 }
 
+int check_sizes(const char* fn, int64_t m, int64_t n, int64_t k) {
+  if (m < 0 || n <= 0 || k <= 0 || m >= (1 << 30) || n >= (1 << 28) || k > (1 << 22))
+    return fail(RUS_ERR_INVALID, "%s: bad sizes m=%lld n=%lld k=%lld", fn, (long long)m, (long long)n,
+                (long long)k);
+  return RUS_OK;
+}
+
+// What a plan depends on: nothing is planned, or remembered, for formats that do not exist.
+int check_plan(const char* fn, int64_t m, int64_t n, int64_t k, int32_t x_fmt, int32_t w_fmt) {
+  if (int e = check_sizes(fn, m, n, k)) return e;
+  if (int e = check_format(fn, x_fmt, "x")) return e;
+  return check_format(fn, w_fmt, "w");
+}
+
 // Checks shared by the three entry points; fills what they share.
 int prepare(const char* fn, MxArgs& g, const void* xc, const void* xs, int32_t x_fmt, const void* wc,
             const void* ws, int32_t w_fmt, int64_t m, int64_t n, int64_t k, void* y,
             int64_t ldy, int64_t y_cols, int32_t dtype, bool raw = false) {
-  if (m < 0 || n <= 0 || k <= 0 || m >= (1 << 30) || n >= (1 << 28) || k > (1 << 22))
-    return fail(RUS_ERR_INVALID, "%s: bad sizes m=%lld n=%lld k=%lld", fn, (long long)m,
-                (long long)n, (long long)k);
+  if (int e = check_sizes(fn, m, n, k)) return e;
   if (dtype != RUS_DTYPE_F16 && dtype != RUS_DTYPE_BF16)
     return fail(RUS_ERR_UNSUPPORTED, "%s: results are fp16 or bf16, not dtype %d", fn, (int)dtype);
   if (ldy < y_cols && m > 1)
@@ -900,9 +912,7 @@ extern "C" int rus_mx_gemm_workspace(int64_t m, int64_t n, int64_t k, int32_t x_
                                      int64_t* floats) {
   const char* fn = "rus_mx_gemm_workspace";
   if (!floats) return fail(RUS_ERR_INVALID, "%s: null result", fn);
-  if (m < 0 || n <= 0 || k <= 0 || m >= (1 << 30) || n >= (1 << 28) || k > (1 << 22))
-    return fail(RUS_ERR_INVALID, "%s: bad sizes m=%lld n=%lld k=%lld", fn, (long long)m, (long long)n,
-                (long long)k);
+  if (int e = check_plan(fn, m, n, k, x_fmt, w_fmt)) return e;
   const GemmPlan p = gemm_plan(m, n, mx_blocks(k), x_fmt, w_fmt, false);
   *floats = m > 0 && !few_tokens(m, n, mx_blocks(k)) && p.splits > 1 ? p.splits * m * n : 0;
   return RUS_OK;
@@ -920,12 +930,6 @@ RowsScratch rows_scratch(int64_t m, int64_t n, int64_t k, int32_t act, int32_t w
   if (few_tokens(m, n, nb)) return {0, 0, 0};
   const GemmPlan p = gemm_plan(m, n, nb, act, w_fmt, glu);
   return {m * nb * (act == RUS_MX_FP4 ? 16 : 32), (m * nb + 15) / 16 * 16, p.splits > 1 ? p.splits * m * n : 0};
-}
-int check_sizes(const char* fn, int64_t m, int64_t n, int64_t k) {
-  if (m < 0 || n <= 0 || k <= 0 || m >= (1 << 30) || n >= (1 << 28) || k > (1 << 22))
-    return fail(RUS_ERR_INVALID, "%s: bad sizes m=%lld n=%lld k=%lld", fn, (long long)m, (long long)n,
-                (long long)k);
-  return RUS_OK;
 }
 // The scratch's parts, or a refusal.
 int place(const char* fn, const RowsScratch& need, void* scratch, int64_t n_scratch, char*& codes, char*& scales,
@@ -986,8 +990,6 @@ int run_tokens(const char* fn, const void* x, int64_t ldx, int32_t act, const vo
                int32_t dtype, bool glu, void* stream) {
   MxArgs g;
   if (int e = prepare(fn, g, nullptr, nullptr, act, wc, ws, w_fmt, m, n, k, y, ldy, n, dtype, true)) return e;
-  if (act != RUS_MX_FP4 && act != RUS_MX_FP8)
-    return fail(RUS_ERR_INVALID, "%s: unknown activation format %d", fn, (int)act);
   if (ldx < k && m > 1) return fail(RUS_ERR_INVALID, "%s: stride_x=%lld smaller than a row", fn, (long long)ldx);
   if (!x || !aligned(x, 2)) return fail(RUS_ERR_INVALID, "%s: x is null or misaligned", fn);
   if (bias && !aligned(bias, 2)) return fail(RUS_ERR_INVALID, "%s: misaligned bias", fn);
@@ -1012,7 +1014,7 @@ extern "C" int rus_mx_rows_scratch(int64_t m, int64_t n, int64_t k, int32_t act,
                                    int64_t* bytes) {
   const char* fn = "rus_mx_rows_scratch";
   if (!bytes) return fail(RUS_ERR_INVALID, "%s: null result", fn);
-  if (int e = check_sizes(fn, m, n, k)) return e;
+  if (int e = check_plan(fn, m, n, k, act, w_fmt)) return e;
   *bytes = m > 0 ? rows_scratch(m, n, k, act, w_fmt, glu != 0).bytes() : 0;
   return RUS_OK;
 }
@@ -1024,6 +1026,7 @@ extern "C" int rus_mx_gemm_rows(const void* x, int64_t stride_x, int32_t act, co
   const char* fn = "rus_mx_gemm_rows";
   if (int e = check_sizes(fn, m, n, k)) return e;
   if (m == 0) return RUS_OK;
+  if (int e = check_plan(fn, m, n, k, act, w_fmt)) return e;
   if (few_tokens(m, n, mx_blocks(k)))
     return run_tokens(fn, x, stride_x, act, w_codes, w_scales, w_fmt, m, n, k, bias, y, stride_y, dtype, false,
                       stream);
@@ -1045,6 +1048,7 @@ extern "C" int rus_mx_glu_fwd_rows(const void* x, int64_t stride_x, int32_t act,
   const char* fn = "rus_mx_glu_fwd_rows";
   if (int e = check_sizes(fn, m, n, k)) return e;
   if (m == 0) return RUS_OK;
+  if (int e = check_plan(fn, m, n, k, act, w_fmt)) return e;
   if (few_tokens(m, n, mx_blocks(k)))
     return run_tokens(fn, x, stride_x, act, w_codes, w_scales, w_fmt, m, n, k, nullptr, h, stride_h, dtype, true,
                       stream);

@@ -3,10 +3,13 @@
 
 from __future__ import annotations
 
+import ctypes
+import threading
+
 import pytest
 import torch
 
-from rus_amd import kernels as K, ops
+from rus_amd import _lib, kernels as K, ops
 
 
 def _mx(rows, cols, fmt="fp4"):
@@ -75,3 +78,59 @@ def test_first_derivatives_under_create_graph(plain_kernels):
     z = ops.mx_mlp_glu(x, _mx(16, 64)).sum() + (x * x).sum()
     (dx,) = torch.autograd.grad(z, x, create_graph=True)
     assert torch.equal(dx, 2 * x)
+
+
+# ---- formats that do not exist -------------------------------------------------------------------
+
+F16, FP4, FP8 = 0, 0, 1
+
+
+def _query(name, *sizes):
+    got = ctypes.c_int64()
+    _lib.call(name, *sizes, ctypes.byref(got))
+    return got.value
+
+
+@pytest.mark.parametrize("x_fmt,w_fmt,which", [(2, FP4, "x"), (-1, FP8, "x"), (FP8, 2, "w"), (FP8, -2, "w"),
+                                               (FP4, 2, "w")])
+def test_size_queries_refuse_unknown_formats(x_fmt, w_fmt, which):
+    for call in (lambda: _query("rus_mx_gemm_workspace", 64, 2048, 8960, x_fmt, w_fmt),
+                 lambda: _query("rus_mx_rows_scratch", 64, 2048, 8960, x_fmt, w_fmt, 0),
+                 lambda: _query("rus_mx_rows_scratch", 64, 2048, 8960, x_fmt, w_fmt, 1)):
+        with pytest.raises(RuntimeError, match=f"{which} has unknown format"):
+            call()
+
+
+def test_a_refused_format_leaves_other_plans_alone():
+    """Sizes are planned once per thread and remembered: a thread whose first calls name formats that do not
+    exist sees the sizes that every thread sees."""
+    bad = [(x_fmt, w_fmt) for x_fmt in (-1, 0, 1, 2) for w_fmt in (-2, 0, 1, 2, 4) if not {x_fmt, w_fmt} <= {0, 1}]
+
+    def refused(m, n, k, x_fmt, w_fmt):
+        rows = (16, k, x_fmt, 16, 16, w_fmt, m, n, k)
+        return (lambda: _query("rus_mx_gemm_workspace", m, n, k, x_fmt, w_fmt),
+                lambda: _query("rus_mx_rows_scratch", m, n, k, x_fmt, w_fmt, 0),
+                # (no scratch: refused before anything is launched)
+                lambda: _lib.call("rus_mx_gemm_rows", *rows, None, 16, n, F16, None, 0, None),
+                lambda: _lib.call("rus_mx_glu_fwd_rows", *rows, 16, n, F16, None, 0, None))
+
+    def ask(before):
+        got = []
+        for size in [(64, 512, 20000), (64, 2048, 8960), (100, 4096, 4096)]:
+            for good in [(FP4, FP4), (FP8, FP4), (FP4, FP8), (FP8, FP8)]:
+                for i in range(4 * len(bad)):
+                    _query("rus_mx_gemm_workspace", *size, FP8 - good[0], good[1])  # (takes the other's place)
+                    if before:
+                        try:
+                            refused(*size, *bad[i // 4])[i % 4]()
+                        except RuntimeError:
+                            pass
+                    got.append(_query("rus_mx_gemm_workspace", *size, *good))
+        return got
+
+    got = []
+    for before in (False, True):
+        t = threading.Thread(target=lambda: got.append(ask(before)))
+        t.start()
+        t.join()
+    assert len(got) == 2 and got[0] == got[1]
