@@ -168,6 +168,20 @@ __device__ __forceinline__ void sum_parts(const float* __restrict__ p, int64_t s
 // Whether a sum of that many threads is of the first kind.
 inline bool deep_sum(int64_t threads, int64_t parts) { return threads <= 32768 && parts > 8; }
 
+// A dispatch counts its work-items in 32 bits.
+constexpr int64_t kMaxItems = int64_t(1) << 32;
+
+// launch(first, count) for slices of the rows that a dispatch holds: one, below 2^31 work-items.
+template <typename F>
+int by_rows(const char* fn, int64_t rows, int64_t threads_per_row, F launch) {
+  const int64_t most = (kMaxItems / 2 + threads_per_row - 1) / threads_per_row;
+  for (int64_t first = 0; first < rows; first += most) {
+    launch(first, rows - first < most ? rows - first : most);
+    if (int e = check_launch(fn)) return e;
+  }
+  return RUS_OK;
+}
+
 // A thread's last plans by the sizes they are for: finding one goes over all choices, a few us.
 template <typename Plan>
 class PlanMemo {

@@ -299,18 +299,18 @@ int quantize_rows(const char* fn, const void* x, int32_t dtype, int64_t n_rows, 
     if (int e = check_mx(fn, codes, scales, fmt, "output")) return e;
     if (!x || !aligned(x, sizeof(T))) return fail(RUS_ERR_INVALID, "%s: x is null or misaligned", fn);
     const int nb = static_cast<int>(mx_blocks(n_cols));
-    const int64_t total = n_rows * nb * 4;
-    const dim3 grid(static_cast<unsigned>((total + 255) / 256));
-    auto go = [&](auto k) {
-      hipLaunchKernelGGL(k, grid, dim3(256), 0, stream, static_cast<const T*>(x), stride_row,
-                         static_cast<int>(n_cols), nb, total, static_cast<uint8_t*>(codes),
-                         static_cast<uint8_t*>(scales));
+    auto go = [&](auto k, int64_t bytes) {
+      return by_rows(fn, n_rows, nb * 4, [&](int64_t first, int64_t rows) {
+        const int64_t total = rows * nb * 4;
+        hipLaunchKernelGGL(k, dim3(static_cast<unsigned>((total + 255) / 256)), dim3(256), 0, stream,
+                           static_cast<const T*>(x) + first * stride_row, stride_row,
+                           static_cast<int>(n_cols), nb, total,
+                           static_cast<uint8_t*>(codes) + first * nb * bytes,
+                           static_cast<uint8_t*>(scales) + first * nb);
+      });
     };
-    if (fmt == RUS_MX_FP4)
-      go(mx_quantize_kernel<T, kFp4>);
-    else
-      go(mx_quantize_kernel<T, kFp8>);
-    return check_launch(fn);
+    return fmt == RUS_MX_FP4 ? go(mx_quantize_kernel<T, kFp4>, kCodeBytes<kFp4>)
+                             : go(mx_quantize_kernel<T, kFp8>, kCodeBytes<kFp8>);
   });
 }
 
@@ -340,18 +340,18 @@ extern "C" int rus_mx_dequantize(const void* codes, const void* scales, int32_t 
       return fail(RUS_ERR_INVALID, "%s: out is null or misaligned", fn);
     const int nb = static_cast<int>(mx_blocks(n_cols));
     const int packs = static_cast<int>((n_cols + 7) / 8);
-    const int64_t total = n_rows * packs;
-    const dim3 grid(static_cast<unsigned>((total + 255) / 256));
-    auto go = [&](auto k) {
-      hipLaunchKernelGGL(k, grid, dim3(256), 0, static_cast<hipStream_t>(stream),
-                         static_cast<const uint8_t*>(codes), static_cast<const uint8_t*>(scales),
-                         static_cast<int>(n_cols), nb, packs, total, static_cast<T*>(out), stride_row);
+    auto go = [&](auto k, int64_t bytes) {
+      return by_rows(fn, n_rows, packs, [&](int64_t first, int64_t rows) {
+        const int64_t total = rows * packs;
+        hipLaunchKernelGGL(k, dim3(static_cast<unsigned>((total + 255) / 256)), dim3(256), 0,
+                           static_cast<hipStream_t>(stream),
+                           static_cast<const uint8_t*>(codes) + first * nb * bytes,
+                           static_cast<const uint8_t*>(scales) + first * nb, static_cast<int>(n_cols),
+                           nb, packs, total, static_cast<T*>(out) + first * stride_row, stride_row);
+      });
     };
-    if (fmt == RUS_MX_FP4)
-      go(mx_dequantize_kernel<T, kFp4>);
-    else
-      go(mx_dequantize_kernel<T, kFp8>);
-    return check_launch(fn);
+    return fmt == RUS_MX_FP4 ? go(mx_dequantize_kernel<T, kFp4>, kCodeBytes<kFp4>)
+                             : go(mx_dequantize_kernel<T, kFp8>, kCodeBytes<kFp8>);
   });
 }
 
@@ -389,18 +389,20 @@ extern "C" int rus_rmsnorm_mx_fwd(const void* x, const void* residual, const voi
         const int steps = (packs + 1023) / 1024;
         const int threads = ((packs + steps - 1) / steps + 63) / 64 * 64;
         auto go = [&](auto k) {
-          hipLaunchKernelGGL(k, dim3(static_cast<unsigned>(n_rows)), dim3(threads), 0,
-                             static_cast<hipStream_t>(stream), static_cast<const T*>(x),
-                             static_cast<const T*>(residual), static_cast<const W*>(weight),
-                             static_cast<T*>(sum_out), static_cast<uint8_t*>(codes),
-                             static_cast<uint8_t*>(scales), rstd, static_cast<int>(n_cols), nb,
-                             stride_row, eps, 1.0 / static_cast<double>(n_cols));
+          return by_rows(fn, n_rows, threads, [&](int64_t first, int64_t rows) {
+            const int64_t at = first * stride_row;
+            hipLaunchKernelGGL(k, dim3(static_cast<unsigned>(rows)), dim3(threads), 0,
+                               static_cast<hipStream_t>(stream), static_cast<const T*>(x) + at,
+                               residual ? static_cast<const T*>(residual) + at : nullptr,
+                               static_cast<const W*>(weight),
+                               sum_out ? static_cast<T*>(sum_out) + at : nullptr,
+                               static_cast<uint8_t*>(codes) + first * nb * kCodeBytes<kFp8>,
+                               static_cast<uint8_t*>(scales) + first * nb, rstd + first,
+                               static_cast<int>(n_cols), nb, stride_row, eps,
+                               1.0 / static_cast<double>(n_cols));
+          });
         };
-        if (residual)
-          go(rmsnorm_mx_kernel<T, W, true>);
-        else
-          go(rmsnorm_mx_kernel<T, W, false>);
-        return check_launch(fn);
+        return residual ? go(rmsnorm_mx_kernel<T, W, true>) : go(rmsnorm_mx_kernel<T, W, false>);
       }
     });
   });
