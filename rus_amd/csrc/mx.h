@@ -170,6 +170,11 @@ inline bool deep_sum(int64_t threads, int64_t parts) { return threads <= 32768 &
 
 // A dispatch counts its work-items in 32 bits.
 constexpr int64_t kMaxItems = int64_t(1) << 32;
+inline int check_items(const char* fn, int64_t workgroups, int64_t threads) {
+  if (workgroups * threads < kMaxItems) return RUS_OK;
+  return fail(RUS_ERR_UNSUPPORTED, "%s: %lld workgroups of %lld are beyond one dispatch", fn,
+              (long long)workgroups, (long long)threads);
+}
 
 // launch(first, count) for slices of the rows that a dispatch holds: one, below 2^31 work-items.
 template <typename F>

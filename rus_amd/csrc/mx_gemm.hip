@@ -787,6 +787,13 @@ GemmPlan gemm_plan(int64_t m, int64_t n, int64_t nb, int x_fmt, int w_fmt, bool 
                   [&] { return find_gemm_plan(m, n, nb, x_fmt, w_fmt, glu); });
 }
 
+// (The 32 x 32 kernel always fits: below 2^23 workgroups of 256 along the features.)
+int check_tiles(const char* fn, const GemmPlan& plan, int64_t m, int64_t n, bool glu) {
+  if (plan.bt == 32) return RUS_OK;
+  const int64_t nf = glu ? plan.bf / 2 : plan.bf;
+  return check_items(fn, ((n + nf - 1) / nf) * ((m + plan.bt - 1) / plan.bt) + 7, plan.bt == 256 ? 512 : 256);
+}
+
 template <int EPI, typename T, int FX, int FW>
 void launch(const MxArgs& g, const GemmPlan& plan, hipStream_t st) {
   constexpr int G = FX == kFp4 && FW == kFp4 ? 2 : 1;
@@ -818,9 +825,12 @@ void by_format(const MxArgs& g, const GemmPlan& plan, int32_t x_fmt, int32_t w_f
   return w_fmt == RUS_MX_FP4 ? launch<EPI, T, kFp4, kFp4>(g, plan, st) : launch<EPI, T, kFp4, kFp8>(g, plan, st);
 }
 
-template <int EPI>
-int dispatch(const char* fn, const MxArgs& g, int32_t x_fmt, int32_t w_fmt, int32_t dtype, hipStream_t st) {
+// The gated products; `first` runs once nothing is left to refuse.
+template <int EPI, typename F>
+int dispatch(const char* fn, const MxArgs& g, int32_t x_fmt, int32_t w_fmt, int32_t dtype, hipStream_t st, F first) {
   const GemmPlan plan = gemm_plan(g.m, g.n, g.nb, x_fmt, w_fmt, true);
+  if (int e = check_tiles(fn, plan, g.m, g.n, true)) return e;
+  if (int e = first()) return e;
   if (dtype == RUS_DTYPE_BF16)
     by_format<EPI, bf16>(g, plan, x_fmt, w_fmt, st);
   else
@@ -845,6 +855,7 @@ int product(const char* fn, MxArgs g, const GemmPlan& plan, int32_t x_fmt, int32
   g.vec = g.n % 4 == 0;
   g.y = parts;
   by_format<kParts, f16>(g, plan, x_fmt, w_fmt, st);
+  if (int e = check_launch(fn)) return e;
   const dim3 grid(static_cast<unsigned>((static_cast<int64_t>(g.m) * packs + 255) / 256));
   auto add = [&](auto k) {
     hipLaunchKernelGGL(k, grid, dim3(256), 0, st, parts, plan.splits, static_cast<int64_t>(g.m), packs, g.n, bias, y,
@@ -886,8 +897,6 @@ int prepare(const char* fn, MxArgs& g, const void* xc, const void* xs, int32_t x
     if (int e = check_mx(fn, xc, xs, x_fmt, "x")) return e;
   if (int e = check_mx(fn, wc, ws, w_fmt, "w")) return e;
   if (!y || !aligned(y, 2)) return fail(RUS_ERR_INVALID, "%s: output is null or misaligned", fn);
-  if (((m + 63) / 64) * ((n + 63) / 64) >= (int64_t(1) << 28))
-    return fail(RUS_ERR_UNSUPPORTED, "%s: m=%lld x n=%lld is beyond 2^28 tiles", fn, (long long)m, (long long)n);
   g = MxArgs{};
   g.xc = static_cast<const uint8_t*>(xc);
   g.xs = static_cast<const uint8_t*>(xs);
@@ -947,7 +956,7 @@ TokenArgs token_args(const MxArgs& g, int x_fmt, int64_t k, const void* bias) {
   return {nullptr, 0, g.xc, g.xs, g.wc, g.ws, x_fmt, g.m, g.n, static_cast<int>(k), g.nb, bias, g.y, g.ldy};
 }
 
-// rus_mx_gemm and rus_mx_glu_fwd; `first` runs once nothing is left to refuse.
+// rus_mx_gemm and rus_mx_glu_fwd.
 template <typename F>
 int run_gemm(const char* fn, const void* xc, const void* xs, int32_t x_fmt, const void* wc, const void* ws,
              int32_t w_fmt, int64_t m, int64_t n, int64_t k, const void* bias, void* y, int64_t ldy,
@@ -960,6 +969,7 @@ int run_gemm(const char* fn, const void* xc, const void* xs, int32_t x_fmt, cons
   if (few_tokens(m, n, g.nb))
     return token_product(fn, token_args(g, x_fmt, k, bias), w_fmt, false, dtype == RUS_DTYPE_BF16, st);
   const GemmPlan plan = gemm_plan(m, n, g.nb, x_fmt, w_fmt, false);
+  if (int e = check_tiles(fn, plan, m, n, false)) return e;
   if (plan.splits > 1 && (n_workspace < plan.splits * m * n || !workspace || !aligned(workspace, 16)))
     return fail(RUS_ERR_INVALID, "%s: workspace holds %lld floats (16-byte aligned), needs %lld", fn,
                 (long long)n_workspace, (long long)(plan.splits * m * n));
@@ -980,8 +990,7 @@ int run_glu(const char* fn, const void* xc, const void* xs, int32_t x_fmt, const
   const hipStream_t st = static_cast<hipStream_t>(stream);
   if (few_tokens(m, n, g.nb))
     return token_product(fn, token_args(g, x_fmt, k, nullptr), w_fmt, true, dtype == RUS_DTYPE_BF16, st);
-  if (int e = first()) return e;
-  return dispatch<kGluFwd>(fn, g, x_fmt, w_fmt, dtype, st);
+  return dispatch<kGluFwd>(fn, g, x_fmt, w_fmt, dtype, st, first);
 }
 
 // A few tokens that are rounded to blocks inside the product.
@@ -1085,5 +1094,5 @@ extern "C" int rus_mx_glu_bwd(const void* dh, int64_t stride_dh, const void* x_c
   g.dh = dh;
   g.ld_dh = stride_dh;
   g.vec = g.vec && aligned(dh, 16) && stride_dh % 8 == 0;
-  return dispatch<kGluBwd>(fn, g, x_fmt, w_fmt, dtype, static_cast<hipStream_t>(stream));
+  return dispatch<kGluBwd>(fn, g, x_fmt, w_fmt, dtype, static_cast<hipStream_t>(stream), [] { return RUS_OK; });
 }

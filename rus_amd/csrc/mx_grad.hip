@@ -409,9 +409,7 @@ extern "C" int rus_mx_gemm_t(const void* dy, int64_t stride_dy, int32_t dtype, c
   g.k = static_cast<int>(k);
   g.nb = static_cast<int>(mx_blocks(k));
   const int64_t tiles = ((m + plan.tm - 1) / plan.tm) * ((k + kGradN - 1) / kGradN);
-  if (tiles * plan.splits >= (int64_t(1) << 30))
-    return fail(RUS_ERR_UNSUPPORTED, "%s: m=%lld x k=%lld is beyond 2^30 tiles", fn, (long long)m,
-                (long long)k);
+  if (int e = check_items(fn, tiles * plan.splits + 7, kGradThreads)) return e;
   g.tiles_m = static_cast<int>((m + plan.tm - 1) / plan.tm);
   g.tiles_k = static_cast<int>((k + kGradN - 1) / kGradN);
   g.splits = plan.splits;
@@ -435,13 +433,14 @@ extern "C" int rus_mx_gemm_t(const void* dy, int64_t stride_dy, int32_t dtype, c
         return go(mx_grad_kernel<T, F, 32>);
     }
   };
-  auto types = [&](auto t) {
+  auto types = [&](auto t) -> int {
     typedef decltype(t) T;
     if (w_fmt == RUS_MX_FP4)
       tile(t, std::integral_constant<int, kFp4>{});
     else
       tile(t, std::integral_constant<int, kFp8>{});
-    if (!split) return;
+    if (!split) return RUS_OK;
+    if (int e = check_launch(fn)) return e;
     const bool wide = k % 4 == 0 && stride_dx % 4 == 0 && aligned(dx, 8);
     const int packs = static_cast<int>(wide ? k / 4 : k);
     const dim3 sum(static_cast<unsigned>((m * packs + 255) / 256));
@@ -453,10 +452,8 @@ extern "C" int rus_mx_gemm_t(const void* dy, int64_t stride_dy, int32_t dtype, c
       wide ? add(mx_grad_sum_kernel<T, 4, true>) : add(mx_grad_sum_kernel<T, 1, true>);
     else
       wide ? add(mx_grad_sum_kernel<T, 4, false>) : add(mx_grad_sum_kernel<T, 1, false>);
+    return RUS_OK;
   };
-  if (dtype == RUS_DTYPE_F16)
-    types(f16{});
-  else
-    types(bf16{});
+  if (int e = dtype == RUS_DTYPE_F16 ? types(f16{}) : types(bf16{})) return e;
   return check_launch(fn);
 }

@@ -180,10 +180,11 @@ __global__ __launch_bounds__(512) void mx_token_kernel(TokenArgs g) {
 // Eight waves where the contraction is long or workgroups are few, four else (each workgroup rounds x for
 // itself). One token, W from memory: 1,536 x 8,960 fp4 10.4, 7.4 and 5.5 us with 2, 4 and 8 waves, 2 x
 // 8,960 x 1,536 with the gate 6.9, 6.2 and 8.7; four tokens x 2,048 x 1,536 7.2, 5.6 and 4.7.
+int token_waves(int64_t n, int64_t nb) { return (nb + 7) / 8 > 16 || n <= 4096 ? 8 : 4; }
+
 template <int FW, int EPI, typename T>
 void launch(const TokenArgs& g, hipStream_t st) {
-  const int chunks = (g.nb + 7) / 8;
-  const int waves = chunks > 16 || g.n <= 4096 ? 8 : 4;
+  const int waves = token_waves(g.n, g.nb);
   const size_t lds = static_cast<size_t>(g.m) * g.nb * (kPitch + 4);
   auto go = [&](auto k) {
     hipLaunchKernelGGL(k, dim3((g.n + 7) / 8), dim3(waves * kWave), lds, st, g);
@@ -212,7 +213,8 @@ void by_weight(const TokenArgs& g, int w_fmt, hipStream_t st) {
 // and 8.8, two 9.4 and 8.9 (one launch less for the host), four 13.5 and 10.8; with the gate, 2 x 8,960 x
 // 1,536, one 6.2 and 10.9, two 9.1 and 10.7, four 12.3 and 11.0.
 bool few_tokens(int64_t m, int64_t n, int64_t nb) {
-  return m <= (n <= 4096 ? 4 : 2) && m * nb * (kPitch + 4) <= 61440;
+  return m <= (n <= 4096 ? 4 : 2) && m * nb * (kPitch + 4) <= 61440 &&
+         (n + 7) / 8 * token_waves(n, nb) * kWave < kMaxItems;  // (else the 32 x 32 kernel)
 }
 
 int token_product(const char* fn, const TokenArgs& g, int w_fmt, bool glu, bool bf, hipStream_t st) {

@@ -91,3 +91,32 @@ def test_norm_more_rows_than_a_dispatch(residual):
         p, ph, pr = K.rms_norm_mx_fwd(x[a:b], w, residual=None if res is None else res[a:b])
         assert torch.equal(q.codes[a:b], p.codes) and torch.equal(q.scales[a:b], p.scales), (a, b)
         assert torch.equal(h[a:b], ph) and torch.equal(rstd[a:b], pr), (a, b)
+
+
+@pytest.mark.parametrize("glu", [False, True])
+def test_few_tokens_with_more_features_than_a_dispatch(glu):
+    """The few-token kernel takes 32 threads a feature here: from 2^27 features on another one has to."""
+    n, k = (1 << 27) + 40, 32
+    rows = 2 * n if glu else n
+    g = torch.Generator(device=DEV).manual_seed(4)
+    codes = torch.zeros(rows, 64, device=DEV, dtype=torch.uint8)
+    codes[:, :16] = torch.randint(0, 256, (rows, 16), generator=g, device=DEV, dtype=torch.uint8)
+    scales = torch.zeros(rows, 4, device=DEV, dtype=torch.uint8)
+    scales[:, 0] = 125
+    w = K.MXTensor(codes, scales, (rows, k), "fp4")
+    x = torch.randint(-3, 4, (1, k), generator=g, device=DEV).to(BF16)
+    got = K.mx_mlp_glu_fwd(x, w) if glu else K.mx_gemm(x, w)
+    step = 1 << 23
+    for a in range(0, n, step):
+        b = min(a + step, n)
+        part = [K.mx_dequantize(K.MXTensor(codes[o + a: o + b], scales[o + a: o + b], (b - a, k), "fp4"), F32)
+                for o in ((0, n) if glu else (0,))]
+        y = [torch.matmul(p, x[0].float()) for p in part]  # multiples of 1/8 below 2^8: exact
+        if not glu:
+            assert torch.equal(got[0, a:b], y[0].to(BF16)), a
+            continue
+        gate, up = y[0].double(), y[1].double()
+        want = gate / (1 + torch.exp(-gate)) * up
+        # the sigmoid's error in units of 2^-23 and the result's rounding
+        tol = ((10 + gate.abs()) * 2.0**-23 + 2.0**-8) * want.abs() + 2.0**-130
+        assert ((got[0, a:b].double() - want).abs() <= tol).all(), a

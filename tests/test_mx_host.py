@@ -134,3 +134,20 @@ def test_a_refused_format_leaves_other_plans_alone():
         t.start()
         t.join()
     assert len(got) == 2 and got[0] == got[1]
+
+
+# ---- results that one dispatch cannot hold -------------------------------------------------------
+
+
+@pytest.mark.parametrize("name,args", [
+    ("rus_mx_gemm", (16, 16, FP8, 16, 16, FP8, 1 << 19, 1 << 20, 64, None, 16, 1 << 20, F16, None, 0, None)),
+    ("rus_mx_gemm_rows", (16, 64, FP8, 16, 16, FP8, 1 << 19, 1 << 20, 64, None, 16, 1 << 20, F16, 16, 1 << 60, None)),
+    ("rus_mx_glu_fwd", (16, 16, FP8, 16, 16, FP8, 1 << 19, 1 << 19, 64, 16, 1 << 19, F16, None)),
+    ("rus_mx_glu_fwd_rows", (16, 64, FP8, 16, 16, FP8, 1 << 19, 1 << 19, 64, 16, 1 << 19, F16, 16, 1 << 60, None)),
+    ("rus_mx_glu_bwd", (16, 1 << 19, 16, 16, FP8, 16, 16, FP8, 1 << 19, 1 << 19, 64, 16, 1 << 20, F16, None)),
+    ("rus_mx_gemm_t", (16, 64, F16, 16, 16, FP4, 1 << 20, 64, 1 << 20, 16, 1 << 20, None, 0, None)),
+])
+def test_results_beyond_a_dispatch_are_refused(name, args):
+    """2^39 values, a terabyte: refused by name, with nothing launched."""
+    with pytest.raises(RuntimeError, match=f"{name}: .* beyond one dispatch"):
+        _lib.call(name, *args)
