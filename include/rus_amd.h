@@ -23,7 +23,7 @@
 extern "C" {
 #endif
 
-#define RUS_ABI_VERSION 20
+#define RUS_ABI_VERSION 21
 
 #define RUS_DTYPE_F16 0
 #define RUS_DTYPE_F32 1
@@ -867,6 +867,14 @@ int rus_mx_gemm(const void* x_codes, const void* x_scales, int32_t x_fmt, const 
                 int64_t n_workspace, void* stream);
 
 /*
+ * Diagnostic: how a product of these sizes would run. glu: 1 rus_mx_glu_fwd, 2 _bwd, 0 neither.
+ * plan[0] x plan[1]: rows of W x tokens of a workgroup's tile (8 x m: the few-token kernel), plan[2]: parts
+ * of the contraction.
+ */
+int rus_mx_gemm_plan(int64_t m, int64_t n, int64_t k, int32_t x_fmt, int32_t w_fmt, int32_t glu,
+                     int32_t* plan);
+
+/*
  * rus_mx_gemm of activations that are not in blocks yet: x [m, k] in T, quantised to `act` first
  * (rus_mx_quantize; the same bits), a few tokens inside the product's own launch. scratch: the bytes
  * rus_mx_rows_scratch names (glu = 0; 0: none; 16-byte aligned), not shared by calls that overlap.
@@ -889,6 +897,9 @@ int rus_mx_gemm_t_workspace(int64_t m, int64_t n, int64_t k, int64_t* floats);
 int rus_mx_gemm_t(const void* dy, int64_t stride_dy, int32_t dtype, const void* w_codes,
                   const void* w_scales, int32_t w_fmt, int64_t m, int64_t n, int64_t k, void* dx,
                   int64_t stride_dx, float* workspace, int64_t n_workspace, void* stream);
+
+/* Diagnostic: how rus_mx_gemm_t would run. plan[0]: tokens of a tile, plan[1]: parts of the contraction. */
+int rus_mx_gemm_t_plan(int64_t m, int64_t n, int64_t k, int32_t* plan);
 
 /*
  * Gated feed-forward, first half, in one kernel: G = X W[0:n]^T, U = X W[n:2n]^T (W [2n, k]: gate

@@ -11,7 +11,7 @@ import threading
 from pathlib import Path
 
 LIB_PATH = Path(__file__).resolve().parent / "librus_amd.so"
-ABI_VERSION = 20
+ABI_VERSION = 21
 
 DTYPE_F16 = 0
 DTYPE_F32 = 1
@@ -155,6 +155,8 @@ SIGNATURES: dict[str, list] = {
     "rus_rmsnorm_mx_fwd": [_vp, _vp, _vp, _i32, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _f32, _i32,
                            _vp],
     "rus_mx_gemm_workspace": [_i64, _i64, _i64, _i32, _i32, ctypes.POINTER(_i64)],
+    "rus_mx_gemm_plan": [_i64, _i64, _i64, _i32, _i32, _i32, ctypes.POINTER(_i32)],
+    "rus_mx_gemm_t_plan": [_i64, _i64, _i64, ctypes.POINTER(_i32)],
     "rus_mx_gemm": [_vp, _vp, _i32, _vp, _vp, _i32, _i64, _i64, _i64, _vp, _vp, _i64, _i32, _vp,
                     _i64, _vp],
     "rus_mx_gemm_t_workspace": [_i64, _i64, _i64, ctypes.POINTER(_i64)],

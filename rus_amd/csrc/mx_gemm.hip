@@ -927,6 +927,20 @@ extern "C" int rus_mx_gemm_workspace(int64_t m, int64_t n, int64_t k, int32_t x_
   return RUS_OK;
 }
 
+extern "C" int rus_mx_gemm_plan(int64_t m, int64_t n, int64_t k, int32_t x_fmt, int32_t w_fmt, int32_t glu,
+                                int32_t* plan) {
+  const char* fn = "rus_mx_gemm_plan";
+  if (!plan) return fail(RUS_ERR_INVALID, "%s: null result", fn);
+  if (int e = check_plan(fn, m, n, k, x_fmt, w_fmt)) return e;
+  const int64_t nb = mx_blocks(k);
+  const bool few = glu != 2 && few_tokens(m, n, nb);
+  const GemmPlan p = gemm_plan(m, n, nb, x_fmt, w_fmt, glu != 0);
+  plan[0] = few ? 8 : p.bf;
+  plan[1] = few ? static_cast<int32_t>(m) : p.bt;
+  plan[2] = few ? 1 : p.splits;
+  return RUS_OK;
+}
+
 // Scratch of a call that quantises its activations: codes, scales, sums, each 16-byte aligned.
 namespace rus {
 namespace {

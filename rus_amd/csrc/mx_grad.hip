@@ -361,6 +361,13 @@ GradPlan grad_plan(int64_t m, int64_t n, int64_t k) {
   return memo.get({m, n, k, 0}, [&] { return find_grad_plan(m, n, k); });
 }
 
+int check_sizes(const char* fn, int64_t m, int64_t n, int64_t k) {
+  if (m < 0 || n <= 0 || k <= 0 || m >= (1 << 30) || n >= (1 << 28) || k > (1 << 28))
+    return fail(RUS_ERR_INVALID, "%s: bad sizes m=%lld n=%lld k=%lld", fn, (long long)m,
+                (long long)n, (long long)k);
+  return RUS_OK;
+}
+
 }  // namespace
 }  // namespace rus
 
@@ -369,11 +376,19 @@ using namespace rus;
 extern "C" int rus_mx_gemm_t_workspace(int64_t m, int64_t n, int64_t k, int64_t* floats) {
   const char* fn = "rus_mx_gemm_t_workspace";
   if (!floats) return fail(RUS_ERR_INVALID, "%s: null result", fn);
-  if (m < 0 || n <= 0 || k <= 0 || m >= (1 << 30) || n >= (1 << 28) || k > (1 << 28))
-    return fail(RUS_ERR_INVALID, "%s: bad sizes m=%lld n=%lld k=%lld", fn, (long long)m,
-                (long long)n, (long long)k);
+  if (int e = check_sizes(fn, m, n, k)) return e;
   const GradPlan p = grad_plan(m, n, k);
   *floats = p.splits > 1 ? p.splits * m * k : 0;
+  return RUS_OK;
+}
+
+extern "C" int rus_mx_gemm_t_plan(int64_t m, int64_t n, int64_t k, int32_t* plan) {
+  const char* fn = "rus_mx_gemm_t_plan";
+  if (!plan) return fail(RUS_ERR_INVALID, "%s: null result", fn);
+  if (int e = check_sizes(fn, m, n, k)) return e;
+  const GradPlan p = grad_plan(m, n, k);
+  plan[0] = p.tm;
+  plan[1] = p.splits;
   return RUS_OK;
 }
 
@@ -382,9 +397,7 @@ extern "C" int rus_mx_gemm_t(const void* dy, int64_t stride_dy, int32_t dtype, c
                              void* dx, int64_t stride_dx, float* workspace, int64_t n_workspace,
                              void* stream) {
   const char* fn = "rus_mx_gemm_t";
-  if (m < 0 || n <= 0 || k <= 0 || m >= (1 << 30) || n >= (1 << 28) || k > (1 << 28))
-    return fail(RUS_ERR_INVALID, "%s: bad sizes m=%lld n=%lld k=%lld", fn, (long long)m,
-                (long long)n, (long long)k);
+  if (int e = check_sizes(fn, m, n, k)) return e;
   if (dtype != RUS_DTYPE_F16 && dtype != RUS_DTYPE_BF16)
     return fail(RUS_ERR_UNSUPPORTED, "%s: gradients are fp16 or bf16, not dtype %d", fn, (int)dtype);
   if ((stride_dy < n || stride_dx < k) && m > 1)

@@ -4,10 +4,13 @@ dropped, doubled or scaled by a neighbour's scale."""
 
 from __future__ import annotations
 
+import ctypes
+
 import pytest
 import torch
 
-from rus_amd import kernels as K, ops
+from rus_amd import _lib, kernels as K, ops
+from test_gpu_mx_sizes import FORMATS, bits, exact
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -120,3 +123,114 @@ def test_few_tokens_with_more_features_than_a_dispatch(glu):
         # the sigmoid's error in units of 2^-23 and the result's rounding
         tol = ((10 + gate.abs()) * 2.0**-23 + 2.0**-8) * want.abs() + 2.0**-130
         assert ((got[0, a:b].double() - want).abs() <= tol).all(), a
+
+
+# ---- every tile over many stages -----------------------------------------------------------------
+#
+# Sizes that the plan sends to the named tile (asserted: a change of its costs may not leave one untested),
+# ragged in tokens and features, contractions of even and odd numbers of 128s, past two quads of scales.
+
+
+def plan(m, n, k, fx, fw, glu=0):
+    got = (ctypes.c_int32 * 3)()
+    _lib.call("rus_mx_gemm_plan", m, n, k, _lib.MX_FP8 if fx == "fp8" else _lib.MX_FP4,
+              _lib.MX_FP8 if fw == "fp8" else _lib.MX_FP4, glu, got)
+    return got[0], got[1], got[2] > 1
+
+
+PLAIN = [  # rows of W x tokens of a tile, whether the contraction is split, formats, sizes
+    (256, 128, False, "fp8", "fp4", 1100, 9000, 1200), (256, 128, False, "fp8", "fp4", 2100, 9001, 1100),
+    (256, 128, False, "fp8", "fp4", 521, 7285, 660), (256, 128, False, "fp8", "fp4", 1993, 2058, 633),
+    (256, 128, True, "fp8", "fp4", 38, 12346, 13154), (256, 128, True, "fp8", "fp4", 8, 12303, 6120),
+    (256, 256, False, "fp4", "fp4", 2100, 4500, 1536), (256, 256, False, "fp4", "fp4", 1100, 9000, 1200),
+    (256, 256, False, "fp4", "fp4", 1211, 7069, 637), (256, 256, False, "fp4", "fp4", 666, 11028, 2100),
+    (256, 256, True, "fp4", "fp4", 270, 14218, 9674), (256, 256, True, "fp4", "fp4", 386, 8337, 9226),
+]
+for _fx, _fw in FORMATS:
+    PLAIN += [(128, 128, False, _fx, _fw, 4420, 398, 691), (128, 128, False, _fx, _fw, 195, 9917, 633),
+              (128, 128, True, _fx, _fw, 3664, 33, 5689), (128, 128, True, _fx, _fw, 3359, 32, 5794),
+              (128, 64, False, _fx, _fw, 1345, 120, 1240), (128, 64, False, _fx, _fw, 777, 240, 1074),
+              (128, 64, False, _fx, _fw, 707, 2048, 1536),
+              (128, 64, True, _fx, _fw, 9, 3449, 6585), (128, 64, True, _fx, _fw, 8, 2061, 12304)]
+
+
+@pytest.mark.parametrize("bf,bt,split,fx,fw,m,n,k", PLAIN)
+def test_product_in_each_tile(bf, bt, split, fx, fw, m, n, k):
+    assert plan(m, n, k, fx, fw) == (bf, bt, split)
+    w, wb = exact(n, k, fw, n + 1)
+    x, xb = exact(m, k, fx, m + 1)
+    want = x @ w.T
+    assert float(want.abs().max()) < 2.0**15
+    bits(K.mx_gemm(xb, wb, dtype=BF16), want)
+    bias = torch.arange(n, device=DEV).remainder(7) - 3.0
+    bits(K.mx_gemm(xb, wb, bias=bias.to(F16)), want + bias.double())
+    odd = torch.full((m, n + 3), 7.0, dtype=F16, device=DEV)  # rows at any alignment, neighbours left alone
+    K.mx_gemm(xb, wb, out=odd[:, 1: n + 1])
+    bits(odd[:, 1: n + 1], want)
+    odd[:, 1: n + 1] = 7.0
+    assert (odd == 7.0).all()
+
+
+GATED = [(256, 128, "fp8", "fp4", 2100, 4501, 1100), (256, 128, "fp8", "fp4", 1290, 5001, 1100),
+         (256, 128, "fp8", "fp4", 707, 8960, 1536), (256, 128, "fp8", "fp4", 332, 5657, 645),
+         (256, 256, "fp4", "fp4", 1290, 5001, 1100), (256, 256, "fp4", "fp4", 707, 8960, 1536),
+         (256, 256, "fp4", "fp4", 302, 13408, 650), (128, 128, "fp4", "fp4", 2100, 4501, 1100),
+         (128, 128, "fp8", "fp8", 2100, 2301, 1100), (128, 128, "fp4", "fp8", 1290, 1157, 1200),
+         (128, 64, "fp8", "fp4", 687, 304, 959), (128, 64, "fp8", "fp8", 3245, 34, 1817),
+         (128, 64, "fp4", "fp4", 596, 77, 4364), (128, 64, "fp4", "fp8", 23, 9081, 958)]
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("bf,bt,fx,fw,m,n,k", GATED)
+def test_gated_in_each_tile(bf, bt, fx, fw, m, n, k, dtype):
+    assert plan(m, n, k, fx, fw, 1) == plan(m, n, k, fx, fw, 2) == (bf, bt, False)
+    w, wb = exact(2 * n, k, fw, n, low=119)  # so that g and u stay near one
+    x, xb = exact(m, k, fx, m)
+    y = x @ w.T
+    g, u = y[:, :n], y[:, n:]
+    s = 1 / (1 + torch.exp(-g))
+    half, least = (2.0**-11, 2.0**-25) if dtype == F16 else (2.0**-8, 2.0**-134)
+    tol = (20 + 2 * g.abs()) * 2.0**-23  # the sigmoid's exponential and reciprocal, four products
+
+    def near(got, want, err):
+        return bool(((got.double() - want).abs() <= err + half * (want.abs() + err) + least).all())
+
+    want = g * s * u
+    assert near(K.mx_mlp_glu_fwd(xb, wb, dtype=dtype), want, tol * want.abs())
+    dh = (torch.arange(m * n, device=DEV).remainder(11) - 5.0).view(m, n).to(dtype)
+    d = dh.double()
+    got = K.mx_mlp_glu_bwd(dh, xb, wb)
+    # the two terms of silu' may cancel: each has its own rounding
+    assert near(got[:, :n], d * u * (s + g * s * (1 - s)), tol * (d * u).abs() * (s + g.abs() * s))
+    assert near(got[:, n:], d * g * s, tol * (d * g * s).abs())
+    wide = torch.full((m, 3 * n + 3), 7.0, dtype=dtype, device=DEV)  # dh and the result in one odd matrix
+    wide[:, 1: n + 1] = dh
+    K.mx_mlp_glu_bwd(wide[:, 1: n + 1], xb, wb, out=wide[:, n + 2: 3 * n + 2])
+    assert torch.equal(wide[:, n + 2: 3 * n + 2], got) and torch.equal(wide[:, 1: n + 1], dh)
+    assert (wide[:, [0, n + 1, 3 * n + 2]] == 7.0).all()
+
+
+GRADIENT = [(256, True, 2100, 5000, 1537), (256, False, 4100, 700, 2310), (256, True, 132, 2790, 10810),
+            (256, False, 772, 259, 9627), (128, True, 137, 4114, 1799), (128, False, 399, 267, 9259),
+            (64, True, 37, 2823, 5470), (64, False, 1763, 258, 1042), (32, True, 8, 3175, 4885),
+            (32, False, 86, 383, 1864)]
+
+
+@pytest.mark.parametrize("fw", ["fp4", "fp8"])
+@pytest.mark.parametrize("tm,split,m,n,k", GRADIENT)
+def test_gradient_in_each_tile(tm, split, m, n, k, fw):
+    got = (ctypes.c_int32 * 2)()
+    _lib.call("rus_mx_gemm_t_plan", m, n, k, got)
+    assert (got[0], got[1] > 1) == (tm, split)
+    w, wb = exact(n, k, fw, 1)
+    g = torch.Generator(device=DEV).manual_seed(m)
+    dy = torch.randint(-3, 4, (m, n), generator=g, device=DEV).double()
+    want = dy @ w
+    for dtype in (F16, BF16):
+        bits(K.mx_gemm(dy.to(dtype), wb, trans=True), want)
+        wide = torch.full((m, n + 2), float("nan"), dtype=dtype, device=DEV)  # rows at any alignment
+        wide[:, 1: n + 1] = dy.to(dtype)
+        out = torch.full((m, k + 2), 7.0, dtype=dtype, device=DEV)
+        K.mx_gemm(wide[:, 1: n + 1], wb, trans=True, out=out[:, 1: k + 1])
+        bits(out[:, 1: k + 1], want)
+        assert (out[:, [0, k + 1]] == 7.0).all()

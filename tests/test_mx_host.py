@@ -151,3 +151,35 @@ def test_results_beyond_a_dispatch_are_refused(name, args):
     """2^39 values, a terabyte: refused by name, with nothing launched."""
     with pytest.raises(RuntimeError, match=f"{name}: .* beyond one dispatch"):
         _lib.call(name, *args)
+
+
+# ---- the plans -----------------------------------------------------------------------------------
+
+
+def test_plans_agree_with_the_sizes_they_need():
+    p, t = (ctypes.c_int32 * 3)(), (ctypes.c_int32 * 2)()
+    for m, n, k in [(1, 1536, 8960), (3, 2048, 1536), (8, 1536, 8960), (33, 2051, 4096), (707, 2048, 1536),
+                    (270, 14218, 9674), (2100, 9001, 1100), (4100, 700, 2310)]:
+        for x_fmt in (FP4, FP8):
+            for w_fmt in (FP4, FP8):
+                _lib.call("rus_mx_gemm_plan", m, n, k, x_fmt, w_fmt, 0, p)
+                assert _query("rus_mx_gemm_workspace", m, n, k, x_fmt, w_fmt) == (p[2] * m * n if p[2] > 1 else 0)
+                scratch = _query("rus_mx_rows_scratch", m, n, k, x_fmt, w_fmt, 0)
+                assert (scratch == 0) == ((p[0], p[1]) == (8, m))  # few tokens: a feature's row to 8 lanes
+                _lib.call("rus_mx_gemm_plan", m, n, k, x_fmt, w_fmt, 2, p)
+                assert p[0] >= 32 and p[2] == 1
+        _lib.call("rus_mx_gemm_t_plan", m, n, k, t)
+        assert _query("rus_mx_gemm_t_workspace", m, n, k) == (t[1] * m * k if t[1] > 1 else 0)
+
+
+@pytest.mark.parametrize("name,args,msg", [
+    ("rus_mx_gemm_plan", (4, 64, 64, FP8, FP4, 0, None), "null result"),
+    ("rus_mx_gemm_plan", (4, 0, 64, FP8, FP4, 0, (ctypes.c_int32 * 3)()), "bad sizes"),
+    ("rus_mx_gemm_plan", (4, 64, 64, 2, FP4, 0, (ctypes.c_int32 * 3)()), "x has unknown format"),
+    ("rus_mx_gemm_plan", (4, 64, 64, FP8, -1, 0, (ctypes.c_int32 * 3)()), "w has unknown format"),
+    ("rus_mx_gemm_t_plan", (4, 64, 64, None), "null result"),
+    ("rus_mx_gemm_t_plan", (4, 64, 0, (ctypes.c_int32 * 2)()), "bad sizes"),
+])
+def test_plan_queries_refuse(name, args, msg):
+    with pytest.raises(RuntimeError, match=msg):
+        _lib.call(name, *args)
