@@ -234,3 +234,129 @@ def test_gradient_in_each_tile(tm, split, m, n, k, fw):
         K.mx_gemm(wide[:, 1: n + 1], wb, trans=True, out=out[:, 1: k + 1])
         bits(out[:, 1: k + 1], want)
         assert (out[:, [0, k + 1]] == 7.0).all()
+
+
+# ---- blocks that are not finite, in each tile ----------------------------------------------------
+
+SPECIAL = [(256, 128, False, "fp8", "fp4", 1993, 2058, 633), (256, 256, False, "fp4", "fp4", 2100, 4500, 1100),
+           (128, 128, False, "fp8", "fp8", 2100, 2301, 1100), (128, 128, False, "fp4", "fp8", 2100, 2301, 1100),
+           (128, 64, False, "fp8", "fp4", 707, 2048, 1536), (128, 64, False, "fp4", "fp4", 777, 240, 1074),
+           (32, 32, False, "fp8", "fp4", 40, 700, 640), (128, 64, True, "fp8", "fp8", 9, 3449, 6585),
+           (256, 128, True, "fp8", "fp4", 38, 12346, 13154), (256, 256, True, "fp4", "fp4", 270, 14218, 9674)]
+
+
+def not_finite(m, n, k):
+    """x [m, k] and w [n, k] of ones with single infinities and NaNs, and the results they reach: the rows of x
+    and of w that hold one. A row of zeros in x is no shield: 0 NaN is NaN."""
+    x, w = torch.ones(m, k, device=DEV), torch.ones(n, k, device=DEV)
+    x[2] = 0.0
+    bad_x, bad_w = [1, m // 2, m - 2], [0, n // 3, n - 1]
+    for row, col, v in zip(bad_x, (k - 1, k // 2, 0), ("nan", "inf", "-inf")):
+        x[row, col] = float(v)
+    for row, col, v in zip(bad_w, (0, k - 1, k // 2), ("-inf", "nan", "inf")):
+        w[row, col] = float(v)
+    bad = torch.zeros(m, n, dtype=torch.bool, device=DEV)
+    bad[bad_x], bad[:, bad_w] = True, True
+    return x, w, bad
+
+
+@pytest.mark.parametrize("bf,bt,split,fx,fw,m,n,k", SPECIAL)
+def test_product_of_blocks_that_are_not_finite(bf, bt, split, fx, fw, m, n, k):
+    assert plan(m, n, k, fx, fw) == (bf, bt, split)
+    x, w, bad = not_finite(m, n, k)
+    y = K.mx_gemm(K.mx_quantize(x, fx), K.mx_quantize(w, fw), dtype=F16)
+    want = torch.full((m, n), float(k), dtype=F16, device=DEV)
+    want[2] = 0.0
+    assert torch.equal(torch.isnan(y), bad) and torch.equal(y[~bad], want[~bad])
+
+
+@pytest.mark.parametrize("bf,bt,fx,fw,m,n,k", [
+    (256, 128, "fp8", "fp4", 1290, 5001, 1100), (256, 256, "fp4", "fp4", 1290, 5001, 1100),
+    (128, 128, "fp8", "fp8", 2100, 2301, 1100), (128, 64, "fp8", "fp4", 687, 304, 959),
+    (32, 32, "fp8", "fp4", 40, 70, 640)])
+def test_gated_blocks_that_are_not_finite(bf, bt, fx, fw, m, n, k):
+    """A NaN in a gate's or an up row reaches that feature; in x, its token; in dh, its one result of each."""
+    assert plan(m, n, k, fx, fw, 1) == plan(m, n, k, fx, fw, 2) == (bf, bt, False)
+    x, w, both = not_finite(m, 2 * n, k)
+    bad = both[:, :n] | both[:, n:]
+    xb, wb = K.mx_quantize(x, fx), K.mx_quantize(w * 2.0**-9, fw)
+    clean = K.mx_mlp_glu_fwd(K.mx_quantize(torch.ones(3, k, device=DEV), fx),
+                             K.mx_quantize(torch.full((64, k), 2.0**-9, device=DEV), fw), dtype=F16)[0, 0]
+    h = K.mx_mlp_glu_fwd(xb, wb, dtype=F16)
+    want = clean.expand(m, n).clone()
+    want[2] = 0.0
+    assert torch.equal(torch.isnan(h), bad)
+    # (another kernel, the same exact projections: a step of fp16 at most)
+    assert ((h - want)[~bad].abs() <= 2.0**-10 * clean).all()
+    dh = torch.ones(m, n, dtype=F16, device=DEV)
+    dh[m - 1, 3], dh[0, 5] = float("nan"), float("inf")
+    d = K.mx_mlp_glu_bwd(dh, xb, wb)
+    # d_up = dh silu(g) needs the gate only, d_gate = dh u silu'(g) both
+    bad_up = both[:, :n].clone()
+    for b in (bad, bad_up):
+        b[m - 1, 3] = True
+    assert torch.equal(torch.isnan(d[:, :n]), bad) and torch.equal(torch.isnan(d[:, n:]), bad_up)
+    assert torch.isinf(d[0, [5, n + 5]]).all()
+    finite = torch.isfinite(d)
+    finite[0, [5, n + 5]] = True
+    assert torch.equal(finite, ~torch.cat([bad, bad_up], dim=1))
+
+
+@pytest.mark.parametrize("fw", ["fp4", "fp8"])
+@pytest.mark.parametrize("tm,split,m,n,k", [r for r in GRADIENT if r[2:] != (4100, 700, 2310)])
+def test_gradient_of_blocks_that_are_not_finite(tm, split, m, n, k, fw):
+    """A block of W reaches its 32 columns of every row, a NaN or an infinity of dy its own row."""
+    w = torch.ones(n, k, device=DEV)
+    w[0, 40], w[n // 2, k - 1], w[n - 1, 0] = float("nan"), float("inf"), float("-inf")
+    dy = torch.ones(m, n, dtype=BF16, device=DEV)
+    dy[2] = 0.0
+    dy[1, n - 1], dy[m // 2, 0], dy[m - 2, n // 2] = float("nan"), float("inf"), float("-inf")
+    dx = K.mx_gemm(dy, K.mx_quantize(w, fw), trans=True)
+    nan = torch.zeros(m, k, dtype=torch.bool, device=DEV)
+    nan[1] = True
+    nan[:, :64] = nan[:, (k - 1) // 32 * 32:] = True
+    want = torch.full((m, k), float(n), device=DEV).to(BF16)
+    want[2] = 0.0
+    want[m // 2], want[m - 2] = float("inf"), float("-inf")
+    assert torch.equal(torch.isnan(dx), nan) and torch.equal(dx[~nan], want[~nan])
+
+
+# ---- the layers on inputs of other forms ---------------------------------------------------------
+
+
+def layers():
+    """(name, f of one input) over weights of ragged sizes."""
+    d, inner = 200, 150
+    g = torch.Generator(device=DEV).manual_seed(5)
+    rnd = lambda *s: torch.randn(*s, generator=g, device=DEV, dtype=F16)
+    wg, wd = K.mx_quantize(rnd(2 * inner, d) * 0.1, "fp4"), K.mx_quantize(rnd(d, inner) * 0.1, "fp4")
+    nw, bias, res = rnd(d) * 0.1 + 1, rnd(2 * inner), rnd(d)
+    return d, {"linear": lambda x: ops.mx_linear(x, wg, bias), "glu": lambda x: ops.mx_mlp_glu(x, wg),
+               "norm_mlp": lambda x: ops.mx_norm_mlp(x, nw, wg, wd),
+               "residual": lambda x: sum(ops.mx_norm_mlp(x, nw, wg, wd, residual=res.expand_as(x).contiguous())),
+               "same": lambda x: sum(ops.mx_norm_mlp(x, nw, wg, wd, residual=x))}
+
+
+@pytest.mark.parametrize("layer", ["linear", "glu", "norm_mlp", "residual", "same"])
+def test_layers_on_inputs_of_any_form(layer):
+    """Zero tokens, a single vector, transposed, sliced and broadcast inputs, broadcast gradients: what the
+    same rows give when contiguous."""
+    d, f = layers()
+    f = f[layer]
+    for shape in ((0, d), (2, 0, d), (1, 0, 3, d)):
+        x = torch.zeros(shape, dtype=F16, device=DEV, requires_grad=True)
+        y = f(x)
+        assert y.shape[:-1] == x.shape[:-1]
+        y.sum().backward()
+        assert x.grad.shape == x.shape
+    base = torch.randn(6, 7, d + 5, generator=torch.Generator(device=DEV).manual_seed(6), device=DEV, dtype=F16)
+    views = [base[0, 0, :d], base[:, :, 3: d + 3], base.transpose(0, 1)[..., :d], base[::2, 1:, 5:],
+             base[0, :1, :d].expand(9, d), base[:1, :, :d].expand(4, 7, d)]
+    for v in views:
+        x, c = v.detach().requires_grad_(), v.detach().contiguous().requires_grad_()
+        y, want = f(x), f(c)
+        assert torch.equal(y, want)
+        for dy in (torch.ones((), dtype=F16, device=DEV).expand(y.shape), torch.randn_like(y),
+                   torch.randn(y.shape[-1:] + y.shape[:-1], device=DEV, dtype=F16).movedim(0, -1)):
+            dx = torch.autograd.grad(y, x, dy, retain_graph=True)[0]
+            assert torch.equal(dx, torch.autograd.grad(want, c, dy.contiguous(), retain_graph=True)[0])
