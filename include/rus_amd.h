@@ -856,7 +856,9 @@ int rus_rmsnorm_mx_fwd(const void* x, const void* residual, const void* weight, 
  * y[m, n] = T(sum_k X[m, k] W[n, k] + bias[n]); X [m, k] and W [n, k] in either format, T fp16 or
  * bf16 (dtype), bias in T or NULL; fp32 sums; k at most 2^22. Beyond a few tokens the sums come from
  * the scaled matrix instructions, which with an 8-bit operand keep about 13 bits below the largest of
- * 16 products that they add first. workspace: the fp32 elements rus_mx_gemm_workspace names (0: none;
+ * 16 products that they add first. The bias is the first term of that sum in a tile, the last one for a few
+ * tokens or a contraction in parts: results may differ in their last bit between batch sizes.
+ * workspace: the fp32 elements rus_mx_gemm_workspace names (0: none;
  * 16-byte aligned), for a contraction that few tiles split among them; not shared by calls that overlap.
  */
 int rus_mx_gemm_workspace(int64_t m, int64_t n, int64_t k, int32_t x_fmt, int32_t w_fmt,
@@ -888,10 +890,10 @@ int rus_mx_gemm_rows(const void* x, int64_t stride_x, int32_t act, const void* w
 
 /*
  * The input gradient of rus_mx_gemm: dx[m, k] = T(sum_n dy[m, n] T(W[n, k])), dy and dx in T = fp16
- * or bf16 (dtype), W decoded to T inside the product (an fp16 decode of |W| > 65504 is infinite;
- * bf16 holds every value); fp32 sums. workspace: the fp32 elements rus_mx_gemm_t_workspace names
- * (0: none; 16-byte aligned), the sums of a contraction that few tiles split among them; not
- * shared by calls that overlap.
+ * or bf16 (dtype), W decoded to T inside the product (exact from 2^-14 up to 65504 in fp16 and from 2^-126
+ * to 2^128 in bf16; above infinite, below rounded to a multiple of 2^-24 or 2^-133); fp32 sums. workspace:
+ * the fp32 elements rus_mx_gemm_t_workspace names (0: none; 16-byte aligned), the sums of a contraction
+ * that few tiles split among them; not shared by calls that overlap.
  */
 int rus_mx_gemm_t_workspace(int64_t m, int64_t n, int64_t k, int64_t* floats);
 int rus_mx_gemm_t(const void* dy, int64_t stride_dy, int32_t dtype, const void* w_codes,

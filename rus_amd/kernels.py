@@ -2578,7 +2578,8 @@ def mx_gemm(x, w: MXTensor, trans: bool = False, bias: torch.Tensor | None = Non
     too: an ``MXTensor`` or a tensor, quantised here to ``act`` ("fp8" or "fp4"). The result has
     ``dtype`` (fp16 or bf16; default x's own, fp16 for blocks), fp32 sums rounded once.
     trans=True: x [m, out] (a 16-bit tensor) @ W -> [m, in], the input gradient, with W decoded to
-    x's type inside the product (fp16: infinite above 65504)."""
+    x's type inside the product (fp16: infinite above 65504, rounded to multiples of 2^-24 below 2^-14;
+    bf16: the same at 2^128, 2^-133 and 2^-126)."""
     fn = "mx_gemm"
     if not isinstance(w, MXTensor):
         raise TypeError(f"{fn}: w must be an MXTensor, got {type(w).__name__}")

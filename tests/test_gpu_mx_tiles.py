@@ -6,9 +6,11 @@ from __future__ import annotations
 
 import ctypes
 
+import numpy as np
 import pytest
 import torch
 
+from oracle import ops as ref
 from rus_amd import _lib, kernels as K, ops
 from test_gpu_mx_sizes import FORMATS, bits, exact
 
@@ -360,3 +362,48 @@ def test_layers_on_inputs_of_any_form(layer):
                    torch.randn(y.shape[-1:] + y.shape[:-1], device=DEV, dtype=F16).movedim(0, -1)):
             dx = torch.autograd.grad(y, x, dy, retain_graph=True)[0]
             assert torch.equal(dx, torch.autograd.grad(want, c, dy.contiguous(), retain_graph=True)[0])
+
+
+# ---- every code at every scale -------------------------------------------------------------------
+
+
+def every_value(fmt):
+    """One row with all codes of a format at all finite scales: (their values in float64, codes, scales)."""
+    n = 16 if fmt == "fp4" else 256
+    codes = np.tile(np.arange(n, dtype=np.uint8), 255 * max(1, 32 // n))
+    scales = np.repeat(np.arange(255, dtype=np.uint8), max(1, n // 32))
+    codes = np.pad(codes, (0, -len(codes) % 128))
+    scales = np.pad(scales, (0, -len(scales) % 4))
+    return ref.mx_values(ref.mx_pack(codes[None], fmt), scales[None], len(codes), fmt)[0], codes, scales
+
+
+def same(a, b):
+    return bool(((a == b) | (torch.isnan(a) & torch.isnan(b))).all())
+
+
+@pytest.mark.parametrize("m", [1, 40, 100, 300])
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("fw", ["fp4", "fp8"])
+def test_gradient_decodes_every_value(fw, dtype, m):
+    """One weight row times one: the values rounded once to dy's type, subnormal and infinite ones too."""
+    v, codes, scales = every_value(fw)
+    w = K.MXTensor(torch.from_numpy(ref.mx_pack(codes[None], fw)).to(DEV), torch.from_numpy(scales[None]).to(DEV),
+                   (1, len(v)), fw)
+    want = torch.from_numpy(v).to(dtype).to(DEV)
+    assert same(K.mx_gemm(torch.ones(m, 1, dtype=dtype, device=DEV), w, trans=True), want.expand(m, -1))
+    assert same(K.mx_dequantize(w, dtype)[0], want)
+
+
+@pytest.mark.parametrize("exponent", [-100, 0, 100])
+@pytest.mark.parametrize("m", [1, 5, 40, 300])
+@pytest.mark.parametrize("fx,fw", FORMATS)
+def test_product_of_every_value(fx, fw, m, exponent):
+    """One weight a row times a power of two: fp32 products rounded once, at scales whose own product leaves
+    fp32."""
+    v, codes, scales = every_value(fw)
+    code, scale = np.zeros((len(v), 128), np.uint8), np.zeros((len(v), 4), np.uint8)
+    code[:, 0], scale[:, 0] = codes, np.repeat(scales, 32)
+    w = K.MXTensor(torch.from_numpy(ref.mx_pack(code, fw)).to(DEV), torch.from_numpy(scale).to(DEV), (len(v), 1), fw)
+    x = torch.full((m, 1), 2.0**exponent, device=DEV)
+    want = torch.from_numpy(v * 2.0**exponent).float().to(BF16).to(DEV)
+    assert same(K.mx_gemm(K.mx_quantize(x, fx), w, dtype=BF16), want.expand(m, -1))
