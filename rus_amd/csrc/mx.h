@@ -139,8 +139,8 @@ __device__ __forceinline__ void each(F f) {
 
 // The sum of `parts` groups of V floats, `step` apart, added in order. DEEP: sixteen loads at a time, for
 // few sums of many parts, which take a few rounds of the latency from other XCDs' caches (28 parts of
-// 16 x 1,536: 5.4 us by eights, 3.7 by sixteens); many sums are better served by more waves with fewer
-// registers (5 parts of 4,096 x 1,536: 22 us, by sixteens 27).
+// 16 x 1,536: 5.4 us by eights, 3.7 by sixteens, as 32 parts take); many sums are better served by more
+// waves with fewer registers (5 parts of 4,096 x 1,536: 21 us, by sixteens 27).
 template <bool DEEP, int V>
 __device__ __forceinline__ void sum_parts(const float* __restrict__ p, int64_t step, int parts, float (&v)[V]) {
   load_f32<float, V>(p, v);

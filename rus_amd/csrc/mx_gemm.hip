@@ -149,8 +149,10 @@ __device__ __forceinline__ void finish(const MxArgs& g, int t, int f, const floa
 // 32 features x 32 tokens per workgroup of four waves, the contraction's groups of four blocks dealt to
 // the waves, operands straight from memory to registers, two groups' loads in flight at a time; the
 // waves' sums meet in LDS. Bound by the lines that a CU's address unit takes in (about 2.3 cycles each: a
-// load touches 32 rows for 32 bytes of each), so more waves bring nothing (8,960 x 1,536 at one token:
-// 11.1, 9.3 and 9.6 us with 4, 8 and 16 waves) and what fills the other CUs is a part of the contraction.
+// load touches 32 rows for 32 bytes of each), so eight waves bring nothing where workgroups are many (32
+// tokens fp8 by fp4: 17,920 x 1,536 10.0 us with four and 10.2 with eight, 2,048 x 1,536 5.1 and 5.3). Few
+// of them over a long contraction (1,536 x 8,960, 32 tokens: 16.5 and 15.5) leave CUs idle, which parts of
+// the contraction fill (five parts: 6.2 and 6.1).
 constexpr int kAhead = 2, kRowsWaves = 4;
 
 template <int FX, int FW, int EPI, typename T>
@@ -219,11 +221,12 @@ __global__ __launch_bounds__(kRowsWaves* kWave) void mx_rows_kernel(MxArgs g) {
 // What bounds it is the copies: a CU takes a line from its L2 in about 2.3 cycles whether it needs 128
 // bytes of it or 64 (55 or 28 bytes per cycle, measured with nothing else running). Where both operands
 // are fp4, a stage is therefore two groups, so that rows are whole lines, and where there are tiles
-// enough a tile is 256 x 256, which copies half as much a product (8,161 x 17,920 x 1,536: 139 us, 3.2
-// PFLOP/s, against 165 with 128 x 128; 8,161 x 8,960 x 8,960: 341 and 412); with an fp8 operand the
-// products take twice as long and a taller tile of one group covers the copies (8,161 x 17,920 x 1,536:
-// 194 us with 256 x 128, 195 with 256 x 256, 225 with 128 x 128). They go out between the products, since
-// a wave that issues them in a row waits for each.
+// enough a tile is 256 x 256, which copies half as much a product (8,161 x 17,920 x 1,536: 164 us, 2.7
+// PFLOP/s, against 180 with 128 x 128; 8,161 x 8,960 x 8,960: 353, 3.7 PFLOP/s, and 426); with an fp8
+// operand the products take twice as long and a taller tile of one group covers the copies (8,161 x 17,920
+// x 1,536 with fp4 weights: 208 us, 2.2 PFLOP/s, with 256 x 128, 254 with 128 x 128; fp8 weights, 128 x
+// 128 only: 275). (Averages of 20 calls on the same operands; on three sets of them in turn 169, 407, 234
+// and 327.) They go out between the products, since a wave that issues them in a row waits for each.
 //
 // LDS rows of W are in MFMA order (row 32 q + i holds feature 32 q + feature_of(i)); with a gate, the
 // lower half is gate, the upper half up rows of the same features, and a wave takes the same part of
@@ -738,13 +741,22 @@ __global__ __launch_bounds__(256) void mx_sum_kernel(const float* __restrict__ p
 //
 // The one whose launch is estimated shortest. A launch takes a + groups (b + r (rounds - 1)) us, groups
 // of four blocks of the contraction per workgroup, rounds of 256 workgroups (and c for each after the
-// first); a contraction cut into parts pays for a second launch and 8 bytes a value and part. Measured at
-// 12 and 70 groups (k = 1536, 8960), 1 to 8,161 tokens, 1,536 to 17,920 features: one round of 256 x 128
-// tiles 10.5 / 42 us, of 128 x 128 7.4 / 28.5, of 128 x 64 6.4 / 25, of the 32 x 32 kernel 3.7 / 9.3
-// (one token) and 4.7 / 15.3 (32). 707 tokens x 17,920: 22.9, 25.4, 28.4 and (32 x 32) 121; 192 tokens
-// 12.5, 12.1, 9.9; 2,048 features at 33 tokens 10.3, 7.1, 6.4 and 4.6. With both operands fp4, 256 x 256
-// takes the taller tile's place: one round 12 to 17 / 43 to 61 us, a further one 16 / 64, against 128 x
-// 128's 6.5 / 21 to 33 and 4.8 / 28.
+// first); a contraction cut into parts pays for a second launch and 8 bytes a value and part.
+//
+// Measured (us a kernel, average of 20 on the same operands) at k = 1,536 / 8,960 with 16, 256, 512 and
+// 1,024 workgroups:
+//   fp8 by fp4  128 x 64   7.2, 8.4, 11.5, 19.3 / 29, 42, 50, 96      fp4 by fp4  6.6, 7.4, 9.8, 16.5 / 24, 32, 41, 78
+//               128 x 128  7.8, 10.7, 16.8, 28.5 / 32, 52, 72, 146                6.8, 9.0, 13.1, 21.1 / 22, 35, 49, 97
+//               256 x 128  11.0, 16.2, 25.6, 45.2 / 49, 68, 116, 238   256 x 256  11.8, 20.5, 37.6, 70.0 / 48, 76, 151, 306
+//   fp8 by fp8  128 x 64   8.0, 9.5, 13.1, 23.3 / 32, 47, 57, 114     fp4 by fp8  8.1, 8.8, 12.2, 21.9 / 31, 44, 52, 106
+//               128 x 128  8.7, 11.2, 17.3, 30.1 / 38, 56, 76, 166                7.9, 10.7, 15.9, 27.7 / 32, 50, 69, 147
+// and the 32 x 32 kernel (fp8 by fp4) on 2,048 features 4.4 at one token, 5.1 at 32, 7.9 at 256; on 1,536
+// features with k = 8,960 11.5 and 16.5 whole, 5.0 and 6.2 in five parts (and 2.5 to 3 for their sum).
+// The estimates fit few workgroups and fall up to a third short where a round is full; the choice needs
+// their order. It took the shortest kind measured in 40 of 43 products and gates of 33 to 8,161 tokens
+// (1,536 to 17,920 features, all formats): 707 tokens x 2,048 128 x 64 (8.4; 128 x 128 9.0, 256 x 128
+// 12.1), x 17,920 256 x 128 (23.4; 25.6, 28.4), 4,096 x 1,536 x 8,960 256 x 128 (63.2; 64.0, 73.6). Not
+// at 192 tokens x 17,920 (256 x 128 13.5, 128 x 64 10.9) nor the 4-bit gate at 4,096 (78 and 76).
 struct GemmPlan {
   int bf, bt, splits;  // bt 32: the 32 x 32 kernel
 };

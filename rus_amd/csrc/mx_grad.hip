@@ -9,8 +9,8 @@
 // conversions and writes it transposed-readable; rows of any alignment, and the contraction's end, come
 // in on the same way. W's rows lie along the contraction, so its fragments leave LDS through the
 // transposing ds_read_b64_tr_b16. Reads, decoding, writes and loads go out between the products: bound by
-// the matrix pipe and its clock (2,048 x 17,920 x 1,536 bf16: 105 us and 11 for the sums, 1,073 TFLOP/s,
-// where a library product of 8192^3 reaches 1,197; in groups between bursts of products 113 us).
+// the matrix pipe and its clock (2,048 x 17,920 x 1,536 bf16: 96 us on the same operands each call, 113 on
+// three sets in turn, 1.17 and 1.0 PFLOP/s, where a library product of 8192^3 reaches 1.2; 11 for the sums).
 // A tile count below the chip's 256 CUs splits the contraction; the splits' fp32 sums are added in
 // split order by a second launch.
 #include "mx.h"
@@ -329,9 +329,12 @@ __global__ __launch_bounds__(256) void mx_grad_sum_kernel(const float* __restric
 // The tile height and the number of splits for a shape, by what a launch is estimated to take: rounds of
 // 256 workgroups, each 3 us (5 of 256 tokens) and its stages (1.7, 1.05, 0.9 or 0.65 us of 256, 128, 64
 // or 32 tokens); a split contraction pays for the second launch and 8 bytes a sum, which stay in the
-// caches (10 TB/s). Measured over 1 to 4,096 tokens: 4,096 x 17,920 x 1,536 in 256-token tiles and 5
-// splits 232 us (2: 238; 128-token tiles unsplit 272, in 4 splits 307); 707 tokens 53; 256 tokens in
-// 128-token tiles 29 (256: 34, 64: 34); 16 tokens in 32-token tiles and 28 splits 14.5.
+// caches (10 TB/s). Measured with n x k = 17,920 x 1,536 fp4, fp16 dy, the kernel and the sums: 4,096
+// tokens in 256-token tiles and 5 splits 216 + 21 us (2: 225 + 10, 1: 370; 128-token tiles unsplit 274, in 4
+// splits 268 + 18); 2,048 in 256-token tiles and 5 splits 98 + 11 (4: 105 + 9; 128-token tiles in 3 178 +
+// 7); 707 in 128-token tiles and 7 splits 47 + 6 (4: 67 + 5; 256-token tiles in 14 43 + 10); 256 in
+// 128-token tiles and 20 splits 22 + 6 (256: 25 + 11, 64: 29 + 4). 16 tokens, 2,048 x 1,536, in 32-token
+// tiles and 32 splits 4.8 + 3.6 (16: 4.8 + 2.7, 8: 5.8 + 3.8).
 struct GradPlan {
   int tm, splits;
 };

@@ -57,9 +57,9 @@ __device__ __forceinline__ void store_codes(uint8_t* p, const float (&v)[8], boo
 
 // Thread = eight elements, four neighbouring lanes = one block: a 16-byte load, the block's largest
 // element by two lane exchanges, one store of 4 or 8 bytes of codes. Bound by memory: 17920 x 1536
-// fp16 to 4 bits 13.8 us and back 12.4 us (5.0 / 5.6 TB/s of the bytes named above), fp32 19.2 us
-// (6.5 TB/s). Rows of an odd length go by the same accesses: 16384 x 1111 fp16 to 4 bits took 24.5 us
-// with single-element loads there and takes 13.6, back 26.5 and 10.2; lengths that are multiples of 8
+// fp16 to 4 bits 14.5 us and back 12.4 us (70 MB of rows, codes and scales: 4.8 / 5.6 TB/s), fp32 18.8 us
+// (125 MB). Rows of an odd length go by the same accesses: 16384 x 1111 fp16 to 4 bits took 24.5 us
+// with single-element loads there and takes 13.3, back 26.5 and 10.2; lengths that are multiples of 8
 // took the same either way.
 template <typename T, int FMT>
 __global__ __launch_bounds__(256) void mx_quantize_kernel(const T* __restrict__ x, int64_t stride,
@@ -210,9 +210,10 @@ __device__ __forceinline__ bool fast_blocks(const float (&h)[8], const float (&w
 
 // One workgroup per row, eight columns per thread and step; a row of up to 8192 columns stays in
 // registers between the two passes, a longer one is read again (from this CU's L2). Bound by memory:
-// 16381 x 1536 fp16 with the residual moves 177 MB in 32 us (5.5 TB/s); with fp64 products and a
-// correctly rounded square root and division it took 39 us, bound by arithmetic. Without a residual,
-// where a third of those bytes move, arithmetic still bounds it: 26 us (33 in fp64).
+// 16381 x 1536 fp16 with the residual moves 177 MB in 36 us (4.9 TB/s); on the same rows each call, part
+// of which the last-level cache holds, 31 us, and there it took 39 us with fp64 products and a correctly
+// rounded square root and division, bound by arithmetic. Without a residual, where 76 MB move, arithmetic
+// still bounds it: 26 us (33 in fp64).
 template <typename T, typename W, bool HAS_RES>
 __global__ __launch_bounds__(1024) void rmsnorm_mx_kernel(
     const T* __restrict__ x, const T* __restrict__ res, const W* __restrict__ w, T* sum_out,

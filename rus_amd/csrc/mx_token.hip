@@ -10,8 +10,8 @@
 // would do it. A block's 32 products are summed by v_dot2_f32_f16, exact products and fp32 sums, and join
 // the row's sum times both blocks' scales, as one exponent: the product of the scales alone may pass fp32.
 //
-// One token: 1,536 x 8,960 fp4 (7.3 MB) 5.5 us, 2 x 8,960 x 1,536 with the gate (14.6 MB) 6.2 us, W from
-// memory; an empty launch takes about 2.
+// One token: 1,536 x 8,960 fp4 (7.3 MB) 6.4 us with W from memory and 5.4 from the last-level cache, 2 x
+// 8,960 x 1,536 with the gate (14.6 MB) 7.4 and 6.2; an empty launch takes about 2.
 //
 // Matrix instructions would not help: their operand wants 32 rows at once, 32 bytes of each, four times
 // the line requests; tokens 1 to 32 cost them the same.
@@ -178,8 +178,9 @@ __global__ __launch_bounds__(512) void mx_token_kernel(TokenArgs g) {
 }
 
 // Eight waves where the contraction is long or workgroups are few, four else (each workgroup rounds x for
-// itself). One token, W from memory: 1,536 x 8,960 fp4 10.4, 7.4 and 5.5 us with 2, 4 and 8 waves, 2 x
-// 8,960 x 1,536 with the gate 6.9, 6.2 and 8.7; four tokens x 2,048 x 1,536 7.2, 5.6 and 4.7.
+// itself). One token, W from memory: 1,536 x 8,960 fp4 11.6, 8.3 and 6.3 us with 2, 4 and 8 waves, 2 x
+// 8,960 x 1,536 with the gate 8.3, 7.0 and 9.8, 17,920 x 1,536 8.3, 8.3 and 12.9; four tokens x 2,048 x
+// 1,536 8.0, 6.2 and 5.2.
 int token_waves(int64_t n, int64_t nb) { return (nb + 7) / 8 > 16 || n <= 4096 ? 8 : 4; }
 
 template <int FW, int EPI, typename T>
@@ -208,10 +209,12 @@ void by_weight(const TokenArgs& g, int w_fmt, hipStream_t st) {
 }  // namespace
 
 // One or two tokens, four where there are few features, as far as x fits into LDS. W from memory, this
-// kernel against rounding x in a launch of its own and the other kernels: 1,536 x 8,960 fp4 one token 5.5
-// and 11.1 us, two 7.5 and 11.2; 2,048 x 1,536 one 3.4 and 6.2, four 4.7 and 6.6; 17,920 x 1,536 one 7.0
-// and 8.8, two 9.4 and 8.9 (one launch less for the host), four 13.5 and 10.8; with the gate, 2 x 8,960 x
-// 1,536, one 6.2 and 10.9, two 9.1 and 10.7, four 12.3 and 11.0.
+// kernel against rounding x in a launch of its own and the other kernels, weights in 4 bits (in 8): 1,536 x
+// 8,960 one token 6.4 and 13.8 us (7.4 and 13.9), two 8.3 and 13.3 (9.1 and 14.2); 2,048 x 1,536 one 4.1
+// and 6.5 (4.5 and 7.1), four 5.2 and 6.9 (5.6 and 7.4); 17,920 x 1,536 one 8.6 and 10.0 (11.3 and 11.9),
+// two 10.9 and 10.3 (13.7 and 12.5; one launch less for the host), four 15.4 and 11.9 (18.1 and 15.5); with
+// the gate, 2 x 8,960 x 1,536, one 7.4 and 12.1 (9.5 and 15.3), two 10.2 and 12.4 (11.2 and 15.7), four
+// 13.6 and 12.3 (15.3 and 15.9).
 bool few_tokens(int64_t m, int64_t n, int64_t nb) {
   return m <= (n <= 4096 ? 4 : 2) && m * nb * (kPitch + 4) <= 61440 &&
          (n + 7) / 8 * token_waves(n, nb) * kWave < kMaxItems;  // (else the 32 x 32 kernel)
