@@ -753,7 +753,7 @@ __global__ __launch_bounds__(256) void mx_sum_kernel(const float* __restrict__ p
 // and the 32 x 32 kernel (fp8 by fp4) on 2,048 features 4.4 at one token, 5.1 at 32, 7.9 at 256; on 1,536
 // features with k = 8,960 11.5 and 16.5 whole, 5.0 and 6.2 in five parts (and 2.5 to 3 for their sum).
 // The estimates fit few workgroups and fall up to a third short where a round is full; the choice needs
-// their order. It took the shortest kind measured in 40 of 43 products and gates of 33 to 8,161 tokens
+// their order. It took the shortest kind measured in 41 of 44 products and gates of 33 to 8,161 tokens
 // (1,536 to 17,920 features, all formats): 707 tokens x 2,048 128 x 64 (8.4; 128 x 128 9.0, 256 x 128
 // 12.1), x 17,920 256 x 128 (23.4; 25.6, 28.4), 4,096 x 1,536 x 8,960 256 x 128 (63.2; 64.0, 73.6). Not
 // at 192 tokens x 17,920 (256 x 128 13.5, 128 x 64 10.9) nor the 4-bit gate at 4,096 (78 and 76).
