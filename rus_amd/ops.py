@@ -150,7 +150,7 @@ class _FirstOrderFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, g, fn):
         ctx.fn = fn
-        return g.view_as(g)
+        return g.clone()  # (a view could not be changed in place)
 
     @staticmethod
     def backward(ctx, dg):

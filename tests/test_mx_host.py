@@ -78,6 +78,8 @@ def test_first_derivatives_under_create_graph(plain_kernels):
     z = ops.mx_mlp_glu(x, _mx(16, 64)).sum() + (x * x).sum()
     (dx,) = torch.autograd.grad(z, x, create_graph=True)
     assert torch.equal(dx, 2 * x)
+    (dx,) = torch.autograd.grad(ops.mx_mlp_glu(x, _mx(16, 64)).sum(), x, create_graph=True)
+    dx.mul_(2.0)  # a gradient is the caller's to change
 
 
 # ---- formats that do not exist -------------------------------------------------------------------
