@@ -1,5 +1,5 @@
-"""The host side of the microscaled operators where a first reading of it went wrong: frozen parameters under
-``no_grad``, second derivatives, size queries of unknown formats, launches that one dispatch cannot hold."""
+"""The host side of the microscaled operators on the CPU: frozen parameters under ``no_grad``, second
+derivatives, size queries of unknown formats, results that one dispatch cannot hold, plans."""
 
 from __future__ import annotations
 
