@@ -23,11 +23,16 @@
 extern "C" {
 #endif
 
-#define RUS_ABI_VERSION 21
+#define RUS_ABI_VERSION 22
 
 #define RUS_DTYPE_F16 0
 #define RUS_DTYPE_F32 1
-#define RUS_DTYPE_BF16 2 /* microscaled entry points only */
+#define RUS_DTYPE_BF16 2 /* microscaled, rope_axes, attn_masked and distillation entry points only */
+
+/* Types of rus_rope_axes' positions. */
+#define RUS_POS_I64 0
+#define RUS_POS_I32 1
+#define RUS_POS_F32 2
 
 /* Element formats of microscaled blocks. */
 #define RUS_MX_FP4 0 /* e2m1, two to a byte, the even element in the low half */
@@ -925,6 +930,100 @@ int rus_mx_glu_bwd(const void* dh, int64_t stride_dh, const void* x_codes, const
                    int32_t x_fmt, const void* w_codes, const void* w_scales, int32_t w_fmt,
                    int64_t m, int64_t n, int64_t k, void* d_gu, int64_t stride_d_gu, int32_t dtype,
                    void* stream);
+
+/*
+ * Rotary positions with several axes. Pair i < pairs of every head of q [n_tokens, h_q, head_dim] and k (h_k heads;
+ * 0 heads: none) turns by a = pos[axis[i]][t] * f[i], turns[i] = f[i] / 2 pi in 64 bits:
+ *   (x1, x2) -> T(x1 cos a - x2 sin a), T(x2 cos a + x1 sin a)
+ * x1, x2 the elements i and i + pairs, or with `adjacent` 2 i and 2 i + 1; elements from 2 pairs on are copied.
+ * inverse: by -a (the backward). Strides of q and k in elements, unit stride within a head; q_out, k_out contiguous,
+ * apart from the inputs or at the same place. pos [n_axes, ld_pos >= n_tokens] of pos_type (RUS_POS_*), any sign;
+ * axis [pairs] (an axis past the last counts as the last), turns [pairs] on the device. T = fp16, bf16 or fp32, at
+ * most 512 pairs. Angles are formed in 64 bits, the rotation in 32.
+ * Beside: rus_qkv_lora_rope_fwd (solution/kernels.py:206-348), which reads one axis' angles from tables.
+ */
+int rus_rope_axes(const void* q, int64_t q_stride_t, int64_t q_stride_h, int32_t h_q, void* q_out, const void* k,
+                  int64_t k_stride_t, int64_t k_stride_h, int32_t h_k, void* k_out, int64_t n_tokens,
+                  int32_t head_dim, int32_t pairs, int32_t adjacent, const void* pos, int32_t pos_type,
+                  int64_t ld_pos, int32_t n_axes, const uint8_t* axis, const double* turns, int32_t inverse,
+                  int32_t dtype, void* stream);
+
+/*
+ * Attention over packed rows with capped scores, a bias by distance, a prefix and fewer queries than keys. Row s has
+ * the queries [cu_q[s], cu_q[s+1]) of q [n_q, h_q, head_dim] and the keys [cu_k[s], cu_k[s+1]) of k, v [n_k, h_kv,
+ * head_dim]; query i of lq stands at p = lk - lq + i, so that a row's queries are the last of its keys. Key j is
+ * visible when causal is 0, j <= p, or j < prefix[s] (prefix NULL: 0; clamped to [0, lk]). Of the visible keys, with
+ * KV head h / (h_q / h_kv):
+ *   z = scale q.k,  softcap > 0: z = softcap tanh(z / softcap),  slopes: z -= slopes[h] |p - j|
+ *   out = softmax(z) v,  lse[h, t] = ln sum e^z (fp32 [h_q, n_q])
+ * A query that sees no key, and one outside every row, gets out = 0 and lse = -inf. Hidden keys take no part whatever
+ * they hold. T = fp16 or bf16, head_dim 64 or 128; q, k, v 16-byte aligned with strides that are multiples of 8
+ * elements (unit stride within a head); out contiguous. cu_q, cu_k, prefix int32 and slopes [h_q] fp32 on the device;
+ * entries out of order or range are clamped into the arrays. max_q, max_k: at least the longest row's queries and
+ * keys (they choose the kernel; rows longer than max_q are not finished). workspace: the fp32 elements that
+ * rus_attn_masked_workspace names for the same sizes (0: none; 16-byte aligned), not shared by calls that overlap.
+ * P is rounded to T for its product with v, sums are fp32.
+ * Beside: rus_attn_varlen_fwd (solution/ops.py:669-696).
+ */
+int rus_attn_masked_workspace(int32_t n_seq, int64_t n_q, int64_t n_k, int32_t max_q, int32_t max_k, int32_t h_q,
+                              int32_t h_kv, int32_t head_dim, int32_t backward, int64_t* floats);
+int rus_attn_masked_fwd(const void* q, int64_t q_stride_t, int64_t q_stride_h, const void* k, int64_t k_stride_t,
+                        int64_t k_stride_h, const void* v, int64_t v_stride_t, int64_t v_stride_h,
+                        const int32_t* cu_q, const int32_t* cu_k, int32_t n_seq, int64_t n_q, int64_t n_k,
+                        int32_t max_q, int32_t max_k, int32_t h_q, int32_t h_kv, int32_t head_dim, float scale,
+                        int32_t causal, const int32_t* prefix, float softcap, const float* slopes, int32_t dtype,
+                        void* out, float* lse, float* workspace, int64_t n_workspace, void* stream);
+
+/*
+ * Its backward, given out and lse: with t = tanh(z / softcap) (1 - t^2 = 1 without a cap), D = dout.out,
+ *   dS = P (dout v^T - D) (1 - t^2),  dq = scale dS k,  dk = scale dS^T q,  dv = P^T dout,
+ * dk and dv summed over the query heads of each KV head in a fixed order in fp32 and rounded once. dout by strides as
+ * q; dq, dk, dv contiguous, zero at tokens that no row or no pair covers. P and dS are rounded to T.
+ */
+int rus_attn_masked_bwd(const void* dout, int64_t do_stride_t, int64_t do_stride_h, const void* q, int64_t q_stride_t,
+                        int64_t q_stride_h, const void* k, int64_t k_stride_t, int64_t k_stride_h, const void* v,
+                        int64_t v_stride_t, int64_t v_stride_h, const void* out, const float* lse,
+                        const int32_t* cu_q, const int32_t* cu_k, int32_t n_seq, int64_t n_q, int64_t n_k,
+                        int32_t max_q, int32_t max_k, int32_t h_q, int32_t h_kv, int32_t head_dim, float scale,
+                        int32_t causal, const int32_t* prefix, float softcap, const float* slopes, int32_t dtype,
+                        void* dq, void* dk, void* dv, float* workspace, int64_t n_workspace, void* stream);
+
+/*
+ * Distillation from a teacher's top logits over the lm_head. Per token n_entries (at most 1024) pairs of a vocabulary
+ * id (int64, or int32 with ids32) and a logit (logits_dtype: fp32, fp16 or bf16), both [n_tok, n_entries] contiguous;
+ * an id outside [0, n_vocab) or a logit of -inf is no entry. q = softmax over a token's entries of logit / T, p =
+ * softmax over the vocabulary of h W^T / T:
+ *   kl = sum q (ln q - ln p),  loss = T^2 sum kl / denom,  dH = T / denom (p W - sum q W[id]) (times 2^16)
+ * denom = max(*num_items or the number of tokens with entries, 1). Tokens without entries: kl 0, dH 0. An id that
+ * comes twice adds its q.
+ *
+ * rus_lmhead_distill_fwd: vocabulary rows [256 part_base, + n_vocab) of the head, as rus_lmhead_ce_fwd_probs: partial
+ * maxima and sums of h W^T / T (fp32 logits) per 256 rows, and, where probs is given, P = fp16(2^(z log2 e - ref)),
+ * half_ref and chunk_max, for rus_lmhead_ce_probs_rescale and rus_lmhead_ce_grad_hidden_scaled. d a multiple of 64.
+ * rus_lmhead_distill_blank: P = 0 at the teacher's entries among rows [vocab_start, + n_rows), before its product.
+ * rus_lmhead_distill_entries: once every chunk is in the partials: kl, lse (of z), taught (1 or 0) [n_tok], coef
+ * [n_tok, n_entries] (NULL: no gradient wanted), loss and denom (one each). weight: all n_vocab rows, in device
+ * memory or page-locked, device-mapped host memory.
+ * rus_lmhead_distill_finish: dH in fp32 [n_tok, d] from the accumulated partials and the entries' rows.
+ * Beside: the chunked cross-entropy (solution/ops.py:174-349).
+ */
+int rus_lmhead_distill_fwd(const void* hidden, const void* weight, int64_t n_tok, int64_t d, int64_t ld_h,
+                           int64_t ld_w, int64_t n_vocab, float temperature, float* part_m, float* part_s,
+                           int64_t part_base, int64_t part_stride, void* probs, int64_t ld_p, const float* ref,
+                           float* half_ref, uint32_t* chunk_max, void* stream);
+int rus_lmhead_distill_blank(void* probs, int64_t ld_p, int64_t n_tok, int64_t n_rows, int64_t vocab_start,
+                             const void* ids, int32_t ids32, const void* logits, int32_t logits_dtype,
+                             int32_t n_entries, int64_t n_vocab, float temperature, void* stream);
+int rus_lmhead_distill_entries(const void* hidden, int64_t ld_h, const void* weight, int64_t ld_w, int64_t n_vocab,
+                               int64_t n_tok, int64_t d, const void* ids, int32_t ids32, const void* logits,
+                               int32_t logits_dtype, int32_t n_entries, float temperature, const float* part_m,
+                               const float* part_s, int64_t n_parts, int64_t part_stride, const float* num_items,
+                               float* kl, float* lse, float* taught, float* coef, float* loss, float* denom,
+                               void* stream);
+int rus_lmhead_distill_finish(const float* parts, int32_t n_parts, int64_t n_tok, int64_t d, const float* m_run,
+                              const float* lse, const float* taught, const float* coef, const void* ids,
+                              int32_t ids32, int32_t n_entries, const void* weight, int64_t ld_w, int64_t n_vocab,
+                              const float* denom, float temperature, float* out, void* stream);
 
 #ifdef __cplusplus
 }

@@ -599,3 +599,59 @@ def mx_glu_bwd(dh: np.ndarray, g: np.ndarray, u: np.ndarray) -> np.ndarray:
 
 
 __all__ = [name for name in dir() if not name.startswith("_") and name not in ("math", "np", "torch")]
+
+
+# ---------------------------------------------------------------------------------------------
+# Rotary positions with several axes, attention with caps / distance bias / prefix, distillation
+# (float64; the definitions in include/rus_amd.h)
+# ---------------------------------------------------------------------------------------------
+
+
+def rope_axes(x, pos, axis, freq, adjacent=False, inverse=False):
+    """x [N, heads, d] with pair i turned by pos[axis[i]] * freq[i], in float64."""
+    p = len(axis)
+    a = pos.double()[torch.tensor(list(axis))].t() * torch.tensor(list(freq), dtype=torch.float64)
+    c, s = torch.cos(a)[:, None], torch.sin(a)[:, None] * (-1.0 if inverse else 1.0)
+    y = x.double().clone()
+    i, j = (slice(0, 2 * p, 2), slice(1, 2 * p, 2)) if adjacent else (slice(0, p), slice(p, 2 * p))
+    u, v = y[..., i].clone(), y[..., j].clone()
+    y[..., i], y[..., j] = u * c - v * s, v * c + u * s
+    return y
+
+
+def masked_scores(q, k, lq, lk, causal=True, prefix=0, softcap=0.0, slopes=None, scale=None):
+    """(scores, visible, 1 - tanh^2) of one row and KV group's heads in float64: q [h, lq, d], k [lk, d]."""
+    scale = q.shape[-1] ** -0.5 if scale is None else scale
+    z = scale * (q.double() @ k.double().t())
+    f = torch.ones_like(z)
+    if softcap:
+        t = torch.tanh(z / softcap)
+        z, f = softcap * t, 1.0 - t * t
+    at, j = torch.arange(lk - lq, lk)[:, None], torch.arange(lk)[None, :]
+    if slopes is not None:
+        z = z - slopes.double()[:, None, None] * (at - j).abs().double()
+    seen = (j <= at) | (j < prefix) if causal else torch.ones(lq, lk, dtype=torch.bool)
+    return z, seen, f
+
+
+def distill_head(hidden, weight, ids, logits, temperature=1.0, num_items=None):
+    """dict(loss, kl, dh) in float64: KL of the student's softmax over the vocabulary from the teacher's over its
+    entries (ids outside the vocabulary and logits of -inf are none)."""
+    n, v, t = hidden.shape[0], weight.shape[0], temperature
+    h, w = hidden.double(), weight.double()
+    log_p = torch.log_softmax(h @ w.t() / t, dim=1)
+    kl = torch.zeros(n, dtype=torch.float64)
+    g = torch.zeros(n, v, dtype=torch.float64)
+    taught = 0
+    for i in range(n):
+        on = (ids[i] >= 0) & (ids[i] < v) & (logits[i] != -math.inf)
+        if not bool(on.any()):
+            continue
+        taught += 1
+        log_q = torch.log_softmax(logits[i][on].double() / t, dim=0)
+        at = ids[i][on].long()
+        kl[i] = (log_q.exp() * (log_q - log_p[i, at])).sum()
+        g[i] = log_p[i].exp()
+        g[i].index_add_(0, at, -log_q.exp())
+    denom = max(float(taught if num_items is None else num_items), 1.0)
+    return {"loss": t * t * kl.sum() / denom, "kl": kl, "dh": (t / denom) * (g @ w)}

@@ -64,6 +64,14 @@ def _warm_up(device) -> None:
     q, _, _ = K.rms_norm_mx_fwd(x, w, residual=x)
     K.mx_gemm(K.mx_gemm(x, wq), wq, trans=True)
     K.mx_mlp_glu_bwd(K.mx_mlp_glu_fwd(q, wq), q, wq)
+    # rotary positions with several axes, attention with a cap, distillation over the lm_head
+    axes = K.RopeAxes.sections((16, 24, 24), 1e6, 128, dev)
+    q, k = qkv[:, :1536].view(4, 12, 128), qkv[:, 1536:1792].view(4, 2, 128)
+    q, k = K.rope_axes_fwd(q, k, torch.zeros(3, 4, dtype=torch.int64, device=dev), axes)
+    cu = torch.tensor([0, 4], dtype=torch.int32, device=dev)
+    out, lse = K.attn_masked_fwd(q, k, k, cu, softcap=50.0)
+    K.attn_masked_bwd(out, q, k, k, out, lse, cu, softcap=50.0)
+    K.lm_head_distill(hid, head, lab.view(4, 1), torch.zeros(4, 1, device=dev))
     torch.cuda.synchronize(dev)
 
 

@@ -11,11 +11,12 @@ import threading
 from pathlib import Path
 
 LIB_PATH = Path(__file__).resolve().parent / "librus_amd.so"
-ABI_VERSION = 21
+ABI_VERSION = 22
 
 DTYPE_F16 = 0
 DTYPE_F32 = 1
-DTYPE_BF16 = 2  # microscaled entry points only
+DTYPE_BF16 = 2  # microscaled, rope_axes, attn_masked and distillation entry points only
+POS_I64, POS_I32, POS_F32 = 0, 1, 2
 MX_FP4, MX_FP8 = 0, 1
 
 _vp = ctypes.c_void_p
@@ -170,6 +171,21 @@ SIGNATURES: dict[str, list] = {
     "rus_mx_glu_fwd": [_vp, _vp, _i32, _vp, _vp, _i32, _i64, _i64, _i64, _vp, _i64, _i32, _vp],
     "rus_mx_glu_bwd": [_vp, _i64, _vp, _vp, _i32, _vp, _vp, _i32, _i64, _i64, _i64, _vp, _i64,
                        _i32, _vp],
+    "rus_rope_axes": [_vp, _i64, _i64, _i32, _vp, _vp, _i64, _i64, _i32, _vp, _i64, _i32, _i32, _i32, _vp,
+                      _i32, _i64, _i32, _vp, _vp, _i32, _i32, _vp],
+    "rus_attn_masked_workspace": [_i32, _i64, _i64, _i32, _i32, _i32, _i32, _i32, _i32, ctypes.POINTER(_i64)],
+    "rus_attn_masked_fwd": [_vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _vp, _i32, _i64, _i64, _i32,
+                            _i32, _i32, _i32, _i32, _f32, _i32, _vp, _f32, _vp, _i32, _vp, _vp, _vp, _i64, _vp],
+    "rus_attn_masked_bwd": [_vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _vp, _vp, _vp,
+                            _i32, _i64, _i64, _i32, _i32, _i32, _i32, _i32, _f32, _i32, _vp, _f32, _vp, _i32, _vp,
+                            _vp, _vp, _vp, _i64, _vp],
+    "rus_lmhead_distill_fwd": [_vp, _vp, _i64, _i64, _i64, _i64, _i64, _f32, _vp, _vp, _i64, _i64, _vp, _i64, _vp,
+                               _vp, _vp, _vp],
+    "rus_lmhead_distill_blank": [_vp, _i64, _i64, _i64, _i64, _vp, _i32, _vp, _i32, _i32, _i64, _f32, _vp],
+    "rus_lmhead_distill_entries": [_vp, _i64, _vp, _i64, _i64, _i64, _i64, _vp, _i32, _vp, _i32, _i32, _f32, _vp,
+                                   _vp, _i64, _i64, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp],
+    "rus_lmhead_distill_finish": [_vp, _i32, _i64, _i64, _vp, _vp, _vp, _vp, _vp, _i32, _i32, _vp, _i64, _i64, _vp,
+                                  _f32, _vp, _vp],
 }
 
 _lock = threading.Lock()

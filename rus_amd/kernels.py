@@ -82,6 +82,13 @@ __all__ = [
     "rms_norm_mx_fwd",
     "mx_mlp_glu_fwd",
     "mx_mlp_glu_bwd",
+    "RopeAxes",
+    "rope_axes_fwd",
+    "rope_axes_bwd",
+    "attn_masked_fwd",
+    "attn_masked_bwd",
+    "LMHeadDistill",
+    "lm_head_distill",
 ]
 
 
@@ -1831,6 +1838,15 @@ def lm_head_weight_t(weight: torch.Tensor) -> torch.Tensor:
     return wt
 
 
+def _num_items(num_items_in_batch, dev) -> torch.Tensor | None:
+    """``num_items_in_batch`` (None, a number or a tensor) as a float32 device scalar."""
+    if isinstance(num_items_in_batch, torch.Tensor):
+        return num_items_in_batch.detach().to(device=dev, dtype=torch.float32).reshape(1)
+    if num_items_in_batch is not None:
+        return torch.full((1,), float(num_items_in_batch), dtype=torch.float32, device=dev)
+    return None
+
+
 def lm_head_ce_loss(nll: torch.Tensor, labels: torch.Tensor, num_items_in_batch=None):
     """(loss, denom) as one-element float32 device tensors: denom = max(num_items_in_batch, 1)
     if given, else max(#(labels != -100), 1); loss = sum(nll) / denom (no host read)."""
@@ -1840,11 +1856,7 @@ def lm_head_ce_loss(nll: torch.Tensor, labels: torch.Tensor, num_items_in_batch=
     n = nll.numel()
     if labels.numel() != n or nll.dtype != torch.float32 or labels.dtype != torch.int64:
         raise ValueError(f"{fn}: nll float32 [n] and labels int64 [n] expected")
-    ni = None
-    if isinstance(num_items_in_batch, torch.Tensor):
-        ni = num_items_in_batch.detach().to(device=dev, dtype=torch.float32).reshape(1)
-    elif num_items_in_batch is not None:
-        ni = torch.full((1,), float(num_items_in_batch), dtype=torch.float32, device=dev)
+    ni = _num_items(num_items_in_batch, dev)
     out = torch.empty(2, dtype=torch.float32, device=dev)
     _launch("lmhead_ce_loss", n * 12, 0, "rus_lmhead_ce_loss", nll.contiguous().data_ptr(),
             labels.contiguous().data_ptr(), n, _ptr(ni), out.data_ptr(), out.data_ptr() + 4,
@@ -2703,3 +2715,402 @@ def mx_mlp_glu_bwd(dh: torch.Tensor, x, w: MXTensor, act: str = "fp8",
                _MX_FMT[x.fmt][0], w.codes.data_ptr(), w.scales.data_ptr(), _MX_FMT[w.fmt][0], m, n, k,
                out.data_ptr(), _ld(out), dt)
     return out
+
+
+# ---------------------------------------------------------------------------------------------
+# Rotary positions with several axes (beside kernels.py:206-348, whose angles are one axis' tables)
+# ---------------------------------------------------------------------------------------------
+
+ROPE_AXES_PAIRS = 512  # rotated pairs of a head at most
+_WIDE_DTYPES = {torch.float16: DTYPE_F16, torch.bfloat16: _lib.DTYPE_BF16, torch.float32: DTYPE_F32}
+_POS_TYPES = {torch.int64: _lib.POS_I64, torch.int32: _lib.POS_I32, torch.float32: _lib.POS_F32}
+
+
+class RopeAxes:
+    """Which axis and frequency turn each pair of a head: pair i by pos[axis[i]] * freq[i] (radians per
+    position). The pairs are the elements (i, i + P) of a head, or (2 i, 2 i + 1) with ``adjacent``;
+    elements past the P pairs are left as they are."""
+
+    def __init__(self, axis, freq, head_dim: int, adjacent: bool = False, device="cuda"):
+        axis, freq = [int(a) for a in axis], [float(f) for f in freq]
+        self.pairs, self.head_dim, self.adjacent = len(axis), int(head_dim), bool(adjacent)
+        if not axis or len(freq) != len(axis):
+            raise ValueError(f"RopeAxes: {len(axis)} axes for {len(freq)} frequencies")
+        if 2 * self.pairs > self.head_dim or self.pairs > ROPE_AXES_PAIRS:
+            raise ValueError(f"RopeAxes: {self.pairs} pairs in heads of {head_dim} (at most {ROPE_AXES_PAIRS})")
+        if min(axis) < 0 or max(axis) > 255:
+            raise ValueError("RopeAxes: axes are numbered 0 to 255")
+        if not all(math.isfinite(f) for f in freq):
+            raise ValueError("RopeAxes: a frequency is not finite")
+        self.n_axes = max(axis) + 1
+        self.axis = torch.tensor(axis, dtype=torch.uint8, device=device)
+        self.turns = torch.tensor([f / (2.0 * math.pi) for f in freq], dtype=torch.float64, device=device)
+
+    @classmethod
+    def sections(cls, sections, theta: float, head_dim: int, device="cuda", order: str = "blocks",
+                 restart: bool = False, adjacent: bool = False) -> "RopeAxes":
+        """``sections``: pairs per axis. ``order`` "blocks" gives the first sections[0] pairs to axis 0, the
+        next to axis 1 and so on; "cycle" deals them in turn (0, 1, 2, 0, 1, ...) while an axis has pairs
+        left. Frequencies theta^(-i / P) by the pair's place i, or, with ``restart``, theta^(-j / S) by its
+        place j among the S pairs of its axis."""
+        sections = [int(n) for n in sections]
+        if not sections or min(sections) < 0 or sum(sections) == 0:
+            raise ValueError(f"RopeAxes: bad sections {sections}")
+        if not theta > 0:
+            raise ValueError(f"RopeAxes: theta must be positive, got {theta}")
+        if order == "blocks":
+            axis = [a for a, n in enumerate(sections) for _ in range(n)]
+        elif order == "cycle":
+            axis = [a for j in range(max(sections)) for a, n in enumerate(sections) if j < n]
+        else:
+            raise ValueError(f"RopeAxes: order must be 'blocks' or 'cycle', got {order!r}")
+        total, seen, freq = len(axis), [0] * len(sections), []
+        for i, a in enumerate(axis):
+            freq.append(theta ** (-(seen[a] / sections[a] if restart else i / total)))
+            seen[a] += 1
+        return cls(axis, freq, head_dim, adjacent, device)
+
+    @property
+    def device(self) -> torch.device:
+        return self.axis.device
+
+
+def _rope_axes_heads(fn: str, x: torch.Tensor, axes: RopeAxes, name: str) -> torch.Tensor:
+    if x.dim() != 3 or x.shape[2] != axes.head_dim:
+        raise ValueError(f"{fn}: {name} must be [N, heads, {axes.head_dim}], got {tuple(x.shape)}")
+    if x.dtype not in _WIDE_DTYPES:
+        raise TypeError(f"{fn}: unsupported dtype {x.dtype} (fp16, bf16 or fp32)")
+    return x if x.stride(2) == 1 else x.contiguous()
+
+
+def _rope_axes(fn: str, q: torch.Tensor, k: torch.Tensor | None, pos: torch.Tensor, axes: RopeAxes,
+               inverse: bool):
+    q = _rope_axes_heads(fn, q, axes, "q")
+    n, hq, d = q.shape
+    hk = 0
+    if k is not None:
+        k = _rope_axes_heads(fn, k, axes, "k")
+        hk = k.shape[1]
+        if k.dtype != q.dtype or k.shape[0] != n:
+            raise ValueError(f"{fn}: k must be {q.dtype} with {n} tokens")
+    if pos.dtype not in _POS_TYPES:
+        raise TypeError(f"{fn}: positions must be int64, int32 or fp32, got {pos.dtype}")
+    if pos.dim() != 2 or pos.shape[1] != n or pos.shape[0] < axes.n_axes:
+        raise ValueError(f"{fn}: positions must be [{axes.n_axes}, {n}], got {tuple(pos.shape)}")
+    _same_device(fn, q, k, pos, axes.axis)
+    if pos.stride(1) != 1 and n > 1:
+        pos = pos.contiguous()
+    q_out = torch.empty((n, hq, d), dtype=q.dtype, device=q.device)
+    k_out = None if k is None else torch.empty((n, hk, d), dtype=q.dtype, device=q.device)
+    if n == 0 or hq + hk == 0:
+        return q_out, k_out
+    _mx_launch("rope_axes", lambda: (2 * n * (hq + hk) * d * q.element_size() + pos.numel() * pos.element_size(),
+                                     6.0 * n * (hq + hk) * axes.pairs),
+               q, "rus_rope_axes", q.data_ptr(), q.stride(0), q.stride(1), hq, q_out.data_ptr(),
+               _ptr(k), 0 if k is None else k.stride(0), 0 if k is None else k.stride(1), hk, _ptr(k_out), n, d,
+               axes.pairs, 1 if axes.adjacent else 0, pos.data_ptr(), _POS_TYPES[pos.dtype], pos.stride(0),
+               axes.n_axes, axes.axis.data_ptr(), axes.turns.data_ptr(), 1 if inverse else 0, _WIDE_DTYPES[q.dtype])
+    return q_out, k_out
+
+
+def rope_axes_fwd(q: torch.Tensor, k: torch.Tensor | None, pos: torch.Tensor, axes: RopeAxes):
+    """(q, k) with their pairs turned by ``axes`` at the positions pos [axes, N] (int64, int32 or fp32):
+    q [N, h_q, d] and k [N, h_k, d] (or None) fp16, bf16 or fp32, views of a fused projection's rows as they
+    are; the results are contiguous."""
+    return _rope_axes("rope_axes_fwd", q, k, pos, axes, False)
+
+
+def rope_axes_bwd(dq: torch.Tensor, dk: torch.Tensor | None, pos: torch.Tensor, axes: RopeAxes):
+    """Gradients of ``rope_axes_fwd``'s inputs: its results' gradients turned back."""
+    return _rope_axes("rope_axes_bwd", dq, dk, pos, axes, True)
+
+
+# ---------------------------------------------------------------------------------------------
+# Attention with capped scores, a bias by distance and a prefix (beside ops.py:669-696)
+# ---------------------------------------------------------------------------------------------
+
+
+def _masked_heads(fn: str, x: torch.Tensor, name: str, like: torch.Tensor) -> torch.Tensor:
+    if x.dim() != 3 or x.shape[2] != like.shape[2]:
+        raise ValueError(f"{fn}: {name} must be [tokens, heads, {like.shape[2]}], got {tuple(x.shape)}")
+    if x.dtype != like.dtype:
+        raise TypeError(f"{fn}: {name} must be {like.dtype}, got {x.dtype}")
+    if x.numel() and (x.stride(2) != 1 or x.stride(0) % 8 or x.stride(1) % 8 or x.data_ptr() % 16):
+        return x.contiguous()
+    return x
+
+
+def _masked_ints(fn: str, t: torch.Tensor, name: str, n: int | None) -> None:
+    if t.dtype != torch.int32 or t.dim() != 1 or not t.is_contiguous() or (n is not None and t.numel() != n):
+        raise ValueError(f"{fn}: {name} must be a contiguous int32 tensor"
+                         f"{'' if n is None else f' with {n} entries'}")
+
+
+class _MaskedCall:
+    """Checked operands of one call: tensors that the launch addresses, and its arguments in order."""
+
+    def __init__(self, fn, q, k, v, cu_q, cu_k, causal, prefix, softcap, slopes, scale, max_q, max_k):
+        if q.dim() != 3 or q.shape[2] not in (64, 128):
+            raise ValueError(f"{fn}: q must be [tokens, heads, 64 or 128], got {tuple(q.shape)}")
+        if q.dtype not in (torch.float16, torch.bfloat16):
+            raise TypeError(f"{fn}: unsupported dtype {q.dtype} (fp16 or bf16)")
+        self.q, self.k, self.v = (_masked_heads(fn, t, name, q) for t, name in ((q, "q"), (k, "k"), (v, "v")))
+        nq, hq, d = q.shape
+        nk, hkv = k.shape[:2]
+        if v.shape != k.shape:
+            raise ValueError(f"{fn}: k {tuple(k.shape)} and v {tuple(v.shape)} differ")
+        if hkv == 0 or hq == 0 or hq % hkv:
+            raise ValueError(f"{fn}: h_q={hq} is not a multiple of h_kv={hkv}")
+        _masked_ints(fn, cu_q, "cu_q", None)
+        if cu_q.numel() < 2:
+            raise ValueError(f"{fn}: cu_q must have a start and an end for each row")
+        if cu_k is None:
+            if nq != nk:
+                raise ValueError(f"{fn}: {nq} queries and {nk} keys need a cu_k of their own")
+            cu_k = cu_q
+        n_seq = cu_q.numel() - 1
+        _masked_ints(fn, cu_k, "cu_k", n_seq + 1)
+        if prefix is not None:
+            _masked_ints(fn, prefix, "prefix", n_seq)
+        if slopes is not None and (slopes.dtype != torch.float32 or slopes.shape != (hq,) or not slopes.is_contiguous()):
+            raise ValueError(f"{fn}: slopes must be contiguous fp32 [{hq}]")
+        softcap = 0.0 if softcap is None else float(softcap)
+        scale = 1.0 / math.sqrt(d) if scale is None else float(scale)
+        if not 0.0 <= softcap < math.inf:
+            raise ValueError(f"{fn}: softcap must be positive, or 0 for none, got {softcap}")
+        if not 0.0 < scale < math.inf:
+            raise ValueError(f"{fn}: scale must be positive and finite, got {scale}")
+        _same_device(fn, q, k, v, cu_q, cu_k, prefix, slopes)
+        self.max_q = nq if max_q is None else int(max_q)
+        self.max_k = nk if max_k is None else int(max_k)
+        if self.max_q < 0 or self.max_k < 0:
+            raise ValueError(f"{fn}: max_q={max_q} max_k={max_k}")
+        self.nq, self.nk, self.hq, self.hkv, self.d, self.n_seq = nq, nk, hq, hkv, d, n_seq
+        self.kept = cu_q, cu_k, prefix, slopes
+        self.sizes = (n_seq, nq, nk, self.max_q, self.max_k, hq, hkv, d)
+        self.qkv = (self.q.data_ptr(), self.q.stride(0), self.q.stride(1), self.k.data_ptr(), self.k.stride(0),
+                    self.k.stride(1), self.v.data_ptr(), self.v.stride(0), self.v.stride(1))
+        self.scores = (scale, 1 if causal else 0, _ptr(prefix), softcap, _ptr(slopes), _WIDE_DTYPES[q.dtype])
+
+    def workspace(self, backward: int) -> tuple:
+        got = ctypes.c_int64()
+        _lib.call("rus_attn_masked_workspace", *self.sizes, backward, ctypes.byref(got))
+        self.ws = torch.empty(got.value, dtype=torch.float32, device=self.q.device) if got.value else None
+        return _ptr(self.ws), got.value
+
+    def cost(self, backward: bool):  # visible pairs are known on the device only: every pair of the longest rows
+        pairs = float(self.max_k) * self.nq * self.hq * self.d
+        nbytes = 2 * (2 * self.nq * self.hq + 2 * self.nk * self.hkv) * self.d * (2 if backward else 1)
+        return nbytes, (10.0 if backward else 4.0) * pairs
+
+
+def attn_masked_fwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: torch.Tensor,
+                    cu_k: torch.Tensor | None = None, causal: bool = True, prefix: torch.Tensor | None = None,
+                    softcap: float | None = None, slopes: torch.Tensor | None = None,
+                    scale: float | None = None, max_q: int | None = None, max_k: int | None = None):
+    """(out [n_q, h_q, d] like q, lse [h_q, n_q] fp32) of attention over packed rows: row s has the queries
+    [cu_q[s], cu_q[s + 1]) and the keys [cu_k[s], cu_k[s + 1]) (int32 on the device; cu_k None: the same
+    rows), its queries standing at the end of its keys (one new token over a cache: a row of one query).
+
+    A query at position p sees key j when ``causal`` is false, j <= p, or j < prefix[s] (int32 [rows]). Scores are
+    scale q.k (default d^-1/2), with ``softcap`` c > 0 capped to c tanh(. / c), with ``slopes`` (fp32 [h_q]) less
+    slopes[h] |p - j|. A query that sees nothing, or belongs to no row, gets zeros and lse -inf; what hidden keys
+    hold does not matter. q, k, v fp16 or bf16, d 64 or 128, h_q a multiple of h_kv, strided as a fused projection
+    leaves them. ``max_q`` and ``max_k``: the longest row's queries and keys (default: all tokens); they choose
+    how the work is split, and a row may not have more queries than max_q."""
+    fn = "attn_masked_fwd"
+    c = _MaskedCall(fn, q, k, v, cu_q, cu_k, causal, prefix, softcap, slopes, scale, max_q, max_k)
+    out = torch.empty((c.nq, c.hq, c.d), dtype=q.dtype, device=q.device)
+    lse = torch.empty((c.hq, c.nq), dtype=torch.float32, device=q.device)
+    if c.nq:
+        cu_q, cu_k = c.kept[:2]
+        _mx_launch("attn_masked_fwd", lambda: c.cost(False), q, "rus_attn_masked_fwd", *c.qkv, cu_q.data_ptr(),
+                   cu_k.data_ptr(), *c.sizes, *c.scores, out.data_ptr(), lse.data_ptr(), *c.workspace(0))
+    return out, lse
+
+
+def attn_masked_bwd(dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: torch.Tensor,
+                    lse: torch.Tensor, cu_q: torch.Tensor, cu_k: torch.Tensor | None = None, causal: bool = True,
+                    prefix: torch.Tensor | None = None, softcap: float | None = None,
+                    slopes: torch.Tensor | None = None, scale: float | None = None, max_q: int | None = None,
+                    max_k: int | None = None):
+    """(dq, dk, dv) of ``attn_masked_fwd`` for the gradient of its out, given its out and lse. dk and dv add the
+    query heads of a KV head in a fixed order in fp32 and are rounded once."""
+    fn = "attn_masked_bwd"
+    c = _MaskedCall(fn, q, k, v, cu_q, cu_k, causal, prefix, softcap, slopes, scale, max_q, max_k)
+    if dout.shape != q.shape or out.shape != q.shape:
+        raise ValueError(f"{fn}: dout and out must be {tuple(q.shape)}, got {tuple(dout.shape)}, {tuple(out.shape)}")
+    dout = _masked_heads(fn, dout, "dout", q)
+    if out.dtype != q.dtype or not out.is_contiguous():
+        raise ValueError(f"{fn}: out must be contiguous {q.dtype}")
+    if lse.dtype != torch.float32 or lse.shape != (c.hq, c.nq) or not lse.is_contiguous():
+        raise ValueError(f"{fn}: lse must be contiguous fp32 [{c.hq}, {c.nq}]")
+    _same_device(fn, q, dout, out, lse)
+    dq = torch.empty((c.nq, c.hq, c.d), dtype=q.dtype, device=q.device)
+    dk, dv = (torch.empty((c.nk, c.hkv, c.d), dtype=q.dtype, device=q.device) for _ in range(2))
+    if c.nq or c.nk:
+        cu_q, cu_k = c.kept[:2]
+        _mx_launch("attn_masked_bwd", lambda: c.cost(True), q, "rus_attn_masked_bwd", dout.data_ptr(), dout.stride(0),
+                   dout.stride(1), *c.qkv, out.data_ptr(), lse.data_ptr(), cu_q.data_ptr(), cu_k.data_ptr(),
+                   *c.sizes, *c.scores, dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), *c.workspace(1))
+    return dq, dk, dv
+
+
+# ---------------------------------------------------------------------------------------------
+# Distillation from a teacher's top logits over the lm_head (beside ops.py:174-349)
+# ---------------------------------------------------------------------------------------------
+
+DISTILL_ENTRIES = 1024  # teacher entries per token at most
+
+
+def _teacher(fn: str, ids: torch.Tensor, logits: torch.Tensor, n_tok: int):
+    """(ids, logits) as contiguous [n_tok, K] rows."""
+    if ids.dtype not in (torch.int64, torch.int32):
+        raise TypeError(f"{fn}: teacher ids must be int64 or int32, got {ids.dtype}")
+    if logits.dtype not in _WIDE_DTYPES:
+        raise TypeError(f"{fn}: teacher logits must be fp32, fp16 or bf16, got {logits.dtype}")
+    if ids.dim() < 1 or ids.shape != logits.shape or ids.numel() != n_tok * ids.shape[-1]:
+        raise ValueError(f"{fn}: teacher ids {tuple(ids.shape)} and logits {tuple(logits.shape)} must both be "
+                         f"[{n_tok}, K]")
+    if not 1 <= ids.shape[-1] <= DISTILL_ENTRIES:
+        raise ValueError(f"{fn}: {ids.shape[-1]} teacher entries per token (1 to {DISTILL_ENTRIES})")
+    k = ids.shape[-1]
+    return ids.reshape(n_tok, k).contiguous(), logits.detach().reshape(n_tok, k).contiguous()
+
+
+class LMHeadDistill:
+    """One pass of the distillation loss over vocabulary chunks (in order), as ``LMHeadPass``: per chunk the
+    statistics GEMM with P, the rescaling of half tiles, the teacher's entries taken out of P, and the split-K
+    product into fp32 partials; ``finish`` forms the loss and, with the entries back in fp32, the hidden gradient."""
+
+    def __init__(self, n_tok: int, d: int, n_vocab: int, chunk: int, ids: torch.Tensor, logits: torch.Tensor,
+                 temperature: float, need_grad: bool):
+        device = ids.device
+        self.n_tok, self.d, self.n_vocab, self.chunk = n_tok, d, n_vocab, int(chunk)
+        self.ids, self.logits, self.t, self.need_grad = ids, logits, float(temperature), need_grad
+        self.entries = (ids.data_ptr(), 1 if ids.dtype == torch.int32 else 0)
+        self.teacher = (*self.entries, logits.data_ptr(), _WIDE_DTYPES[logits.dtype], ids.shape[1])
+        self.parts = torch.empty((2, lm_head_num_parts(n_vocab), n_tok), dtype=torch.float32, device=device)
+        self.done = 0
+        if need_grad:
+            cols = min(self.chunk, n_vocab)
+            self.chunk_max = torch.zeros((-(-n_vocab // self.chunk), n_tok), dtype=torch.float32, device=device)
+            self.p = torch.empty((n_tok, _round_up(cols, LM_K)), dtype=torch.float16, device=device)
+            self.half_ref = torch.empty((2 * lm_head_num_parts(cols), n_tok), dtype=torch.float32, device=device)
+            rows = torch.empty((6, n_tok), dtype=torch.float32, device=device).unbind(0)
+            self.state, self.m_run, self.alpha = (rows[0:2], rows[2:4]), rows[4], rows[5]
+            n_cu = cu_count(device)
+            tiles = -(-n_tok // 256) * -(-d // 256)
+            splits = lm_head_split_count(n_tok, d, cols, n_cu, max_split=max(1, n_cu // tiles))
+            self.dparts = torch.empty((splits, n_tok, d), dtype=torch.float32, device=device)
+
+    def add_chunk(self, hidden: torch.Tensor, w_rows: torch.Tensor, w_t: torch.Tensor | None, start: int) -> None:
+        """Vocabulary rows [start, start + len(w_rows)) with their transpose ``w_t`` [d, >= rows] (needed with
+        the gradient only)."""
+        n, c, tok = w_rows.shape[0], self.done, self.n_tok
+        m, s = self.parts.unbind(0)
+        before = self.state[(c + 1) % 2] if self.need_grad and c else (None, None)
+        probs = (None, 0, None, None, None)
+        if self.need_grad:
+            probs = (self.p.data_ptr(), self.p.stride(0), _ptr(before[0]), self.half_ref.data_ptr(),
+                     self.chunk_max[c].data_ptr())
+        _launch("lmhead_distill_fwd", 2 * ((tok + n) * self.d + (tok * n if self.need_grad else 0)),
+                2.0 * tok * n * self.d, "rus_lmhead_distill_fwd", hidden.data_ptr(), w_rows.data_ptr(), tok, self.d,
+                hidden.stride(0), w_rows.stride(0), n, self.t, m.data_ptr(), s.data_ptr(), start // LM_TILE, tok,
+                *probs, _stream(hidden))
+        if self.need_grad:
+            after = self.state[c % 2]
+            _launch("lmhead_ce_probs_rescale", 20 * tok, 0, "rus_lmhead_ce_probs_rescale", self.p.data_ptr(),
+                    self.p.stride(0), tok, n, self.half_ref.data_ptr(), tok, self.chunk_max[c].data_ptr(),
+                    _ptr(before[0]), _ptr(before[1]), after[0].data_ptr(), after[1].data_ptr(),
+                    self.alpha.data_ptr(), self.m_run.data_ptr(), _stream(hidden))
+            _launch("lmhead_distill_blank", 14 * self.ids.numel(), 0, "rus_lmhead_distill_blank", self.p.data_ptr(),
+                    self.p.stride(0), tok, n, start, *self.teacher, self.n_vocab, self.t, _stream(hidden))
+            lm_head_ce_grad_hidden_scaled(self.p, w_t, n, self.dparts, c > 0, self.alpha)
+        self.done = c + 1
+
+    def finish(self, hidden: torch.Tensor, w_rows: torch.Tensor, num_items_in_batch=None):
+        """(loss, kl, denom, dh): loss and denom one element each, kl [n_tok], dh fp32 [n_tok, d] times 2^16
+        (None without the gradient). ``w_rows``: the whole weight, on the device or pinned on the host."""
+        tok, k, dev = self.n_tok, self.ids.shape[1], hidden.device
+        rows = torch.empty((3, tok), dtype=torch.float32, device=dev)
+        kl, lse, taught = rows.unbind(0)
+        out = torch.empty(2, dtype=torch.float32, device=dev)
+        coef = torch.empty((tok, k), dtype=torch.float32, device=dev) if self.need_grad else None
+        m, s = self.parts.unbind(0)
+        items = _num_items(num_items_in_batch, dev)
+        _launch("lmhead_distill_entries", 2 * tok * k * self.d + 8 * m.numel(), 2.0 * tok * k * self.d,
+                "rus_lmhead_distill_entries", hidden.data_ptr(), hidden.stride(0), w_rows.data_ptr(),
+                w_rows.stride(0), self.n_vocab, tok, self.d, *self.teacher, self.t, m.data_ptr(), s.data_ptr(),
+                m.shape[0], tok, _ptr(items), kl.data_ptr(), lse.data_ptr(), taught.data_ptr(), _ptr(coef),
+                out.data_ptr(), out.data_ptr() + 4, _stream(hidden))
+        dh = None
+        if self.need_grad:
+            dh = torch.empty((tok, self.d), dtype=torch.float32, device=dev)
+            _launch("lmhead_distill_finish", 4 * self.dparts.numel() + 2 * tok * k * self.d + 4 * dh.numel(),
+                    2.0 * tok * k * self.d, "rus_lmhead_distill_finish", self.dparts.data_ptr(),
+                    self.dparts.shape[0], tok, self.d, self.m_run.data_ptr(), lse.data_ptr(), taught.data_ptr(),
+                    coef.data_ptr(), *self.entries, k, w_rows.data_ptr(), w_rows.stride(0), self.n_vocab,
+                    out.data_ptr() + 4, self.t, dh.data_ptr(), _stream(hidden))
+        return out[0:1], kl, out[1:2], dh
+
+
+def _temperature(fn: str, t) -> float:
+    t = float(t)
+    if not 1e-6 <= t <= 1e6:
+        raise ValueError(f"{fn}: temperature must lie in [1e-6, 1e6], got {t}")
+    return t
+
+
+def lm_head_distill(hidden: torch.Tensor, weight: torch.Tensor, teacher_ids: torch.Tensor,
+                    teacher_logits: torch.Tensor, temperature: float = 1.0, num_items_in_batch=None,
+                    v_chunk: int | None = None, need_grad: bool = True, weight_t: torch.Tensor | None = None):
+    """Distillation from a teacher's top logits over a device-resident fp16 lm_head weight [V, d], d a multiple
+    of 64: (loss, kl, denom, dh).
+
+    Token by token the teacher gives K vocabulary ids and their logits ([n_tok, K]; int64 or int32, fp32, fp16 or
+    bf16). q is the softmax of its logits / T over them, p the student's softmax of hidden W^T / T over the whole
+    vocabulary: kl [n_tok] = sum q (ln q - ln p), loss = T^2 sum(kl) / denom, dh = 2^16 times the loss' gradient
+    in fp32 [n_tok, d] (None without ``need_grad``; ``lm_head_dh_reduce`` undoes the factor). An id outside the
+    vocabulary or a logit of -inf is no entry; a token without entries has kl 0 and gradient 0. denom is
+    num_items_in_batch, else the tokens with entries, at least 1. No [n_tok, V] array exists: ``v_chunk`` (a
+    multiple of 256) rows of the vocabulary at a time, by default as ``ops.lm_head_layout`` chooses. ``weight_t`` is
+    W^T [d, >= round_up(V, 64)] (built and cached on the weight when not given)."""
+    fn = "lm_head_distill"
+    t = _temperature(fn, temperature)
+    if hidden.dim() != 2 or weight.dim() != 2 or weight.shape[1] != hidden.shape[1] or weight.shape[0] == 0:
+        raise ValueError(f"{fn}: hidden [N, d] and weight [V, d] expected, got {tuple(hidden.shape)}, "
+                         f"{tuple(weight.shape)}")
+    n_tok, d = hidden.shape
+    if d % LM_K or d == 0:
+        raise ValueError(f"{fn}: the hidden size must be a multiple of {LM_K}, got {d}")
+    ids, logits = _teacher(fn, teacher_ids, teacher_logits, n_tok)
+    h = _lm_operand(fn, hidden, d, "hidden")
+    w = _lm_operand(fn, weight, d, "weight")
+    _same_device(fn, h, w, ids, logits, weight_t)
+    n_vocab = w.shape[0]
+    with torch.cuda.device(h.device):
+        if n_tok == 0:
+            out = torch.zeros(1, dtype=torch.float32, device=h.device)
+            denom = torch.clamp(_num_items(num_items_in_batch, h.device), min=1.0) \
+                if num_items_in_batch is not None else torch.ones_like(out)
+            return out, torch.empty(0, dtype=torch.float32, device=h.device), denom, \
+                torch.empty((0, d), dtype=torch.float32, device=h.device) if need_grad else None
+        chunk = lm_head_chunk_cols(n_tok, n_vocab, cu_count(h.device), at_least_two=True) if v_chunk is None \
+            else int(v_chunk)
+        if chunk <= 0 or (chunk < n_vocab and chunk % LM_TILE):
+            raise ValueError(f"{fn}: v_chunk must be a positive multiple of {LM_TILE}")
+        wt = None
+        if need_grad:
+            wt = weight_t if weight_t is not None else lm_head_weight_t(weight)
+            if wt.dtype != torch.float16 or wt.dim() != 2 or wt.shape[0] != d or wt.stride(1) != 1 or \
+                    wt.shape[1] < _round_up(n_vocab, LM_K):
+                raise ValueError(f"{fn}: weight_t must be fp16 [{d}, >= {_round_up(n_vocab, LM_K)}] with "
+                                 "contiguous rows")
+        else:
+            chunk = n_vocab  # no P is kept: one launch over the whole vocabulary
+        hp = LMHeadDistill(n_tok, d, n_vocab, chunk, ids, logits, t, need_grad)
+        for start in range(0, n_vocab, chunk):
+            end = min(start + chunk, n_vocab)
+            hp.add_chunk(h, w[start:end], None if wt is None else wt[:, start:], start)
+        return hp.finish(h, w, num_items_in_batch)

@@ -256,6 +256,66 @@ def mx_norm_mlp(x, weight, w_gate_up, w_down, eps: float = 1e-6, residual=None):
 
 
 # ---------------------------------------------------------------------------------------------
+# Rotary positions with several axes, and attention with caps, a bias by distance and a prefix
+# ---------------------------------------------------------------------------------------------
+
+
+class FusedRopeAxesFn(torch.autograd.Function):
+    """(q, k) turned by ``kernels.RopeAxes`` at their positions; the backward turns the gradients back."""
+
+    @staticmethod
+    def forward(ctx, q, k, pos, axes, inverse=False):
+        ctx.axes, ctx.inverse, ctx.with_k = axes, inverse, k is not None
+        ctx.save_for_backward(pos)
+        q, k = (K.rope_axes_bwd if inverse else K.rope_axes_fwd)(q, k, pos, axes)
+        return (q, k) if ctx.with_k else q
+
+    @staticmethod
+    def backward(ctx, dq, dk=None):
+        (pos,) = ctx.saved_tensors
+        out = FusedRopeAxesFn.apply(dq, dk, pos, ctx.axes, not ctx.inverse)
+        return (*out, None, None, None) if ctx.with_k else (out, None, None, None, None)
+
+
+def rope_axes(q, k, pos, axes):
+    """``kernels.rope_axes_fwd`` with gradients of q and k: (q, k), or q alone where k is None."""
+    _no_weight_grad("rope_axes", positions=pos)
+    kept = _leaf_streams("rope_axes", q, k)
+    out = FusedRopeAxesFn.apply(q, k, pos, axes)
+    del kept
+    return out
+
+
+class FusedMaskedAttentionFn(torch.autograd.Function):
+    """``kernels.attn_masked_fwd`` / ``attn_masked_bwd``; keeps q, k, v, the output and lse."""
+
+    @staticmethod
+    def forward(ctx, q, k, v, cu_q, cu_k, prefix, slopes, kw):
+        ctx.kw = kw
+        out, lse = K.attn_masked_fwd(q, k, v, cu_q, cu_k, prefix=prefix, slopes=slopes, **kw)
+        ctx.save_for_backward(q, k, v, out, lse, cu_q, cu_k, prefix, slopes)
+        return out
+
+    @staticmethod
+    def backward(ctx, dout):
+        q, k, v, out, lse, cu_q, cu_k, prefix, slopes = ctx.saved_tensors
+        grads = K.attn_masked_bwd(dout, q, k, v, out, lse, cu_q, cu_k, prefix=prefix, slopes=slopes, **ctx.kw)
+        return (*(_first_order("masked_attention", g) for g in grads), None, None, None, None, None)
+
+
+def masked_attention(q, k, v, cu_q, cu_k=None, causal: bool = True, prefix=None, softcap=None, slopes=None,
+                     scale=None, max_q=None, max_k=None):
+    """Attention over packed rows with gradients of q, k and v (``kernels.attn_masked_fwd`` has the arguments):
+    the output [n_q, h_q, d]. The slopes of the distance bias are fixed."""
+    _no_weight_grad("masked_attention", slopes=slopes)
+    kept = _leaf_streams("masked_attention", q, k, v)
+    out = FusedMaskedAttentionFn.apply(q, k, v, cu_q, cu_k, prefix, slopes, dict(
+        causal=causal, softcap=softcap, scale=scale, max_q=max_q, max_k=max_k))
+    del kept
+    return out
+
+
+# ---------------------------------------------------------------------------------------------
 # Chunked lm_head cross-entropy (solution/ops.py:174-349)
 # ---------------------------------------------------------------------------------------------
 
@@ -347,6 +407,84 @@ def chunked_lm_head(hidden_states, shift_labels, weight_or_host_head, num_items_
     streamed HostHead uses its own chunk)."""
     return FusedChunkedLMHeadFn.apply(hidden_states, shift_labels, weight_or_host_head,
                                       num_items_in_batch, v_chunk)
+
+
+def _distill_streamed(h_2d, ids, logits, head: HostHead, temperature, num_items_in_batch, need_grad):
+    """The distillation loss over a HostHead streamed from pinned host memory, chunk by chunk as
+    ``_lm_head_streamed``; the teacher's rows of W are read from the host by the finishing kernels."""
+    fn = "chunked_distill_head"
+    n_tok, d = h_2d.shape
+    V, vc = head.vocab_size, head.v_chunk
+    ids, logits = K._teacher(fn, ids, logits, n_tok)
+    h = K._lm_operand(fn, h_2d, d, "hidden")
+    K._same_device(fn, h, ids, logits)
+    if head.hidden_size != d or d % K.LM_K:
+        raise ValueError(f"{fn}: the head's hidden size is {head.hidden_size}, got {d} (a multiple of {K.LM_K})")
+    t = K._temperature(fn, temperature)
+    if n_tok == 0:
+        raise ValueError(f"{fn}: no tokens")
+    starts = list(range(0, V, vc))
+    hp = K.LMHeadDistill(n_tok, d, V, vc, ids, logits, t, need_grad)
+    head.prefetch_chunk(0, 0, min(vc, V))
+    for c, s in enumerate(starts):
+        e = min(s + vc, V)
+        if c + 1 < len(starts):
+            head.prefetch_chunk(c + 1, starts[c + 1], min(starts[c + 1] + vc, V))
+        rows = head.get_chunk(c, s, e)
+        rows_t = head.get_chunk_t(c, s, e) if need_grad else None
+        hp.add_chunk(h, rows, rows_t, s)
+        head.release_chunk(c)
+    return hp.finish(h, head.cpu_weight, num_items_in_batch)
+
+
+class FusedDistillHeadFn(torch.autograd.Function):
+    """Loss and per-token KL divergence from a teacher's top logits without the [N, V] logits
+    (``kernels.lm_head_distill``); the hidden gradient (times 2^16) is formed in forward and scaled by the
+    incoming gradient of the loss in backward, as ``FusedChunkedLMHeadFn`` does."""
+
+    @staticmethod
+    def forward(ctx, hidden_states, teacher_ids, teacher_logits, weight_or_host_head, temperature=1.0,
+                num_items_in_batch=None, v_chunk=None):
+        h_2d = hidden_states.reshape(-1, hidden_states.shape[-1])
+        need_grad = bool(ctx.needs_input_grad[0])
+        is_head = isinstance(weight_or_host_head, HostHead)
+        if is_head and not weight_or_host_head.resident:
+            loss, kl, _, dh = _distill_streamed(h_2d, teacher_ids, teacher_logits, weight_or_host_head, temperature,
+                                                num_items_in_batch, need_grad)
+        else:
+            w, wt = weight_or_host_head, None
+            if is_head:
+                w, wt = weight_or_host_head.gpu_weight, weight_or_host_head.gpu_weight_t
+            loss, kl, _, dh = K.lm_head_distill(h_2d, w.detach(), teacher_ids, teacher_logits, temperature,
+                                                num_items_in_batch, v_chunk, need_grad, wt)
+        ctx.save_for_backward(dh)
+        ctx.orig_shape, ctx.orig_dtype = hidden_states.shape, hidden_states.dtype
+        ctx.mark_non_differentiable(kl)
+        return loss[0], kl
+
+    @staticmethod
+    def backward(ctx, grad_loss, _g_kl=None):
+        (dh,) = ctx.saved_tensors
+        if dh is None:
+            return (None,) * 7
+        g = grad_loss.detach().to(torch.float32).reshape(1)
+        d_h = K.lm_head_dh_reduce(dh.unsqueeze(0), 1.0 / PRESCALE_GRAD, ctx.orig_dtype, scale_dev=g)
+        return (_first_order("chunked_distill_head", d_h.view(ctx.orig_shape)),) + (None,) * 6
+
+
+def chunked_distill_head(hidden_states, teacher_ids, teacher_logits, weight_or_host_head, temperature: float = 1.0,
+                         num_items_in_batch=None, v_chunk=None):
+    """(loss, kl) of the distillation loss over the lm_head: hidden_states [..., d] fp16, the teacher's ids and
+    logits [..., K], the frozen head as a weight [V, d] or a ``HostHead`` (``kernels.lm_head_distill`` has the
+    definition). The loss has a gradient with respect to hidden_states; kl [tokens] has none."""
+    fn = "chunked_distill_head"
+    _no_weight_grad(fn, teacher_logits=teacher_logits,
+                    weight=None if isinstance(weight_or_host_head, HostHead) else weight_or_host_head)
+    kept = _leaf_streams(fn, hidden_states)
+    out = FusedDistillHeadFn.apply(hidden_states, teacher_ids, teacher_logits, weight_or_host_head, temperature,
+                                   num_items_in_batch, v_chunk)
+    del kept
+    return out
 
 
 # ---------------------------------------------------------------------------------------------
