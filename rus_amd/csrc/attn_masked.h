@@ -126,14 +126,15 @@ __device__ __forceinline__ bool find_span_block(const int32_t* cu, int n_seq, in
 }
 
 // ---------------------------------------------------------------------------------------------
-// Scores, in log2 units. tanh x = 1 - 2 / (1 + e^{2x}) is good to 2^-23 absolute, i.e. to that part of the cap,
-// which counts where the cap is far above the scores: up to |x| = 1/16 the odd polynomial, 5e-12 away.
+// Scores, in log2 units. tanh x = 1 - 2 / (1 + e^{2x}) is good to 2^-22 absolute, i.e. to that part of the cap, which
+// counts where the cap is far above the scores: up to |x| = 1/4 the odd polynomial to x^9, 9e-9 of x away.
 // ---------------------------------------------------------------------------------------------
-constexpr float kSmallTanh = 0.0625f;
+constexpr float kSmallTanh = 0.25f;
 
 __device__ __forceinline__ float tanh_small(float x) {
   const float z = x * x;
-  float p = __builtin_fmaf(z, -5.3968254e-2f, 1.3333333e-1f);
+  float p = __builtin_fmaf(z, 2.1869489e-2f, -5.3968254e-2f);
+  p = __builtin_fmaf(z, p, 1.3333333e-1f);
   p = __builtin_fmaf(z, p, -3.3333333e-1f);
   return __builtin_fmaf(z * p, x, x);
 }

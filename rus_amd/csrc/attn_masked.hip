@@ -1,40 +1,524 @@
 // Attention over packed rows with a tanh cap on the scores, a bias by distance, a prefix that every query sees, and
 // fewer queries than keys where a cache is read: forward and backward, fp16 / bf16, head dims 64 and 128. The
 // definition is in attn_masked.h.
+#include <type_traits>
+
 #include "attn_masked.h"
+#include "attn_masked_tiles.h"
 
 namespace rus {
 namespace {
 
 constexpr int kWaves = 4, kRows = 128;  // waves of a block, tokens of a block
+constexpr int kFwdTiles = 2;             // key tiles per stage of the forward
 
+// Block id -> (item, head): the query heads of a KV group that work on one item take ids 8 apart, i.e. one XCD (ids go
+// round robin over the 8), so that they read their shared keys from one L2. False past the last item.
+__device__ __forceinline__ bool head_item(const MaskedArgs& a, int n_items, int& item, int& head) {
+  const int grp = a.h_q / a.h_kv, chunk = 8 * grp;
+  const int t = blockIdx.x / chunk, r = blockIdx.x % chunk;
+  const int64_t i = static_cast<int64_t>(t) * chunk + (r & 7) * grp + (r >> 3);
+  item = static_cast<int>(i / a.h_q);
+  head = static_cast<int>(i % a.h_q);
+  return i / a.h_q < n_items;
+}
+
+__device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
+
+__device__ __forceinline__ MaskedRow uniform(MaskedRow r) {
+  return MaskedRow{uniform(r.qa), uniform(r.lq), uniform(r.ka), uniform(r.lk), uniform(r.pre)};
+}
+
+// ---------------------------------------------------------------------------------------------
+// Forward. S^T = K Q^T on 32 NT keys: a lane owns one query (column) and half of the keys; the running maximum and sum
+// are per-lane scalars, and P^T feeds O^T += V^T P^T from the accumulator. m is the running maximum itself at every
+// step, and O is divided by lr, the sum of the rounded P, in which their common rounding cancels (l, of the unrounded,
+// gives the lse).
+// ---------------------------------------------------------------------------------------------
+template <int ND>
+struct FwdState {
+  f32x16 o[ND];
+  float m, l, lr;
+  __device__ __forceinline__ FwdState() : m(-INFINITY), l(0.0f), lr(0.0f) {
+#pragma unroll
+    for (int d = 0; d < ND; ++d) o[d] = f32x16{};
+  }
+};
+
+// left: keys of the lane's query from the first of these on that it sees; whole: every query of the wave sees all.
+// d0: distance of the lane's first element (key 4 h).
+template <typename T, int HD, bool CAP, bool BIAS, int NT>
+__device__ __forceinline__ void fwd_keys(const MaskedArgs& a, const FragLane<HD>& fl, const char* kt, const char* vt,
+                                         const Frag (&qf)[HD / 16], FwdState<HD / 32>& w, float slope2, bool whole,
+                                         int left, float d0, int h) {
+  using L = Tiles<HD>;
+  f32x16 st[NT];
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+    st[n] = f32x16{};
+#pragma unroll
+    for (int s = 0; s < L::kSteps; ++s) st[n] = mfma<T>(fl.frag(kt + n * L::kBytes, s), qf[s], st[n]);
+  }
+  constexpr bool kRaw = !CAP && !BIAS;  // scaled inside the exponential
+  if constexpr (!kRaw) tile_scores<CAP, BIAS, NT, false>(a, slope2, st, st, d0, 1.0f);
+  if (!whole) {
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) st[n][r] = 32 * n + acc_row(r, h) < left ? st[n][r] : -INFINITY;
+  }
+  float mx = -INFINITY;
+#pragma unroll
+  for (int n = 0; n < NT; ++n)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) mx = fmaxf(mx, st[n][r]);
+  const float2 mp = half_pair(mx);
+  mx = fmaxf(mp.x, mp.y);
+  if constexpr (kRaw) mx *= a.sl2;  // scale > 0
+  const float mn = fmaxf(w.m, mx);
+  const float ref = mn == -INFINITY ? 0.0f : mn;  // nothing seen yet: every P is 2^-inf
+  if (__ballot(mx > w.m)) {
+    const float alpha = exp2_raw(w.m - ref);
+    w.l *= alpha;
+    w.lr *= alpha;
+    w.m = mn;
+#pragma unroll
+    for (int d = 0; d < L::kDims; ++d)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) w.o[d][r] *= alpha;
+  }
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+    float rs = 0.0f;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      const float p = exp2_raw(kRaw ? __builtin_fmaf(st[n][r], a.sl2, -ref) : st[n][r] - ref);
+      st[n][r] = p;
+      rs += p;
+    }
+    w.l += rs;  // this lane's 16 keys; the other half's join at the end
+  }
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+    const Frag p0 = frag_acc<T>(st[n], 0), p1 = frag_acc<T>(st[n], 1);
+    w.lr = sum8<T>(p1, sum8<T>(p0, w.lr));
+#pragma unroll
+    for (int d = 0; d < L::kDims; ++d) {
+      w.o[d] = mfma<T>(fl.frag_t(vt + n * L::kBytes, 0, d), p0, w.o[d]);  // O^T += V^T P^T
+      w.o[d] = mfma<T>(fl.frag_t(vt + n * L::kBytes, 1, d), p1, w.o[d]);
+    }
+  }
+}
+
+template <typename T, int HD>
+__device__ __forceinline__ void load_row_frags(Frag (&f)[HD / 16], const T* row, int h) {
+#pragma unroll
+  for (int s = 0; s < HD / 16; ++s) f[s] = *reinterpret_cast<const Frag*>(row + 16 * s + 8 * h);
+}
+
+// 128 queries of one head, 32 to a wave; tiles of 32 keys stream through double-buffered LDS, two to a stage, each
+// copied once for all four waves while the previous stage is used. Hidden keys reach the product as 0 x V: where V is
+// not finite the sums are not either, and such a query is formed again by itself (plain_fwd_row).
 template <typename T, int HD, bool CAP, bool BIAS>
-__global__ __launch_bounds__(64 * kWaves) void masked_fwd_kernel(MaskedArgs a) {
-  int s, b, nb;
-  if (!find_span_block<kRows>(a.cu_q, a.n_seq, static_cast<int>(a.n_q), blockIdx.x, s, b, nb)) return;
-  const MaskedRow r = as_queries(masked_row(a, s), s, a.n_seq);
-  const int wave = threadIdx.x >> 6;
-  for (int i = b * kRows + wave; i < min((b + 1) * kRows, r.lq); i += kWaves)
-    plain_fwd_row<T, HD, CAP, BIAS>(a, r, i, blockIdx.y);
+__device__ __forceinline__ void fwd_block(const MaskedArgs& a, char* buf0, char* buf1) {
+  using L = Tiles<HD>;
+  constexpr int NT = kFwdTiles;
+  int item, head, s, b, nb;
+  if (!head_item(a, a.n_blocks, item, head)) return;
+  if (!find_span_block<kRows>(a.cu_q, a.n_seq, static_cast<int>(a.n_q), item, s, b, nb)) return;
+  const MaskedRow r = uniform(as_queries(masked_row(a, s), s, a.n_seq));
+  b = uniform(nb - 1 - b);  // the last queries see the most keys: first
+  const int g = head / (a.h_q / a.h_kv);
+  const int wave = uniform(static_cast<int>(threadIdx.x) >> 6);
+  const int lane = threadIdx.x & 63, h = lane >> 5, col = lane & 31;
+  const int i0 = b * kRows, iw = i0 + 32 * wave, i = min(iw + col, r.lq - 1);
+  const bool valid = iw + col < r.lq;
+  const int vis = r.vis(i, a.causal);
+  const int tiles = (r.vis(min(i0 + kRows, r.lq) - 1, a.causal) + 31) / 32;
+  const int stages = (tiles + NT - 1) / NT;
+  // Keys that all of the wave's queries see, and that any does.
+  const int vis_all = iw < r.lq ? r.vis(iw, a.causal) : 0;
+  const int mine = iw < r.lq ? (r.vis(min(iw + 31, r.lq - 1), a.causal) + 31) / 32 : 0;
+  const T* kh = token<T>(a.k, r.ka, a.k_st, g, a.k_sh);
+  const T* vh = token<T>(a.v, r.ka, a.v_st, g, a.v_sh);
+  constexpr int C = L::kCopies / kWaves;
+  const TileLane<HD, C> tk(C * wave, lane, a.k_st), tv(C * wave, lane, a.v_st);
+  const FragLane<HD> fl0(lane);
+  const Scorer<CAP, BIAS> sc(a, head);
+  auto copy = [&](char* dst, int j) {
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      const int t = NT * j + n;
+      if (t >= tiles) break;
+      const int rows = r.lk - 32 * t;
+      tk.copy(dst + n * L::kBytes, kh + 32 * t * a.k_st, rows);
+      tv.copy(dst + (NT + n) * L::kBytes, vh + 32 * t * a.v_st, rows);
+    }
+  };
+  if (stages) copy(buf0, 0);
+  Frag qf[L::kSteps];
+  load_row_frags<T, HD>(qf, token<T>(a.q, r.qa + i, a.q_st, head, a.q_sh), h);
+  FwdState<L::kDims> w;
+  stage_barrier();
+  auto stage = [&](const char* cur, char* next, int j) {
+    if (j + 1 < stages) copy(next, j + 1);
+    const char* vt = cur + NT * L::kBytes;
+    const FragLane<HD> fl = fl0.fresh();
+    const int mt = mine - NT * j, k0 = 32 * NT * j;  // this wave's tiles from here on, first key
+    const float d0 = static_cast<float>(r.off() + i - k0 - 4 * h);
+    if (mt >= 2)
+      fwd_keys<T, HD, CAP, BIAS, 2>(a, fl, cur, vt, qf, w, sc.slope2, k0 + 64 <= vis_all, vis - k0, d0, h);
+    else if (mt == 1)
+      fwd_keys<T, HD, CAP, BIAS, 1>(a, fl, cur, vt, qf, w, sc.slope2, k0 + 32 <= vis_all, vis - k0, d0, h);
+    stage_barrier();
+  };
+  for (int j = 0; j < stages; j += 2) {
+    stage(buf0, buf1, j);
+    if (j + 1 < stages) stage(buf1, buf0, j + 1);
+  }
+  if (iw >= r.lq) return;
+  const float2 lp = half_pair(w.l), rp = half_pair(w.lr);
+  const float f = vis > 0 ? 1.0f / (rp.x + rp.y) : 0.0f;
+  if (vis <= 0) {
+#pragma unroll
+    for (int d = 0; d < L::kDims; ++d) w.o[d] = f32x16{};
+  }
+  uint64_t again = __ballot(valid && !all_finite(w.o, f));
+  uint32_t cols = static_cast<uint32_t>(again) | static_cast<uint32_t>(again >> 32);
+  const bool keep = valid && !((cols >> col) & 1);
+  const int64_t t = r.qa + i;
+  store_row<T, L::kDims>(static_cast<T*>(a.out) + (t * a.h_q + head) * HD, w.o, f, h, keep);
+  if (h == 0 && keep) a.lse[head * a.n_q + t] = vis > 0 ? (w.m + log2f(lp.x + lp.y)) * kLn2 : -INFINITY;
+  for (; cols; cols &= cols - 1) plain_fwd_row<T, HD, CAP, BIAS>(a, r, iw + __builtin_ctz(cols), head);
 }
 
 template <typename T, int HD, bool CAP, bool BIAS>
-__global__ __launch_bounds__(64 * kWaves) void masked_bwd_kernel(MaskedArgs a) {
+__global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2, 2))) void masked_fwd_kernel(
+    MaskedArgs a) {
+  __shared__ __attribute__((aligned(16))) char buf0[2 * kFwdTiles * Tiles<HD>::kBytes];
+  __shared__ __attribute__((aligned(16))) char buf1[2 * kFwdTiles * Tiles<HD>::kBytes];
+  fwd_block<T, HD, CAP, BIAS>(a, buf0, buf1);
+}
+
+// ---------------------------------------------------------------------------------------------
+// Backward.
+// ---------------------------------------------------------------------------------------------
+
+// LDS of the backward: the streamed tiles' two buffers, and for the dK / dV blocks the block's V rows and the streamed
+// queries' lse and D.
+struct BwdLds {
+  char* buf0;
+  char* buf1;
+  char* v;
+  float* ld0;  // lse (log2 units) of 32 queries, then D
+  float* ld1;
+};
+
+// dQ of 128 queries: key tiles stream through LDS, each wave owns 32 queries (Q and dO fragments in registers; D from
+// the same fragments).
+template <typename T, int HD, bool CAP, bool BIAS>
+__device__ __forceinline__ void bwd_dq(const MaskedArgs& a, int blk, int head, const BwdLds& lds) {
+  using L = Tiles<HD>;
   int s, b, nb;
-  const int wave = threadIdx.x >> 6, blk = blockIdx.x;
-  if (blk < a.n_kblocks) {
-    const int grp = a.h_q / a.h_kv, head = blockIdx.y;
-    if (head % grp) return;
-    if (!find_span_block<kRows>(a.cu_k, a.n_seq, static_cast<int>(a.n_k), blk, s, b, nb)) return;
-    const MaskedRow r = as_keys(masked_row(a, s), s, a.n_seq);
-    for (int j = b * kRows + wave; j < min((b + 1) * kRows, r.lk); j += kWaves)
-      plain_dkv_row<T, HD, CAP, BIAS>(a, r, j, head, head + grp, nullptr, nullptr);
-    return;
+  if (!find_span_block<kRows>(a.cu_q, a.n_seq, static_cast<int>(a.n_q), blk, s, b, nb)) return;
+  const MaskedRow r = uniform(as_queries(masked_row(a, s), s, a.n_seq));
+  b = uniform(nb - 1 - b);
+  const int g = head / (a.h_q / a.h_kv);
+  const int wave = uniform(static_cast<int>(threadIdx.x) >> 6);
+  const int lane = threadIdx.x & 63, h = lane >> 5, col = lane & 31;
+  const int i0 = b * kRows, iw = i0 + 32 * wave, i = min(iw + col, r.lq - 1);
+  const bool valid = iw + col < r.lq;
+  const int vis = r.vis(i, a.causal);
+  const int tiles = (r.vis(min(i0 + kRows, r.lq) - 1, a.causal) + 31) / 32;
+  const int vis_all = iw < r.lq ? r.vis(iw, a.causal) : 0;
+  const int mine = iw < r.lq ? (r.vis(min(iw + 31, r.lq - 1), a.causal) + 31) / 32 : 0;
+  const T* kh = token<T>(a.k, r.ka, a.k_st, g, a.k_sh);
+  const T* vh = token<T>(a.v, r.ka, a.v_st, g, a.v_sh);
+  constexpr int C = L::kCopies / kWaves;
+  const TileLane<HD, C> tk(C * wave, lane, a.k_st), tv(C * wave, lane, a.v_st);
+  const FragLane<HD> fl0(lane);
+  const Scorer<CAP, BIAS> sc(a, head);
+  auto copy = [&](char* dst, int j) {
+    const int rows = r.lk - 32 * j;
+    tk.copy(dst, kh + 32 * j * a.k_st, rows);
+    tv.copy(dst + L::kBytes, vh + 32 * j * a.v_st, rows);
+  };
+  if (tiles) copy(lds.buf0, 0);
+  const int64_t t = r.qa + i;
+  Frag qf[L::kSteps], df[L::kSteps];
+  load_row_frags<T, HD>(qf, token<T>(a.q, t, a.q_st, head, a.q_sh), h);
+  load_row_frags<T, HD>(df, token<T>(a.dout, t, a.do_st, head, a.do_sh), h);
+  float ds = 0.0f;
+  {
+    Frag of[L::kSteps];
+    load_row_frags<T, HD>(of, static_cast<const T*>(a.o) + (t * a.h_q + head) * HD, h);
+#pragma unroll
+    for (int k = 0; k < L::kSteps; ++k) ds = dot8<T>(of[k], df[k], ds);
   }
-  if (!find_span_block<kRows>(a.cu_q, a.n_seq, static_cast<int>(a.n_q), blk - a.n_kblocks, s, b, nb)) return;
-  const MaskedRow r = as_queries(masked_row(a, s), s, a.n_seq);
-  for (int i = b * kRows + wave; i < min((b + 1) * kRows, r.lq); i += kWaves)
-    plain_dq_row<T, HD, CAP, BIAS>(a, r, i, blockIdx.y);
+  const float2 dp2 = half_pair(ds);
+  const float dsum = dp2.x + dp2.y;
+  const float lse2 = a.lse[head * a.n_q + t] * kLog2e;
+  f32x16 dq[L::kDims];
+#pragma unroll
+  for (int d = 0; d < L::kDims; ++d) dq[d] = f32x16{};
+  stage_barrier();
+  auto stage = [&](const char* kt, char* next, int j) {
+    if (j + 1 < tiles) copy(next, j + 1);
+    const char* vt = kt + L::kBytes;
+    const FragLane<HD> fl = fl0.fresh();
+    if (j < mine) {
+      f32x16 st[1] = {f32x16{}}, dp = f32x16{}, f[1];
+#pragma unroll
+      for (int k = 0; k < L::kSteps; ++k) {
+        st[0] = mfma<T>(fl.frag(kt, k), qf[k], st[0]);  // S^T = K Q^T
+        dp = mfma<T>(fl.frag(vt, k), df[k], dp);        // dP^T = V dO^T
+      }
+      constexpr bool kRaw = !CAP && !BIAS;
+      if constexpr (!kRaw)
+        tile_scores<CAP, BIAS, 1, true>(a, sc.slope2, st, f, static_cast<float>(r.off() + i - 32 * j - 4 * h), 1.0f);
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        const float p = exp2_raw(kRaw ? __builtin_fmaf(st[0][e], a.sl2, -lse2) : st[0][e] - lse2);
+        st[0][e] = p * (dp[e] - dsum);
+        if constexpr (CAP) st[0][e] *= f[0][e];
+      }
+      if (32 * j + 32 > vis_all) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) st[0][e] = 32 * j + acc_row(e, h) < vis ? st[0][e] : 0.0f;
+      }
+      const Frag s0 = frag_acc<T>(st[0], 0), s1 = frag_acc<T>(st[0], 1);
+#pragma unroll
+      for (int d = 0; d < L::kDims; ++d) {
+        dq[d] = mfma<T>(fl.frag_t(kt, 0, d), s0, dq[d]);  // dQ^T += K^T dS^T
+        dq[d] = mfma<T>(fl.frag_t(kt, 1, d), s1, dq[d]);
+      }
+    }
+    stage_barrier();
+  };
+  for (int j = 0; j < tiles; j += 2) {
+    stage(lds.buf0, lds.buf1, j);
+    if (j + 1 < tiles) stage(lds.buf1, lds.buf0, j + 1);
+  }
+  if (iw >= r.lq) return;
+  uint64_t again = __ballot(valid && !all_finite(dq, a.scale));
+  uint32_t cols = static_cast<uint32_t>(again) | static_cast<uint32_t>(again >> 32);
+  store_row<T, L::kDims>(static_cast<T*>(a.out) + (t * a.h_q + head) * HD, dq, a.scale, h,
+                         valid && !((cols >> col) & 1));
+  for (; cols; cols &= cols - 1) plain_dq_row<T, HD, CAP, BIAS>(a, r, iw + __builtin_ctz(cols), head);
+}
+
+// dK and dV of 128 keys for one query head: Q and dO tiles stream through LDS with their lse and D, each wave owns 32
+// keys (K fragments in registers, V fragments from LDS). A lane owns one key (column of S = Q K^T) and half of the
+// queries.
+template <typename T, int HD, bool CAP, bool BIAS>
+__device__ __forceinline__ void bwd_dkdv(const MaskedArgs& a, int blk, int head, const BwdLds& lds) {
+  using L = Tiles<HD>;
+  int s, b, nb;
+  if (!find_span_block<kRows>(a.cu_k, a.n_seq, static_cast<int>(a.n_k), blk, s, b, nb)) return;
+  const MaskedRow r = uniform(as_keys(masked_row(a, s), s, a.n_seq));
+  b = uniform(b);
+  const int grp = a.h_q / a.h_kv, g = head / grp;
+  const int tid = threadIdx.x, wave = uniform(tid >> 6);
+  const int lane = tid & 63, h = lane >> 5, col = lane & 31;
+  const int k0 = b * kRows, kw = k0 + 32 * wave, kj = kw + col, kc = min(kj, r.lk - 1);
+  // The block's query tiles run from the first query that sees its first key; a wave's from its own first.
+  const int t0 = r.first(k0, a.causal) / 32, tiles = (r.lq + 31) / 32;
+  const int q_lane = r.first(kc, a.causal);                         // the lane's first query
+  const int q_wave = kw < r.lk ? r.first(kw, a.causal) / 32 : tiles;  // the wave's first tile
+  const int q_all = r.first(min(kw + 31, r.lk - 1), a.causal);      // from here on every key of the wave is seen
+  const T* qh = token<T>(a.q, r.qa, a.q_st, head, a.q_sh);
+  const T* doh = token<T>(a.dout, r.qa, a.do_st, head, a.do_sh);
+  const int64_t o_st = static_cast<int64_t>(a.h_q) * HD;
+  const T* oh = static_cast<const T*>(a.o) + r.qa * o_st + head * HD;
+  const float* lse = a.lse + head * a.n_q + r.qa;
+  constexpr int C = L::kCopies / kWaves;
+  const TileLane<HD, C> tq(C * wave, lane, a.q_st), td(C * wave, lane, a.do_st), to(C * wave, lane, o_st);
+  const FragLane<HD> fl0(lane);
+  const Scorer<CAP, BIAS> sc(a, head);
+  Frag orow[C];  // the O chunks of the dO chunks this lane copies
+  float lr = 0.0f;
+  auto copy = [&](char* dst, int j) {
+    const int rows = r.lq - 32 * j;
+    tq.copy(dst, qh + 32 * j * a.q_st, rows);
+    td.copy(dst + L::kBytes, doh + 32 * j * a.do_st, rows);
+#pragma unroll
+    for (int i = 0; i < C; ++i)
+      orow[i] = *reinterpret_cast<const Frag*>(reinterpret_cast<const char*>(oh + 32 * j * o_st) + to.at(i, rows));
+    if (tid < 32) lr = lse[32 * j + min(tid, rows - 1)];
+  };
+  // D of the rows this wave copied (its copies have landed): each lane's 8 products, then the sum over a row's lanes.
+  auto finish = [&](const char* dst, float* ld) {
+    __builtin_amdgcn_s_waitcnt(0x0070 | 0x0F00);  // vmcnt(0)
+    if (tid < 32) ld[tid] = lr * kLog2e;
+#pragma unroll
+    for (int i = 0; i < C; ++i) {
+      const Frag y = *reinterpret_cast<const Frag*>(dst + L::kBytes + (C * wave + i) * 1024 + lane * 16);
+      float x = dot8<T>(orow[i], y, 0.0f);
+#pragma unroll
+      for (int o = L::kChunks / 2; o >= 1; o >>= 1) x += __shfl_xor(x, o, 64);
+      if (lane % L::kChunks == 0) ld[32 + tq.row[i]] = x;
+    }
+  };
+  if (t0 < tiles) copy(lds.buf0, t0);
+  {
+    const TileLane<HD, C> tv(C * wave, lane, a.v_st);
+#pragma unroll
+    for (int n = 0; n < 4; ++n)
+      if (k0 + 32 * n < r.lk)
+        tv.copy(lds.v + n * L::kBytes, token<T>(a.v, static_cast<int64_t>(r.ka) + k0 + 32 * n, a.v_st, g, a.v_sh),
+                r.lk - k0 - 32 * n);
+  }
+  Frag kf[L::kSteps];
+  load_row_frags<T, HD>(kf, token<T>(a.k, static_cast<int64_t>(r.ka) + kc, a.k_st, g, a.k_sh), h);
+  f32x16 dk[L::kDims], dv[L::kDims];
+#pragma unroll
+  for (int d = 0; d < L::kDims; ++d) {
+    dk[d] = f32x16{};
+    dv[d] = f32x16{};
+  }
+  if (t0 < tiles) finish(lds.buf0, lds.ld0);
+  stage_barrier();
+  const char* vt = lds.v + wave * L::kBytes;
+  auto stage = [&](const char* qt, const float* ld, char* next, float* ldn, int j) {
+    if (j + 1 < tiles) copy(next, j + 1);
+    const char* dt = qt + L::kBytes;
+    const FragLane<HD> fl = fl0.fresh();
+    if (j >= q_wave) {
+      f32x16 st[1] = {f32x16{}}, dp = f32x16{}, f[1];
+#pragma unroll
+      for (int k = 0; k < L::kSteps; ++k) {
+        st[0] = mfma<T>(fl.frag(qt, k), kf[k], st[0]);      // S = Q K^T
+        dp = mfma<T>(fl.frag(dt, k), fl.frag(vt, k), dp);   // dP = dO V^T
+      }
+      constexpr bool kRaw = !CAP && !BIAS;
+      if constexpr (!kRaw)
+        tile_scores<CAP, BIAS, 1, true>(a, sc.slope2, st, f, static_cast<float>(r.off() + 32 * j + 4 * h - kc), -1.0f);
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const f32x4 lv = *reinterpret_cast<const f32x4*>(ld + 8 * q + 4 * h);
+        const f32x4 dd = *reinterpret_cast<const f32x4*>(ld + 32 + 8 * q + 4 * h);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int e = 4 * q + i;
+          const float p = exp2_raw(kRaw ? __builtin_fmaf(st[0][e], a.sl2, -lv[i]) : st[0][e] - lv[i]);
+          st[0][e] = p;                    // P
+          dp[e] = p * (dp[e] - dd[i]);     // dS
+          if constexpr (CAP) dp[e] *= f[0][e];
+        }
+      }
+      if (32 * j < q_all || 32 * j + 32 > r.lq) {  // queries that do not see a key, and rows past the last
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const int i = 32 * j + acc_row(e, h);
+          const bool in = i >= q_lane && i < r.lq;
+          st[0][e] = in ? st[0][e] : 0.0f;
+          dp[e] = in ? dp[e] : 0.0f;
+        }
+      }
+      const Frag p0 = frag_acc<T>(st[0], 0), p1 = frag_acc<T>(st[0], 1);
+      const Frag s0 = frag_acc<T>(dp, 0), s1 = frag_acc<T>(dp, 1);
+#pragma unroll
+      for (int d = 0; d < L::kDims; ++d) {
+        dv[d] = mfma<T>(p0, fl.frag_t(dt, 0, d), dv[d]);  // dV += P^T dO
+        dv[d] = mfma<T>(p1, fl.frag_t(dt, 1, d), dv[d]);
+        dk[d] = mfma<T>(s0, fl.frag_t(qt, 0, d), dk[d]);  // dK += dS^T Q
+        dk[d] = mfma<T>(s1, fl.frag_t(qt, 1, d), dk[d]);
+      }
+    }
+    if (j + 1 < tiles) finish(next, ldn);
+    stage_barrier();
+  };
+  for (int j = t0; j < tiles; j += 2) {
+    stage(lds.buf0, lds.ld0, lds.buf1, lds.ld1, j);
+    if (j + 1 < tiles) stage(lds.buf1, lds.ld1, lds.buf0, lds.ld0, j + 1);
+  }
+  if (kw >= r.lk) return;
+  // Keys are accumulator rows, head dims lanes. A key with a sum that is not finite is formed again by itself.
+  uint32_t bad = 0;
+#pragma unroll
+  for (int e = 0; e < 16; ++e) {
+    bool fine = true;
+#pragma unroll
+    for (int d = 0; d < L::kDims; ++d)
+      fine = fine && fabsf(dk[d][e] * a.scale) <= 3.402823466e38f && fabsf(dv[d][e]) <= 3.402823466e38f;
+    const uint64_t no = __ballot(!fine);
+    if (no & 0xffffffffu) bad |= 1u << acc_row(e, 0);
+    if (no >> 32) bad |= 1u << acc_row(e, 1);
+  }
+#pragma unroll
+  for (int e = 0; e < 16; ++e) {
+    const int row = acc_row(e, h), key = kw + row;
+    if (key >= r.lk || ((bad >> row) & 1)) continue;
+#pragma unroll
+    for (int d = 0; d < L::kDims; ++d) {
+      const int64_t t = r.ka + key;
+      if (grp > 1) {  // this head's part, past the L2: other blocks' parts join it in the next launch
+        const int64_t o = (head * a.n_k + t) * HD + 32 * d + col;
+        store_partial(a.dk_part + o, dk[d][e] * a.scale);
+        store_partial(a.dv_part + o, dv[d][e]);
+      } else {
+        const int64_t o = (t * a.h_kv + g) * HD + 32 * d + col;
+        static_cast<T*>(a.dk)[o] = from_f32<T>(dk[d][e] * a.scale);
+        static_cast<T*>(a.dv)[o] = from_f32<T>(dv[d][e]);
+      }
+    }
+  }
+  for (; bad; bad &= bad - 1) {
+    const int key = kw + __builtin_ctz(bad);
+    if (key >= r.lk) break;
+    const int64_t o = (head * a.n_k + r.ka + key) * HD;
+    plain_dkv_row<T, HD, CAP, BIAS>(a, r, key, head, head + 1, grp > 1 ? a.dk_part + o : nullptr,
+                                    grp > 1 ? a.dv_part + o : nullptr);
+  }
+}
+
+// Blocks of the first n_kblocks items are dK / dV blocks (the heavier ones, dispatched first), the rest dQ blocks.
+template <typename T, int HD, bool CAP, bool BIAS>
+__global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2, 2))) void masked_bwd_kernel(
+    MaskedArgs a) {
+  using L = Tiles<HD>;
+  __shared__ __attribute__((aligned(16))) char buf0[2 * L::kBytes];
+  __shared__ __attribute__((aligned(16))) char buf1[2 * L::kBytes];
+  __shared__ __attribute__((aligned(16))) char v[4 * L::kBytes];
+  __shared__ __attribute__((aligned(16))) float ld0[64];
+  __shared__ __attribute__((aligned(16))) float ld1[64];
+  int item, head;
+  if (!head_item(a, a.n_kblocks + a.n_blocks, item, head)) return;
+  const BwdLds lds{buf0, buf1, v, ld0, ld1};
+  if (item < a.n_kblocks)
+    bwd_dkdv<T, HD, CAP, BIAS>(a, item, head, lds);
+  else
+    bwd_dq<T, HD, CAP, BIAS>(a, item - a.n_kblocks, head, lds);
+}
+
+// dk / dv [key, g, :] = T(sum over the KV group's heads, in head order, of the parts). Thread = 4 head dims of a key.
+template <typename T>
+__global__ __launch_bounds__(256) void masked_group_sum_kernel(MaskedArgs a, int hd4) {
+  const int64_t t = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  const int c = 4 * static_cast<int>(t % hd4), grp = a.h_q / a.h_kv, hd = 4 * hd4;
+  const int g = static_cast<int>((t / hd4) % a.h_kv);
+  const int64_t key = t / hd4 / a.h_kv;
+  if (key >= a.n_k) return;
+  const int64_t step = a.n_k * hd;
+  const float* src = (blockIdx.y == 0 ? a.dk_part : a.dv_part) + g * grp * step + key * hd + c;
+  f32x4 sum = *reinterpret_cast<const f32x4*>(src);
+  int j = 1;
+  for (; j + 4 < grp; j += 4) {  // four heads' loads in flight
+    f32x4 x[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = *reinterpret_cast<const f32x4*>(src + (j + i) * step);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) sum += x[i];
+  }
+  f32x4 x[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (j + i < grp) x[i] = *reinterpret_cast<const f32x4*>(src + (j + i) * step);
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (j + i < grp) sum += x[i];
+  float o[4] = {sum[0], sum[1], sum[2], sum[3]};
+  store_from_f32<T, 4>(static_cast<T*>(blockIdx.y == 0 ? a.dk : a.dv) + (key * a.h_kv + g) * hd + c, o);
 }
 
 // Calls f<T, HD, CAP, BIAS>() for the call's types.
@@ -66,6 +550,15 @@ void dispatch(int dtype, int hd, bool cap, bool bias, F f) {
 
 int64_t blocks_bound(int64_t n, int32_t n_seq) { return (n + kRows - 1) / kRows + n_seq + 2; }
 
+// Launch size of n_items for every head (whole chunks of head_item's).
+int item_grid(const char* fn, int64_t n_items, const MaskedArgs& a, int64_t& grid) {
+  const int64_t chunk = 8 * (a.h_q / a.h_kv), items = n_items * a.h_q;
+  grid = (items + chunk - 1) / chunk * chunk;
+  if (grid * 64 * kWaves >= (int64_t(1) << 32) || a.n_k * a.h_kv * 32 >= (int64_t(1) << 32))
+    return fail(RUS_ERR_UNSUPPORTED, "%s: %lld blocks beyond one dispatch", fn, (long long)grid);
+  return RUS_OK;
+}
+
 // Sizes that every entry point takes.
 int check_sizes(const char* fn, int32_t n_seq, int64_t n_q, int64_t n_k, int32_t max_q, int32_t max_k, int32_t h_q,
                 int32_t h_kv, int32_t head_dim) {
@@ -73,7 +566,7 @@ int check_sizes(const char* fn, int32_t n_seq, int64_t n_q, int64_t n_k, int32_t
     return fail(RUS_ERR_UNSUPPORTED, "%s: head_dim %d (64 or 128)", fn, head_dim);
   if (h_q <= 0 || h_kv <= 0 || h_q % h_kv || h_q > 65535)
     return fail(RUS_ERR_INVALID, "%s: h_q=%d must be a multiple of h_kv=%d, at most 65535", fn, h_q, h_kv);
-  if (n_seq <= 0 || n_q < 0 || n_k < 0 || n_q >= (int64_t(1) << 31) - 256 || n_k >= (int64_t(1) << 31) - 256 ||
+  if (n_seq <= 0 || n_seq > (1 << 22) || n_q < 0 || n_k < 0 || n_q >= (int64_t(1) << 31) - 256 || n_k >= (int64_t(1) << 31) - 256 ||
       max_q < 0 || max_k < 0)
     return fail(RUS_ERR_INVALID, "%s: n_seq=%d n_q=%lld n_k=%lld max_q=%d max_k=%d", fn, n_seq, (long long)n_q,
                 (long long)n_k, max_q, max_k);
@@ -82,6 +575,7 @@ int check_sizes(const char* fn, int32_t n_seq, int64_t n_q, int64_t n_k, int32_t
 
 int check_rows(const char* fn, const char* name, const void* p, int64_t n, int64_t st, int64_t sh) {
   if (n == 0) return RUS_OK;
+  if (st >= (1 << 26)) return fail(RUS_ERR_UNSUPPORTED, "%s: %s has a token stride of 2^26 elements or more", fn, name);
   if (!p || !aligned(p, 16) || st % 8 || sh % 8 || st < 0 || sh < 0)
     return fail(RUS_ERR_INVALID, "%s: %s must be 16-byte aligned with strides that are multiples of 8", fn, name);
   return RUS_OK;
@@ -122,7 +616,7 @@ extern "C" int rus_attn_masked_workspace(int32_t n_seq, int64_t n_q, int64_t n_k
   const char* fn = "rus_attn_masked_workspace";
   if (!floats) return fail(RUS_ERR_INVALID, "%s: null result", fn);
   if (int e = check_sizes(fn, n_seq, n_q, n_k, max_q, max_k, h_q, h_kv, head_dim)) return e;
-  *floats = 0;
+  *floats = backward && h_q > h_kv ? 2 * static_cast<int64_t>(h_q) * n_k * head_dim : 0;
   return RUS_OK;
 }
 
@@ -151,9 +645,11 @@ extern "C" int rus_attn_masked_fwd(const void* q, int64_t q_stride_t, int64_t q_
   a.cu_q = cu_q, a.cu_k = cu_k, a.n_seq = n_seq, a.n_q = n_q, a.n_k = n_k, a.h_q = h_q, a.h_kv = h_kv;
   set_scores(a, scale, softcap, slopes, prefix, causal);
   a.n_blocks = static_cast<int>(blocks_bound(n_q, n_seq));
+  int64_t grid;
+  if (int e = item_grid(fn, a.n_blocks, a, grid)) return e;
   dispatch(dtype, head_dim, softcap > 0.0f, slopes != nullptr, [&](auto t, auto d, auto c, auto b) {
     hipLaunchKernelGGL((masked_fwd_kernel<decltype(t), decltype(d)::value, decltype(c)::value, decltype(b)::value>),
-                       dim3(a.n_blocks, h_q), dim3(64 * kWaves), 0, static_cast<hipStream_t>(stream), a);
+                       dim3(grid), dim3(64 * kWaves), 0, static_cast<hipStream_t>(stream), a);
   });
   return check_launch(fn);
 }
@@ -189,9 +685,27 @@ extern "C" int rus_attn_masked_bwd(const void* dout, int64_t do_stride_t, int64_
   set_scores(a, scale, softcap, slopes, prefix, causal);
   a.n_blocks = static_cast<int>(blocks_bound(n_q, n_seq));
   a.n_kblocks = static_cast<int>(blocks_bound(n_k, n_seq));
+  int64_t grid;
+  if (int e = item_grid(fn, a.n_blocks + a.n_kblocks, a, grid)) return e;
+  const int64_t half = static_cast<int64_t>(h_q) * n_k * head_dim;
+  if (h_q > h_kv && n_k > 0) {
+    if (!workspace || n_workspace < 2 * half || !aligned(workspace, 16))
+      return fail(RUS_ERR_INVALID, "%s: workspace of %lld floats, %lld needed", fn, (long long)n_workspace,
+                  (long long)(2 * half));
+    a.dk_part = workspace;
+    a.dv_part = workspace + half;
+  }
   dispatch(dtype, head_dim, softcap > 0.0f, slopes != nullptr, [&](auto t, auto d, auto c, auto b) {
     hipLaunchKernelGGL((masked_bwd_kernel<decltype(t), decltype(d)::value, decltype(c)::value, decltype(b)::value>),
-                       dim3(a.n_blocks + a.n_kblocks, h_q), dim3(64 * kWaves), 0, static_cast<hipStream_t>(stream), a);
+                       dim3(grid), dim3(64 * kWaves), 0, static_cast<hipStream_t>(stream), a);
   });
+  if (int e = check_launch(fn)) return e;
+  if (h_q == h_kv || n_k == 0) return RUS_OK;
+  const int hd4 = head_dim / 4;
+  const dim3 blocks(static_cast<unsigned>((n_k * h_kv * hd4 + 255) / 256), 2);
+  if (dtype == RUS_DTYPE_F16)
+    hipLaunchKernelGGL(masked_group_sum_kernel<f16>, blocks, dim3(256), 0, static_cast<hipStream_t>(stream), a, hd4);
+  else
+    hipLaunchKernelGGL(masked_group_sum_kernel<bf16>, blocks, dim3(256), 0, static_cast<hipStream_t>(stream), a, hd4);
   return check_launch(fn);
 }
