@@ -36,7 +36,7 @@ struct MaskedArgs {
   int n_seq, h_q, h_kv, causal;
   int n_blocks;    // blocks of 128 queries, bound over all rows
   int n_kblocks;   // blocks of 128 keys
-  int splits, split_tiles, col_tiles;
+  int splits, split_tiles;
   float scale;
   float sl2;        // scale log2 e
   float kc;         // scale / cap
@@ -97,15 +97,15 @@ __device__ __forceinline__ MaskedRow as_keys(MaskedRow r, int s, int n_seq) {
   return r;
 }
 
-// Block id -> (row, block within it) for blocks of kB tokens, over rows 0 .. n_seq + 1 in order; false past the last.
+// Block id -> (row, block within it) for blocks of kb tokens, over rows 0 .. n_seq + 1 in order; false past the last.
 // Uniform over the block.
-template <int kB>
-__device__ __forceinline__ bool find_span_block(const int32_t* cu, int n_seq, int n, int blk, int& s, int& b, int& nb) {
+__device__ __forceinline__ bool find_span_block(const int32_t* cu, int n_seq, int n, int blk, int kb, int& s, int& b,
+                                                int& nb) {
   const int lane = threadIdx.x & 63;
   for (int c = 0; c < n_seq + 2; c += 64) {
     int a = 0, e = 0;
     if (c + lane < n_seq + 2) row_span(cu, c + lane, n_seq, n, a, e);
-    const int mine = (e - a + kB - 1) / kB;
+    const int mine = (e - a + kb - 1) / kb;
     int sum = mine;  // inclusive over the lanes
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) {
@@ -123,6 +123,21 @@ __device__ __forceinline__ bool find_span_block(const int32_t* cu, int n_seq, in
     blk -= total;
   }
   return false;
+}
+
+// The row that query t belongs to.
+__device__ __forceinline__ int row_of(const MaskedArgs& a, int t) {
+  if (t < a.cu_q[0]) return a.n_seq + 1;
+  if (t >= a.cu_q[a.n_seq]) return a.n_seq;
+  int lo = 0, hi = a.n_seq;  // cu_q[lo] <= t < cu_q[hi]
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) / 2;
+    if (a.cu_q[mid] <= t)
+      lo = mid;
+    else
+      hi = mid;
+  }
+  return lo;
 }
 
 // ---------------------------------------------------------------------------------------------

@@ -1,6 +1,7 @@
 // Attention over packed rows with a tanh cap on the scores, a bias by distance, a prefix that every query sees, and
 // fewer queries than keys where a cache is read: forward and backward, fp16 / bf16, head dims 64 and 128. The
 // definition is in attn_masked.h.
+#include <algorithm>
 #include <type_traits>
 
 #include "attn_masked.h"
@@ -125,7 +126,7 @@ __device__ __forceinline__ void fwd_block(const MaskedArgs& a, char* buf0, char*
   constexpr int NT = kFwdTiles;
   int item, head, s, b, nb;
   if (!head_item(a, a.n_blocks, item, head)) return;
-  if (!find_span_block<kRows>(a.cu_q, a.n_seq, static_cast<int>(a.n_q), item, s, b, nb)) return;
+  if (!find_span_block(a.cu_q, a.n_seq, static_cast<int>(a.n_q), item, kRows, s, b, nb)) return;
   const MaskedRow r = uniform(as_queries(masked_row(a, s), s, a.n_seq));
   b = uniform(nb - 1 - b);  // the last queries see the most keys: first
   const int g = head / (a.h_q / a.h_kv);
@@ -201,6 +202,220 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2, 
 }
 
 // ---------------------------------------------------------------------------------------------
+// Few queries over many keys: a block holds up to 32 (query, head) pairs of one KV head as the columns of S^T, so that
+// K and V are read once for all of the group's heads, its waves take key tiles in turn (each with LDS of its own, no
+// barrier in the loop), and the keys are split over blocks whose parts another launch joins. Part: per column the sum
+// of P V on the part's own maximum, then that maximum, the sum of P and the sum of the rounded P.
+// ---------------------------------------------------------------------------------------------
+constexpr int kMaxSplitGroup = 32;
+
+__host__ __device__ inline int split_tokens(int grp) { return 32 / grp; }  // queries of a block
+
+constexpr int max_of(int x, int y) { return x > y ? x : y; }
+
+// One of a block's tile buffers, which the merge of the waves' sums uses again.
+template <int HD>
+constexpr int kSplitLds = max_of(2 * kWaves * Tiles<HD>::kBytes, kWaves * HD * 33 * 4);
+
+template <typename T, int HD, bool CAP, bool BIAS>
+__device__ __forceinline__ void split_block(const MaskedArgs& a, char* buf0, char* buf1) {
+  using L = Tiles<HD>;
+  const int grp = a.h_q / a.h_kv, tpb = split_tokens(grp);
+  const int z = blockIdx.x % a.splits, rest = blockIdx.x / a.splits;
+  const int g = rest % a.h_kv, item = rest / a.h_kv;
+  int s, b, nb;
+  if (!find_span_block(a.cu_q, a.n_seq, static_cast<int>(a.n_q), item, tpb, s, b, nb)) return;
+  const MaskedRow r = uniform(as_queries(masked_row(a, s), s, a.n_seq));
+  b = uniform(b);
+  const int wave = uniform(static_cast<int>(threadIdx.x) >> 6);
+  const int lane = threadIdx.x & 63, h = lane >> 5, col = lane & 31;
+  const int i0 = b * tpb, nq = min(tpb, r.lq - i0);  // the block's first query, its queries
+  const bool valid = col < nq * grp;
+  const int i = i0 + (valid ? col / grp : 0), head = g * grp + (valid ? col % grp : 0);
+  const int vis = r.vis(i, a.causal), vis_all = r.vis(i0, a.causal);
+  const int tiles = (r.vis(i0 + nq - 1, a.causal) + 31) / 32;
+  const int first = z * a.split_tiles;
+  if (first >= tiles && z > 0) return;  // the join knows
+  const int last = z == a.splits - 1 ? tiles : min(tiles, first + a.split_tiles);
+  const T* kh = token<T>(a.k, r.ka, a.k_st, g, a.k_sh);
+  const T* vh = token<T>(a.v, r.ka, a.v_st, g, a.v_sh);
+  const TileLane<HD, L::kCopies> tk(0, lane, a.k_st), tv(0, lane, a.v_st);
+  const FragLane<HD> fl0(lane);
+  const Scorer<CAP, BIAS> sc(a, head);
+  char* b0 = buf0 + wave * 2 * L::kBytes;
+  char* b1 = buf1 + wave * 2 * L::kBytes;
+  auto copy = [&](char* dst, int t) {
+    const int rows = r.lk - 32 * t;
+    tk.copy(dst, kh + 32 * t * a.k_st, rows);
+    tv.copy(dst + L::kBytes, vh + 32 * t * a.v_st, rows);
+  };
+  if (first + wave < last) copy(b0, first + wave);
+  Frag qf[L::kSteps];
+  load_row_frags<T, HD>(qf, token<T>(a.q, r.qa + i, a.q_st, head, a.q_sh), h);
+  FwdState<L::kDims> w;
+  stage_wait();
+  auto stage = [&](const char* cur, char* next, int t) {
+    if (t + kWaves < last) copy(next, t + kWaves);
+    const FragLane<HD> fl = fl0.fresh();
+    const int k0 = 32 * t;
+    fwd_keys<T, HD, CAP, BIAS, 1>(a, fl, cur, cur + L::kBytes, qf, w, sc.slope2, k0 + 32 <= vis_all, vis - k0,
+                                  static_cast<float>(r.off() + i - k0 - 4 * h), h);
+    stage_wait();
+  };
+  for (int t = first + wave; t < last; t += 2 * kWaves) {
+    stage(b0, b1, t);
+    if (t + kWaves < last) stage(b1, b0, t + kWaves);
+  }
+  // The waves' sums meet in the LDS, two waves at a time: [wave][HD][32 columns], then m, l, lr.
+  float* acc = reinterpret_cast<float*>(buf0);
+  __shared__ float ml[kWaves][3][32];
+  __shared__ uint32_t again;
+  const float2 lp = half_pair(w.l), rp = half_pair(w.lr);
+  if (threadIdx.x == 0) again = 0;
+  if (h == 0) {
+    ml[wave][0][col] = w.m;
+    ml[wave][1][col] = lp.x + lp.y;
+    ml[wave][2][col] = rp.x + rp.y;
+  }
+  __syncthreads();  // every wave is done with its tiles
+  float M = -INFINITY;
+#pragma unroll
+  for (int v = 0; v < kWaves; ++v) M = fmaxf(M, ml[v][0][col]);
+  const float ref = M == -INFINITY ? 0.0f : M;
+  float l = 0.0f, lr = 0.0f;
+#pragma unroll
+  for (int v = 0; v < kWaves; ++v) {
+    const float f = exp2_raw(ml[v][0][col] - ref);
+    l += ml[v][1][col] * f;
+    lr += ml[v][2][col] * f;
+  }
+  const float mine = exp2_raw(w.m - ref);
+#pragma unroll
+  for (int d = 0; d < L::kDims; ++d)
+#pragma unroll
+    for (int e = 0; e < 16; ++e)
+      acc[(wave * HD + 32 * d + acc_row(e, h)) * 33 + col] = w.o[d][e] * mine;
+  __syncthreads();
+  // Thread: 8 head dims of a column; the waves' sums in wave order.
+  constexpr int N = 8;
+  const bool direct = a.splits == 1;
+  for (int x = threadIdx.x; x < 32 * (HD / N); x += 64 * kWaves) {
+    const int c = x / (HD / N), d0 = x % (HD / N) * N;
+    if (c >= nq * grp) break;
+    const int64_t t = r.qa + i0 + c / grp, hd = g * grp + c % grp;
+    float o[N];
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+      o[e] = 0.0f;
+#pragma unroll
+      for (int v = 0; v < kWaves; ++v) o[e] += acc[(v * HD + d0 + e) * 33 + c];
+    }
+    if (direct) {
+      // sums of the column: every thread of it forms them again
+      float mc = -INFINITY, rc = 0.0f;
+#pragma unroll
+      for (int v = 0; v < kWaves; ++v) mc = fmaxf(mc, ml[v][0][c]);
+      mc = mc == -INFINITY ? 0.0f : mc;
+#pragma unroll
+      for (int v = 0; v < kWaves; ++v) rc += ml[v][2][c] * exp2_raw(ml[v][0][c] - mc);
+      const bool any = r.vis(i0 + c / grp, a.causal) > 0;
+      const float f = any ? 1.0f / rc : 0.0f;
+      bool fine = true;
+#pragma unroll
+      for (int e = 0; e < N; ++e) {
+        o[e] = any ? o[e] * f : 0.0f;
+        fine = fine && fabsf(o[e]) <= 3.402823466e38f;
+      }
+      if (!fine) atomicOr(&again, 1u << c);
+      store_from_f32<T, N>(static_cast<T*>(a.out) + (t * a.h_q + hd) * HD + d0, o);
+    } else {
+      store_pack<float, N>(a.part + ((static_cast<int64_t>(z) * a.n_q + t) * a.h_q + hd) * (HD + 4) + d0,
+                           __builtin_bit_cast(Pack<float, N>, o));
+    }
+  }
+  if (wave == 0 && h == 0 && valid) {
+    const int64_t t = r.qa + i;
+    if (direct) {
+      a.lse[head * a.n_q + t] = vis > 0 ? (M + log2f(l)) * kLn2 : -INFINITY;
+    } else {
+      float* p = a.part + ((static_cast<int64_t>(z) * a.n_q + t) * a.h_q + head) * (HD + 4) + HD;
+      p[0] = M;
+      p[1] = l;
+      p[2] = lr;
+    }
+  }
+  if (!direct) return;
+  stage_wait();  // the stores above come before those below
+  __syncthreads();
+  uint32_t cols = again;
+  for (; cols; cols &= cols - 1) {  // (uniform over the block; the waves take columns in turn)
+    const int c = __builtin_ctz(cols);
+    if (c % kWaves == wave) plain_fwd_row<T, HD, CAP, BIAS>(a, r, i0 + c / grp, g * grp + c % grp);
+  }
+}
+
+template <typename T, int HD, bool CAP, bool BIAS>
+__global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(1, 2))) void masked_split_kernel(
+    MaskedArgs a) {
+  __shared__ __attribute__((aligned(16))) char buf0[kSplitLds<HD>];
+  __shared__ __attribute__((aligned(16))) char buf1[2 * kWaves * Tiles<HD>::kBytes];
+  split_block<T, HD, CAP, BIAS>(a, buf0, buf1);
+}
+
+// Joins the parts of one (query, head) a wave, in order.
+template <typename T, int HD, bool CAP, bool BIAS>
+__global__ __launch_bounds__(64 * kWaves) void masked_join_kernel(MaskedArgs a) {
+  constexpr int N = HD / 64;
+  const int64_t x = static_cast<int64_t>(blockIdx.x) * kWaves + (threadIdx.x >> 6);
+  if (x >= a.n_q * a.h_q) return;
+  const int lane = threadIdx.x & 63, head = static_cast<int>(x % a.h_q);
+  const int64_t t = x / a.h_q;
+  const int tpb = split_tokens(a.h_q / a.h_kv);
+  const int s = row_of(a, static_cast<int>(t));
+  const MaskedRow r = as_queries(masked_row(a, s), s, a.n_seq);
+  const int i = static_cast<int>(t) - r.qa, i0 = i / tpb * tpb;
+  const int vis = r.vis(i, a.causal);
+  // The parts that the query's block wrote.
+  const int tiles = (r.vis(min(i0 + tpb, r.lq) - 1, a.causal) + 31) / 32;
+  const int n = max(1, min(a.splits, (tiles + a.split_tiles - 1) / a.split_tiles));
+  const int64_t step = a.n_q * a.h_q * (HD + 4);
+  const float* p = a.part + x * (HD + 4);
+  float m = -INFINITY;
+  for (int z = lane; z < n; z += 64) m = fmaxf(m, p[z * step + HD]);
+  m = wave_max(m);
+  const float ref = m == -INFINITY ? 0.0f : m;
+  float l = 0.0f, lr = 0.0f, o[N] = {};
+  for (int z = lane; z < n; z += 64) {
+    const float f = exp2_raw(p[z * step + HD] - ref);
+    l += p[z * step + HD + 1] * f;
+    lr += p[z * step + HD + 2] * f;
+  }
+  l = wave_sum(l);
+  lr = wave_sum(lr);
+#pragma unroll 4
+  for (int z = 0; z < n; ++z) {
+    const float f = exp2_raw(p[z * step + HD] - ref);
+    float y[N];
+    load_f32<float, N>(p + z * step + lane * N, y);
+#pragma unroll
+    for (int d = 0; d < N; ++d) o[d] = __builtin_fmaf(y[d], f, o[d]);
+  }
+  const float f = 1.0f / lr;
+  bool fine = true;
+#pragma unroll
+  for (int d = 0; d < N; ++d) {
+    o[d] = vis > 0 ? o[d] * f : 0.0f;
+    fine = fine && fabsf(o[d]) <= 3.402823466e38f;
+  }
+  if (__ballot(!fine)) {
+    plain_fwd_row<T, HD, CAP, BIAS>(a, r, i, head);
+    return;
+  }
+  store_from_f32<T, N>(static_cast<T*>(a.out) + x * HD + lane * N, o);
+  if (lane == 0) a.lse[head * a.n_q + t] = vis > 0 ? (m + log2f(l)) * kLn2 : -INFINITY;
+}
+
+// ---------------------------------------------------------------------------------------------
 // Backward.
 // ---------------------------------------------------------------------------------------------
 
@@ -220,7 +435,7 @@ template <typename T, int HD, bool CAP, bool BIAS>
 __device__ __forceinline__ void bwd_dq(const MaskedArgs& a, int blk, int head, const BwdLds& lds) {
   using L = Tiles<HD>;
   int s, b, nb;
-  if (!find_span_block<kRows>(a.cu_q, a.n_seq, static_cast<int>(a.n_q), blk, s, b, nb)) return;
+  if (!find_span_block(a.cu_q, a.n_seq, static_cast<int>(a.n_q), blk, kRows, s, b, nb)) return;
   const MaskedRow r = uniform(as_queries(masked_row(a, s), s, a.n_seq));
   b = uniform(nb - 1 - b);
   const int g = head / (a.h_q / a.h_kv);
@@ -314,7 +529,7 @@ template <typename T, int HD, bool CAP, bool BIAS>
 __device__ __forceinline__ void bwd_dkdv(const MaskedArgs& a, int blk, int head, const BwdLds& lds) {
   using L = Tiles<HD>;
   int s, b, nb;
-  if (!find_span_block<kRows>(a.cu_k, a.n_seq, static_cast<int>(a.n_k), blk, s, b, nb)) return;
+  if (!find_span_block(a.cu_k, a.n_seq, static_cast<int>(a.n_k), blk, kRows, s, b, nb)) return;
   const MaskedRow r = uniform(as_keys(masked_row(a, s), s, a.n_seq));
   b = uniform(b);
   const int grp = a.h_q / a.h_kv, g = head / grp;
@@ -550,6 +765,28 @@ void dispatch(int dtype, int hd, bool cap, bool bias, F f) {
 
 int64_t blocks_bound(int64_t n, int32_t n_seq) { return (n + kRows - 1) / kRows + n_seq + 2; }
 
+// How a forward runs: splits = 0: blocks of 128 queries; otherwise blocks of few queries, the keys in `splits` parts of
+// `tiles` tiles each.
+struct SplitPlan {
+  int splits, tiles;
+  int64_t items;  // blocks of few queries, bound over all rows
+};
+
+SplitPlan split_plan(int32_t n_seq, int64_t n_q, int32_t max_k, int32_t h_q, int32_t h_kv) {
+  SplitPlan p{0, 0, 0};
+  const int grp = h_q / h_kv;
+  if (grp > kMaxSplitGroup) return p;
+  if (std::max<int64_t>((n_q + kRows - 1) / kRows, n_seq) * h_q >= 256) return p;
+  const int tpb = split_tokens(grp);
+  p.items = (n_q + tpb - 1) / tpb + n_seq + 2;
+  const int64_t base = std::max<int64_t>((n_q + tpb - 1) / tpb, n_seq) * h_kv;
+  const int64_t tiles = std::max<int64_t>((static_cast<int64_t>(max_k) + 31) / 32, 1);
+  const int64_t want = std::min<int64_t>(512 / base, (tiles + 7) / 8);
+  p.splits = static_cast<int>(std::max<int64_t>(want, 1));
+  p.tiles = static_cast<int>((tiles + p.splits - 1) / p.splits);
+  return p;
+}
+
 // Launch size of n_items for every head (whole chunks of head_item's).
 int item_grid(const char* fn, int64_t n_items, const MaskedArgs& a, int64_t& grid) {
   const int64_t chunk = 8 * (a.h_q / a.h_kv), items = n_items * a.h_q;
@@ -616,7 +853,12 @@ extern "C" int rus_attn_masked_workspace(int32_t n_seq, int64_t n_q, int64_t n_k
   const char* fn = "rus_attn_masked_workspace";
   if (!floats) return fail(RUS_ERR_INVALID, "%s: null result", fn);
   if (int e = check_sizes(fn, n_seq, n_q, n_k, max_q, max_k, h_q, h_kv, head_dim)) return e;
-  *floats = backward && h_q > h_kv ? 2 * static_cast<int64_t>(h_q) * n_k * head_dim : 0;
+  if (backward) {
+    *floats = h_q > h_kv ? 2 * static_cast<int64_t>(h_q) * n_k * head_dim : 0;
+    return RUS_OK;
+  }
+  const SplitPlan p = split_plan(n_seq, n_q, max_k, h_q, h_kv);
+  *floats = p.splits > 1 ? p.splits * n_q * h_q * (head_dim + 4) : 0;
   return RUS_OK;
 }
 
@@ -644,6 +886,28 @@ extern "C" int rus_attn_masked_fwd(const void* q, int64_t q_stride_t, int64_t q_
   a.out = out, a.lse = lse;
   a.cu_q = cu_q, a.cu_k = cu_k, a.n_seq = n_seq, a.n_q = n_q, a.n_k = n_k, a.h_q = h_q, a.h_kv = h_kv;
   set_scores(a, scale, softcap, slopes, prefix, causal);
+  const SplitPlan p = split_plan(n_seq, n_q, max_k, h_q, h_kv);
+  if (p.splits) {
+    a.splits = p.splits;
+    a.split_tiles = p.tiles;
+    a.part = workspace;
+    const int64_t need = p.splits > 1 ? p.splits * n_q * h_q * (head_dim + 4) : 0;
+    if (need && (!workspace || n_workspace < need || !aligned(workspace, 16)))
+      return fail(RUS_ERR_INVALID, "%s: workspace of %lld floats, %lld needed", fn, (long long)n_workspace,
+                  (long long)need);
+    const int64_t blocks = p.items * h_kv * p.splits;
+    if (blocks * 64 * kWaves >= (int64_t(1) << 32))
+      return fail(RUS_ERR_UNSUPPORTED, "%s: %lld blocks beyond one dispatch", fn, (long long)blocks);
+    dispatch(dtype, head_dim, softcap > 0.0f, slopes != nullptr, [&](auto t, auto d, auto c, auto b) {
+      hipLaunchKernelGGL((masked_split_kernel<decltype(t), decltype(d)::value, decltype(c)::value, decltype(b)::value>),
+                         dim3(static_cast<unsigned>(blocks)), dim3(64 * kWaves), 0, static_cast<hipStream_t>(stream), a);
+      if (p.splits > 1)
+        hipLaunchKernelGGL((masked_join_kernel<decltype(t), decltype(d)::value, decltype(c)::value, decltype(b)::value>),
+                           dim3(static_cast<unsigned>((n_q * h_q + kWaves - 1) / kWaves)), dim3(64 * kWaves), 0,
+                           static_cast<hipStream_t>(stream), a);
+    });
+    return check_launch(fn);
+  }
   a.n_blocks = static_cast<int>(blocks_bound(n_q, n_seq));
   int64_t grid;
   if (int e = item_grid(fn, a.n_blocks, a, grid)) return e;
