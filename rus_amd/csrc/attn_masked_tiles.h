@@ -160,7 +160,20 @@ struct FragLane {
 // Every copy of this wave has landed and every LDS read of it has returned.
 __device__ __forceinline__ void stage_wait() { __builtin_amdgcn_s_waitcnt(0x0070); }  // vmcnt(0) lgkmcnt(0)
 
-// ... and the block's barrier: the buffer just filled may be read, the buffer just read may be filled.
+// All but the last N copies of this wave have landed.
+template <int N>
+__device__ __forceinline__ void wait_copies() {
+  __builtin_amdgcn_s_waitcnt(N | (7 << 4) | (15 << 8));
+  asm volatile("" ::: "memory");
+}
+
+// This wave's LDS reads have returned: a copy may now overwrite the tile they read.
+__device__ __forceinline__ void wait_reads() {
+  __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0), vmcnt / expcnt not waited on
+  asm volatile("" ::: "memory");
+}
+
+// stage_wait and the block's barrier: the buffer just filled may be read, the buffer just read may be filled.
 __device__ __forceinline__ void stage_barrier() {
   stage_wait();
   __syncthreads();

@@ -10,6 +10,7 @@ raises ``RuntimeError``.
 from __future__ import annotations
 
 import ctypes
+import functools
 import math
 
 import torch
@@ -2745,6 +2746,7 @@ class RopeAxes:
         self.n_axes = max(axis) + 1
         self.axis = torch.tensor(axis, dtype=torch.uint8, device=device)
         self.turns = torch.tensor([f / (2.0 * math.pi) for f in freq], dtype=torch.float64, device=device)
+        self.tables = self.axis.data_ptr(), self.turns.data_ptr()
 
     @classmethod
     def sections(cls, sections, theta: float, head_dim: int, device="cuda", order: str = "blocks",
@@ -2775,41 +2777,50 @@ class RopeAxes:
         return self.axis.device
 
 
-def _rope_axes_heads(fn: str, x: torch.Tensor, axes: RopeAxes, name: str) -> torch.Tensor:
+def _rope_axes_heads(fn: str, x: torch.Tensor, axes: RopeAxes, name: str):
+    """x as [N, heads, d] with unit stride within a head, and its strides."""
     if x.dim() != 3 or x.shape[2] != axes.head_dim:
         raise ValueError(f"{fn}: {name} must be [N, heads, {axes.head_dim}], got {tuple(x.shape)}")
-    if x.dtype not in _WIDE_DTYPES:
-        raise TypeError(f"{fn}: unsupported dtype {x.dtype} (fp16, bf16 or fp32)")
-    return x if x.stride(2) == 1 else x.contiguous()
+    st, sh, sd = x.stride()
+    if sd == 1:
+        return x, st, sh
+    x = x.contiguous()
+    return x, *x.stride()[:2]
 
 
 def _rope_axes(fn: str, q: torch.Tensor, k: torch.Tensor | None, pos: torch.Tensor, axes: RopeAxes,
                inverse: bool):
-    q = _rope_axes_heads(fn, q, axes, "q")
+    q, q_st, q_sh = _rope_axes_heads(fn, q, axes, "q")
     n, hq, d = q.shape
-    hk = 0
+    dt = q.dtype
+    code = _WIDE_DTYPES.get(dt)
+    if code is None:
+        raise TypeError(f"{fn}: unsupported dtype {dt} (fp16, bf16 or fp32)")
+    hk = k_st = k_sh = 0
     if k is not None:
-        k = _rope_axes_heads(fn, k, axes, "k")
-        hk = k.shape[1]
-        if k.dtype != q.dtype or k.shape[0] != n:
-            raise ValueError(f"{fn}: k must be {q.dtype} with {n} tokens")
-    if pos.dtype not in _POS_TYPES:
+        k, k_st, k_sh = _rope_axes_heads(fn, k, axes, "k")
+        nk, hk, _ = k.shape
+        if k.dtype != dt or nk != n:
+            raise ValueError(f"{fn}: k must be {dt} with {n} tokens")
+    pos_type = _POS_TYPES.get(pos.dtype)
+    if pos_type is None:
         raise TypeError(f"{fn}: positions must be int64, int32 or fp32, got {pos.dtype}")
     if pos.dim() != 2 or pos.shape[1] != n or pos.shape[0] < axes.n_axes:
         raise ValueError(f"{fn}: positions must be [{axes.n_axes}, {n}], got {tuple(pos.shape)}")
     _same_device(fn, q, k, pos, axes.axis)
-    if pos.stride(1) != 1 and n > 1:
+    ld_pos, step = pos.stride()
+    if step != 1 and n > 1:
         pos = pos.contiguous()
-    q_out = torch.empty((n, hq, d), dtype=q.dtype, device=q.device)
-    k_out = None if k is None else torch.empty((n, hk, d), dtype=q.dtype, device=q.device)
+        ld_pos = n
+    q_out = q.new_empty((n, hq, d))
+    k_out = None if k is None else q.new_empty((n, hk, d))
     if n == 0 or hq + hk == 0:
         return q_out, k_out
     _mx_launch("rope_axes", lambda: (2 * n * (hq + hk) * d * q.element_size() + pos.numel() * pos.element_size(),
                                      6.0 * n * (hq + hk) * axes.pairs),
-               q, "rus_rope_axes", q.data_ptr(), q.stride(0), q.stride(1), hq, q_out.data_ptr(),
-               _ptr(k), 0 if k is None else k.stride(0), 0 if k is None else k.stride(1), hk, _ptr(k_out), n, d,
-               axes.pairs, 1 if axes.adjacent else 0, pos.data_ptr(), _POS_TYPES[pos.dtype], pos.stride(0),
-               axes.n_axes, axes.axis.data_ptr(), axes.turns.data_ptr(), 1 if inverse else 0, _WIDE_DTYPES[q.dtype])
+               q, "rus_rope_axes", q.data_ptr(), q_st, q_sh, hq, q_out.data_ptr(), _ptr(k), k_st, k_sh, hk,
+               _ptr(k_out), n, d, axes.pairs, axes.adjacent, pos.data_ptr(), pos_type, ld_pos, axes.n_axes,
+               *axes.tables, inverse, code)
     return q_out, k_out
 
 
@@ -2830,14 +2841,17 @@ def rope_axes_bwd(dq: torch.Tensor, dk: torch.Tensor | None, pos: torch.Tensor, 
 # ---------------------------------------------------------------------------------------------
 
 
-def _masked_heads(fn: str, x: torch.Tensor, name: str, like: torch.Tensor) -> torch.Tensor:
-    if x.dim() != 3 or x.shape[2] != like.shape[2]:
-        raise ValueError(f"{fn}: {name} must be [tokens, heads, {like.shape[2]}], got {tuple(x.shape)}")
-    if x.dtype != like.dtype:
-        raise TypeError(f"{fn}: {name} must be {like.dtype}, got {x.dtype}")
-    if x.numel() and (x.stride(2) != 1 or x.stride(0) % 8 or x.stride(1) % 8 or x.data_ptr() % 16):
-        return x.contiguous()
-    return x
+def _masked_heads(fn: str, x: torch.Tensor, name: str, d: int, dt: torch.dtype):
+    """x as [tokens, heads, d] that the kernels address, and its address and strides."""
+    if x.dim() != 3 or x.shape[2] != d:
+        raise ValueError(f"{fn}: {name} must be [tokens, heads, {d}], got {tuple(x.shape)}")
+    if x.dtype != dt:
+        raise TypeError(f"{fn}: {name} must be {dt}, got {x.dtype}")
+    st, sh, sd = x.stride()
+    if sd != 1 or (st | sh) & 7 or x.data_ptr() & 15:
+        x = x.contiguous()
+        st, sh, _ = x.stride()
+    return x, (x.data_ptr(), st, sh)
 
 
 def _masked_ints(fn: str, t: torch.Tensor, name: str, n: int | None) -> None:
@@ -2846,62 +2860,65 @@ def _masked_ints(fn: str, t: torch.Tensor, name: str, n: int | None) -> None:
                          f"{'' if n is None else f' with {n} entries'}")
 
 
-class _MaskedCall:
-    """Checked operands of one call: tensors that the launch addresses, and its arguments in order."""
-
-    def __init__(self, fn, q, k, v, cu_q, cu_k, causal, prefix, softcap, slopes, scale, max_q, max_k):
-        if q.dim() != 3 or q.shape[2] not in (64, 128):
-            raise ValueError(f"{fn}: q must be [tokens, heads, 64 or 128], got {tuple(q.shape)}")
-        if q.dtype not in (torch.float16, torch.bfloat16):
-            raise TypeError(f"{fn}: unsupported dtype {q.dtype} (fp16 or bf16)")
-        self.q, self.k, self.v = (_masked_heads(fn, t, name, q) for t, name in ((q, "q"), (k, "k"), (v, "v")))
-        nq, hq, d = q.shape
-        nk, hkv = k.shape[:2]
-        if v.shape != k.shape:
-            raise ValueError(f"{fn}: k {tuple(k.shape)} and v {tuple(v.shape)} differ")
-        if hkv == 0 or hq == 0 or hq % hkv:
-            raise ValueError(f"{fn}: h_q={hq} is not a multiple of h_kv={hkv}")
-        _masked_ints(fn, cu_q, "cu_q", None)
-        if cu_q.numel() < 2:
-            raise ValueError(f"{fn}: cu_q must have a start and an end for each row")
-        if cu_k is None:
-            if nq != nk:
-                raise ValueError(f"{fn}: {nq} queries and {nk} keys need a cu_k of their own")
-            cu_k = cu_q
-        n_seq = cu_q.numel() - 1
+def _masked_call(fn, q, k, v, cu_q, cu_k, causal, prefix, softcap, slopes, scale, max_q, max_k):
+    """Checked operands of one call: ((q, k, v) as addressed, their addresses and strides, (cu_q, cu_k) addresses,
+    sizes, what the scores take). Everything else that the launch reads belongs to the caller."""
+    if q.dim() != 3 or q.shape[2] not in (64, 128):
+        raise ValueError(f"{fn}: q must be [tokens, heads, 64 or 128], got {tuple(q.shape)}")
+    dt = q.dtype
+    if dt is not torch.float16 and dt is not torch.bfloat16:
+        raise TypeError(f"{fn}: unsupported dtype {dt} (fp16 or bf16)")
+    nq, hq, d = q.shape
+    q, q_at = _masked_heads(fn, q, "q", d, dt)
+    k, k_at = _masked_heads(fn, k, "k", d, dt)
+    v, v_at = _masked_heads(fn, v, "v", d, dt)
+    nk, hkv, _ = k.shape
+    if v.shape != k.shape:
+        raise ValueError(f"{fn}: k {tuple(k.shape)} and v {tuple(v.shape)} differ")
+    if hkv == 0 or hq == 0 or hq % hkv:
+        raise ValueError(f"{fn}: h_q={hq} is not a multiple of h_kv={hkv}")
+    _masked_ints(fn, cu_q, "cu_q", None)
+    n_seq = cu_q.numel() - 1
+    if n_seq < 1:
+        raise ValueError(f"{fn}: cu_q must have a start and an end for each row")
+    if cu_k is None:
+        if nq != nk:
+            raise ValueError(f"{fn}: {nq} queries and {nk} keys need a cu_k of their own")
+        cu_k = cu_q
+    else:
         _masked_ints(fn, cu_k, "cu_k", n_seq + 1)
-        if prefix is not None:
-            _masked_ints(fn, prefix, "prefix", n_seq)
-        if slopes is not None and (slopes.dtype != torch.float32 or slopes.shape != (hq,) or not slopes.is_contiguous()):
-            raise ValueError(f"{fn}: slopes must be contiguous fp32 [{hq}]")
-        softcap = 0.0 if softcap is None else float(softcap)
-        scale = 1.0 / math.sqrt(d) if scale is None else float(scale)
-        if not 0.0 <= softcap < math.inf:
-            raise ValueError(f"{fn}: softcap must be positive, or 0 for none, got {softcap}")
-        if not 0.0 < scale < math.inf:
-            raise ValueError(f"{fn}: scale must be positive and finite, got {scale}")
-        _same_device(fn, q, k, v, cu_q, cu_k, prefix, slopes)
-        self.max_q = nq if max_q is None else int(max_q)
-        self.max_k = nk if max_k is None else int(max_k)
-        if self.max_q < 0 or self.max_k < 0:
-            raise ValueError(f"{fn}: max_q={max_q} max_k={max_k}")
-        self.nq, self.nk, self.hq, self.hkv, self.d, self.n_seq = nq, nk, hq, hkv, d, n_seq
-        self.kept = cu_q, cu_k, prefix, slopes
-        self.sizes = (n_seq, nq, nk, self.max_q, self.max_k, hq, hkv, d)
-        self.qkv = (self.q.data_ptr(), self.q.stride(0), self.q.stride(1), self.k.data_ptr(), self.k.stride(0),
-                    self.k.stride(1), self.v.data_ptr(), self.v.stride(0), self.v.stride(1))
-        self.scores = (scale, 1 if causal else 0, _ptr(prefix), softcap, _ptr(slopes), _WIDE_DTYPES[q.dtype])
+    if prefix is not None:
+        _masked_ints(fn, prefix, "prefix", n_seq)
+    if slopes is not None and (slopes.dtype != torch.float32 or slopes.shape != (hq,) or not slopes.is_contiguous()):
+        raise ValueError(f"{fn}: slopes must be contiguous fp32 [{hq}]")
+    softcap = 0.0 if softcap is None else float(softcap)
+    scale = d**-0.5 if scale is None else float(scale)
+    if not 0.0 <= softcap < math.inf:
+        raise ValueError(f"{fn}: softcap must be positive, or 0 for none, got {softcap}")
+    if not 0.0 < scale < math.inf:
+        raise ValueError(f"{fn}: scale must be positive and finite, got {scale}")
+    max_q = nq if max_q is None else int(max_q)
+    max_k = nk if max_k is None else int(max_k)
+    if max_q < 0 or max_k < 0:
+        raise ValueError(f"{fn}: max_q={max_q} max_k={max_k}")
+    _same_device(fn, q, k, v, cu_q, cu_k, prefix, slopes)
+    return ((q, k, v), (*q_at, *k_at, *v_at), (cu_q.data_ptr(), cu_k.data_ptr()),
+            (n_seq, nq, nk, max_q, max_k, hq, hkv, d),
+            (scale, bool(causal), _ptr(prefix), softcap, _ptr(slopes), _WIDE_DTYPES[dt]))
 
-    def workspace(self, backward: int) -> tuple:
-        got = ctypes.c_int64()
-        _lib.call("rus_attn_masked_workspace", *self.sizes, backward, ctypes.byref(got))
-        self.ws = torch.empty(got.value, dtype=torch.float32, device=self.q.device) if got.value else None
-        return _ptr(self.ws), got.value
 
-    def cost(self, backward: bool):  # visible pairs are known on the device only: every pair of the longest rows
-        pairs = float(self.max_k) * self.nq * self.hq * self.d
-        nbytes = 2 * (2 * self.nq * self.hq + 2 * self.nk * self.hkv) * self.d * (2 if backward else 1)
-        return nbytes, (10.0 if backward else 4.0) * pairs
+@functools.lru_cache(maxsize=1024)
+def _masked_workspace(sizes: tuple, backward: bool) -> int:
+    got = ctypes.c_int64()
+    _lib.call("rus_attn_masked_workspace", *sizes, backward, ctypes.byref(got))
+    return got.value
+
+
+def _masked_cost(sizes: tuple, backward: bool):
+    """(bytes, FLOPs) with every pair of the longest rows: the visible ones are known on the device only."""
+    _, nq, nk, _, max_k, hq, hkv, d = sizes
+    return (2 * (2 * nq * hq + 2 * nk * hkv) * d * (2 if backward else 1),
+            (10.0 if backward else 4.0) * max_k * nq * hq * d)
 
 
 def attn_masked_fwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: torch.Tensor,
@@ -2919,13 +2936,16 @@ def attn_masked_fwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: tor
     leaves them. ``max_q`` and ``max_k``: the longest row's queries and keys (default: all tokens); they choose
     how the work is split, and a row may not have more queries than max_q."""
     fn = "attn_masked_fwd"
-    c = _MaskedCall(fn, q, k, v, cu_q, cu_k, causal, prefix, softcap, slopes, scale, max_q, max_k)
-    out = torch.empty((c.nq, c.hq, c.d), dtype=q.dtype, device=q.device)
-    lse = torch.empty((c.hq, c.nq), dtype=torch.float32, device=q.device)
-    if c.nq:
-        cu_q, cu_k = c.kept[:2]
-        _mx_launch("attn_masked_fwd", lambda: c.cost(False), q, "rus_attn_masked_fwd", *c.qkv, cu_q.data_ptr(),
-                   cu_k.data_ptr(), *c.sizes, *c.scores, out.data_ptr(), lse.data_ptr(), *c.workspace(0))
+    rows, at, cu, sizes, scores = _masked_call(fn, q, k, v, cu_q, cu_k, causal, prefix, softcap, slopes, scale,
+                                               max_q, max_k)
+    _, nq, _, _, _, hq, _, d = sizes
+    out = q.new_empty((nq, hq, d))
+    lse = torch.empty((hq, nq), dtype=torch.float32, device=q.device)
+    if nq:
+        floats = _masked_workspace(sizes, False)
+        ws = _floats(floats, q)
+        _mx_launch(fn, lambda: _masked_cost(sizes, False), q, "rus_attn_masked_fwd", *at, *cu, *sizes, *scores,
+                   out.data_ptr(), lse.data_ptr(), _ptr(ws), floats)
     return out, lse
 
 
@@ -2937,22 +2957,24 @@ def attn_masked_bwd(dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: tor
     """(dq, dk, dv) of ``attn_masked_fwd`` for the gradient of its out, given its out and lse. dk and dv add the
     query heads of a KV head in a fixed order in fp32 and are rounded once."""
     fn = "attn_masked_bwd"
-    c = _MaskedCall(fn, q, k, v, cu_q, cu_k, causal, prefix, softcap, slopes, scale, max_q, max_k)
+    rows, at, cu, sizes, scores = _masked_call(fn, q, k, v, cu_q, cu_k, causal, prefix, softcap, slopes, scale,
+                                               max_q, max_k)
+    _, nq, nk, _, _, hq, hkv, d = sizes
     if dout.shape != q.shape or out.shape != q.shape:
         raise ValueError(f"{fn}: dout and out must be {tuple(q.shape)}, got {tuple(dout.shape)}, {tuple(out.shape)}")
-    dout = _masked_heads(fn, dout, "dout", q)
+    dout, do_at = _masked_heads(fn, dout, "dout", d, q.dtype)
     if out.dtype != q.dtype or not out.is_contiguous():
         raise ValueError(f"{fn}: out must be contiguous {q.dtype}")
-    if lse.dtype != torch.float32 or lse.shape != (c.hq, c.nq) or not lse.is_contiguous():
-        raise ValueError(f"{fn}: lse must be contiguous fp32 [{c.hq}, {c.nq}]")
+    if lse.dtype != torch.float32 or lse.shape != (hq, nq) or not lse.is_contiguous():
+        raise ValueError(f"{fn}: lse must be contiguous fp32 [{hq}, {nq}]")
     _same_device(fn, q, dout, out, lse)
-    dq = torch.empty((c.nq, c.hq, c.d), dtype=q.dtype, device=q.device)
-    dk, dv = (torch.empty((c.nk, c.hkv, c.d), dtype=q.dtype, device=q.device) for _ in range(2))
-    if c.nq or c.nk:
-        cu_q, cu_k = c.kept[:2]
-        _mx_launch("attn_masked_bwd", lambda: c.cost(True), q, "rus_attn_masked_bwd", dout.data_ptr(), dout.stride(0),
-                   dout.stride(1), *c.qkv, out.data_ptr(), lse.data_ptr(), cu_q.data_ptr(), cu_k.data_ptr(),
-                   *c.sizes, *c.scores, dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), *c.workspace(1))
+    dq = q.new_empty((nq, hq, d))
+    dk, dv = q.new_empty((nk, hkv, d)), q.new_empty((nk, hkv, d))
+    if nq or nk:
+        floats = _masked_workspace(sizes, True)
+        ws = _floats(floats, q)
+        _mx_launch(fn, lambda: _masked_cost(sizes, True), q, "rus_attn_masked_bwd", *do_at, *at, out.data_ptr(),
+                   lse.data_ptr(), *cu, *sizes, *scores, dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), _ptr(ws), floats)
     return dq, dk, dv
 
 
