@@ -157,7 +157,9 @@ __device__ __forceinline__ float tanh_small(float x) {
 template <bool CAP, bool BIAS>
 struct Scorer {
   float slope2;  // slope log2 e of the head
-  __device__ __forceinline__ Scorer(const MaskedArgs& a, int head) : slope2(BIAS ? a.slopes[head] * kLog2e : 0.0f) {}
+  float slope;   // slope / scale: in the products' unit
+  __device__ __forceinline__ Scorer(const MaskedArgs& a, int head)
+      : slope2(BIAS ? a.slopes[head] * kLog2e : 0.0f), slope(BIAS ? a.slopes[head] / a.scale : 0.0f) {}
 
   // Score of the product st at distance d, and (1 - t^2) of the cap.
   __device__ __forceinline__ float score(const MaskedArgs& a, float st, float d, float& factor) const {

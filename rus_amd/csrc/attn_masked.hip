@@ -51,24 +51,26 @@ struct FwdState {
 // values_ready() before the V tiles are.
 template <typename T, int HD, bool CAP, bool BIAS, int NT, typename F, typename G>
 __device__ __forceinline__ void fwd_keys(const MaskedArgs& a, const FragLane<HD>& fl, const char* kt, const char* vt,
-                                         const Frag (&qf)[HD / 16], FwdState<HD / 32>& w, float slope2, bool whole,
-                                         int left, float d0, int h, F keys_read, G values_ready) {
+                                         const Frag (&qf)[HD / 16], FwdState<HD / 32>& w,
+                                         const Scorer<CAP, BIAS>& sc, bool whole, int left, float d0, bool ahead, int h,
+                                         F keys_read, G values_ready) {
   using L = Tiles<HD>;
   f32x16 st[NT];
+  start_scores<CAP, BIAS, NT>(st, sc.slope, d0, 1.0f, ahead);
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
-    st[n] = f32x16{};
 #pragma unroll
     for (int s = 0; s < L::kSteps; ++s) st[n] = mfma<T>(fl.frag(kt + n * L::kBytes, s), qf[s], st[n]);
   }
   keys_read();
-  constexpr bool kRaw = !CAP && !BIAS;  // scaled inside the exponential
-  if constexpr (!kRaw) tile_scores<CAP, BIAS, NT, false>(a, slope2, st, st, d0, 1.0f);
+  // (without a cap scaled inside the exponential)
+  if constexpr (CAP) capped_scores<BIAS, NT, false>(a, sc.slope2, st, st, d0, 1.0f);
   if (!whole) {
+    const int most = left - 4 * h;
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) st[n][r] = 32 * n + acc_row(r, h) < left ? st[n][r] : -INFINITY;
+      for (int r = 0; r < 16; ++r) st[n][r] = 32 * n + acc_row(r, 0) < most ? st[n][r] : -INFINITY;
   }
   float mx = -INFINITY;
 #pragma unroll
@@ -77,7 +79,7 @@ __device__ __forceinline__ void fwd_keys(const MaskedArgs& a, const FragLane<HD>
     for (int r = 0; r < 16; ++r) mx = fmaxf(mx, st[n][r]);
   const float2 mp = half_pair(mx);
   mx = fmaxf(mp.x, mp.y);
-  if constexpr (kRaw) mx *= a.sl2;  // scale > 0
+  if constexpr (!CAP) mx *= a.sl2;  // scale > 0
   const float mn = fmaxf(w.m, mx);
   const float ref = mn == -INFINITY ? 0.0f : mn;  // nothing seen yet: every P is 2^-inf
   if (__ballot(mx > w.m)) {
@@ -95,7 +97,7 @@ __device__ __forceinline__ void fwd_keys(const MaskedArgs& a, const FragLane<HD>
     float rs = 0.0f;
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
-      const float p = exp2_raw(kRaw ? __builtin_fmaf(st[n][r], a.sl2, -ref) : st[n][r] - ref);
+      const float p = exp2_raw(CAP ? st[n][r] - ref : __builtin_fmaf(st[n][r], a.sl2, -ref));
       st[n][r] = p;
       rs += p;
     }
@@ -152,8 +154,7 @@ __device__ __forceinline__ void fwd_block(const MaskedArgs& a, char* buf0, char*
   auto copy = [&](char* dst, int j) {
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
-      const int t = NT * j + n;
-      if (t >= tiles) break;
+      const int t = min(NT * j + n, tiles - 1);  // (behind the last tile: the last again, hidden)
       const int rows = r.lk - 32 * t;
       tk.copy(dst + n * L::kBytes, kh + 32 * t * a.k_st, rows);
       tv.copy(dst + (NT + n) * L::kBytes, vh + 32 * t * a.v_st, rows);
@@ -170,12 +171,9 @@ __device__ __forceinline__ void fwd_block(const MaskedArgs& a, char* buf0, char*
     const FragLane<HD> fl = fl0.fresh();
     const int mt = mine - NT * j, k0 = 32 * NT * j;  // this wave's tiles from here on, first key
     const float d0 = static_cast<float>(r.off() + i - k0 - 4 * h);
-    if (mt >= 2)
-      fwd_keys<T, HD, CAP, BIAS, 2>(a, fl, cur, vt, qf, w, sc.slope2, k0 + 64 <= vis_all, vis - k0, d0, h,
-                                    [] {}, [] {});
-    else if (mt == 1)
-      fwd_keys<T, HD, CAP, BIAS, 1>(a, fl, cur, vt, qf, w, sc.slope2, k0 + 32 <= vis_all, vis - k0, d0, h,
-                                    [] {}, [] {});
+    if (mt > 0)
+      fwd_keys<T, HD, CAP, BIAS, NT>(a, fl, cur, vt, qf, w, sc, k0 + 32 * NT <= vis_all, vis - k0, d0,
+                                     k0 + 32 * NT - 1 <= r.off() + iw, h, [] {}, [] {});
     stage_barrier();
   };
   for (int j = 0; j < stages; j += 2) {
@@ -261,7 +259,8 @@ __device__ __forceinline__ void split_block(const MaskedArgs& a, char* kbuf, cha
     const bool more = t + kWaves < last;
     if (t > first + wave) wait_copies<L::kCopies>();  // this K tile; the V tile behind it may be on its way
     fwd_keys<T, HD, CAP, BIAS, 1>(
-        a, fl, kt, vt, qf, w, sc.slope2, k0 + 32 <= vis_all, vis - k0, static_cast<float>(r.off() + i - k0 - 4 * h), h,
+        a, fl, kt, vt, qf, w, sc, k0 + 32 <= vis_all, vis - k0, static_cast<float>(r.off() + i - k0 - 4 * h),
+        k0 + 31 <= r.off() + i0, h,
         [&] {
           wait_reads();
           if (more) copy_k(t + kWaves);
@@ -472,6 +471,57 @@ struct BwdLds {
   float* ld1;
 };
 
+// dS^T of a 32 x 32 tile in st, a lane owning a query: st holds the products, dp dP^T. left: keys of the lane's query from
+// the tile's first on that it sees, edge: whether any query of the wave misses one.
+template <typename T, bool CAP, bool BIAS>
+__device__ __forceinline__ void query_scores(const MaskedArgs& a, float slope2, f32x16 (&st)[1], f32x16 (&f)[1],
+                                             const f32x16& dp, float dsum, float lse2, float d0, bool edge, int left,
+                                             int h) {
+  if constexpr (CAP) capped_scores<BIAS, 1, true>(a, slope2, st, f, d0, 1.0f);
+#pragma unroll
+  for (int e = 0; e < 16; ++e) {
+    const float p = exp2_raw(CAP ? st[0][e] - lse2 : __builtin_fmaf(st[0][e], a.sl2, -lse2));
+    st[0][e] = p * (dp[e] - dsum);
+    if constexpr (CAP) st[0][e] *= f[0][e];
+  }
+  if (edge) {
+    const int most = left - 4 * h;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) st[0][e] = acc_row(e, 0) < most ? st[0][e] : 0.0f;
+  }
+}
+
+// P in st and dS in dp of a 32 x 32 tile, a lane owning a key; stats(q, lse, D): those of the queries 8 q + 4 h .. + 4
+// (lse in log2 units). edge: whether a
+// query of the tile (below `first`: those that miss the lane's key; from `rows` on: none) stays out.
+template <typename T, bool CAP, bool BIAS, typename F>
+__device__ __forceinline__ void key_scores(const MaskedArgs& a, float slope2, f32x16 (&st)[1], f32x16 (&f)[1], f32x16& dp,
+                                           F stats, float d0, bool edge, int first, int rows, int h) {
+  if constexpr (CAP) capped_scores<BIAS, 1, true>(a, slope2, st, f, d0, -1.0f);
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    f32x4 lv, dd;
+    stats(q, lv, dd);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int e = 4 * q + i;
+      const float p = exp2_raw(CAP ? st[0][e] - lv[i] : __builtin_fmaf(st[0][e], a.sl2, -lv[i]));
+      st[0][e] = p;
+      dp[e] = p * (dp[e] - dd[i]);
+      if constexpr (CAP) dp[e] *= f[0][e];
+    }
+  }
+  if (edge) {
+    const int least = first - 4 * h, most = rows - 4 * h;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      const bool in = acc_row(e, 0) >= least && acc_row(e, 0) < most;
+      st[0][e] = in ? st[0][e] : 0.0f;
+      dp[e] = in ? dp[e] : 0.0f;
+    }
+  }
+}
+
 // dQ of 128 queries: key tiles stream through LDS, each wave owns 32 queries (Q and dO fragments in registers; D from
 // the same fragments).
 template <typename T, int HD, bool CAP, bool BIAS>
@@ -525,25 +575,16 @@ __device__ __forceinline__ void bwd_dq(const MaskedArgs& a, int blk, int head, c
     const char* vt = kt + L::kBytes;
     const FragLane<HD> fl = fl0.fresh();
     if (j < mine) {
-      f32x16 st[1] = {f32x16{}}, dp = f32x16{}, f[1];
+      f32x16 st[1], dp = f32x16{}, f[1];
+      start_scores<CAP, BIAS, 1>(st, sc.slope, static_cast<float>(r.off() + i - 32 * j - 4 * h), 1.0f, 32 * j + 31 <= r.off() + iw);
 #pragma unroll
       for (int k = 0; k < L::kSteps; ++k) {
         st[0] = mfma<T>(fl.frag(kt, k), qf[k], st[0]);  // S^T = K Q^T
         dp = mfma<T>(fl.frag(vt, k), df[k], dp);        // dP^T = V dO^T
       }
-      constexpr bool kRaw = !CAP && !BIAS;
-      if constexpr (!kRaw)
-        tile_scores<CAP, BIAS, 1, true>(a, sc.slope2, st, f, static_cast<float>(r.off() + i - 32 * j - 4 * h), 1.0f);
-#pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        const float p = exp2_raw(kRaw ? __builtin_fmaf(st[0][e], a.sl2, -lse2) : st[0][e] - lse2);
-        st[0][e] = p * (dp[e] - dsum);
-        if constexpr (CAP) st[0][e] *= f[0][e];
-      }
-      if (32 * j + 32 > vis_all) {
-#pragma unroll
-        for (int e = 0; e < 16; ++e) st[0][e] = 32 * j + acc_row(e, h) < vis ? st[0][e] : 0.0f;
-      }
+      query_scores<T, CAP, BIAS>(a, sc.slope2, st, f, dp, dsum, lse2,
+                                 static_cast<float>(r.off() + i - 32 * j - 4 * h), 32 * j + 32 > vis_all,
+                                 vis - 32 * j, h);
       const Frag s0 = frag_acc<T>(st[0], 0), s1 = frag_acc<T>(st[0], 1);
 #pragma unroll
       for (int d = 0; d < L::kDims; ++d) {
@@ -611,10 +652,8 @@ __device__ __forceinline__ void bwd_dkdv(const MaskedArgs& a, int blk, int head,
 #pragma unroll
     for (int i = 0; i < C; ++i) {
       const Frag y = *reinterpret_cast<const Frag*>(dst + L::kBytes + (C * wave + i) * 1024 + lane * 16);
-      float x = dot8<T>(orow[i], y, 0.0f);
-#pragma unroll
-      for (int o = L::kChunks / 2; o >= 1; o >>= 1) x += __shfl_xor(x, o, 64);
-      if (lane % L::kChunks == 0) ld[32 + tq.row[i]] = x;
+      const float x = group_sum<L::kChunks>(dot8<T>(orow[i], y, 0.0f));
+      if (lane % L::kChunks == 0) ld[32 + tq.row(i)] = x;
     }
   };
   if (t0 < tiles) copy(lds.buf0, t0);
@@ -642,37 +681,21 @@ __device__ __forceinline__ void bwd_dkdv(const MaskedArgs& a, int blk, int head,
     const char* dt = qt + L::kBytes;
     const FragLane<HD> fl = fl0.fresh();
     if (j >= q_wave) {
-      f32x16 st[1] = {f32x16{}}, dp = f32x16{}, f[1];
+      f32x16 st[1], dp = f32x16{}, f[1];
+      start_scores<CAP, BIAS, 1>(st, sc.slope, static_cast<float>(r.off() + 32 * j + 4 * h - kc), -1.0f, r.off() + 32 * j >= kw + 31);
 #pragma unroll
       for (int k = 0; k < L::kSteps; ++k) {
         st[0] = mfma<T>(fl.frag(qt, k), kf[k], st[0]);      // S = Q K^T
         dp = mfma<T>(fl.frag(dt, k), fl.frag(vt, k), dp);   // dP = dO V^T
       }
-      constexpr bool kRaw = !CAP && !BIAS;
-      if constexpr (!kRaw)
-        tile_scores<CAP, BIAS, 1, true>(a, sc.slope2, st, f, static_cast<float>(r.off() + 32 * j + 4 * h - kc), -1.0f);
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const f32x4 lv = *reinterpret_cast<const f32x4*>(ld + 8 * q + 4 * h);
-        const f32x4 dd = *reinterpret_cast<const f32x4*>(ld + 32 + 8 * q + 4 * h);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int e = 4 * q + i;
-          const float p = exp2_raw(kRaw ? __builtin_fmaf(st[0][e], a.sl2, -lv[i]) : st[0][e] - lv[i]);
-          st[0][e] = p;                    // P
-          dp[e] = p * (dp[e] - dd[i]);     // dS
-          if constexpr (CAP) dp[e] *= f[0][e];
-        }
-      }
-      if (32 * j < q_all || 32 * j + 32 > r.lq) {  // queries that do not see a key, and rows past the last
-#pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          const int i = 32 * j + acc_row(e, h);
-          const bool in = i >= q_lane && i < r.lq;
-          st[0][e] = in ? st[0][e] : 0.0f;
-          dp[e] = in ? dp[e] : 0.0f;
-        }
-      }
+      key_scores<T, CAP, BIAS>(
+          a, sc.slope2, st, f, dp,
+          [&](int q, f32x4& lv, f32x4& dd) {
+            lv = *reinterpret_cast<const f32x4*>(ld + 8 * q + 4 * h);
+            dd = *reinterpret_cast<const f32x4*>(ld + 32 + 8 * q + 4 * h);
+          },
+          static_cast<float>(r.off() + 32 * j + 4 * h - kc), 32 * j < q_all || 32 * j + 32 > r.lq, q_lane - 32 * j,
+          r.lq - 32 * j, h);
       const Frag p0 = frag_acc<T>(st[0], 0), p1 = frag_acc<T>(st[0], 1);
       const Frag s0 = frag_acc<T>(dp, 0), s1 = frag_acc<T>(dp, 1);
 #pragma unroll
@@ -749,6 +772,276 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2, 
     bwd_dq<T, HD, CAP, BIAS>(a, item - a.n_kblocks, head, lds);
 }
 
+// ---------------------------------------------------------------------------------------------
+// The backward of batches that leave the chip idle in blocks of 128: a block owns 32 tokens of one side, its four waves
+// take the other side's tiles in turn (each with LDS of its own) and their sums meet in the LDS in wave order.
+// ---------------------------------------------------------------------------------------------
+template <int HD>
+constexpr int kNarrowLds = (2 + 2 * kWaves) * Tiles<HD>::kBytes;  // two shared tiles, two a wave; then the sums
+
+// The waves' sums of one set of accumulators: every wave's tiles into LDS (lane-contiguous), then each wave adds 4 ND of
+// the 16 ND registers over the waves, in wave order: register wave * 4 ND + x.
+template <int ND>
+__device__ __forceinline__ void merge_waves(float* buf, const f32x16 (&acc)[ND], int wave, int lane, float (&x)[4 * ND]) {
+  __syncthreads();
+  if (threadIdx.x == 0) reinterpret_cast<uint32_t*>(buf)[kWaves * 64 * 16 * ND] = 0;  // the rows to form again
+#pragma unroll
+  for (int d = 0; d < ND; ++d)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) buf[(wave * 16 * ND + 16 * d + e) * 64 + lane] = acc[d][e];
+  __syncthreads();
+#pragma unroll
+  for (int y = 0; y < 4 * ND; ++y) {
+    x[y] = 0.0f;
+#pragma unroll
+    for (int v = 0; v < kWaves; ++v) x[y] += buf[(v * 16 * ND + wave * 4 * ND + y) * 64 + lane];
+  }
+}
+
+template <typename T, int HD, bool CAP, bool BIAS>
+__device__ __forceinline__ void narrow_dq(const MaskedArgs& a, int blk, int head, char* smem) {
+  uint32_t* again = reinterpret_cast<uint32_t*>(smem + kWaves * 64 * 16 * (HD / 32) * 4);  // behind the waves' sums
+  using L = Tiles<HD>;
+  constexpr int ND = L::kDims;
+  int s, b, nb;
+  if (!find_span_block(a.cu_q, a.n_seq, static_cast<int>(a.n_q), blk, 32, s, b, nb)) return;
+  const MaskedRow r = uniform(as_queries(masked_row(a, s), s, a.n_seq));
+  b = uniform(nb - 1 - b);
+  const int g = head / (a.h_q / a.h_kv);
+  const int wave = uniform(static_cast<int>(threadIdx.x) >> 6);
+  const int lane = threadIdx.x & 63, h = lane >> 5, col = lane & 31;
+  const int i0 = 32 * b, i = min(i0 + col, r.lq - 1);
+  const bool valid = i0 + col < r.lq;
+  const int vis = r.vis(i, a.causal), vis_all = r.vis(i0, a.causal);
+  const int tiles = (r.vis(min(i0 + 31, r.lq - 1), a.causal) + 31) / 32;
+  const T* kh = token<T>(a.k, r.ka, a.k_st, g, a.k_sh);
+  const T* vh = token<T>(a.v, r.ka, a.v_st, g, a.v_sh);
+  const TileLane<HD, L::kCopies> tk(0, lane, a.k_st), tv(0, lane, a.v_st);
+  const FragLane<HD> fl(lane);
+  const Scorer<CAP, BIAS> sc(a, head);
+  char* kt = smem + 2 * wave * L::kBytes;
+  char* vt = kt + L::kBytes;
+  auto copy = [&](int j) {
+    tk.fresh().copy(kt, kh + 32 * j * a.k_st, r.lk - 32 * j);
+    tv.fresh().copy(vt, vh + 32 * j * a.v_st, r.lk - 32 * j);
+  };
+  if (wave < tiles) copy(wave);
+  const int64_t t = r.qa + i;
+  Frag qf[L::kSteps], df[L::kSteps];
+  load_row_frags<T, HD>(qf, token<T>(a.q, t, a.q_st, head, a.q_sh), h);
+  load_row_frags<T, HD>(df, token<T>(a.dout, t, a.do_st, head, a.do_sh), h);
+  float ds = 0.0f;
+  {
+    Frag of[L::kSteps];
+    load_row_frags<T, HD>(of, static_cast<const T*>(a.o) + (t * a.h_q + head) * HD, h);
+#pragma unroll
+    for (int k = 0; k < L::kSteps; ++k) ds = dot8<T>(of[k], df[k], ds);
+  }
+  const float2 dp2 = half_pair(ds);
+  const float dsum = dp2.x + dp2.y;
+  const float lse2 = a.lse[head * a.n_q + t] * kLog2e;
+  f32x16 dq[ND];
+#pragma unroll
+  for (int d = 0; d < ND; ++d) dq[d] = f32x16{};
+  stage_wait();
+  for (int j = wave; j < tiles; j += kWaves) {
+    f32x16 st[1], dp = f32x16{}, f[1];
+    start_scores<CAP, BIAS, 1>(st, sc.slope, static_cast<float>(r.off() + i - 32 * j - 4 * h), 1.0f, 32 * j + 31 <= r.off() + i0);
+#pragma unroll
+    for (int k = 0; k < L::kSteps; ++k) {
+      st[0] = mfma<T>(fl.frag(kt, k), qf[k], st[0]);  // S^T = K Q^T
+      dp = mfma<T>(fl.frag(vt, k), df[k], dp);        // dP^T = V dO^T
+    }
+    query_scores<T, CAP, BIAS>(a, sc.slope2, st, f, dp, dsum, lse2, static_cast<float>(r.off() + i - 32 * j - 4 * h),
+                               32 * j + 32 > vis_all, vis - 32 * j, h);
+    const Frag s0 = frag_acc<T>(st[0], 0), s1 = frag_acc<T>(st[0], 1);
+#pragma unroll
+    for (int d = 0; d < ND; ++d) {
+      dq[d] = mfma<T>(fl.frag_t(kt, 0, d), s0, dq[d]);  // dQ^T += K^T dS^T
+      dq[d] = mfma<T>(fl.frag_t(kt, 1, d), s1, dq[d]);
+    }
+    if (j + kWaves < tiles) {
+      wait_reads();
+      copy(j + kWaves);
+      wait_copies<0>();
+    }
+  }
+  float x[4 * ND];
+  merge_waves<ND>(reinterpret_cast<float*>(smem), dq, wave, lane, x);
+  bool fine = true;
+#pragma unroll
+  for (int y = 0; y < 4 * ND; ++y) {
+    x[y] *= a.scale;
+    fine = fine && fabsf(x[y]) <= 3.402823466e38f;
+  }
+  if (valid && !fine) atomicOr(again, 1u << col);
+  __syncthreads();
+  uint32_t cols = *again;
+  if (valid && !((cols >> col) & 1)) {
+    T* row = static_cast<T*>(a.out) + (t * a.h_q + head) * HD;
+#pragma unroll
+    for (int q = 0; q < ND; ++q) {  // four registers: head dims 32 d + 8 (e / 4) + 4 h .. + 4
+      const int e = wave * 4 * ND + 4 * q;
+      const float o[4] = {x[4 * q], x[4 * q + 1], x[4 * q + 2], x[4 * q + 3]};
+      store_from_f32<T, 4>(row + 32 * (e >> 4) + acc_row(e & 15, h), o);
+    }
+  }
+  for (; cols; cols &= cols - 1)
+    if (__builtin_ctz(cols) % kWaves == wave) plain_dq_row<T, HD, CAP, BIAS>(a, r, i0 + __builtin_ctz(cols), head);
+}
+
+template <typename T, int HD, bool CAP, bool BIAS>
+__device__ __forceinline__ void narrow_dkdv(const MaskedArgs& a, int blk, int head, char* smem) {
+  // (the word behind the waves' sums: the tiles leave no other room for two blocks a CU)
+  uint32_t* again = reinterpret_cast<uint32_t*>(smem + kWaves * 64 * 16 * (HD / 32) * 4);
+  using L = Tiles<HD>;
+  constexpr int ND = L::kDims;
+  int s, b, nb;
+  if (!find_span_block(a.cu_k, a.n_seq, static_cast<int>(a.n_k), blk, 32, s, b, nb)) return;
+  const MaskedRow r = uniform(as_keys(masked_row(a, s), s, a.n_seq));
+  const int grp = a.h_q / a.h_kv, g = head / grp;
+  const int wave = uniform(static_cast<int>(threadIdx.x) >> 6);
+  const int lane = threadIdx.x & 63, h = lane >> 5, col = lane & 31;
+  const int k0 = 32 * uniform(b), kc = min(k0 + col, r.lk - 1);
+  const int t0 = r.first(k0, a.causal) / 32, tiles = (r.lq + 31) / 32;
+  const int q_lane = r.first(kc, a.causal);                     // the lane's first query
+  const int q_all = r.first(min(k0 + 31, r.lk - 1), a.causal);  // from here on every key is seen
+  const T* qh = token<T>(a.q, r.qa, a.q_st, head, a.q_sh);
+  const T* doh = token<T>(a.dout, r.qa, a.do_st, head, a.do_sh);
+  const int64_t o_st = static_cast<int64_t>(a.h_q) * HD;
+  const T* oh = static_cast<const T*>(a.o) + r.qa * o_st + head * HD;
+  const float* lse = a.lse + head * a.n_q + r.qa;
+  const TileLane<HD, L::kCopies> tq(0, lane, a.q_st), td(0, lane, a.do_st), to(0, lane, o_st);
+  const FragLane<HD> fl(lane);
+  const Scorer<CAP, BIAS> sc(a, head);
+  char* kt = smem;
+  char* vt = smem + L::kBytes;
+  char* qt = smem + (2 + 2 * wave) * L::kBytes;
+  char* dt = qt + L::kBytes;
+  Frag orow[L::kCopies];  // the O chunks of the dO chunks this lane copies
+  float lr = 0.0f;
+  auto copy = [&](int j) {
+    const int rows = r.lq - 32 * j;
+    tq.fresh().copy(qt, qh + 32 * j * a.q_st, rows);
+    td.fresh().copy(dt, doh + 32 * j * a.do_st, rows);
+    const auto o = to.fresh();
+#pragma unroll
+    for (int i = 0; i < L::kCopies; ++i)
+      orow[i] = *reinterpret_cast<const Frag*>(reinterpret_cast<const char*>(oh + 32 * j * o_st) + o.at(i, rows));
+    lr = lse[32 * j + min(col, rows - 1)];
+  };
+  // lse and D of tile row c in lanes c and c + 32.
+  float lse2 = 0.0f, dsum = 0.0f;
+  auto finish = [&] {
+    wait_copies<0>();
+    lse2 = lr * kLog2e;
+    constexpr int kRowsPerCopy = 64 / L::kChunks;
+#pragma unroll
+    for (int i = 0; i < L::kCopies; ++i) {
+      const Frag y = *reinterpret_cast<const Frag*>(dt + i * 1024 + lane * 16);
+      const float x = group_sum<L::kChunks>(dot8<T>(orow[i], y, 0.0f));
+      const float v = __shfl(x, col % kRowsPerCopy * L::kChunks, 64);
+      if (col / kRowsPerCopy == i) dsum = v;
+    }
+  };
+  constexpr int C = L::kCopies / kWaves;
+  TileLane<HD, C>(C * wave, lane, a.k_st)
+      .copy(kt, token<T>(a.k, static_cast<int64_t>(r.ka) + k0, a.k_st, g, a.k_sh), r.lk - k0);
+  TileLane<HD, C>(C * wave, lane, a.v_st)
+      .copy(vt, token<T>(a.v, static_cast<int64_t>(r.ka) + k0, a.v_st, g, a.v_sh), r.lk - k0);
+  if (t0 + wave < tiles) copy(t0 + wave);
+  f32x16 dk[ND], dv[ND];
+#pragma unroll
+  for (int d = 0; d < ND; ++d) {
+    dk[d] = f32x16{};
+    dv[d] = f32x16{};
+  }
+  stage_barrier();
+  if (t0 + wave < tiles) finish();
+  for (int j = t0 + wave; j < tiles; j += kWaves) {
+    f32x16 st[1], dp = f32x16{}, f[1];
+    start_scores<CAP, BIAS, 1>(st, sc.slope, static_cast<float>(r.off() + 32 * j + 4 * h - kc), -1.0f, r.off() + 32 * j >= k0 + 31);
+#pragma unroll
+    for (int k = 0; k < L::kSteps; ++k) {
+      st[0] = mfma<T>(fl.frag(qt, k), fl.frag(kt, k), st[0]);  // S = Q K^T
+      dp = mfma<T>(fl.frag(dt, k), fl.frag(vt, k), dp);        // dP = dO V^T
+    }
+    key_scores<T, CAP, BIAS>(
+        a, sc.slope2, st, f, dp,
+        [&](int q, f32x4& lv, f32x4& dd) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            lv[i] = __shfl(lse2, 8 * q + 4 * h + i, 64);
+            dd[i] = __shfl(dsum, 8 * q + 4 * h + i, 64);
+          }
+        },
+        static_cast<float>(r.off() + 32 * j + 4 * h - kc), 32 * j < q_all || 32 * j + 32 > r.lq, q_lane - 32 * j,
+        r.lq - 32 * j, h);
+    const Frag p0 = frag_acc<T>(st[0], 0), p1 = frag_acc<T>(st[0], 1);
+    const Frag s0 = frag_acc<T>(dp, 0), s1 = frag_acc<T>(dp, 1);
+#pragma unroll
+    for (int d = 0; d < ND; ++d) {
+      dv[d] = mfma<T>(p0, fl.frag_t(dt, 0, d), dv[d]);  // dV += P^T dO
+      dv[d] = mfma<T>(p1, fl.frag_t(dt, 1, d), dv[d]);
+      dk[d] = mfma<T>(s0, fl.frag_t(qt, 0, d), dk[d]);  // dK += dS^T Q
+      dk[d] = mfma<T>(s1, fl.frag_t(qt, 1, d), dk[d]);
+    }
+    if (j + kWaves < tiles) {
+      wait_reads();
+      copy(j + kWaves);
+      finish();
+    }
+  }
+  // Keys are accumulator rows, head dims lanes.
+  float x[4 * ND], y[4 * ND];
+  merge_waves<ND>(reinterpret_cast<float*>(smem), dk, wave, lane, x);
+  merge_waves<ND>(reinterpret_cast<float*>(smem), dv, wave, lane, y);
+#pragma unroll
+  for (int e = 0; e < 4 * ND; ++e) {
+    x[e] *= a.scale;
+    if (!(fabsf(x[e]) <= 3.402823466e38f && fabsf(y[e]) <= 3.402823466e38f))
+      atomicOr(again, 1u << acc_row((wave * 4 * ND + e) & 15, h));
+  }
+  __syncthreads();
+  uint32_t bad = *again;
+#pragma unroll
+  for (int e = 0; e < 4 * ND; ++e) {
+    const int reg = wave * 4 * ND + e, row = acc_row(reg & 15, h), key = k0 + row;
+    if (key >= r.lk || ((bad >> row) & 1)) continue;
+    const int64_t t = r.ka + key;
+    const int dim = 32 * (reg >> 4) + col;
+    if (grp > 1) {
+      const int64_t o = (head * a.n_k + t) * HD + dim;
+      store_partial(a.dk_part + o, x[e]);
+      store_partial(a.dv_part + o, y[e]);
+    } else {
+      const int64_t o = (t * a.h_kv + g) * HD + dim;
+      static_cast<T*>(a.dk)[o] = from_f32<T>(x[e]);
+      static_cast<T*>(a.dv)[o] = from_f32<T>(y[e]);
+    }
+  }
+  for (; bad; bad &= bad - 1) {
+    const int key = k0 + __builtin_ctz(bad);
+    if (key >= r.lk) break;
+    if (__builtin_ctz(bad) % kWaves != wave) continue;
+    const int64_t o = (head * a.n_k + r.ka + key) * HD;
+    plain_dkv_row<T, HD, CAP, BIAS>(a, r, key, head, head + 1, grp > 1 ? a.dk_part + o : nullptr,
+                                    grp > 1 ? a.dv_part + o : nullptr);
+  }
+}
+
+template <typename T, int HD, bool CAP, bool BIAS>
+__global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2, 2))) void masked_narrow_bwd_kernel(
+    MaskedArgs a) {
+  __shared__ __attribute__((aligned(16))) char smem[kNarrowLds<HD>];
+  int item, head;
+  if (!head_item(a, a.n_kblocks + a.n_blocks, item, head)) return;
+  if (item < a.n_kblocks)
+    narrow_dkdv<T, HD, CAP, BIAS>(a, item, head, smem);
+  else
+    narrow_dq<T, HD, CAP, BIAS>(a, item - a.n_kblocks, head, smem);
+}
+
 // dk / dv [key, g, :] = T(sum over the KV group's heads, in head order, of the parts). Thread = 4 head dims of a key.
 template <typename T>
 __global__ __launch_bounds__(256) void masked_group_sum_kernel(MaskedArgs a, int hd4) {
@@ -806,28 +1099,51 @@ void dispatch(int dtype, int hd, bool cap, bool bias, F f) {
     by_dim(bf16{});
 }
 
-int64_t blocks_bound(int64_t n, int32_t n_seq) { return (n + kRows - 1) / kRows + n_seq + 2; }
+// Blocks of `rows` tokens over all rows, bound: each holds a token at least.
+int64_t blocks_bound(int64_t n, int32_t n_seq, int rows) { return std::min<int64_t>((n + rows - 1) / rows + n_seq + 2, n); }
 
 // How a forward runs: splits = 0: blocks of 128 queries; otherwise blocks of few queries, the keys in `splits` parts of
-// `tiles` tiles each.
+// `tiles` tiles each. The former walk a row's keys alone (1.6 us per 64 of them, whatever else runs), so they win where
+// rows are short or blocks many; the latter share them among four waves and the parts, but read K and V again for every
+// 32 / group queries (2.2 us per 128 keys and round of two blocks a CU, 4 us a round aside; heads of 64 half as long).
+// How long the rows are beyond the longest is known on the device only: on average tokens over rows. Measured, 12 / 2
+// heads of 128, us in blocks of 128 / of few: 100 tokens 9.7 / 8.2, 707 23.3 / 15.6, 2,048 53 / 45, 3,000 75 / 75, 4,096
+// 104 / 120, ten rows of 256 13.9 / 23.0, four of 1,024 52 / 57, 1,500 and 27 rows of 64 44 / 37; 4 / 1 heads, 4,096
+// 98 / 51; 16 heads of 64 without a causal mask, eight rows of 700 35 / 59, 1,025 + 577 + 257 + 64 31 / 29.
 struct SplitPlan {
   int splits, tiles;
   int64_t items;  // blocks of few queries, bound over all rows
 };
 
-SplitPlan split_plan(int32_t n_seq, int64_t n_q, int32_t max_k, int32_t h_q, int32_t h_kv) {
+SplitPlan split_plan(int32_t n_seq, int64_t n_q, int64_t n_k, int32_t max_k, int32_t h_q, int32_t h_kv,
+                     int32_t head_dim) {
   SplitPlan p{0, 0, 0};
   const int grp = h_q / h_kv;
   if (grp > kMaxSplitGroup) return p;
-  if (std::max<int64_t>((n_q + kRows - 1) / kRows, n_seq) * h_q >= 256) return p;
   const int tpb = split_tokens(grp);
-  p.items = std::min<int64_t>((n_q + tpb - 1) / tpb + n_seq + 2, n_q);  // a block has a query at least
   const int64_t base = std::max<int64_t>((n_q + tpb - 1) / tpb, n_seq) * h_kv;
   const int64_t tiles = std::max<int64_t>((static_cast<int64_t>(max_k) + 31) / 32, 1);
-  const int64_t want = std::min<int64_t>(512 / base, (tiles + 7) / 8);
-  p.splits = static_cast<int>(std::max<int64_t>(want, 1));
-  p.tiles = static_cast<int>((tiles + p.splits - 1) / p.splits);
+  const int64_t splits = std::max<int64_t>(std::min<int64_t>(512 / base, (tiles + 7) / 8), 1);
+  const int64_t part = (tiles + splits - 1) / splits;
+  const double wide_load = std::max(1.0, std::max<int64_t>((n_q + kRows - 1) / kRows, n_seq) * h_q / 512.0);
+  const double wide_us = 7.0 + 0.8 * tiles * wide_load;
+  const double row = std::min<double>(static_cast<double>(max_k), static_cast<double>(n_k) / n_seq);
+  const double step_us = head_dim == 64 ? 1.1 : 2.2, steps = n_q < n_k ? row / 128 : row / 256;
+  const double few_us =
+      4.0 + std::max(0.4 * part, std::max(1.0, base * splits / 512.0) * (4.0 + step_us * steps / splits)) +
+      (splits > 1 ? 4.0 : 0.0);
+  if (wide_us <= few_us) return p;
+  p.items = std::min<int64_t>((n_q + tpb - 1) / tpb + n_seq + 2, n_q);  // a block has a query at least
+  p.splits = static_cast<int>(splits);
+  p.tiles = static_cast<int>(part);
   return p;
+}
+
+// Whether a backward runs in blocks of 32 tokens: where blocks of 128 would leave the chip idle. 12 / 2 heads of 128, us in
+// blocks of 128 / of 32: 100 tokens 22 / 15, 707 52 / 37, 1,024 65 / 46, 1,024 and ten rows of 64 (156 blocks of 128)
+// 67 / 59; from 192 blocks on the other way round: 2,048 117 / 120, four rows of 512 46 / 64, ten of 256 37 / 67.
+bool narrow_bwd(int32_t n_seq, int64_t n_q, int64_t n_k, int32_t h_q) {
+  return std::max<int64_t>((std::max(n_q, n_k) + kRows - 1) / kRows, n_seq) * h_q < 192;
 }
 
 // Launch size of n_items for every head (whole chunks of head_item's).
@@ -900,7 +1216,7 @@ extern "C" int rus_attn_masked_workspace(int32_t n_seq, int64_t n_q, int64_t n_k
     *floats = h_q > h_kv ? 2 * static_cast<int64_t>(h_q) * n_k * head_dim : 0;
     return RUS_OK;
   }
-  const SplitPlan p = split_plan(n_seq, n_q, max_k, h_q, h_kv);
+  const SplitPlan p = split_plan(n_seq, n_q, n_k, max_k, h_q, h_kv, head_dim);
   *floats = p.splits > 1 ? p.splits * n_q * h_q * (head_dim + 4) : 0;
   return RUS_OK;
 }
@@ -929,7 +1245,7 @@ extern "C" int rus_attn_masked_fwd(const void* q, int64_t q_stride_t, int64_t q_
   a.out = out, a.lse = lse;
   a.cu_q = cu_q, a.cu_k = cu_k, a.n_seq = n_seq, a.n_q = n_q, a.n_k = n_k, a.h_q = h_q, a.h_kv = h_kv;
   set_scores(a, scale, softcap, slopes, prefix, causal);
-  const SplitPlan p = split_plan(n_seq, n_q, max_k, h_q, h_kv);
+  const SplitPlan p = split_plan(n_seq, n_q, n_k, max_k, h_q, h_kv, head_dim);
   if (p.splits) {
     a.splits = p.splits;
     a.split_tiles = p.tiles;
@@ -958,7 +1274,7 @@ extern "C" int rus_attn_masked_fwd(const void* q, int64_t q_stride_t, int64_t q_
     });
     return check_launch(fn);
   }
-  a.n_blocks = static_cast<int>(blocks_bound(n_q, n_seq));
+  a.n_blocks = static_cast<int>(blocks_bound(n_q, n_seq, kRows));
   int64_t grid;
   if (int e = item_grid(fn, a.n_blocks, a, grid)) return e;
   dispatch(dtype, head_dim, softcap > 0.0f, slopes != nullptr, [&](auto t, auto d, auto c, auto b) {
@@ -997,8 +1313,10 @@ extern "C" int rus_attn_masked_bwd(const void* dout, int64_t do_stride_t, int64_
   a.out = dq, a.dk = dk, a.dv = dv;
   a.cu_q = cu_q, a.cu_k = cu_k, a.n_seq = n_seq, a.n_q = n_q, a.n_k = n_k, a.h_q = h_q, a.h_kv = h_kv;
   set_scores(a, scale, softcap, slopes, prefix, causal);
-  a.n_blocks = static_cast<int>(blocks_bound(n_q, n_seq));
-  a.n_kblocks = static_cast<int>(blocks_bound(n_k, n_seq));
+  const bool narrow = narrow_bwd(n_seq, n_q, n_k, h_q);
+  const int rows = narrow ? 32 : kRows;
+  a.n_blocks = static_cast<int>(blocks_bound(n_q, n_seq, rows));
+  a.n_kblocks = static_cast<int>(blocks_bound(n_k, n_seq, rows));
   int64_t grid;
   if (int e = item_grid(fn, a.n_blocks + a.n_kblocks, a, grid)) return e;
   const int64_t half = static_cast<int64_t>(h_q) * n_k * head_dim;
@@ -1009,17 +1327,24 @@ extern "C" int rus_attn_masked_bwd(const void* dout, int64_t do_stride_t, int64_
     a.dk_part = workspace;
     a.dv_part = workspace + half;
   }
+  const dim3 blocks(static_cast<unsigned>(grid)), threads(64 * kWaves);
+  hipStream_t st = static_cast<hipStream_t>(stream);
   dispatch(dtype, head_dim, softcap > 0.0f, slopes != nullptr, [&](auto t, auto d, auto c, auto b) {
-    hipLaunchKernelGGL((masked_bwd_kernel<decltype(t), decltype(d)::value, decltype(c)::value, decltype(b)::value>),
-                       dim3(grid), dim3(64 * kWaves), 0, static_cast<hipStream_t>(stream), a);
+    using T = decltype(t);
+    constexpr int kDim = decltype(d)::value;
+    constexpr bool kCap = decltype(c)::value, kBias = decltype(b)::value;
+    if (narrow)
+      hipLaunchKernelGGL((masked_narrow_bwd_kernel<T, kDim, kCap, kBias>), blocks, threads, 0, st, a);
+    else
+      hipLaunchKernelGGL((masked_bwd_kernel<T, kDim, kCap, kBias>), blocks, threads, 0, st, a);
   });
   if (int e = check_launch(fn)) return e;
   if (h_q == h_kv || n_k == 0) return RUS_OK;
   const int hd4 = head_dim / 4;
-  const dim3 blocks(static_cast<unsigned>((n_k * h_kv * hd4 + 255) / 256), 2);
+  const dim3 sums(static_cast<unsigned>((n_k * h_kv * hd4 + 255) / 256), 2);
   if (dtype == RUS_DTYPE_F16)
-    hipLaunchKernelGGL(masked_group_sum_kernel<f16>, blocks, dim3(256), 0, static_cast<hipStream_t>(stream), a, hd4);
+    hipLaunchKernelGGL(masked_group_sum_kernel<f16>, sums, dim3(256), 0, st, a, hd4);
   else
-    hipLaunchKernelGGL(masked_group_sum_kernel<bf16>, blocks, dim3(256), 0, static_cast<hipStream_t>(stream), a, hd4);
+    hipLaunchKernelGGL(masked_group_sum_kernel<bf16>, sums, dim3(256), 0, st, a, hd4);
   return check_launch(fn);
 }

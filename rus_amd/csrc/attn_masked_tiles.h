@@ -76,6 +76,24 @@ __device__ __forceinline__ float2 half_pair(float x) {
                 __builtin_bit_cast(float, static_cast<uint32_t>(p[1]))};
 }
 
+template <int CTRL>
+__device__ __forceinline__ float dpp(float x) {
+  return __builtin_bit_cast(float,
+                            __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), CTRL, 0xF, 0xF, false));
+}
+
+// Sum over groups of 16 (or 8) neighbouring lanes, in every lane, by VALU moves: lanes c ^ 1, c ^ 2, then, each group of 4
+// holding its sum, 7 - c within 8 and 15 - c within 16.
+template <int N>
+__device__ __forceinline__ float group_sum(float x) {
+  static_assert(N == 8 || N == 16, "groups of 8 or 16 lanes");
+  x += dpp<0xB1>(x);   // quad_perm 1 0 3 2
+  x += dpp<0x4E>(x);   // quad_perm 2 3 0 1
+  x += dpp<0x141>(x);  // row_half_mirror
+  if constexpr (N == 16) x += dpp<0x140>(x);  // row_mirror
+  return x;
+}
+
 template <int HD>
 struct Tiles {
   static constexpr int kRow = 2 * HD;          // bytes of a tile row
@@ -93,28 +111,36 @@ struct Tiles {
   }
 };
 
-// A wave's share, C copies from copy c0 on, of the kCopies that fill a tile. The tile's first row is a uniform pointer;
+// A wave's share, C copies from copy c0 (a multiple of C) on, of the kCopies that fill a tile: copy i fills kStep whole
+// rows, lane l the position l % kChunks of row kStep i + l / kChunks, i.e. it loads that position's chunk. From copy to
+// copy the swizzle changes in a bit or two that do not depend on the lane. The tile's first row is a uniform pointer;
 // rows past the last repeat it (finite or not: hidden either way).
 template <int HD, int C>
 struct TileLane {
   using L = Tiles<HD>;
-  int c0;
-  int row[C];       // tile row of copy i
-  uint32_t ch[C];   // byte offset of its chunk within the row
-  uint32_t off[C];
-  uint32_t stride;  // bytes per token
+  static constexpr int kStep = 64 / L::kChunks;
+  int c0, row0;       // first copy, the lane's row in it
+  uint32_t ch0, off0;  // byte offset of the lane's chunk within that row, of that row
+  uint32_t stride;    // bytes per token
 
   __device__ __forceinline__ TileLane(int first, int lane, int64_t stride_el)
-      : c0(first), stride(static_cast<uint32_t>(stride_el) * 2) {
-#pragma unroll
-    for (int i = 0; i < C; ++i) {
-      row[i] = (64 / L::kChunks) * (first + i) + lane / L::kChunks;
-      ch[i] = ((lane % L::kChunks) ^ L::swz(row[i])) << 4;
-      off[i] = row[i] * stride + ch[i];
-    }
+      : c0(first), row0(kStep * first + lane / L::kChunks), stride(static_cast<uint32_t>(stride_el) * 2) {
+    ch0 = ((lane % L::kChunks) ^ L::swz(row0)) << 4;
+    off0 = row0 * stride;
   }
-  __device__ __forceinline__ uint32_t at(int i, int rows) const {  // rows: tokens left in the row of the batch
-    return rows >= 32 ? off[i] : min(row[i], rows - 1) * stride + ch[i];
+  __device__ __forceinline__ int row(int i) const { return row0 + kStep * i; }
+  // A copy whose offsets the compiler forms again rather than keep each copy's in a register across the loop.
+  __device__ __forceinline__ TileLane fresh() const {
+    TileLane t = *this;
+    asm("" : "+v"(t.ch0), "+v"(t.off0));
+    return t;
+  }
+  __device__ __forceinline__ uint32_t chunk(int i) const {
+    return ch0 ^ (HD == 128 ? (i & 3) << 4 : (i & 1) << 5);
+  }
+  // Byte offset from the tile's first row of what copy i reads; rows: tokens left in the row of the batch.
+  __device__ __forceinline__ uint32_t at(int i, int rows) const {
+    return (rows >= 32 ? off0 + static_cast<uint32_t>(i * kStep) * stride : min(row(i), rows - 1) * stride) + chunk(i);
   }
   // The builtin's LDS target must be a __shared__ array of its own, so that the compiler knows which LDS reads have to
   // wait for it.
@@ -213,43 +239,61 @@ __device__ __forceinline__ bool all_finite(const f32x16 (&x)[ND], float f) {
   return z == 0.0f;
 }
 
-// Scores of NT tiles of products, log2 units: the same as Scorer::score, the choice of tanh made for a whole wave (its
-// largest |x|: where that is above 1/4 the fast form's error is 2^-20 of the largest score, as that of its product is).
-// d0: distance of the lane's first element; tile n's register r is d0 - step * (32 n + acc_row(r, 0)) away. factor: 1 -
-// t^2.
-template <bool CAP, bool BIAS, int NT, bool FACTOR>
-__device__ __forceinline__ void tile_scores(const MaskedArgs& a, float slope2, f32x16 (&st)[NT], f32x16 (&factor)[NT],
-                                            float d0, float step) {
-  if constexpr (CAP) {
-    float top = 0.0f;
-#pragma unroll
-    for (int n = 0; n < NT; ++n)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) top = fmaxf(top, fabsf(st[n][r]));
-    if (__ballot(!(top * a.kc <= kSmallTanh))) {
+// What the products of NT tiles start from: 0, or, where only a bias by distance is added, the bias in the products' own
+// unit (slope / scale), so that it costs no instruction behind the products. d0: distance of the lane's first element;
+// tile n's register r is d0 - step * (32 n + acc_row(r, 0)) away. ahead: none of these distances is negative.
+template <bool CAP, bool BIAS, int NT>
+__device__ __forceinline__ void start_scores(f32x16 (&st)[NT], float slope, float d0, float step, bool ahead) {
+  if constexpr (BIAS && !CAP) {
+    const float at0 = -slope * d0, per = slope * step;
+    if (ahead) {
 #pragma unroll
       for (int n = 0; n < NT; ++n)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          const float u = __builtin_amdgcn_rcpf(1.0f + exp2_raw(st[n][r] * a.k2));
-          if constexpr (FACTOR) factor[n][r] = 4.0f * __builtin_fmaf(-u, u, u);
-          st[n][r] = __builtin_fmaf(-2.0f * a.cap2, u, a.cap2);
-        }
+        for (int r = 0; r < 16; ++r)
+          st[n][r] = __builtin_fmaf(per, static_cast<float>(32 * n + acc_row(r, 0)), at0);
     } else {
 #pragma unroll
       for (int n = 0; n < NT; ++n)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          const float t = tanh_small(st[n][r] * a.kc);
-          if constexpr (FACTOR) factor[n][r] = __builtin_fmaf(-t, t, 1.0f);
-          st[n][r] = t * a.cap2;
-        }
+        for (int r = 0; r < 16; ++r)
+          st[n][r] = -slope * fabsf(d0 - step * static_cast<float>(32 * n + acc_row(r, 0)));
     }
+  } else {
+#pragma unroll
+    for (int n = 0; n < NT; ++n) st[n] = f32x16{};
+  }
+}
+
+// With a cap: scores of NT tiles of products, log2 units, and 1 - t^2 in factor. The choice of tanh is made for a whole
+// wave (its largest |x|: where that is above 1/4 the fast form's error is 2^-20 of the largest score, as that of its
+// product is). slope2, d0, step: the bias, as above.
+template <bool BIAS, int NT, bool FACTOR>
+__device__ __forceinline__ void capped_scores(const MaskedArgs& a, float slope2, f32x16 (&st)[NT], f32x16 (&factor)[NT],
+                                              float d0, float step) {
+  float top = 0.0f;
+#pragma unroll
+  for (int n = 0; n < NT; ++n)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) top = fmaxf(top, fabsf(st[n][r]));
+  if (__ballot(!(top * a.kc <= kSmallTanh))) {
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const float u = __builtin_amdgcn_rcpf(1.0f + exp2_raw(st[n][r] * a.k2));
+        if constexpr (FACTOR) factor[n][r] = 4.0f * __builtin_fmaf(-u, u, u);
+        st[n][r] = __builtin_fmaf(-2.0f * a.cap2, u, a.cap2);
+      }
   } else {
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) st[n][r] *= a.sl2;
+      for (int r = 0; r < 16; ++r) {
+        const float t = tanh_small(st[n][r] * a.kc);
+        if constexpr (FACTOR) factor[n][r] = __builtin_fmaf(-t, t, 1.0f);
+        st[n][r] = t * a.cap2;
+      }
   }
   if constexpr (BIAS) {
 #pragma unroll
