@@ -997,33 +997,28 @@ int rus_attn_masked_bwd(const void* dout, int64_t do_stride_t, int64_t do_stride
  * denom = max(*num_items or the number of tokens with entries, 1). Tokens without entries: kl 0, dH 0. An id that
  * comes twice adds its q.
  *
- * rus_lmhead_distill_fwd: vocabulary rows [256 part_base, + n_vocab) of the head, as rus_lmhead_ce_fwd_probs: partial
- * maxima and sums of h W^T / T (fp32 logits) per 256 rows, and, where probs is given, P = fp16(2^(z log2 e - ref)),
- * half_ref and chunk_max, for rus_lmhead_ce_probs_rescale and rus_lmhead_ce_grad_hidden_scaled. d a multiple of 64.
- * rus_lmhead_distill_blank: P = 0 at the teacher's entries among rows [vocab_start, + n_rows), before its product.
- * rus_lmhead_distill_entries: once every chunk is in the partials: kl, lse (of z), taught (1 or 0) [n_tok], coef
- * [n_tok, n_entries] (NULL: no gradient wanted), loss and denom (one each). weight: all n_vocab rows, in device
- * memory or page-locked, device-mapped host memory.
- * rus_lmhead_distill_finish: dH in fp32 [n_tok, d] from the accumulated partials and the entries' rows.
+ * A pass goes over the vocabulary in chunks of `chunk` rows (a multiple of 256, or all of it), in order:
+ * rus_lmhead_distill_chunk for the rows [vocab_start, + n_rows) with their transpose weight_t [d, >= round_up(n_rows,
+ * 64)] (read where n_split > 0; zeros past n_rows), then rus_lmhead_distill_finish once. weight: all rows of W, in device
+ * memory or page-locked, device-mapped host memory (the first chunk and the end read the entries' rows). n_split: partial sums of the hidden gradient, as
+ * rus_lmhead_ce_grad_hidden's (0: no gradient, dh and weight_t are not touched). workspace: the floats that
+ * rus_lmhead_distill_workspace names, the same ones through a pass, not shared by passes that overlap. d a multiple of
+ * 64; hidden, weight and weight_t fp16. kl [n_tok], loss and denom one each, dh [n_tok, d], all fp32; logits are fp32.
  * Beside: the chunked cross-entropy (solution/ops.py:174-349).
  */
-int rus_lmhead_distill_fwd(const void* hidden, const void* weight, int64_t n_tok, int64_t d, int64_t ld_h,
-                           int64_t ld_w, int64_t n_vocab, float temperature, float* part_m, float* part_s,
-                           int64_t part_base, int64_t part_stride, void* probs, int64_t ld_p, const float* ref,
-                           float* half_ref, uint32_t* chunk_max, void* stream);
-int rus_lmhead_distill_blank(void* probs, int64_t ld_p, int64_t n_tok, int64_t n_rows, int64_t vocab_start,
-                             const void* ids, int32_t ids32, const void* logits, int32_t logits_dtype,
-                             int32_t n_entries, int64_t n_vocab, float temperature, void* stream);
-int rus_lmhead_distill_entries(const void* hidden, int64_t ld_h, const void* weight, int64_t ld_w, int64_t n_vocab,
-                               int64_t n_tok, int64_t d, const void* ids, int32_t ids32, const void* logits,
-                               int32_t logits_dtype, int32_t n_entries, float temperature, const float* part_m,
-                               const float* part_s, int64_t n_parts, int64_t part_stride, const float* num_items,
-                               float* kl, float* lse, float* taught, float* coef, float* loss, float* denom,
-                               void* stream);
-int rus_lmhead_distill_finish(const float* parts, int32_t n_parts, int64_t n_tok, int64_t d, const float* m_run,
-                              const float* lse, const float* taught, const float* coef, const void* ids,
-                              int32_t ids32, int32_t n_entries, const void* weight, int64_t ld_w, int64_t n_vocab,
-                              const float* denom, float temperature, float* out, void* stream);
+int rus_lmhead_distill_workspace(int64_t n_tok, int64_t d, int64_t n_vocab, int64_t chunk, int32_t n_entries,
+                                 int32_t n_split, int64_t* floats);
+int rus_lmhead_distill_chunk(const void* hidden, int64_t ld_h, const void* weight_rows, int64_t ld_w,
+                             const void* weight_t, int64_t ld_wt, const void* weight, int64_t ld_all,
+                             int64_t n_tok, int64_t d, int64_t n_rows, int64_t vocab_start, int64_t n_vocab,
+                             int64_t chunk, const void* ids, int32_t ids32, const void* logits,
+                             int32_t logits_dtype, int32_t n_entries, float temperature, int32_t n_split,
+                             float* workspace, int64_t n_workspace, void* stream);
+int rus_lmhead_distill_finish(const void* weight, int64_t ld_w, int64_t n_tok, int64_t d,
+                              int64_t n_vocab, int64_t chunk, const void* ids, int32_t ids32,
+                              const void* logits, int32_t logits_dtype, int32_t n_entries, float temperature,
+                              int32_t n_split, const float* num_items, float* kl, float* loss, float* denom,
+                              float* dh, float* workspace, int64_t n_workspace, void* stream);
 
 #ifdef __cplusplus
 }

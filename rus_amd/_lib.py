@@ -179,13 +179,11 @@ SIGNATURES: dict[str, list] = {
     "rus_attn_masked_bwd": [_vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _vp, _vp, _vp,
                             _i32, _i64, _i64, _i32, _i32, _i32, _i32, _i32, _f32, _i32, _vp, _f32, _vp, _i32, _vp,
                             _vp, _vp, _vp, _i64, _vp],
-    "rus_lmhead_distill_fwd": [_vp, _vp, _i64, _i64, _i64, _i64, _i64, _f32, _vp, _vp, _i64, _i64, _vp, _i64, _vp,
-                               _vp, _vp, _vp],
-    "rus_lmhead_distill_blank": [_vp, _i64, _i64, _i64, _i64, _vp, _i32, _vp, _i32, _i32, _i64, _f32, _vp],
-    "rus_lmhead_distill_entries": [_vp, _i64, _vp, _i64, _i64, _i64, _i64, _vp, _i32, _vp, _i32, _i32, _f32, _vp,
-                                   _vp, _i64, _i64, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp],
-    "rus_lmhead_distill_finish": [_vp, _i32, _i64, _i64, _vp, _vp, _vp, _vp, _vp, _i32, _i32, _vp, _i64, _i64, _vp,
-                                  _f32, _vp, _vp],
+    "rus_lmhead_distill_workspace": [_i64, _i64, _i64, _i64, _i32, _i32, ctypes.POINTER(_i64)],
+    "rus_lmhead_distill_chunk": [_vp, _i64, _vp, _i64, _vp, _i64, _vp, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _vp, _i32, _vp,
+                                 _i32, _i32, _f32, _i32, _vp, _i64, _vp],
+    "rus_lmhead_distill_finish": [_vp, _i64, _i64, _i64, _i64, _i64, _vp, _i32, _vp, _i32, _i32, _f32,
+                                  _i32, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _vp],
 }
 
 _lock = threading.Lock()

@@ -3000,80 +3000,71 @@ def _teacher(fn: str, ids: torch.Tensor, logits: torch.Tensor, n_tok: int):
     return ids.reshape(n_tok, k).contiguous(), logits.detach().reshape(n_tok, k).contiguous()
 
 
-class LMHeadDistill:
-    """One pass of the distillation loss over vocabulary chunks (in order), as ``LMHeadPass``: per chunk the
-    statistics GEMM with P, the rescaling of half tiles, the teacher's entries taken out of P, and the split-K
-    product into fp32 partials; ``finish`` forms the loss and, with the entries back in fp32, the hidden gradient."""
+@functools.lru_cache(maxsize=1024)
+def _distill_splits(n_tok: int, d: int, cols: int, n_cu: int) -> int:
+    """Partial sums of the hidden gradient: at most one round of the CUs, as ``LMHeadPass`` has them."""
+    tiles = -(-n_tok // 256) * -(-d // 256)
+    return lm_head_split_count(n_tok, d, cols, n_cu, max_split=max(1, n_cu // tiles))
 
-    def __init__(self, n_tok: int, d: int, n_vocab: int, chunk: int, ids: torch.Tensor, logits: torch.Tensor,
+
+@functools.lru_cache(maxsize=1024)
+def _distill_chunk(n_tok: int, n_vocab: int, n_cu: int) -> int:
+    return lm_head_chunk_cols(n_tok, n_vocab, n_cu, at_least_two=True)
+
+
+@functools.lru_cache(maxsize=1024)
+def _distill_workspace(n_tok: int, d: int, n_vocab: int, chunk: int, entries: int, n_split: int) -> int:
+    got = ctypes.c_int64()
+    _lib.call("rus_lmhead_distill_workspace", n_tok, d, n_vocab, chunk, entries, n_split, ctypes.byref(got))
+    return got.value
+
+
+class LMHeadDistill:
+    """One pass of the distillation loss over vocabulary chunks (in order), as ``LMHeadPass``, with ``weight`` all
+    rows of W on the device or pinned on the host: the logits of the teacher's entries first, per chunk the
+    statistics GEMM with P, half tiles brought to one reference and the teacher's entries taken out of P, and the
+    split-K product into fp32 partials; ``finish`` forms the loss and, with the entries back in fp32, the hidden
+    gradient."""
+
+    def __init__(self, n_tok: int, weight: torch.Tensor, chunk: int, ids: torch.Tensor, logits: torch.Tensor,
                  temperature: float, need_grad: bool):
-        device = ids.device
-        self.n_tok, self.d, self.n_vocab, self.chunk = n_tok, d, n_vocab, int(chunk)
-        self.ids, self.logits, self.t, self.need_grad = ids, logits, float(temperature), need_grad
-        self.entries = (ids.data_ptr(), 1 if ids.dtype == torch.int32 else 0)
-        self.teacher = (*self.entries, logits.data_ptr(), _WIDE_DTYPES[logits.dtype], ids.shape[1])
-        self.parts = torch.empty((2, lm_head_num_parts(n_vocab), n_tok), dtype=torch.float32, device=device)
-        self.done = 0
-        if need_grad:
-            cols = min(self.chunk, n_vocab)
-            self.chunk_max = torch.zeros((-(-n_vocab // self.chunk), n_tok), dtype=torch.float32, device=device)
-            self.p = torch.empty((n_tok, _round_up(cols, LM_K)), dtype=torch.float16, device=device)
-            self.half_ref = torch.empty((2 * lm_head_num_parts(cols), n_tok), dtype=torch.float32, device=device)
-            rows = torch.empty((6, n_tok), dtype=torch.float32, device=device).unbind(0)
-            self.state, self.m_run, self.alpha = (rows[0:2], rows[2:4]), rows[4], rows[5]
-            n_cu = cu_count(device)
-            tiles = -(-n_tok // 256) * -(-d // 256)
-            splits = lm_head_split_count(n_tok, d, cols, n_cu, max_split=max(1, n_cu // tiles))
-            self.dparts = torch.empty((splits, n_tok, d), dtype=torch.float32, device=device)
+        n_vocab, d = weight.shape
+        self.n_tok, self.d, self.n_vocab, self.chunk, self.weight = n_tok, d, n_vocab, int(chunk), weight
+        self.ids, self.logits, self.need_grad = ids, logits, need_grad
+        entries = ids.shape[1]
+        self.n_split = _distill_splits(n_tok, d, min(self.chunk, n_vocab), cu_count(ids.device)) if need_grad else 0
+        floats = _distill_workspace(n_tok, d, n_vocab, self.chunk, entries, self.n_split)
+        self.ws = torch.empty(floats, dtype=torch.float32, device=ids.device)
+        self.teacher = (ids.data_ptr(), ids.dtype is torch.int32, logits.data_ptr(), _WIDE_DTYPES[logits.dtype],
+                        entries, float(temperature), self.n_split)
+        self.tail = self.ws.data_ptr(), floats
 
     def add_chunk(self, hidden: torch.Tensor, w_rows: torch.Tensor, w_t: torch.Tensor | None, start: int) -> None:
         """Vocabulary rows [start, start + len(w_rows)) with their transpose ``w_t`` [d, >= rows] (needed with
         the gradient only)."""
-        n, c, tok = w_rows.shape[0], self.done, self.n_tok
-        m, s = self.parts.unbind(0)
-        before = self.state[(c + 1) % 2] if self.need_grad and c else (None, None)
-        probs = (None, 0, None, None, None)
+        n, tok, d = w_rows.shape[0], self.n_tok, self.d
+        nbytes = 2 * (tok + n) * d
         if self.need_grad:
-            probs = (self.p.data_ptr(), self.p.stride(0), _ptr(before[0]), self.half_ref.data_ptr(),
-                     self.chunk_max[c].data_ptr())
-        _launch("lmhead_distill_fwd", 2 * ((tok + n) * self.d + (tok * n if self.need_grad else 0)),
-                2.0 * tok * n * self.d, "rus_lmhead_distill_fwd", hidden.data_ptr(), w_rows.data_ptr(), tok, self.d,
-                hidden.stride(0), w_rows.stride(0), n, self.t, m.data_ptr(), s.data_ptr(), start // LM_TILE, tok,
-                *probs, _stream(hidden))
-        if self.need_grad:
-            after = self.state[c % 2]
-            _launch("lmhead_ce_probs_rescale", 20 * tok, 0, "rus_lmhead_ce_probs_rescale", self.p.data_ptr(),
-                    self.p.stride(0), tok, n, self.half_ref.data_ptr(), tok, self.chunk_max[c].data_ptr(),
-                    _ptr(before[0]), _ptr(before[1]), after[0].data_ptr(), after[1].data_ptr(),
-                    self.alpha.data_ptr(), self.m_run.data_ptr(), _stream(hidden))
-            _launch("lmhead_distill_blank", 14 * self.ids.numel(), 0, "rus_lmhead_distill_blank", self.p.data_ptr(),
-                    self.p.stride(0), tok, n, start, *self.teacher, self.n_vocab, self.t, _stream(hidden))
-            lm_head_ce_grad_hidden_scaled(self.p, w_t, n, self.dparts, c > 0, self.alpha)
-        self.done = c + 1
+            nbytes += 2 * (2 * tok * n + n * d) + 4 * self.n_split * tok * d * (2 if start else 1)
+        _launch("lmhead_distill_chunk", nbytes, (4.0 if self.need_grad else 2.0) * tok * n * d,
+                "rus_lmhead_distill_chunk", hidden.data_ptr(), hidden.stride(0), w_rows.data_ptr(), w_rows.stride(0),
+                _ptr(w_t), 0 if w_t is None else w_t.stride(0), self.weight.data_ptr(), self.weight.stride(0),
+                tok, d, n, start, self.n_vocab, self.chunk,
+                *self.teacher, *self.tail, _stream(hidden))
 
-    def finish(self, hidden: torch.Tensor, w_rows: torch.Tensor, num_items_in_batch=None):
+    def finish(self, num_items_in_batch=None):
         """(loss, kl, denom, dh): loss and denom one element each, kl [n_tok], dh fp32 [n_tok, d] times 2^16
-        (None without the gradient). ``w_rows``: the whole weight, on the device or pinned on the host."""
-        tok, k, dev = self.n_tok, self.ids.shape[1], hidden.device
-        rows = torch.empty((3, tok), dtype=torch.float32, device=dev)
-        kl, lse, taught = rows.unbind(0)
+        (None without the gradient)."""
+        tok, d, dev = self.n_tok, self.d, self.ids.device
+        kl = torch.empty(tok, dtype=torch.float32, device=dev)
         out = torch.empty(2, dtype=torch.float32, device=dev)
-        coef = torch.empty((tok, k), dtype=torch.float32, device=dev) if self.need_grad else None
-        m, s = self.parts.unbind(0)
+        dh = torch.empty((tok, d), dtype=torch.float32, device=dev) if self.need_grad else None
         items = _num_items(num_items_in_batch, dev)
-        _launch("lmhead_distill_entries", 2 * tok * k * self.d + 8 * m.numel(), 2.0 * tok * k * self.d,
-                "rus_lmhead_distill_entries", hidden.data_ptr(), hidden.stride(0), w_rows.data_ptr(),
-                w_rows.stride(0), self.n_vocab, tok, self.d, *self.teacher, self.t, m.data_ptr(), s.data_ptr(),
-                m.shape[0], tok, _ptr(items), kl.data_ptr(), lse.data_ptr(), taught.data_ptr(), _ptr(coef),
-                out.data_ptr(), out.data_ptr() + 4, _stream(hidden))
-        dh = None
-        if self.need_grad:
-            dh = torch.empty((tok, self.d), dtype=torch.float32, device=dev)
-            _launch("lmhead_distill_finish", 4 * self.dparts.numel() + 2 * tok * k * self.d + 4 * dh.numel(),
-                    2.0 * tok * k * self.d, "rus_lmhead_distill_finish", self.dparts.data_ptr(),
-                    self.dparts.shape[0], tok, self.d, self.m_run.data_ptr(), lse.data_ptr(), taught.data_ptr(),
-                    coef.data_ptr(), *self.entries, k, w_rows.data_ptr(), w_rows.stride(0), self.n_vocab,
-                    out.data_ptr() + 4, self.t, dh.data_ptr(), _stream(hidden))
+        rows = 2 * self.ids.numel() * d
+        _launch("lmhead_distill_finish", (2 * rows + 4 * tok * d * (self.n_split + 1)) if self.need_grad else rows,
+                2.0 * rows, "rus_lmhead_distill_finish", self.weight.data_ptr(), self.weight.stride(0), tok, d,
+                self.n_vocab, self.chunk, *self.teacher, _ptr(items), kl.data_ptr(), out.data_ptr(),
+                out.data_ptr() + 4, _ptr(dh), *self.tail, _stream(kl))
         return out[0:1], kl, out[1:2], dh
 
 
@@ -3118,8 +3109,7 @@ def lm_head_distill(hidden: torch.Tensor, weight: torch.Tensor, teacher_ids: tor
                 if num_items_in_batch is not None else torch.ones_like(out)
             return out, torch.empty(0, dtype=torch.float32, device=h.device), denom, \
                 torch.empty((0, d), dtype=torch.float32, device=h.device) if need_grad else None
-        chunk = lm_head_chunk_cols(n_tok, n_vocab, cu_count(h.device), at_least_two=True) if v_chunk is None \
-            else int(v_chunk)
+        chunk = _distill_chunk(n_tok, n_vocab, cu_count(h.device)) if v_chunk is None else int(v_chunk)
         if chunk <= 0 or (chunk < n_vocab and chunk % LM_TILE):
             raise ValueError(f"{fn}: v_chunk must be a positive multiple of {LM_TILE}")
         wt = None
@@ -3131,8 +3121,8 @@ def lm_head_distill(hidden: torch.Tensor, weight: torch.Tensor, teacher_ids: tor
                                  "contiguous rows")
         else:
             chunk = n_vocab  # no P is kept: one launch over the whole vocabulary
-        hp = LMHeadDistill(n_tok, d, n_vocab, chunk, ids, logits, t, need_grad)
+        hp = LMHeadDistill(n_tok, w, chunk, ids, logits, t, need_grad)
         for start in range(0, n_vocab, chunk):
             end = min(start + chunk, n_vocab)
             hp.add_chunk(h, w[start:end], None if wt is None else wt[:, start:], start)
-        return hp.finish(h, w, num_items_in_batch)
+        return hp.finish(num_items_in_batch)

@@ -424,7 +424,7 @@ def _distill_streamed(h_2d, ids, logits, head: HostHead, temperature, num_items_
     if n_tok == 0:
         raise ValueError(f"{fn}: no tokens")
     starts = list(range(0, V, vc))
-    hp = K.LMHeadDistill(n_tok, d, V, vc, ids, logits, t, need_grad)
+    hp = K.LMHeadDistill(n_tok, head.cpu_weight, vc, ids, logits, t, need_grad)
     head.prefetch_chunk(0, 0, min(vc, V))
     for c, s in enumerate(starts):
         e = min(s + vc, V)
@@ -434,7 +434,7 @@ def _distill_streamed(h_2d, ids, logits, head: HostHead, temperature, num_items_
         rows_t = head.get_chunk_t(c, s, e) if need_grad else None
         hp.add_chunk(h, rows, rows_t, s)
         head.release_chunk(c)
-    return hp.finish(h, head.cpu_weight, num_items_in_batch)
+    return hp.finish(num_items_in_batch)
 
 
 class FusedDistillHeadFn(torch.autograd.Function):
