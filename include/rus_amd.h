@@ -959,8 +959,8 @@ int rus_rope_axes(const void* q, int64_t q_stride_t, int64_t q_stride_h, int32_t
  * A query that sees no key, and one outside every row, gets out = 0 and lse = -inf. Hidden keys take no part whatever
  * they hold. T = fp16 or bf16, head_dim 64 or 128; q, k, v 16-byte aligned with strides that are multiples of 8
  * elements (unit stride within a head); out contiguous. cu_q, cu_k, prefix int32 and slopes [h_q] fp32 on the device;
- * entries out of order or range are clamped into the arrays. max_q, max_k: at least the longest row's queries and
- * keys (they choose the kernel; rows longer than max_q are not finished). workspace: the fp32 elements that
+ * entries out of order or range are clamped into the arrays. max_q, max_k: the longest row's queries and keys, by which
+ * the work is laid out (other values cost time only). workspace: the fp32 elements that
  * rus_attn_masked_workspace names for the same sizes (0: none; 16-byte aligned), not shared by calls that overlap.
  * P is rounded to T for its product with v, sums are fp32.
  * Beside: rus_attn_varlen_fwd (solution/ops.py:669-696).
@@ -975,7 +975,14 @@ int rus_attn_masked_fwd(const void* q, int64_t q_stride_t, int64_t q_stride_h, c
                         void* out, float* lse, float* workspace, int64_t n_workspace, void* stream);
 
 /*
- * Its backward, given out and lse: with t = tanh(z / softcap) (1 - t^2 = 1 without a cap), D = dout.out,
+ * Diagnostic: how the two would run. plan[0]: parts that the keys of a block of few queries are split into (0: blocks of
+ * 128 queries, all keys), plan[1]: tiles of 32 keys in a part, plan[2]: tokens of a block of the backward (32 or 128).
+ */
+int rus_attn_masked_plan(int32_t n_seq, int64_t n_q, int64_t n_k, int32_t max_q, int32_t max_k, int32_t h_q,
+                         int32_t h_kv, int32_t head_dim, int32_t* plan);
+
+/*
+ * The backward of rus_attn_masked_fwd, given out and lse: with t = tanh(z / softcap) (1 - t^2 = 1 without a cap), D = dout.out,
  *   dS = P (dout v^T - D) (1 - t^2),  dq = scale dS k,  dk = scale dS^T q,  dv = P^T dout,
  * dk and dv summed over the query heads of each KV head in a fixed order in fp32 and rounded once. dout by strides as
  * q; dq, dk, dv contiguous, zero at tokens that no row or no pair covers. P and dS are rounded to T.

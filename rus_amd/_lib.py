@@ -174,6 +174,7 @@ SIGNATURES: dict[str, list] = {
     "rus_rope_axes": [_vp, _i64, _i64, _i32, _vp, _vp, _i64, _i64, _i32, _vp, _i64, _i32, _i32, _i32, _vp,
                       _i32, _i64, _i32, _vp, _vp, _i32, _i32, _vp],
     "rus_attn_masked_workspace": [_i32, _i64, _i64, _i32, _i32, _i32, _i32, _i32, _i32, ctypes.POINTER(_i64)],
+    "rus_attn_masked_plan": [_i32, _i64, _i64, _i32, _i32, _i32, _i32, _i32, ctypes.POINTER(_i32)],
     "rus_attn_masked_fwd": [_vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _vp, _i32, _i64, _i64, _i32,
                             _i32, _i32, _i32, _i32, _f32, _i32, _vp, _f32, _vp, _i32, _vp, _vp, _vp, _i64, _vp],
     "rus_attn_masked_bwd": [_vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _vp, _vp, _vp,

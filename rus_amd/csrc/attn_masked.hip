@@ -1115,7 +1115,7 @@ struct SplitPlan {
   int64_t items;  // blocks of few queries, bound over all rows
 };
 
-SplitPlan split_plan(int32_t n_seq, int64_t n_q, int64_t n_k, int32_t max_k, int32_t h_q, int32_t h_kv,
+SplitPlan split_plan(int32_t n_seq, int64_t n_q, int64_t n_k, int32_t max_q, int32_t max_k, int32_t h_q, int32_t h_kv,
                      int32_t head_dim) {
   SplitPlan p{0, 0, 0};
   const int grp = h_q / h_kv;
@@ -1123,12 +1123,14 @@ SplitPlan split_plan(int32_t n_seq, int64_t n_q, int64_t n_k, int32_t max_k, int
   const int tpb = split_tokens(grp);
   const int64_t base = std::max<int64_t>((n_q + tpb - 1) / tpb, n_seq) * h_kv;
   const int64_t tiles = std::max<int64_t>((static_cast<int64_t>(max_k) + 31) / 32, 1);
-  const int64_t splits = std::max<int64_t>(std::min<int64_t>(512 / base, (tiles + 7) / 8), 1);
+  // (a part is worth its share of the join from two tiles a wave on, parts at all from some 1,000 keys)
+  const int64_t splits = tiles < 32 ? 1 : std::max<int64_t>(std::min<int64_t>(512 / base, (tiles + 7) / 8), 1);
   const int64_t part = (tiles + splits - 1) / splits;
   const double wide_load = std::max(1.0, std::max<int64_t>((n_q + kRows - 1) / kRows, n_seq) * h_q / 512.0);
   const double wide_us = 7.0 + 0.8 * tiles * wide_load;
   const double row = std::min<double>(static_cast<double>(max_k), static_cast<double>(n_k) / n_seq);
-  const double step_us = head_dim == 64 ? 1.1 : 2.2, steps = n_q < n_k ? row / 128 : row / 256;
+  // (queries of a causal row see half of it on average, a few at the end of a cache nearly all)
+  const double step_us = head_dim == 64 ? 1.1 : 2.2, steps = max_q < max_k ? row / 128 : row / 256;
   const double few_us =
       4.0 + std::max(0.4 * part, std::max(1.0, base * splits / 512.0) * (4.0 + step_us * steps / splits)) +
       (splits > 1 ? 4.0 : 0.0);
@@ -1216,8 +1218,21 @@ extern "C" int rus_attn_masked_workspace(int32_t n_seq, int64_t n_q, int64_t n_k
     *floats = h_q > h_kv ? 2 * static_cast<int64_t>(h_q) * n_k * head_dim : 0;
     return RUS_OK;
   }
-  const SplitPlan p = split_plan(n_seq, n_q, n_k, max_k, h_q, h_kv, head_dim);
+  const SplitPlan p = split_plan(n_seq, n_q, n_k, max_q, max_k, h_q, h_kv, head_dim);
   *floats = p.splits > 1 ? p.splits * n_q * h_q * (head_dim + 4) : 0;
+  return RUS_OK;
+}
+
+extern "C" int rus_attn_masked_plan(int32_t n_seq, int64_t n_q, int64_t n_k, int32_t max_q, int32_t max_k, int32_t h_q,
+                                    int32_t h_kv, int32_t head_dim, int32_t* plan) {
+  using namespace rus;
+  const char* fn = "rus_attn_masked_plan";
+  if (!plan) return fail(RUS_ERR_INVALID, "%s: null result", fn);
+  if (int e = check_sizes(fn, n_seq, n_q, n_k, max_q, max_k, h_q, h_kv, head_dim)) return e;
+  const SplitPlan p = split_plan(n_seq, n_q, n_k, max_q, max_k, h_q, h_kv, head_dim);
+  plan[0] = p.splits;
+  plan[1] = p.tiles;
+  plan[2] = narrow_bwd(n_seq, n_q, n_k, h_q) ? 32 : kRows;
   return RUS_OK;
 }
 
@@ -1245,7 +1260,7 @@ extern "C" int rus_attn_masked_fwd(const void* q, int64_t q_stride_t, int64_t q_
   a.out = out, a.lse = lse;
   a.cu_q = cu_q, a.cu_k = cu_k, a.n_seq = n_seq, a.n_q = n_q, a.n_k = n_k, a.h_q = h_q, a.h_kv = h_kv;
   set_scores(a, scale, softcap, slopes, prefix, causal);
-  const SplitPlan p = split_plan(n_seq, n_q, n_k, max_k, h_q, h_kv, head_dim);
+  const SplitPlan p = split_plan(n_seq, n_q, n_k, max_q, max_k, h_q, h_kv, head_dim);
   if (p.splits) {
     a.splits = p.splits;
     a.split_tiles = p.tiles;

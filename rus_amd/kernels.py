@@ -2933,8 +2933,8 @@ def attn_masked_fwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: tor
     scale q.k (default d^-1/2), with ``softcap`` c > 0 capped to c tanh(. / c), with ``slopes`` (fp32 [h_q]) less
     slopes[h] |p - j|. A query that sees nothing, or belongs to no row, gets zeros and lse -inf; what hidden keys
     hold does not matter. q, k, v fp16 or bf16, d 64 or 128, h_q a multiple of h_kv, strided as a fused projection
-    leaves them. ``max_q`` and ``max_k``: the longest row's queries and keys (default: all tokens); they choose
-    how the work is split, and a row may not have more queries than max_q."""
+    leaves them. ``max_q`` and ``max_k``: the longest row's queries and keys (default: all tokens), by which the
+    work is laid out."""
     fn = "attn_masked_fwd"
     rows, at, cu, sizes, scores = _masked_call(fn, q, k, v, cu_q, cu_k, causal, prefix, softcap, slopes, scale,
                                                max_q, max_k)

@@ -10,12 +10,14 @@ absolute step of 2^-24.
 
 from __future__ import annotations
 
+import ctypes
 import math
 
 import pytest
 import torch
 
 from oracle import ops as ref
+from rus_amd import _lib
 from rus_amd import kernels as K
 from rus_amd import ops
 
@@ -317,3 +319,152 @@ def test_long_cache_offsets_past_32_bits():
     torch.cuda.synchronize()
     want = _definition(q.cpu(), k[n - lk:].cpu(), v[n - lk:].cpu(), dout.cpu(), [4], [lk])
     _check({"out": out, "lse": lse}, want, torch.float16)
+
+
+def _plan(ql, kl, hq, hkv, d):
+    got = (ctypes.c_int32 * 3)()
+    _lib.call("rus_attn_masked_plan", len(ql), sum(ql), sum(kl), max(ql), max(kl), hq, hkv, d, got)
+    return tuple(got)
+
+
+_LONG = [33, 255, 64, 200, 190, 129, 256, 90, 255, 161, 128, 97, 200]
+_ODD = [161] * 3 + [255, 97, 3, 128, 127, 200, 90, 1]
+# (rows of queries, of keys, heads, plan: parts (0: blocks of 128 queries), backward block)
+LAYOUTS = {
+    "blocks_of_128": (_LONG, _LONG, 24, 4, 0, 128),
+    "blocks_of_128_few_queries": ([20, 1, 64, 131, 7, 129, 100, 90, 255, 161, 128, 97, 200], _LONG, 24, 4, 0, 128),
+    "blocks_of_128_odd_ends": (_ODD, _ODD, 28, 2, 0, 128),
+    "few_queries_one_part": ([300, 150], [300, 150], 6, 2, 1, 32),
+    "few_queries_many_parts": ([1, 2, 3], [900, 1500, 64], 6, 2, None, 32),
+    "one_head_per_kv": ([257, 64, 130], [257, 64, 130], 8, 8, 1, 32),
+    "many_rows": ([3] * 90 + [40], [3] * 45 + [70] * 45 + [40], 4, 2, None, 128),  # more rows than a wave has lanes
+}
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16], ids=["fp16", "bf16"])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("layout", list(LAYOUTS))
+@pytest.mark.parametrize("form", ["causal", "prefix_cap", "prefix_bias", "full_cap_bias"])
+def test_layouts_against_float64(dtype, d, layout, form):
+    ql, kl, hq, hkv, parts, block = LAYOUTS[layout]
+    got_plan = _plan(ql, kl, hq, hkv, d)
+    assert (got_plan[0] > 1 if layout == "few_queries_many_parts" else parts is None or got_plan[0] == parts), got_plan
+    assert got_plan[2] == block, got_plan
+    q, k, v, dout = _inputs(ql, kl, hq, hkv, d, dtype, seed=d + len(layout))
+    prefix = [(50 * s + 3) % 150 for s in range(len(ql))]
+    kw = {"causal": {}, "prefix_cap": dict(softcap=5.0, prefix=prefix), "prefix_bias": dict(slopes=_slopes(hq), prefix=prefix),
+          "full_cap_bias": dict(causal=False, softcap=30.0, slopes=-0.01 * _slopes(hq))}[form]
+    _check(_run(q, k, v, dout, ql, kl, **kw), _definition(q, k, v, dout, ql, kl, **kw), dtype)
+
+
+@pytest.mark.parametrize("where", ["q", "k", "v", "dout"])
+@pytest.mark.parametrize("layout", ["blocks_of_128", "few_queries_many_parts", "one_head_per_kv"])
+def test_hidden_elements_in_every_layout(where, layout):
+    """The last token of each row is not finite: of it, every other query (and what only those see) knows nothing."""
+    ql, kl, hq, hkv, *_ = LAYOUTS[layout]
+    t = dict(zip(("q", "k", "v", "dout"), _inputs(ql, kl, hq, hkv, 128, torch.float16, seed=21)))
+    kw = dict(slopes=_slopes(hq))
+    clean = _run(*t.values(), ql, kl, **kw)
+    cq, ck = _cu(ql), _cu(kl)
+    x = t[where].clone()
+    for e in (cq if where in ("q", "dout") else ck)[1:]:
+        x[e - 1, :, 7] = math.nan
+    t[where] = x
+    got = _run(*t.values(), ql, kl, **kw)
+    last_q = torch.tensor([e - 1 for e in cq[1:]])
+    keep = torch.ones(cq[-1], dtype=torch.bool)
+    keep[last_q] = False
+    for name in ("out", "dq"):
+        a, b = got[name].cpu()[keep], clean[name].cpu()[keep]
+        assert torch.isfinite(a).all() and torch.allclose(a.float(), b.float(), rtol=4e-3, atol=4e-3), name
+        if name == "dq" or where != "dout":
+            assert torch.isnan(got[name].cpu()[last_q]).flatten(1).any(1).all(), name
+    if where != "dout":  # every key of a row is seen by its last query, whose P is no number (v: dS is not, P is)
+        assert torch.isnan(got["dk"].cpu()).any()
+    else:
+        seen = got["dv"].cpu()[..., 7]
+        assert torch.isnan(seen).all() and torch.isfinite(got["dv"].cpu()[..., :7]).all()
+
+
+def test_a_captured_step_beside_eager_work():
+    """Forward and backward in one graph, replayed with other inputs, eager calls and another stream's between: every
+    replay has the eager call's bits."""
+    ql, kl = [70, 33], [90, 33]
+    cu_q, cu_k = _ints(_cu(ql)), _ints(_cu(kl))
+    args = dict(cu_k=cu_k, max_q=70, max_k=90, softcap=9.0)
+    sets = [[t.to(DEV) for t in _inputs(ql, kl, 6, 2, 128, torch.float16, seed=s)] for s in range(4)]
+    static = [t.clone() for t in sets[0]]
+
+    def step(q, k, v, do):
+        out, lse = K.attn_masked_fwd(q, k, v, cu_q, **args)
+        return out, lse, *K.attn_masked_bwd(do, q, k, v, out, lse, cu_q, **args)
+
+    step(*static)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = step(*static)
+    other = torch.cuda.Stream()
+    for rep in range(6):
+        data = sets[rep % 4]
+        want = step(*data)
+        for s, t in zip(static, data):
+            s.copy_(t)
+        graph.replay()
+        other.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(other):
+            beside = step(*sets[(rep + 1) % 4])
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(captured, want)), rep
+        assert all(torch.equal(a, b) for a, b in zip(beside, step(*sets[(rep + 1) % 4]))), rep
+
+
+def test_parts_are_joined_alike_on_two_streams_at_once():
+    q, k, v, _ = (t.to(DEV) for t in _inputs([1] * 4, [5000, 70, 3000, 1], 12, 2, 128, torch.bfloat16, seed=30))
+    cu_q, cu_k = _ints(range(5)), _ints(_cu([5000, 70, 3000, 1]))
+    call = lambda: K.attn_masked_fwd(q, k, v, cu_q, cu_k, max_q=1, max_k=5000)
+    want = call()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    got = []
+    for _ in range(5):
+        for s in streams:
+            with torch.cuda.stream(s):
+                got.append(call())
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for g in got for a, b in zip(g, want))
+
+
+def test_malformed_rows_stay_inside_the_arrays():
+    """Starts out of order or range are clamped: nothing is read or written outside (results of such rows say nothing)."""
+    q, k, v, dout = (t.to(DEV) for t in _inputs([64], [64], 4, 2, 64, torch.float16, seed=31))
+    for cu in ([0, 100, 64], [-5, 30, 64], [60, 10, 64], [64, 64, 0], [2**31 - 1, -(2**31), 7]):
+        cu = _ints(cu)
+        out, lse = K.attn_masked_fwd(q, k, v, cu, softcap=3.0)
+        K.attn_masked_bwd(dout, q, k, v, out, lse, cu, softcap=3.0)
+        torch.cuda.synchronize()
+
+
+def test_other_longest_rows_cost_time_only():
+    ql, kl = [5, 40], [700, 40]
+    q, k, v, dout = _inputs(ql, kl, 4, 2, 64, torch.float16, seed=32)
+    want = _definition(q, k, v, dout, ql, kl)
+    d = [t.to(DEV) for t in (q, k, v)]
+    for max_q, max_k in ((0, 0), (1, 1), (45, 740), (10000, 1 << 30), (None, None)):
+        out, lse = K.attn_masked_fwd(*d, _ints(_cu(ql)), _ints(_cu(kl)), max_q=max_q, max_k=max_k)
+        _check({"out": out, "lse": lse}, want, torch.float16)
+
+
+def test_no_queries_or_no_keys():
+    z = lambda n, h: torch.zeros(n, h, 64, dtype=torch.float16, device=DEV)
+    cu0, cu4 = _ints([0, 0]), _ints([0, 4])
+    out, lse = K.attn_masked_fwd(z(0, 4), z(4, 2), z(4, 2), cu0, cu4)
+    assert out.shape == (0, 4, 64)
+    dq, dk, dv = K.attn_masked_bwd(out, z(0, 4), z(4, 2), z(4, 2), out, lse, cu0, cu4)
+    assert not bool(dk.any()) and not bool(dv.any())
+    q = z(4, 4) + 1
+    out, lse = K.attn_masked_fwd(q, z(0, 2), z(0, 2), cu4, cu0)
+    assert not bool(out.any()) and bool((lse == -math.inf).all())
+    dq, dk, dv = K.attn_masked_bwd(q, q, z(0, 2), z(0, 2), out, lse, cu4, cu0)
+    assert not bool(dq.any()) and dk.shape == (0, 2, 64)
