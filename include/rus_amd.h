@@ -982,7 +982,8 @@ int rus_attn_masked_plan(int32_t n_seq, int64_t n_q, int64_t n_k, int32_t max_q,
                          int32_t h_kv, int32_t head_dim, int32_t* plan);
 
 /*
- * The backward of rus_attn_masked_fwd, given out and lse: with t = tanh(z / softcap) (1 - t^2 = 1 without a cap), D = dout.out,
+ * The backward of rus_attn_masked_fwd, given out and lse: with t = tanh(z / softcap) (1 - t^2 = 1 without a cap),
+ * D = sum_j P_j (dout v^T)_j (not dout.out: out has been rounded),
  *   dS = P (dout v^T - D) (1 - t^2),  dq = scale dS k,  dk = scale dS^T q,  dv = P^T dout,
  * dk and dv summed over the query heads of each KV head in a fixed order in fp32 and rounded once. dout by strides as
  * q; dq, dk, dv contiguous, zero at tokens that no row or no pair covers. P and dS are rounded to T.

@@ -8,8 +8,11 @@
 // P = softmax z, O = P V, lse = ln sum e^z. No visible key: O = 0, lse = -inf, gradients 0. Hidden keys and the
 // queries that do not see a key take no part whatever they hold: neither an infinity nor a NaN of theirs gets through
 // (see nonfinite rows below).
-// Backward, with t = tanh(z / cap): D = dO.O, dS = P (dO V^T - D) (1 - t^2), dQ = scale dS K, dK = scale dS^T Q,
-// dV = P^T dO.
+// Backward, with t = tanh(z / cap): D = sum_j P_j (dO V^T)_j, dS = P (dO V^T - D) (1 - t^2), dQ = scale dS K, dK = scale
+// dS^T Q, dV = P^T dO. D is dO.O of the unrounded O; the O at hand is rounded, and the gradients of 16-bit rows would
+// carry half again the error that their own roundings give (bf16 0.34% against 0.24%). Since the P of a row sum to 1,
+// D' = dO.(rounded O) is off by exactly r = sum_j P_j (dP_j - D'): the dQ blocks sum r as they go, and leave D' + r for
+// the blocks of dK and dV and dQ = scale (sum dS' K - r sum P (1 - t^2) K), dS' with D'.
 #pragma once
 
 #include <math.h>
@@ -28,6 +31,7 @@ struct MaskedArgs {
   void *out, *dk, *dv;         // out: O, in the backward dQ (both [n_q, h_q, HD] contiguous); dk, dv contiguous
   float* lse;                  // [h_q, n_q] natural log
   float *dk_part, *dv_part;    // [h_q, n_k, HD] where query heads share keys
+  float* dsum;                 // [h_q, n_q] D
   float* part;                 // parts of a split over keys
   const int32_t *cu_q, *cu_k, *prefix;
   const float* slopes;
@@ -259,17 +263,22 @@ __device__ void plain_dq_row(const MaskedArgs& a, const MaskedRow& r, int i, int
   const T* q = token<T>(a.q, t, a.q_st, head, a.q_sh);
   const T* go = token<T>(a.dout, t, a.do_st, head, a.do_sh);
   const int vis = r.vis(i, a.causal), p0 = r.off() + i;
-  float dq[N] = {};
-  if (vis > 0) {
-    const float dsum = dot_rows<T, HD>(go, static_cast<const T*>(a.o) + (t * a.h_q + head) * HD);
-    const float lse2 = a.lse[head * a.n_q + t] * kLog2e;
+  float dq[N] = {}, dsum = 0.0f;
+  const float lse2 = a.lse[head * a.n_q + t] * kLog2e;
+  for (int pass = 0; pass < 2; ++pass) {  // D first
+    float sum = 0.0f;
     for (int jb = 0; jb < vis; jb += 64) {
       const int j = min(jb + lane, vis - 1), n = min(64, vis - jb);
       float f;
       const float y = sc.score(a, dot_rows<T, HD>(q, token<T>(a.k, r.ka + j, a.k_st, g, a.k_sh)),
                                static_cast<float>(p0 - j), f);
       const float dp = dot_rows<T, HD>(go, token<T>(a.v, r.ka + j, a.v_st, g, a.v_sh));
-      const float ds = exp2_raw(y - lse2) * (dp - dsum) * f;
+      const float p = exp2_raw(y - lse2);
+      if (pass == 0) {
+        sum += lane < n ? p * dp : 0.0f;
+        continue;
+      }
+      const float ds = p * (dp - dsum) * f;
       for (int jj = 0; jj < n; ++jj) {
         const float dj = lane_value(ds, jj);
         const T* k = token<T>(a.k, r.ka + jb + jj, a.k_st, g, a.k_sh) + lane * N;
@@ -277,7 +286,9 @@ __device__ void plain_dq_row(const MaskedArgs& a, const MaskedRow& r, int i, int
         for (int d = 0; d < N; ++d) dq[d] = __builtin_fmaf(dj, static_cast<float>(k[d]), dq[d]);
       }
     }
+    if (pass == 0) dsum = wave_sum(sum);
   }
+  if (lane == 0) a.dsum[head * a.n_q + t] = dsum;
 #pragma unroll
   for (int d = 0; d < N; ++d) dq[d] *= a.scale;
   store_from_f32<T, N>(static_cast<T*>(a.out) + (t * a.h_q + head) * HD + lane * N, dq);
@@ -303,7 +314,7 @@ __device__ void plain_dkv_row(const MaskedArgs& a, const MaskedRow& r, int j, in
       float f;
       const float y = sc.score(a, dot_rows<T, HD>(token<T>(a.q, tq, a.q_st, head, a.q_sh), k),
                                static_cast<float>(r.off() + i - j), f);
-      const float dsum = dot_rows<T, HD>(go, static_cast<const T*>(a.o) + (tq * a.h_q + head) * HD);
+      const float dsum = a.dsum[head * a.n_q + tq];
       const float p = exp2_raw(y - a.lse[head * a.n_q + tq] * kLog2e);
       const float ds = p * (dot_rows<T, HD>(go, v) - dsum) * f;
       for (int ii = 0; ii < n; ++ii) {

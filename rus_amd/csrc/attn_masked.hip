@@ -471,29 +471,43 @@ struct BwdLds {
   float* ld1;
 };
 
-// dS^T of a 32 x 32 tile in st, a lane owning a query: st holds the products, dp dP^T. left: keys of the lane's query from
-// the tile's first on that it sees, edge: whether any query of the wave misses one.
+// A 32 x 32 tile, a lane owning a query: st holds the products, dp dP^T; then st P (1 - t^2) and dp dS'^T, whose sum
+// before the factor joins r. left: keys of the lane's query from the tile's first on that it sees, edge: whether any query
+// of the wave misses one.
 template <typename T, bool CAP, bool BIAS>
-__device__ __forceinline__ void query_scores(const MaskedArgs& a, float slope2, f32x16 (&st)[1], f32x16 (&f)[1],
-                                             const f32x16& dp, float dsum, float lse2, float d0, bool edge, int left,
-                                             int h) {
+__device__ __forceinline__ void query_scores(const MaskedArgs& a, float slope2, f32x16 (&st)[1], f32x16& dp, float dsum,
+                                             float lse2, float d0, bool edge, int left, int h, float& r) {
+  f32x16 f[1];
   if constexpr (CAP) capped_scores<BIAS, 1, true>(a, slope2, st, f, d0, 1.0f);
 #pragma unroll
-  for (int e = 0; e < 16; ++e) {
-    const float p = exp2_raw(CAP ? st[0][e] - lse2 : __builtin_fmaf(st[0][e], a.sl2, -lse2));
-    st[0][e] = p * (dp[e] - dsum);
-    if constexpr (CAP) st[0][e] *= f[0][e];
-  }
+  for (int e = 0; e < 16; ++e)
+    st[0][e] = exp2_raw(CAP ? st[0][e] - lse2 : __builtin_fmaf(st[0][e], a.sl2, -lse2));
+#pragma unroll
+  for (int e = 0; e < 16; ++e) dp[e] = st[0][e] * (dp[e] - dsum);
   if (edge) {
     const int most = left - 4 * h;
 #pragma unroll
-    for (int e = 0; e < 16; ++e) st[0][e] = acc_row(e, 0) < most ? st[0][e] : 0.0f;
+    for (int e = 0; e < 16; ++e) {
+      const bool in = acc_row(e, 0) < most;
+      st[0][e] = in ? st[0][e] : 0.0f;
+      dp[e] = in ? dp[e] : 0.0f;
+      if constexpr (CAP) f[0][e] = in ? f[0][e] : 0.0f;
+    }
+  }
+#pragma unroll
+  for (int e = 0; e < 16; ++e) r += dp[e];
+  if constexpr (CAP) {
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      dp[e] *= f[0][e];
+      st[0][e] *= f[0][e];
+    }
   }
 }
 
 // P in st and dS in dp of a 32 x 32 tile, a lane owning a key; stats(q, lse, D): those of the queries 8 q + 4 h .. + 4
-// (lse in log2 units). edge: whether a
-// query of the tile (below `first`: those that miss the lane's key; from `rows` on: none) stays out.
+// (lse in log2 units). edge: whether a query of the tile (below `first`: those that miss the lane's key; from `rows` on:
+// none) stays out.
 template <typename T, bool CAP, bool BIAS, typename F>
 __device__ __forceinline__ void key_scores(const MaskedArgs& a, float slope2, f32x16 (&st)[1], f32x16 (&f)[1], f32x16& dp,
                                            F stats, float d0, bool edge, int first, int rows, int h) {
@@ -522,10 +536,10 @@ __device__ __forceinline__ void key_scores(const MaskedArgs& a, float slope2, f3
   }
 }
 
-// dQ of 128 queries: key tiles stream through LDS, each wave owns 32 queries (Q and dO fragments in registers; D from
-// the same fragments).
+// dQ and D of 128 queries: key tiles stream through LDS, each wave owns 32 queries (Q fragments in registers, its dO
+// tile in LDS: the two sums leave no registers for it).
 template <typename T, int HD, bool CAP, bool BIAS>
-__device__ __forceinline__ void bwd_dq(const MaskedArgs& a, int blk, int head, const BwdLds& lds) {
+__device__ __forceinline__ void bwd_dq(const MaskedArgs& a, int blk, int head, char* buf0, char* buf1, char* dot) {
   using L = Tiles<HD>;
   int s, b, nb;
   if (!find_span_block(a.cu_q, a.n_seq, static_cast<int>(a.n_q), blk, kRows, s, b, nb)) return;
@@ -551,14 +565,18 @@ __device__ __forceinline__ void bwd_dq(const MaskedArgs& a, int blk, int head, c
     tk.copy(dst, kh + 32 * j * a.k_st, rows);
     tv.copy(dst + L::kBytes, vh + 32 * j * a.v_st, rows);
   };
-  if (tiles) copy(lds.buf0, 0);
+  if (tiles) copy(buf0, 0);
   const int64_t t = r.qa + i;
-  Frag qf[L::kSteps], df[L::kSteps];
+  char* dt = dot + wave * L::kBytes;
+  if (iw < r.lq)
+    TileLane<HD, L::kCopies>(0, lane, a.do_st)
+        .copy(dt, token<T>(a.dout, static_cast<int64_t>(r.qa) + iw, a.do_st, head, a.do_sh), r.lq - iw);
+  Frag qf[L::kSteps];
   load_row_frags<T, HD>(qf, token<T>(a.q, t, a.q_st, head, a.q_sh), h);
-  load_row_frags<T, HD>(df, token<T>(a.dout, t, a.do_st, head, a.do_sh), h);
   float ds = 0.0f;
   {
-    Frag of[L::kSteps];
+    Frag df[L::kSteps], of[L::kSteps];
+    load_row_frags<T, HD>(df, token<T>(a.dout, t, a.do_st, head, a.do_sh), h);
     load_row_frags<T, HD>(of, static_cast<const T*>(a.o) + (t * a.h_q + head) * HD, h);
 #pragma unroll
     for (int k = 0; k < L::kSteps; ++k) ds = dot8<T>(of[k], df[k], ds);
@@ -566,43 +584,57 @@ __device__ __forceinline__ void bwd_dq(const MaskedArgs& a, int blk, int head, c
   const float2 dp2 = half_pair(ds);
   const float dsum = dp2.x + dp2.y;
   const float lse2 = a.lse[head * a.n_q + t] * kLog2e;
-  f32x16 dq[L::kDims];
+  f32x16 dq[L::kDims], pk[L::kDims];  // sum dS' K, sum P (1 - t^2) K
+  float rest = 0.0f;
 #pragma unroll
-  for (int d = 0; d < L::kDims; ++d) dq[d] = f32x16{};
+  for (int d = 0; d < L::kDims; ++d) {
+    dq[d] = f32x16{};
+    pk[d] = f32x16{};
+  }
   stage_barrier();
   auto stage = [&](const char* kt, char* next, int j) {
     if (j + 1 < tiles) copy(next, j + 1);
     const char* vt = kt + L::kBytes;
     const FragLane<HD> fl = fl0.fresh();
     if (j < mine) {
-      f32x16 st[1], dp = f32x16{}, f[1];
+      f32x16 st[1], dp = f32x16{};
       start_scores<CAP, BIAS, 1>(st, sc.slope, static_cast<float>(r.off() + i - 32 * j - 4 * h), 1.0f, 32 * j + 31 <= r.off() + iw);
 #pragma unroll
       for (int k = 0; k < L::kSteps; ++k) {
         st[0] = mfma<T>(fl.frag(kt, k), qf[k], st[0]);  // S^T = K Q^T
-        dp = mfma<T>(fl.frag(vt, k), df[k], dp);        // dP^T = V dO^T
+        dp = mfma<T>(fl.frag(vt, k), fl.frag(dt, k), dp);  // dP^T = V dO^T
       }
-      query_scores<T, CAP, BIAS>(a, sc.slope2, st, f, dp, dsum, lse2,
-                                 static_cast<float>(r.off() + i - 32 * j - 4 * h), 32 * j + 32 > vis_all,
-                                 vis - 32 * j, h);
-      const Frag s0 = frag_acc<T>(st[0], 0), s1 = frag_acc<T>(st[0], 1);
+      query_scores<T, CAP, BIAS>(a, sc.slope2, st, dp, dsum, lse2, static_cast<float>(r.off() + i - 32 * j - 4 * h),
+                                 32 * j + 32 > vis_all, vis - 32 * j, h, rest);
+      const Frag p0 = frag_acc<T>(st[0], 0), p1 = frag_acc<T>(st[0], 1);
+      const Frag s0 = frag_acc<T>(dp, 0), s1 = frag_acc<T>(dp, 1);
 #pragma unroll
       for (int d = 0; d < L::kDims; ++d) {
-        dq[d] = mfma<T>(fl.frag_t(kt, 0, d), s0, dq[d]);  // dQ^T += K^T dS^T
-        dq[d] = mfma<T>(fl.frag_t(kt, 1, d), s1, dq[d]);
+        const Frag k0 = fl.frag_t(kt, 0, d), k1 = fl.frag_t(kt, 1, d);
+        dq[d] = mfma<T>(k0, s0, dq[d]);  // dQ^T += K^T dS'^T
+        pk[d] = mfma<T>(k0, p0, pk[d]);
+        dq[d] = mfma<T>(k1, s1, dq[d]);
+        pk[d] = mfma<T>(k1, p1, pk[d]);
       }
     }
     stage_barrier();
   };
   for (int j = 0; j < tiles; j += 2) {
-    stage(lds.buf0, lds.buf1, j);
-    if (j + 1 < tiles) stage(lds.buf1, lds.buf0, j + 1);
+    stage(buf0, buf1, j);
+    if (j + 1 < tiles) stage(buf1, buf0, j + 1);
   }
   if (iw >= r.lq) return;
-  uint64_t again = __ballot(valid && !all_finite(dq, a.scale));
+  const float2 rp = half_pair(rest);
+  rest = rp.x + rp.y;
+#pragma unroll
+  for (int d = 0; d < L::kDims; ++d)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) dq[d][e] = __builtin_fmaf(-rest, pk[d][e], dq[d][e]);
+  const uint64_t again = __ballot(valid && !(all_finite(dq, a.scale) && fabsf(rest) <= 3.402823466e38f));
   uint32_t cols = static_cast<uint32_t>(again) | static_cast<uint32_t>(again >> 32);
-  store_row<T, L::kDims>(static_cast<T*>(a.out) + (t * a.h_q + head) * HD, dq, a.scale, h,
-                         valid && !((cols >> col) & 1));
+  const bool keep = valid && !((cols >> col) & 1);
+  store_row<T, L::kDims>(static_cast<T*>(a.out) + (t * a.h_q + head) * HD, dq, a.scale, h, keep);
+  if (h == 0 && keep) a.dsum[head * a.n_q + t] = vis > 0 ? dsum + rest : 0.0f;
   for (; cols; cols &= cols - 1) plain_dq_row<T, HD, CAP, BIAS>(a, r, iw + __builtin_ctz(cols), head);
 }
 
@@ -627,34 +659,21 @@ __device__ __forceinline__ void bwd_dkdv(const MaskedArgs& a, int blk, int head,
   const int q_all = r.first(min(kw + 31, r.lk - 1), a.causal);      // from here on every key of the wave is seen
   const T* qh = token<T>(a.q, r.qa, a.q_st, head, a.q_sh);
   const T* doh = token<T>(a.dout, r.qa, a.do_st, head, a.do_sh);
-  const int64_t o_st = static_cast<int64_t>(a.h_q) * HD;
-  const T* oh = static_cast<const T*>(a.o) + r.qa * o_st + head * HD;
   const float* lse = a.lse + head * a.n_q + r.qa;
+  const float* dsum = a.dsum + head * a.n_q + r.qa;
   constexpr int C = L::kCopies / kWaves;
-  const TileLane<HD, C> tq(C * wave, lane, a.q_st), td(C * wave, lane, a.do_st), to(C * wave, lane, o_st);
+  const TileLane<HD, C> tq(C * wave, lane, a.q_st), td(C * wave, lane, a.do_st);
   const FragLane<HD> fl0(lane);
   const Scorer<CAP, BIAS> sc(a, head);
-  Frag orow[C];  // the O chunks of the dO chunks this lane copies
-  float lr = 0.0f;
+  float stat = 0.0f;  // of threads 0 to 31 a query's lse (log2 units), of 32 to 63 its D
   auto copy = [&](char* dst, int j) {
     const int rows = r.lq - 32 * j;
     tq.copy(dst, qh + 32 * j * a.q_st, rows);
     td.copy(dst + L::kBytes, doh + 32 * j * a.do_st, rows);
-#pragma unroll
-    for (int i = 0; i < C; ++i)
-      orow[i] = *reinterpret_cast<const Frag*>(reinterpret_cast<const char*>(oh + 32 * j * o_st) + to.at(i, rows));
-    if (tid < 32) lr = lse[32 * j + min(tid, rows - 1)];
+    if (wave == 0) stat = h == 0 ? lse[32 * j + min(col, rows - 1)] * kLog2e : dsum[32 * j + min(col, rows - 1)];
   };
-  // D of the rows this wave copied (its copies have landed): each lane's 8 products, then the sum over a row's lanes.
-  auto finish = [&](const char* dst, float* ld) {
-    __builtin_amdgcn_s_waitcnt(0x0070 | 0x0F00);  // vmcnt(0)
-    if (tid < 32) ld[tid] = lr * kLog2e;
-#pragma unroll
-    for (int i = 0; i < C; ++i) {
-      const Frag y = *reinterpret_cast<const Frag*>(dst + L::kBytes + (C * wave + i) * 1024 + lane * 16);
-      const float x = group_sum<L::kChunks>(dot8<T>(orow[i], y, 0.0f));
-      if (lane % L::kChunks == 0) ld[32 + tq.row(i)] = x;
-    }
+  auto finish = [&](float* ld) {
+    if (wave == 0) ld[lane] = stat;
   };
   if (t0 < tiles) copy(lds.buf0, t0);
   {
@@ -673,7 +692,7 @@ __device__ __forceinline__ void bwd_dkdv(const MaskedArgs& a, int blk, int head,
     dk[d] = f32x16{};
     dv[d] = f32x16{};
   }
-  if (t0 < tiles) finish(lds.buf0, lds.ld0);
+  if (t0 < tiles) finish(lds.ld0);
   stage_barrier();
   const char* vt = lds.v + wave * L::kBytes;
   auto stage = [&](const char* qt, const float* ld, char* next, float* ldn, int j) {
@@ -706,7 +725,7 @@ __device__ __forceinline__ void bwd_dkdv(const MaskedArgs& a, int blk, int head,
         dk[d] = mfma<T>(s1, fl.frag_t(qt, 1, d), dk[d]);
       }
     }
-    if (j + 1 < tiles) finish(next, ldn);
+    if (j + 1 < tiles) finish(ldn);
     stage_barrier();
   };
   for (int j = t0; j < tiles; j += 2) {
@@ -753,9 +772,18 @@ __device__ __forceinline__ void bwd_dkdv(const MaskedArgs& a, int blk, int head,
   }
 }
 
-// Blocks of the first n_kblocks items are dK / dV blocks (the heavier ones, dispatched first), the rest dQ blocks.
 template <typename T, int HD, bool CAP, bool BIAS>
-__global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2, 2))) void masked_bwd_kernel(
+__global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2, 2))) void masked_dq_kernel(MaskedArgs a) {
+  __shared__ __attribute__((aligned(16))) char buf0[2 * Tiles<HD>::kBytes];
+  __shared__ __attribute__((aligned(16))) char buf1[2 * Tiles<HD>::kBytes];
+  __shared__ __attribute__((aligned(16))) char dot[kWaves * Tiles<HD>::kBytes];
+  int item, head;
+  if (!head_item(a, a.n_blocks, item, head)) return;
+  bwd_dq<T, HD, CAP, BIAS>(a, item, head, buf0, buf1, dot);
+}
+
+template <typename T, int HD, bool CAP, bool BIAS>
+__global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2, 2))) void masked_dkdv_kernel(
     MaskedArgs a) {
   using L = Tiles<HD>;
   __shared__ __attribute__((aligned(16))) char buf0[2 * L::kBytes];
@@ -764,18 +792,17 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2, 
   __shared__ __attribute__((aligned(16))) float ld0[64];
   __shared__ __attribute__((aligned(16))) float ld1[64];
   int item, head;
-  if (!head_item(a, a.n_kblocks + a.n_blocks, item, head)) return;
-  const BwdLds lds{buf0, buf1, v, ld0, ld1};
-  if (item < a.n_kblocks)
-    bwd_dkdv<T, HD, CAP, BIAS>(a, item, head, lds);
-  else
-    bwd_dq<T, HD, CAP, BIAS>(a, item - a.n_kblocks, head, lds);
+  if (!head_item(a, a.n_kblocks, item, head)) return;
+  bwd_dkdv<T, HD, CAP, BIAS>(a, item, head, BwdLds{buf0, buf1, v, ld0, ld1});
 }
 
 // ---------------------------------------------------------------------------------------------
 // The backward of batches that leave the chip idle in blocks of 128: a block owns 32 tokens of one side, its four waves
 // take the other side's tiles in turn (each with LDS of its own) and their sums meet in the LDS in wave order.
 // ---------------------------------------------------------------------------------------------
+// Of the dQ blocks: two tiles a wave (then the sums), a word and the waves' parts of r, the dO tile.
+template <int HD>
+constexpr int kNarrowDo = 2 * kWaves * Tiles<HD>::kBytes + 16 + 32 * kWaves * 4;
 template <int HD>
 constexpr int kNarrowLds = (2 + 2 * kWaves) * Tiles<HD>::kBytes;  // two shared tiles, two a wave; then the sums
 
@@ -827,12 +854,16 @@ __device__ __forceinline__ void narrow_dq(const MaskedArgs& a, int blk, int head
   };
   if (wave < tiles) copy(wave);
   const int64_t t = r.qa + i;
-  Frag qf[L::kSteps], df[L::kSteps];
+  char* dt = smem + kNarrowDo<HD>;  // the block's dO tile
+  constexpr int C = L::kCopies / kWaves;
+  TileLane<HD, C>(C * wave, lane, a.do_st)
+      .copy(dt, token<T>(a.dout, static_cast<int64_t>(r.qa) + i0, a.do_st, head, a.do_sh), r.lq - i0);
+  Frag qf[L::kSteps];
   load_row_frags<T, HD>(qf, token<T>(a.q, t, a.q_st, head, a.q_sh), h);
-  load_row_frags<T, HD>(df, token<T>(a.dout, t, a.do_st, head, a.do_sh), h);
   float ds = 0.0f;
   {
-    Frag of[L::kSteps];
+    Frag df[L::kSteps], of[L::kSteps];
+    load_row_frags<T, HD>(df, token<T>(a.dout, t, a.do_st, head, a.do_sh), h);
     load_row_frags<T, HD>(of, static_cast<const T*>(a.o) + (t * a.h_q + head) * HD, h);
 #pragma unroll
     for (int k = 0; k < L::kSteps; ++k) ds = dot8<T>(of[k], df[k], ds);
@@ -840,25 +871,33 @@ __device__ __forceinline__ void narrow_dq(const MaskedArgs& a, int blk, int head
   const float2 dp2 = half_pair(ds);
   const float dsum = dp2.x + dp2.y;
   const float lse2 = a.lse[head * a.n_q + t] * kLog2e;
-  f32x16 dq[ND];
+  f32x16 dq[ND], pk[ND];  // sum dS' K, sum P (1 - t^2) K
+  float rest = 0.0f;
 #pragma unroll
-  for (int d = 0; d < ND; ++d) dq[d] = f32x16{};
-  stage_wait();
+  for (int d = 0; d < ND; ++d) {
+    dq[d] = f32x16{};
+    pk[d] = f32x16{};
+  }
+  stage_barrier();  // every wave's share of the dO tile has landed
   for (int j = wave; j < tiles; j += kWaves) {
-    f32x16 st[1], dp = f32x16{}, f[1];
+    f32x16 st[1], dp = f32x16{};
     start_scores<CAP, BIAS, 1>(st, sc.slope, static_cast<float>(r.off() + i - 32 * j - 4 * h), 1.0f, 32 * j + 31 <= r.off() + i0);
 #pragma unroll
     for (int k = 0; k < L::kSteps; ++k) {
       st[0] = mfma<T>(fl.frag(kt, k), qf[k], st[0]);  // S^T = K Q^T
-      dp = mfma<T>(fl.frag(vt, k), df[k], dp);        // dP^T = V dO^T
+      dp = mfma<T>(fl.frag(vt, k), fl.frag(dt, k), dp);  // dP^T = V dO^T
     }
-    query_scores<T, CAP, BIAS>(a, sc.slope2, st, f, dp, dsum, lse2, static_cast<float>(r.off() + i - 32 * j - 4 * h),
-                               32 * j + 32 > vis_all, vis - 32 * j, h);
-    const Frag s0 = frag_acc<T>(st[0], 0), s1 = frag_acc<T>(st[0], 1);
+    query_scores<T, CAP, BIAS>(a, sc.slope2, st, dp, dsum, lse2, static_cast<float>(r.off() + i - 32 * j - 4 * h),
+                               32 * j + 32 > vis_all, vis - 32 * j, h, rest);
+    const Frag p0 = frag_acc<T>(st[0], 0), p1 = frag_acc<T>(st[0], 1);
+    const Frag s0 = frag_acc<T>(dp, 0), s1 = frag_acc<T>(dp, 1);
 #pragma unroll
     for (int d = 0; d < ND; ++d) {
-      dq[d] = mfma<T>(fl.frag_t(kt, 0, d), s0, dq[d]);  // dQ^T += K^T dS^T
-      dq[d] = mfma<T>(fl.frag_t(kt, 1, d), s1, dq[d]);
+      const Frag k0 = fl.frag_t(kt, 0, d), k1 = fl.frag_t(kt, 1, d);
+      dq[d] = mfma<T>(k0, s0, dq[d]);  // dQ^T += K^T dS'^T
+      pk[d] = mfma<T>(k0, p0, pk[d]);
+      dq[d] = mfma<T>(k1, s1, dq[d]);
+      pk[d] = mfma<T>(k1, p1, pk[d]);
     }
     if (j + kWaves < tiles) {
       wait_reads();
@@ -866,18 +905,27 @@ __device__ __forceinline__ void narrow_dq(const MaskedArgs& a, int blk, int head
       wait_copies<0>();
     }
   }
-  float x[4 * ND];
+  // (the waves' parts of r behind the merge's words)
+  float* parts = reinterpret_cast<float*>(again + 4);
+  const float2 rp = half_pair(rest);
+  float x[4 * ND], y[4 * ND];
   merge_waves<ND>(reinterpret_cast<float*>(smem), dq, wave, lane, x);
-  bool fine = true;
+  if (h == 0) parts[32 * wave + col] = rp.x + rp.y;
+  merge_waves<ND>(reinterpret_cast<float*>(smem), pk, wave, lane, y);
+  rest = 0.0f;
 #pragma unroll
-  for (int y = 0; y < 4 * ND; ++y) {
-    x[y] *= a.scale;
-    fine = fine && fabsf(x[y]) <= 3.402823466e38f;
+  for (int v = 0; v < kWaves; ++v) rest += parts[32 * v + col];
+  bool fine = fabsf(rest) <= 3.402823466e38f;
+#pragma unroll
+  for (int e = 0; e < 4 * ND; ++e) {
+    x[e] = __builtin_fmaf(-rest, y[e], x[e]) * a.scale;
+    fine = fine && fabsf(x[e]) <= 3.402823466e38f;
   }
   if (valid && !fine) atomicOr(again, 1u << col);
   __syncthreads();
   uint32_t cols = *again;
   if (valid && !((cols >> col) & 1)) {
+    if (wave == 0 && h == 0) a.dsum[head * a.n_q + t] = vis > 0 ? dsum + rest : 0.0f;
     T* row = static_cast<T*>(a.out) + (t * a.h_q + head) * HD;
 #pragma unroll
     for (int q = 0; q < ND; ++q) {  // four registers: head dims 32 d + 8 (e / 4) + 4 h .. + 4
@@ -908,41 +956,22 @@ __device__ __forceinline__ void narrow_dkdv(const MaskedArgs& a, int blk, int he
   const int q_all = r.first(min(k0 + 31, r.lk - 1), a.causal);  // from here on every key is seen
   const T* qh = token<T>(a.q, r.qa, a.q_st, head, a.q_sh);
   const T* doh = token<T>(a.dout, r.qa, a.do_st, head, a.do_sh);
-  const int64_t o_st = static_cast<int64_t>(a.h_q) * HD;
-  const T* oh = static_cast<const T*>(a.o) + r.qa * o_st + head * HD;
   const float* lse = a.lse + head * a.n_q + r.qa;
-  const TileLane<HD, L::kCopies> tq(0, lane, a.q_st), td(0, lane, a.do_st), to(0, lane, o_st);
+  const float* ds = a.dsum + head * a.n_q + r.qa;
+  const TileLane<HD, L::kCopies> tq(0, lane, a.q_st), td(0, lane, a.do_st);
   const FragLane<HD> fl(lane);
   const Scorer<CAP, BIAS> sc(a, head);
   char* kt = smem;
   char* vt = smem + L::kBytes;
   char* qt = smem + (2 + 2 * wave) * L::kBytes;
   char* dt = qt + L::kBytes;
-  Frag orow[L::kCopies];  // the O chunks of the dO chunks this lane copies
-  float lr = 0.0f;
+  float lse2 = 0.0f, dsum = 0.0f;  // lse (log2 units) and D of tile row c in lanes c and c + 32
   auto copy = [&](int j) {
     const int rows = r.lq - 32 * j;
     tq.fresh().copy(qt, qh + 32 * j * a.q_st, rows);
     td.fresh().copy(dt, doh + 32 * j * a.do_st, rows);
-    const auto o = to.fresh();
-#pragma unroll
-    for (int i = 0; i < L::kCopies; ++i)
-      orow[i] = *reinterpret_cast<const Frag*>(reinterpret_cast<const char*>(oh + 32 * j * o_st) + o.at(i, rows));
-    lr = lse[32 * j + min(col, rows - 1)];
-  };
-  // lse and D of tile row c in lanes c and c + 32.
-  float lse2 = 0.0f, dsum = 0.0f;
-  auto finish = [&] {
-    wait_copies<0>();
-    lse2 = lr * kLog2e;
-    constexpr int kRowsPerCopy = 64 / L::kChunks;
-#pragma unroll
-    for (int i = 0; i < L::kCopies; ++i) {
-      const Frag y = *reinterpret_cast<const Frag*>(dt + i * 1024 + lane * 16);
-      const float x = group_sum<L::kChunks>(dot8<T>(orow[i], y, 0.0f));
-      const float v = __shfl(x, col % kRowsPerCopy * L::kChunks, 64);
-      if (col / kRowsPerCopy == i) dsum = v;
-    }
+    lse2 = lse[32 * j + min(col, rows - 1)] * kLog2e;
+    dsum = ds[32 * j + min(col, rows - 1)];
   };
   constexpr int C = L::kCopies / kWaves;
   TileLane<HD, C>(C * wave, lane, a.k_st)
@@ -957,7 +986,6 @@ __device__ __forceinline__ void narrow_dkdv(const MaskedArgs& a, int blk, int he
     dv[d] = f32x16{};
   }
   stage_barrier();
-  if (t0 + wave < tiles) finish();
   for (int j = t0 + wave; j < tiles; j += kWaves) {
     f32x16 st[1], dp = f32x16{}, f[1];
     start_scores<CAP, BIAS, 1>(st, sc.slope, static_cast<float>(r.off() + 32 * j + 4 * h - kc), -1.0f, r.off() + 32 * j >= k0 + 31);
@@ -989,7 +1017,7 @@ __device__ __forceinline__ void narrow_dkdv(const MaskedArgs& a, int blk, int he
     if (j + kWaves < tiles) {
       wait_reads();
       copy(j + kWaves);
-      finish();
+      wait_copies<0>();
     }
   }
   // Keys are accumulator rows, head dims lanes.
@@ -1031,15 +1059,21 @@ __device__ __forceinline__ void narrow_dkdv(const MaskedArgs& a, int blk, int he
 }
 
 template <typename T, int HD, bool CAP, bool BIAS>
-__global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2, 2))) void masked_narrow_bwd_kernel(
+__global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2, 2))) void masked_narrow_dq_kernel(
+    MaskedArgs a) {
+  __shared__ __attribute__((aligned(16))) char smem[kNarrowDo<HD> + Tiles<HD>::kBytes];
+  int item, head;
+  if (!head_item(a, a.n_blocks, item, head)) return;
+  narrow_dq<T, HD, CAP, BIAS>(a, item, head, smem);
+}
+
+template <typename T, int HD, bool CAP, bool BIAS>
+__global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2, 2))) void masked_narrow_dkdv_kernel(
     MaskedArgs a) {
   __shared__ __attribute__((aligned(16))) char smem[kNarrowLds<HD>];
   int item, head;
-  if (!head_item(a, a.n_kblocks + a.n_blocks, item, head)) return;
-  if (item < a.n_kblocks)
-    narrow_dkdv<T, HD, CAP, BIAS>(a, item, head, smem);
-  else
-    narrow_dq<T, HD, CAP, BIAS>(a, item - a.n_kblocks, head, smem);
+  if (!head_item(a, a.n_kblocks, item, head)) return;
+  narrow_dkdv<T, HD, CAP, BIAS>(a, item, head, smem);
 }
 
 // dk / dv [key, g, :] = T(sum over the KV group's heads, in head order, of the parts). Thread = 4 head dims of a key.
@@ -1108,8 +1142,9 @@ int64_t blocks_bound(int64_t n, int32_t n_seq, int rows) { return std::min<int64
 // 32 / group queries (2.2 us per 128 keys and round of two blocks a CU, 4 us a round aside; heads of 64 half as long).
 // How long the rows are beyond the longest is known on the device only: on average tokens over rows. Measured, 12 / 2
 // heads of 128, us in blocks of 128 / of few: 100 tokens 9.7 / 8.2, 707 23.3 / 15.6, 2,048 53 / 45, 3,000 75 / 75, 4,096
-// 104 / 120, ten rows of 256 13.9 / 23.0, four of 1,024 52 / 57, 1,500 and 27 rows of 64 44 / 37; 4 / 1 heads, 4,096
-// 98 / 51; 16 heads of 64 without a causal mask, eight rows of 700 35 / 59, 1,025 + 577 + 257 + 64 31 / 29.
+// 104 / 120, ten rows of 256 13.9 / 23.0, four of 1,024 52 / 57, 4,096 + 2,048 + 1,024 + 993 117 / 165, 1,500 and 27 rows
+// of 64 44 / 37; 4 / 1 heads, 4,096 98 / 51; 16 heads of 64 without a causal mask, eight rows of 700 35 / 59, 1,025 +
+// 577 + 257 + 64 31 / 29.
 struct SplitPlan {
   int splits, tiles;
   int64_t items;  // blocks of few queries, bound over all rows
@@ -1126,9 +1161,9 @@ SplitPlan split_plan(int32_t n_seq, int64_t n_q, int64_t n_k, int32_t max_q, int
   // (a part is worth its share of the join from two tiles a wave on, parts at all from some 1,000 keys)
   const int64_t splits = tiles < 32 ? 1 : std::max<int64_t>(std::min<int64_t>(512 / base, (tiles + 7) / 8), 1);
   const int64_t part = (tiles + splits - 1) / splits;
-  const double wide_load = std::max(1.0, std::max<int64_t>((n_q + kRows - 1) / kRows, n_seq) * h_q / 512.0);
-  const double wide_us = 7.0 + 0.8 * tiles * wide_load;
   const double row = std::min<double>(static_cast<double>(max_k), static_cast<double>(n_k) / n_seq);
+  const double wide_load = std::max(1.0, std::max<int64_t>((n_q + kRows - 1) / kRows, n_seq) * h_q / 512.0);
+  const double wide_us = 7.0 + 0.8 * std::max(static_cast<double>(tiles), wide_load * row / 32);
   // (queries of a causal row see half of it on average, a few at the end of a cache nearly all)
   const double step_us = head_dim == 64 ? 1.1 : 2.2, steps = max_q < max_k ? row / 128 : row / 256;
   const double few_us =
@@ -1141,11 +1176,22 @@ SplitPlan split_plan(int32_t n_seq, int64_t n_q, int64_t n_k, int32_t max_q, int
   return p;
 }
 
-// Whether a backward runs in blocks of 32 tokens: where blocks of 128 would leave the chip idle. 12 / 2 heads of 128, us in
-// blocks of 128 / of 32: 100 tokens 22 / 15, 707 52 / 37, 1,024 65 / 46, 1,024 and ten rows of 64 (156 blocks of 128)
-// 67 / 59; from 192 blocks on the other way round: 2,048 117 / 120, four rows of 512 46 / 64, ten of 256 37 / 67.
-bool narrow_bwd(int32_t n_seq, int64_t n_q, int64_t n_k, int32_t h_q) {
-  return std::max<int64_t>((std::max(n_q, n_k) + kRows - 1) / kRows, n_seq) * h_q < 192;
+// Whether a backward runs in blocks of 32 tokens rather than of 128. The latter walk the longest row's tiles alone (2.8 us
+// a tile for dQ, then dK and dV), the former share them among four waves but read the other side again for every 32
+// tokens. Measured, 12 / 2 heads of 128, us in blocks of 128 / of 32: 100 tokens 32 / 23, 707 80 / 48, 2,048 194 / 109,
+// 4,096 377 / 327, two rows of 256 43 / 29, 1,500 and 27 rows of 64 151 / 106; sixteen rows of 32 23 / 25, ten of 256
+// 52 / 71, four of 512 71 / 75, of 1,024 168 / 164, eight of 1,024 254 / 267, 4,096 + 2,048 + 1,024 + 993 430 / 477;
+// 16 heads of 64, no causal mask, 1,025 + 577 + 257 + 64 89 / 77, eight rows of 700 113 / 164.
+bool narrow_bwd(int32_t n_seq, int64_t n_q, int64_t n_k, int32_t max_q, int32_t max_k, int32_t h_q) {
+  const double n = static_cast<double>(std::max(n_q, n_k)), seqs = std::max(n_seq, 1);
+  const double blocks = std::max(n / 32, seqs) * h_q, row = n / seqs / 32;
+  const double narrow_us = 18.0 + blocks * (0.042 + 0.00125 * row);
+  return narrow_us < 18.0 + 2.8 * std::max(max_q, max_k) / 32;
+}
+
+// The backward's workspace: the heads' parts of dK and dV where heads share keys, and D.
+int64_t bwd_floats(int64_t n_q, int64_t n_k, int32_t h_q, int32_t h_kv, int32_t head_dim) {
+  return (h_q > h_kv ? 2 * static_cast<int64_t>(h_q) * n_k * head_dim : 0) + static_cast<int64_t>(h_q) * n_q;
 }
 
 // Launch size of n_items for every head (whole chunks of head_item's).
@@ -1215,7 +1261,7 @@ extern "C" int rus_attn_masked_workspace(int32_t n_seq, int64_t n_q, int64_t n_k
   if (!floats) return fail(RUS_ERR_INVALID, "%s: null result", fn);
   if (int e = check_sizes(fn, n_seq, n_q, n_k, max_q, max_k, h_q, h_kv, head_dim)) return e;
   if (backward) {
-    *floats = h_q > h_kv ? 2 * static_cast<int64_t>(h_q) * n_k * head_dim : 0;
+    *floats = bwd_floats(n_q, n_k, h_q, h_kv, head_dim);
     return RUS_OK;
   }
   const SplitPlan p = split_plan(n_seq, n_q, n_k, max_q, max_k, h_q, h_kv, head_dim);
@@ -1232,7 +1278,7 @@ extern "C" int rus_attn_masked_plan(int32_t n_seq, int64_t n_q, int64_t n_k, int
   const SplitPlan p = split_plan(n_seq, n_q, n_k, max_q, max_k, h_q, h_kv, head_dim);
   plan[0] = p.splits;
   plan[1] = p.tiles;
-  plan[2] = narrow_bwd(n_seq, n_q, n_k, h_q) ? 32 : kRows;
+  plan[2] = narrow_bwd(n_seq, n_q, n_k, max_q, max_k, h_q) ? 32 : kRows;
   return RUS_OK;
 }
 
@@ -1328,30 +1374,34 @@ extern "C" int rus_attn_masked_bwd(const void* dout, int64_t do_stride_t, int64_
   a.out = dq, a.dk = dk, a.dv = dv;
   a.cu_q = cu_q, a.cu_k = cu_k, a.n_seq = n_seq, a.n_q = n_q, a.n_k = n_k, a.h_q = h_q, a.h_kv = h_kv;
   set_scores(a, scale, softcap, slopes, prefix, causal);
-  const bool narrow = narrow_bwd(n_seq, n_q, n_k, h_q);
+  const bool narrow = narrow_bwd(n_seq, n_q, n_k, max_q, max_k, h_q);
   const int rows = narrow ? 32 : kRows;
   a.n_blocks = static_cast<int>(blocks_bound(n_q, n_seq, rows));
   a.n_kblocks = static_cast<int>(blocks_bound(n_k, n_seq, rows));
-  int64_t grid;
-  if (int e = item_grid(fn, a.n_blocks + a.n_kblocks, a, grid)) return e;
-  const int64_t half = static_cast<int64_t>(h_q) * n_k * head_dim;
-  if (h_q > h_kv && n_k > 0) {
-    if (!workspace || n_workspace < 2 * half || !aligned(workspace, 16))
-      return fail(RUS_ERR_INVALID, "%s: workspace of %lld floats, %lld needed", fn, (long long)n_workspace,
-                  (long long)(2 * half));
-    a.dk_part = workspace;
-    a.dv_part = workspace + half;
-  }
-  const dim3 blocks(static_cast<unsigned>(grid)), threads(64 * kWaves);
+  int64_t dq_grid, dkdv_grid;
+  if (int e = item_grid(fn, a.n_blocks, a, dq_grid)) return e;
+  if (int e = item_grid(fn, a.n_kblocks, a, dkdv_grid)) return e;
+  const int64_t need = bwd_floats(n_q, n_k, h_q, h_kv, head_dim);
+  if (need && (!workspace || n_workspace < need || !aligned(workspace, 16)))
+    return fail(RUS_ERR_INVALID, "%s: workspace of %lld floats, %lld needed", fn, (long long)n_workspace,
+                (long long)need);
+  a.dk_part = workspace;
+  a.dv_part = workspace + static_cast<int64_t>(h_q) * n_k * head_dim;
+  a.dsum = workspace + need - static_cast<int64_t>(h_q) * n_q;
+  const dim3 dq_blocks(static_cast<unsigned>(dq_grid)), dkdv_blocks(static_cast<unsigned>(dkdv_grid)),
+      threads(64 * kWaves);
   hipStream_t st = static_cast<hipStream_t>(stream);
   dispatch(dtype, head_dim, softcap > 0.0f, slopes != nullptr, [&](auto t, auto d, auto c, auto b) {
     using T = decltype(t);
     constexpr int kDim = decltype(d)::value;
     constexpr bool kCap = decltype(c)::value, kBias = decltype(b)::value;
-    if (narrow)
-      hipLaunchKernelGGL((masked_narrow_bwd_kernel<T, kDim, kCap, kBias>), blocks, threads, 0, st, a);
-    else
-      hipLaunchKernelGGL((masked_bwd_kernel<T, kDim, kCap, kBias>), blocks, threads, 0, st, a);
+    if (narrow) {
+      if (n_q) hipLaunchKernelGGL((masked_narrow_dq_kernel<T, kDim, kCap, kBias>), dq_blocks, threads, 0, st, a);
+      if (n_k) hipLaunchKernelGGL((masked_narrow_dkdv_kernel<T, kDim, kCap, kBias>), dkdv_blocks, threads, 0, st, a);
+    } else {
+      if (n_q) hipLaunchKernelGGL((masked_dq_kernel<T, kDim, kCap, kBias>), dq_blocks, threads, 0, st, a);
+      if (n_k) hipLaunchKernelGGL((masked_dkdv_kernel<T, kDim, kCap, kBias>), dkdv_blocks, threads, 0, st, a);
+    }
   });
   if (int e = check_launch(fn)) return e;
   if (h_q == h_kv || n_k == 0) return RUS_OK;
