@@ -2849,7 +2849,7 @@ def _masked_heads(fn: str, x: torch.Tensor, name: str, d: int, dt: torch.dtype):
         raise TypeError(f"{fn}: {name} must be {dt}, got {x.dtype}")
     st, sh, sd = x.stride()
     if sd != 1 or (st | sh) & 7 or x.data_ptr() & 15:
-        x = x.contiguous()
+        x = x.clone(memory_format=torch.contiguous_format)  # (.contiguous() keeps one token's strides, and its address)
         st, sh, _ = x.stride()
     return x, (x.data_ptr(), st, sh)
 
@@ -3075,6 +3075,14 @@ def _temperature(fn: str, t) -> float:
     return t
 
 
+def _distill_nothing(hidden: torch.Tensor, num_items_in_batch, need_grad: bool):
+    """What ``lm_head_distill`` returns for no tokens."""
+    out = torch.zeros(1, dtype=torch.float32, device=hidden.device)
+    items = _num_items(num_items_in_batch, hidden.device)
+    return (out, out.new_empty(0), torch.ones_like(out) if items is None else torch.clamp(items, min=1.0),
+            out.new_empty(hidden.shape) if need_grad else None)
+
+
 def lm_head_distill(hidden: torch.Tensor, weight: torch.Tensor, teacher_ids: torch.Tensor,
                     teacher_logits: torch.Tensor, temperature: float = 1.0, num_items_in_batch=None,
                     v_chunk: int | None = None, need_grad: bool = True, weight_t: torch.Tensor | None = None):
@@ -3104,11 +3112,7 @@ def lm_head_distill(hidden: torch.Tensor, weight: torch.Tensor, teacher_ids: tor
     n_vocab = w.shape[0]
     with torch.cuda.device(h.device):
         if n_tok == 0:
-            out = torch.zeros(1, dtype=torch.float32, device=h.device)
-            denom = torch.clamp(_num_items(num_items_in_batch, h.device), min=1.0) \
-                if num_items_in_batch is not None else torch.ones_like(out)
-            return out, torch.empty(0, dtype=torch.float32, device=h.device), denom, \
-                torch.empty((0, d), dtype=torch.float32, device=h.device) if need_grad else None
+            return _distill_nothing(h, num_items_in_batch, need_grad)
         chunk = _distill_chunk(n_tok, n_vocab, cu_count(h.device)) if v_chunk is None else int(v_chunk)
         if chunk <= 0 or (chunk < n_vocab and chunk % LM_TILE):
             raise ValueError(f"{fn}: v_chunk must be a positive multiple of {LM_TILE}")

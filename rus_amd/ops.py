@@ -422,7 +422,7 @@ def _distill_streamed(h_2d, ids, logits, head: HostHead, temperature, num_items_
         raise ValueError(f"{fn}: the head's hidden size is {head.hidden_size}, got {d} (a multiple of {K.LM_K})")
     t = K._temperature(fn, temperature)
     if n_tok == 0:
-        raise ValueError(f"{fn}: no tokens")
+        return K._distill_nothing(h, num_items_in_batch, need_grad)
     starts = list(range(0, V, vc))
     hp = K.LMHeadDistill(n_tok, head.cpu_weight, vc, ids, logits, t, need_grad)
     head.prefetch_chunk(0, 0, min(vc, V))

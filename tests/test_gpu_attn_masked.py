@@ -253,6 +253,29 @@ def test_views_of_a_fused_projection_and_expanded_gradients():
     assert torch.equal(out, out2) and torch.equal(lse, lse2)
 
 
+def test_operands_that_look_contiguous_but_are_not_addressable():
+    """One token whose token stride is odd, and tensors that start 2 bytes behind an aligned address."""
+    q, k, v, dout = (x.to(DEV) for x in _inputs([1], [1], 4, 2, 64, torch.bfloat16, seed=31))
+    cu = _ints([0, 1])
+
+    def odd(x):
+        rows = torch.empty(3, x.shape[1] * 64 + 3, dtype=x.dtype, device=DEV)
+        view = rows[1:2, : x.shape[1] * 64].unflatten(1, x.shape[1:])
+        return view.copy_(x)
+
+    def shifted(x):
+        return torch.empty(x.numel() + 1, dtype=x.dtype, device=DEV)[1:].view(x.shape).copy_(x)
+
+    out, lse = K.attn_masked_fwd(q, k, v, cu)
+    grads = K.attn_masked_bwd(dout, q, k, v, out, lse, cu)
+    for f in (odd, shifted):
+        assert f(q).is_contiguous()
+        got, _ = K.attn_masked_fwd(f(q), f(k), f(v), cu)
+        assert torch.equal(got, out), f.__name__
+        for a, b in zip(K.attn_masked_bwd(f(dout), f(q), f(k), f(v), out, lse, cu), grads):
+            assert torch.equal(a, b), f.__name__
+
+
 def test_gradients_against_differences():
     """(f(x + h e) - f(x - h e)) / 2 h of the definition in float64 along random directions, with the operator's
     gradients from the same inputs."""

@@ -157,6 +157,33 @@ def test_loss_over_a_host_head_and_its_gradient(resident):
     assert abs(float(loss2) - float(loss.detach())) <= 1e-5 * abs(float(loss.detach()))
 
 
+@pytest.mark.parametrize("resident", [True, False])
+@pytest.mark.parametrize("num", [None, 0, 7])
+def test_no_tokens_and_no_teacher(resident, num):
+    h, w, ids, logits = _inputs(9, 64, 700, 3, seed=14)
+    ids[:] = -100
+    head = HostHead(w, DEV, v_chunk=256, resident=resident)
+    for n in (0, 9):
+        x = h[:n].to(DEV).requires_grad_()
+        loss, kl = ops.chunked_distill_head(x, ids[:n].to(DEV), logits[:n].to(DEV), head, 2.0, num)
+        loss.backward()
+        assert float(loss.detach()) == 0.0 and kl.shape == (n,) and not bool(kl.any())
+        assert x.grad.shape == (n, 64) and not bool(x.grad.any())
+
+
+def test_rows_of_wider_buffers_and_rows_that_are_not_addressable():
+    h, w, ids, logits = _inputs(21, 128, 800, 6, seed=15)
+    loss, kl, dh = _run(h, w, ids, logits, 1.5)
+    for cols, first in ((160, 16), (131, 2)):
+        hb, wb = (torch.full((x.shape[0], cols), math.nan, dtype=torch.float16) for x in (h, w))
+        hb[:, first:first + 128], wb[:, first:first + 128] = h, w
+        ib = torch.full((21, 11), -1)
+        ib[:, 3:9] = ids
+        got = K.lm_head_distill(hb.to(DEV)[:, first:first + 128], wb.to(DEV)[:, first:first + 128], ib.to(DEV)[:, 3:9],
+                                logits.t().contiguous().to(DEV).t(), temperature=1.5)
+        assert torch.equal(got[0], loss) and torch.equal(got[1], kl) and torch.equal(got[3], dh)
+
+
 def test_gradient_against_differences():
     h, w, ids, logits = _inputs(7, 64, 400, 6, seed=10)
     _, _, dh = _run(h, w, ids, logits, 1.3)
