@@ -13,6 +13,12 @@ namespace {
 constexpr int kWaves = 4, kRows = 128;  // waves of a block, tokens of a block
 constexpr int kFwdTiles = 2;             // key tiles per stage of the forward
 
+// Blocks a CU that the registers are divided for. 16 heads of 64, us with two / three: eight rows of 700 forward 35 / 31,
+// backward 112 / 89, two of 2,048 59 / 50, 146 / 145; 1,025 + 577 + 257 + 64 with a cap 30 / 27, 77 / 73. The backward's
+// dQ blocks of 32 tokens keep two: their sums would go to scratch memory (the same tokens 73 / 79).
+template <int HD>
+constexpr int kCuBlocks = HD == 64 ? 3 : 2;
+
 // Block id -> (item, head): the query heads of a KV group that work on one item take ids 8 apart, i.e. one XCD (ids go
 // round robin over the 8), so that they read their shared keys from one L2. False past the last item.
 __device__ __forceinline__ bool head_item(const MaskedArgs& a, int n_items, int& item, int& head) {
@@ -34,7 +40,8 @@ __device__ __forceinline__ MaskedRow uniform(MaskedRow r) {
 // Forward. S^T = K Q^T on 32 NT keys: a lane owns one query (column) and half of the keys; the running maximum and sum
 // are per-lane scalars, and P^T feeds O^T += V^T P^T from the accumulator. m is the running maximum itself at every
 // step, and O is divided by lr, the sum of the rounded P, in which their common rounding cancels (l, of the unrounded,
-// gives the lse).
+// gives the lse). P is rounded to T because the matrix instruction takes nothing wider at its rate; everything else
+// stays in 32 bits.
 // ---------------------------------------------------------------------------------------------
 template <int ND>
 struct FwdState {
@@ -124,7 +131,10 @@ __device__ __forceinline__ void load_row_frags(Frag (&f)[HD / 16], const T* row,
 
 // 128 queries of one head, 32 to a wave; tiles of 32 keys stream through double-buffered LDS, two to a stage, each
 // copied once for all four waves while the previous stage is used. Hidden keys reach the product as 0 x V: where V is
-// not finite the sums are not either, and such a query is formed again by itself (plain_fwd_row).
+// not finite the sums are not either, and such a query is formed again by itself (plain_fwd_row). Bound by the products
+// and the exponentials beside them, which two blocks a CU overlap: 4,096 + 2,048 + 1,024 + 993 tokens, 12 / 2 heads of
+// 128, bf16 with a bias 117 us (600 TFLOP/s of what is visible), one row of 4,096 104 us (490): the longest row's last
+// blocks run by themselves.
 template <typename T, int HD, bool CAP, bool BIAS>
 __device__ __forceinline__ void fwd_block(const MaskedArgs& a, char* buf0, char* buf1) {
   using L = Tiles<HD>;
@@ -197,7 +207,8 @@ __device__ __forceinline__ void fwd_block(const MaskedArgs& a, char* buf0, char*
 }
 
 template <typename T, int HD, bool CAP, bool BIAS>
-__global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2, 2))) void masked_fwd_kernel(
+__global__ __launch_bounds__(64 * kWaves)
+__attribute__((amdgpu_waves_per_eu(kCuBlocks<HD>, kCuBlocks<HD>))) void masked_fwd_kernel(
     MaskedArgs a) {
   __shared__ __attribute__((aligned(16))) char buf0[2 * kFwdTiles * Tiles<HD>::kBytes];
   __shared__ __attribute__((aligned(16))) char buf1[2 * kFwdTiles * Tiles<HD>::kBytes];
@@ -208,7 +219,9 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2, 
 // Few queries over many keys: a block holds up to 32 (query, head) pairs of one KV head as the columns of S^T, so that
 // K and V are read once for all of the group's heads, its waves take key tiles in turn (each with LDS of its own, no
 // barrier in the loop), and the keys are split over blocks whose parts another launch joins. Part: per column the sum
-// of P V on the part's own maximum, then that maximum, the sum of P and the sum of the rounded P.
+// of P V on the part's own maximum, then that maximum, the sum of P and the sum of the rounded P. Bound by reading K and
+// V once few queries are left: one token over 131,071 keys, 2 KV heads of 128, 26 us (5.1 TB/s), eight over 15,253 keys
+// in all 12 us; rows of some hundred tokens by a row's tiles in turn (707 tokens 12 us).
 // ---------------------------------------------------------------------------------------------
 constexpr int kMaxSplitGroup = 32;
 
@@ -363,7 +376,8 @@ __device__ __forceinline__ void split_block(const MaskedArgs& a, char* kbuf, cha
 }
 
 template <typename T, int HD, bool CAP, bool BIAS>
-__global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2, 2))) void masked_split_kernel(
+__global__ __launch_bounds__(64 * kWaves)
+__attribute__((amdgpu_waves_per_eu(kCuBlocks<HD>, kCuBlocks<HD>))) void masked_split_kernel(
     MaskedArgs a) {
   __shared__ __attribute__((aligned(16))) char kbuf[kWaves * Tiles<HD>::kBytes];
   __shared__ __attribute__((aligned(16))) char vbuf[kWaves * Tiles<HD>::kBytes];
@@ -371,7 +385,8 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2, 
 }
 
 // Joins the parts of one (query, head), a block each: its waves take the parts in turn, eight loads at a time, and add
-// their sums in wave order.
+// their sums in wave order. What it costs is the loads' latency: 8 tokens of 12 heads, up to 32 parts 4.2 us, one token,
+// 256 parts 7.6 us.
 template <typename T, int HD, bool CAP, bool BIAS, int kJoinWaves>
 __global__ __launch_bounds__(64 * kJoinWaves) void masked_join_kernel(MaskedArgs a) {
   constexpr int N = HD / 64, kDepth = 8;
@@ -458,7 +473,9 @@ __global__ __launch_bounds__(64 * kJoinWaves) void masked_join_kernel(MaskedArgs
 }
 
 // ---------------------------------------------------------------------------------------------
-// Backward.
+// Backward. P and dS are rounded to T for the products that take them; their sums, D and lse are not. Gradients are off
+// the definition by 1.4 times what separate products with 32-bit softmax and its 32-bit gradient are (bf16 0.24% against
+// 0.17%, fp16 0.030% against 0.021%).
 // ---------------------------------------------------------------------------------------------
 
 // LDS of the backward: the streamed tiles' two buffers, and for the dK / dV blocks the block's V rows and the streamed
@@ -537,7 +554,9 @@ __device__ __forceinline__ void key_scores(const MaskedArgs& a, float slope2, f3
 }
 
 // dQ and D of 128 queries: key tiles stream through LDS, each wave owns 32 queries (Q fragments in registers, its dO
-// tile in LDS: the two sums leave no registers for it).
+// tile in LDS: the two sums leave no registers for it, and with it they went to scratch memory). Bound by the four
+// products and the exponentials between them: 4,096 + 2,048 + 1,024 + 993 tokens, 12 / 2 heads of 128, bf16 with a bias
+// 196 us (720 TFLOP/s of what is visible).
 template <typename T, int HD, bool CAP, bool BIAS>
 __device__ __forceinline__ void bwd_dq(const MaskedArgs& a, int blk, int head, char* buf0, char* buf1, char* dot) {
   using L = Tiles<HD>;
@@ -598,7 +617,8 @@ __device__ __forceinline__ void bwd_dq(const MaskedArgs& a, int blk, int head, c
     const FragLane<HD> fl = fl0.fresh();
     if (j < mine) {
       f32x16 st[1], dp = f32x16{};
-      start_scores<CAP, BIAS, 1>(st, sc.slope, static_cast<float>(r.off() + i - 32 * j - 4 * h), 1.0f, 32 * j + 31 <= r.off() + iw);
+      start_scores<CAP, BIAS, 1>(st, sc.slope, static_cast<float>(r.off() + i - 32 * j - 4 * h), 1.0f,
+                                 32 * j + 31 <= r.off() + iw);
 #pragma unroll
       for (int k = 0; k < L::kSteps; ++k) {
         st[0] = mfma<T>(fl.frag(kt, k), qf[k], st[0]);  // S^T = K Q^T
@@ -640,7 +660,7 @@ __device__ __forceinline__ void bwd_dq(const MaskedArgs& a, int blk, int head, c
 
 // dK and dV of 128 keys for one query head: Q and dO tiles stream through LDS with their lse and D, each wave owns 32
 // keys (K fragments in registers, V fragments from LDS). A lane owns one key (column of S = Q K^T) and half of the
-// queries.
+// queries. Bound as dQ, with two products' operands read from LDS by columns: the same tokens 249 us (570 TFLOP/s).
 template <typename T, int HD, bool CAP, bool BIAS>
 __device__ __forceinline__ void bwd_dkdv(const MaskedArgs& a, int blk, int head, const BwdLds& lds) {
   using L = Tiles<HD>;
@@ -701,7 +721,8 @@ __device__ __forceinline__ void bwd_dkdv(const MaskedArgs& a, int blk, int head,
     const FragLane<HD> fl = fl0.fresh();
     if (j >= q_wave) {
       f32x16 st[1], dp = f32x16{}, f[1];
-      start_scores<CAP, BIAS, 1>(st, sc.slope, static_cast<float>(r.off() + 32 * j + 4 * h - kc), -1.0f, r.off() + 32 * j >= kw + 31);
+      start_scores<CAP, BIAS, 1>(st, sc.slope, static_cast<float>(r.off() + 32 * j + 4 * h - kc), -1.0f,
+                                 r.off() + 32 * j >= kw + 31);
 #pragma unroll
       for (int k = 0; k < L::kSteps; ++k) {
         st[0] = mfma<T>(fl.frag(qt, k), kf[k], st[0]);      // S = Q K^T
@@ -773,7 +794,8 @@ __device__ __forceinline__ void bwd_dkdv(const MaskedArgs& a, int blk, int head,
 }
 
 template <typename T, int HD, bool CAP, bool BIAS>
-__global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2, 2))) void masked_dq_kernel(MaskedArgs a) {
+__global__ __launch_bounds__(64 * kWaves)
+__attribute__((amdgpu_waves_per_eu(kCuBlocks<HD>, kCuBlocks<HD>))) void masked_dq_kernel(MaskedArgs a) {
   __shared__ __attribute__((aligned(16))) char buf0[2 * Tiles<HD>::kBytes];
   __shared__ __attribute__((aligned(16))) char buf1[2 * Tiles<HD>::kBytes];
   __shared__ __attribute__((aligned(16))) char dot[kWaves * Tiles<HD>::kBytes];
@@ -783,7 +805,8 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2, 
 }
 
 template <typename T, int HD, bool CAP, bool BIAS>
-__global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2, 2))) void masked_dkdv_kernel(
+__global__ __launch_bounds__(64 * kWaves)
+__attribute__((amdgpu_waves_per_eu(kCuBlocks<HD>, kCuBlocks<HD>))) void masked_dkdv_kernel(
     MaskedArgs a) {
   using L = Tiles<HD>;
   __shared__ __attribute__((aligned(16))) char buf0[2 * L::kBytes];
@@ -798,7 +821,10 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2, 
 
 // ---------------------------------------------------------------------------------------------
 // The backward of batches that leave the chip idle in blocks of 128: a block owns 32 tokens of one side, its four waves
-// take the other side's tiles in turn (each with LDS of its own) and their sums meet in the LDS in wave order.
+// take the other side's tiles in turn (each with LDS of its own) and their sums meet in the LDS in wave order. Bound by
+// the latency of a wave's few tiles: 707 tokens in six rows, 12 / 2 heads of 128 with a cap 22 us dQ, 18 us dK and dV;
+// 1,923 tokens in four, 16 heads of 64 with a cap 41 and 46 us (the cap's arithmetic: 24,560 tiles of some 2,000 cycles
+// over 1,024 SIMDs are 20 us).
 // ---------------------------------------------------------------------------------------------
 // Of the dQ blocks: two tiles a wave (then the sums), a word and the waves' parts of r, the dO tile.
 template <int HD>
@@ -905,20 +931,23 @@ __device__ __forceinline__ void narrow_dq(const MaskedArgs& a, int blk, int head
       wait_copies<0>();
     }
   }
-  // (the waves' parts of r behind the merge's words)
-  float* parts = reinterpret_cast<float*>(again + 4);
+  float* parts = reinterpret_cast<float*>(again + 4);  // the waves' parts of r
   const float2 rp = half_pair(rest);
-  float x[4 * ND], y[4 * ND];
-  merge_waves<ND>(reinterpret_cast<float*>(smem), dq, wave, lane, x);
   if (h == 0) parts[32 * wave + col] = rp.x + rp.y;
-  merge_waves<ND>(reinterpret_cast<float*>(smem), pk, wave, lane, y);
+  __syncthreads();
   rest = 0.0f;
 #pragma unroll
   for (int v = 0; v < kWaves; ++v) rest += parts[32 * v + col];
+#pragma unroll
+  for (int d = 0; d < ND; ++d)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) dq[d][e] = __builtin_fmaf(-rest, pk[d][e], dq[d][e]);
+  float x[4 * ND];
+  merge_waves<ND>(reinterpret_cast<float*>(smem), dq, wave, lane, x);
   bool fine = fabsf(rest) <= 3.402823466e38f;
 #pragma unroll
   for (int e = 0; e < 4 * ND; ++e) {
-    x[e] = __builtin_fmaf(-rest, y[e], x[e]) * a.scale;
+    x[e] *= a.scale;
     fine = fine && fabsf(x[e]) <= 3.402823466e38f;
   }
   if (valid && !fine) atomicOr(again, 1u << col);
@@ -965,13 +994,20 @@ __device__ __forceinline__ void narrow_dkdv(const MaskedArgs& a, int blk, int he
   char* vt = smem + L::kBytes;
   char* qt = smem + (2 + 2 * wave) * L::kBytes;
   char* dt = qt + L::kBytes;
-  float lse2 = 0.0f, dsum = 0.0f;  // lse (log2 units) and D of tile row c in lanes c and c + 32
+  // lse (log2 units) of tile row c in lane c, D in lane c + 32. Heads of 64 leave LDS to spread them from; with 128 the
+  // tiles fill what two blocks a CU have, and lanes ask each other.
+  float* ld = reinterpret_cast<float*>(smem + kNarrowLds<HD>) + 64 * wave;
+  const float* stat_row = h ? ds : lse;
+  float stat = 0.0f;
   auto copy = [&](int j) {
     const int rows = r.lq - 32 * j;
     tq.fresh().copy(qt, qh + 32 * j * a.q_st, rows);
     td.fresh().copy(dt, doh + 32 * j * a.do_st, rows);
-    lse2 = lse[32 * j + min(col, rows - 1)] * kLog2e;
-    dsum = ds[32 * j + min(col, rows - 1)];
+    stat = stat_row[32 * j + min(col, rows - 1)];
+  };
+  auto landed = [&] {
+    stat = h ? stat : stat * kLog2e;
+    if constexpr (HD == 64) ld[lane] = stat;
   };
   constexpr int C = L::kCopies / kWaves;
   TileLane<HD, C>(C * wave, lane, a.k_st)
@@ -986,9 +1022,11 @@ __device__ __forceinline__ void narrow_dkdv(const MaskedArgs& a, int blk, int he
     dv[d] = f32x16{};
   }
   stage_barrier();
+  landed();
   for (int j = t0 + wave; j < tiles; j += kWaves) {
     f32x16 st[1], dp = f32x16{}, f[1];
-    start_scores<CAP, BIAS, 1>(st, sc.slope, static_cast<float>(r.off() + 32 * j + 4 * h - kc), -1.0f, r.off() + 32 * j >= k0 + 31);
+    start_scores<CAP, BIAS, 1>(st, sc.slope, static_cast<float>(r.off() + 32 * j + 4 * h - kc), -1.0f,
+                               r.off() + 32 * j >= k0 + 31);
 #pragma unroll
     for (int k = 0; k < L::kSteps; ++k) {
       st[0] = mfma<T>(fl.frag(qt, k), fl.frag(kt, k), st[0]);  // S = Q K^T
@@ -997,10 +1035,15 @@ __device__ __forceinline__ void narrow_dkdv(const MaskedArgs& a, int blk, int he
     key_scores<T, CAP, BIAS>(
         a, sc.slope2, st, f, dp,
         [&](int q, f32x4& lv, f32x4& dd) {
+          if constexpr (HD == 64) {
+            lv = *reinterpret_cast<const f32x4*>(ld + 8 * q + 4 * h);
+            dd = *reinterpret_cast<const f32x4*>(ld + 32 + 8 * q + 4 * h);
+          } else {
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            lv[i] = __shfl(lse2, 8 * q + 4 * h + i, 64);
-            dd[i] = __shfl(dsum, 8 * q + 4 * h + i, 64);
+            for (int i = 0; i < 4; ++i) {
+              lv[i] = __shfl(stat, 8 * q + 4 * h + i, 64);
+              dd[i] = __shfl(stat, 32 + 8 * q + 4 * h + i, 64);
+            }
           }
         },
         static_cast<float>(r.off() + 32 * j + 4 * h - kc), 32 * j < q_all || 32 * j + 32 > r.lq, q_lane - 32 * j,
@@ -1018,6 +1061,7 @@ __device__ __forceinline__ void narrow_dkdv(const MaskedArgs& a, int blk, int he
       wait_reads();
       copy(j + kWaves);
       wait_copies<0>();
+      landed();
     }
   }
   // Keys are accumulator rows, head dims lanes.
@@ -1068,15 +1112,17 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2, 
 }
 
 template <typename T, int HD, bool CAP, bool BIAS>
-__global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2, 2))) void masked_narrow_dkdv_kernel(
+__global__ __launch_bounds__(64 * kWaves)
+__attribute__((amdgpu_waves_per_eu(kCuBlocks<HD>, kCuBlocks<HD>))) void masked_narrow_dkdv_kernel(
     MaskedArgs a) {
-  __shared__ __attribute__((aligned(16))) char smem[kNarrowLds<HD>];
+  __shared__ __attribute__((aligned(16))) char smem[kNarrowLds<HD> + (HD == 64 ? kWaves * 64 * 4 : 0)];
   int item, head;
   if (!head_item(a, a.n_kblocks, item, head)) return;
   narrow_dkdv<T, HD, CAP, BIAS>(a, item, head, smem);
 }
 
-// dk / dv [key, g, :] = T(sum over the KV group's heads, in head order, of the parts). Thread = 4 head dims of a key.
+// dk / dv [key, g, :] = T(sum over the KV group's heads, in head order, of the parts). Thread = 4 head dims of a
+// key. Bound by reading the parts: 8,161 keys of 12 heads 19 us (5.4 TB/s).
 template <typename T>
 __global__ __launch_bounds__(256) void masked_group_sum_kernel(MaskedArgs a, int hd4) {
   const int64_t t = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
