@@ -9,6 +9,7 @@ raises ``RuntimeError``.
 
 from __future__ import annotations
 
+import array
 import ctypes
 import functools
 import math
@@ -2744,8 +2745,9 @@ class RopeAxes:
         if not all(math.isfinite(f) for f in freq):
             raise ValueError("RopeAxes: a frequency is not finite")
         self.n_axes = max(axis) + 1
-        self.axis = torch.tensor(axis, dtype=torch.uint8, device=device)
-        self.turns = torch.tensor([f / (2.0 * math.pi) for f in freq], dtype=torch.float64, device=device)
+        turns = array.array("d", [f / (2.0 * math.pi) for f in freq])
+        table = torch.frombuffer(bytearray(turns.tobytes() + bytes(axis)), dtype=torch.uint8).to(device)  # one copy
+        self.turns, self.axis = table[: 8 * self.pairs].view(torch.float64), table[8 * self.pairs :]
         self.tables = self.axis.data_ptr(), self.turns.data_ptr()
 
     @classmethod
