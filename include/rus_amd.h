@@ -986,7 +986,8 @@ int rus_attn_masked_plan(int32_t n_seq, int64_t n_q, int64_t n_k, int32_t max_q,
  * D = sum_j P_j (dout v^T)_j (not dout.out: out has been rounded),
  *   dS = P (dout v^T - D) (1 - t^2),  dq = scale dS k,  dk = scale dS^T q,  dv = P^T dout,
  * dk and dv summed over the query heads of each KV head in a fixed order in fp32 and rounded once. dout by strides as
- * q; dq, dk, dv contiguous, zero at tokens that no row or no pair covers. P and dS are rounded to T.
+ * q; dq, dk, dv contiguous, zero at tokens that no row or no pair covers. P and dS are rounded to T
+ * (by the layout, what that leaves is added as a second such value).
  */
 int rus_attn_masked_bwd(const void* dout, int64_t do_stride_t, int64_t do_stride_h, const void* q, int64_t q_stride_t,
                         int64_t q_stride_h, const void* k, int64_t k_stride_t, int64_t k_stride_h, const void* v,

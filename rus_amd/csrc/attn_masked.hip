@@ -473,9 +473,11 @@ __global__ __launch_bounds__(64 * kJoinWaves) void masked_join_kernel(MaskedArgs
 }
 
 // ---------------------------------------------------------------------------------------------
-// Backward. P and dS are rounded to T for the products that take them; their sums, D and lse are not. Gradients are off
-// the definition by 1.4 times what separate products with 32-bit softmax and its 32-bit gradient are (bf16 0.24% against
-// 0.17%, fp16 0.030% against 0.021%).
+// Backward. P and dS are rounded to T for the products that take them; their sums, D and lse are not. In blocks of 128
+// gradients are off the definition by 1.4 times what their own rounding is (bf16 0.24% against 0.17%, fp16 0.030% against
+// 0.021%), which the products at twice the instructions would not be worth; blocks of 32, with instructions to spare, give
+// what these roundings left to the products too, and their gradients are off by their own rounding alone. fp16 loses bits
+// of P and dS below 2^-14: gradients far below 1 want a scaled loss there.
 // ---------------------------------------------------------------------------------------------
 
 // LDS of the backward: the streamed tiles' two buffers, and for the dK / dV blocks the block's V rows and the streamed
@@ -822,7 +824,7 @@ __attribute__((amdgpu_waves_per_eu(kCuBlocks<HD>, kCuBlocks<HD>))) void masked_d
 // ---------------------------------------------------------------------------------------------
 // The backward of batches that leave the chip idle in blocks of 128: a block owns 32 tokens of one side, its four waves
 // take the other side's tiles in turn (each with LDS of its own) and their sums meet in the LDS in wave order. Bound by
-// the latency of a wave's few tiles: 707 tokens in six rows, 12 / 2 heads of 128 with a cap 22 us dQ, 18 us dK and dV;
+// the latency of a wave's few tiles (the remainders' products cost 707 tokens 4%): 707 tokens in six rows, 12 / 2 heads of 128 with a cap 22 us dQ, 18 us dK and dV;
 // 1,923 tokens in four, 16 heads of 64 with a cap 41 and 46 us (the cap's arithmetic: 24,560 tiles of some 2,000 cycles
 // over 1,024 SIMDs are 20 us).
 // ---------------------------------------------------------------------------------------------
@@ -916,14 +918,17 @@ __device__ __forceinline__ void narrow_dq(const MaskedArgs& a, int blk, int head
     query_scores<T, CAP, BIAS>(a, sc.slope2, st, dp, dsum, lse2, static_cast<float>(r.off() + i - 32 * j - 4 * h),
                                32 * j + 32 > vis_all, vis - 32 * j, h, rest);
     const Frag p0 = frag_acc<T>(st[0], 0), p1 = frag_acc<T>(st[0], 1);
-    const Frag s0 = frag_acc<T>(dp, 0), s1 = frag_acc<T>(dp, 1);
+    const Frag s0 = split_acc<T>(dp, 0), s1 = split_acc<T>(dp, 1);
+    const Frag e0 = frag_acc<T>(dp, 0), e1 = frag_acc<T>(dp, 1);
 #pragma unroll
     for (int d = 0; d < ND; ++d) {
       const Frag k0 = fl.frag_t(kt, 0, d), k1 = fl.frag_t(kt, 1, d);
       dq[d] = mfma<T>(k0, s0, dq[d]);  // dQ^T += K^T dS'^T
       pk[d] = mfma<T>(k0, p0, pk[d]);
-      dq[d] = mfma<T>(k1, s1, dq[d]);
+      dq[d] = mfma<T>(k0, e0, dq[d]);
       pk[d] = mfma<T>(k1, p1, pk[d]);
+      dq[d] = mfma<T>(k1, s1, dq[d]);
+      dq[d] = mfma<T>(k1, e1, dq[d]);
     }
     if (j + kWaves < tiles) {
       wait_reads();
@@ -1048,14 +1053,22 @@ __device__ __forceinline__ void narrow_dkdv(const MaskedArgs& a, int blk, int he
         },
         static_cast<float>(r.off() + 32 * j + 4 * h - kc), 32 * j < q_all || 32 * j + 32 > r.lq, q_lane - 32 * j,
         r.lq - 32 * j, h);
-    const Frag p0 = frag_acc<T>(st[0], 0), p1 = frag_acc<T>(st[0], 1);
-    const Frag s0 = frag_acc<T>(dp, 0), s1 = frag_acc<T>(dp, 1);
+    const Frag p0 = split_acc<T>(st[0], 0), p1 = split_acc<T>(st[0], 1);
+    const Frag s0 = split_acc<T>(dp, 0), s1 = split_acc<T>(dp, 1);
+    const Frag c0 = frag_acc<T>(st[0], 0), c1 = frag_acc<T>(st[0], 1);
+    const Frag e0 = frag_acc<T>(dp, 0), e1 = frag_acc<T>(dp, 1);
 #pragma unroll
     for (int d = 0; d < ND; ++d) {
-      dv[d] = mfma<T>(p0, fl.frag_t(dt, 0, d), dv[d]);  // dV += P^T dO
-      dv[d] = mfma<T>(p1, fl.frag_t(dt, 1, d), dv[d]);
-      dk[d] = mfma<T>(s0, fl.frag_t(qt, 0, d), dk[d]);  // dK += dS^T Q
-      dk[d] = mfma<T>(s1, fl.frag_t(qt, 1, d), dk[d]);
+      const Frag o0 = fl.frag_t(dt, 0, d), o1 = fl.frag_t(dt, 1, d);
+      dv[d] = mfma<T>(p0, o0, dv[d]);  // dV += P^T dO
+      dv[d] = mfma<T>(c0, o0, dv[d]);
+      dv[d] = mfma<T>(p1, o1, dv[d]);
+      dv[d] = mfma<T>(c1, o1, dv[d]);
+      const Frag q0 = fl.frag_t(qt, 0, d), q1 = fl.frag_t(qt, 1, d);
+      dk[d] = mfma<T>(s0, q0, dk[d]);  // dK += dS^T Q
+      dk[d] = mfma<T>(e0, q0, dk[d]);
+      dk[d] = mfma<T>(s1, q1, dk[d]);
+      dk[d] = mfma<T>(e1, q1, dk[d]);
     }
     if (j + kWaves < tiles) {
       wait_reads();
@@ -1224,14 +1237,14 @@ SplitPlan split_plan(int32_t n_seq, int64_t n_q, int64_t n_k, int32_t max_q, int
 
 // Whether a backward runs in blocks of 32 tokens rather than of 128. The latter walk the longest row's tiles alone (2.8 us
 // a tile for dQ, then dK and dV), the former share them among four waves but read the other side again for every 32
-// tokens. Measured, 12 / 2 heads of 128, us in blocks of 128 / of 32: 100 tokens 32 / 23, 707 80 / 48, 2,048 194 / 109,
-// 4,096 377 / 327, two rows of 256 43 / 29, 1,500 and 27 rows of 64 151 / 106; sixteen rows of 32 23 / 25, ten of 256
-// 52 / 71, four of 512 71 / 75, of 1,024 168 / 164, eight of 1,024 254 / 267, 4,096 + 2,048 + 1,024 + 993 430 / 477;
-// 16 heads of 64, no causal mask, 1,025 + 577 + 257 + 64 89 / 77, eight rows of 700 113 / 164.
+// tokens. Measured, 12 / 2 heads of 128, us in blocks of 128 / of 32: 100 tokens 32 / 23, 707 79 / 49, 2,048 194 / 119,
+// 3,000 277 / 232, 4,096 378 / 380, two rows of 256 43 / 30, 1,500 and 27 rows of 64 150 / 111; sixteen rows of 32 22 / 25,
+// ten of 256 52 / 71, four of 512 71 / 76, of 1,024 167 / 174, eight of 1,024 254 / 282, 4,096 + 2,048 + 1,024 + 993 429 /
+// 540; 16 heads of 64, no causal mask, 1,025 + 577 + 257 + 64 89 / 84, eight rows of 700 92 / 156.
 bool narrow_bwd(int32_t n_seq, int64_t n_q, int64_t n_k, int32_t max_q, int32_t max_k, int32_t h_q) {
   const double n = static_cast<double>(std::max(n_q, n_k)), seqs = std::max(n_seq, 1);
   const double blocks = std::max(n / 32, seqs) * h_q, row = n / seqs / 32;
-  const double narrow_us = 18.0 + blocks * (0.042 + 0.00125 * row);
+  const double narrow_us = 18.0 + blocks * (0.042 + 0.0014 * row);
   return narrow_us < 18.0 + 2.8 * std::max(max_q, max_k) / 32;
 }
 

@@ -65,6 +65,16 @@ __device__ __forceinline__ Frag frag_acc(const f32x16& c, int s) {
   return __builtin_bit_cast(Frag, r);
 }
 
+// The same, with what the roundings left behind in the registers.
+template <typename T>
+__device__ __forceinline__ Frag split_acc(f32x16& c, int s) {
+  const Frag f = frag_acc<T>(c, s);
+  const Pack<T, 8> r = __builtin_bit_cast(Pack<T, 8>, f);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) c[8 * s + i] -= static_cast<float>(r.v[i]);
+  return f;
+}
+
 // Accumulator row of register r for lane half h.
 __device__ __forceinline__ int acc_row(int r, int h) { return 8 * (r >> 2) + 4 * h + (r & 3); }
 
