@@ -824,9 +824,9 @@ __attribute__((amdgpu_waves_per_eu(kCuBlocks<HD>, kCuBlocks<HD>))) void masked_d
 // ---------------------------------------------------------------------------------------------
 // The backward of batches that leave the chip idle in blocks of 128: a block owns 32 tokens of one side, its four waves
 // take the other side's tiles in turn (each with LDS of its own) and their sums meet in the LDS in wave order. Bound by
-// the latency of a wave's few tiles (the remainders' products cost 707 tokens 4%): 707 tokens in six rows, 12 / 2 heads of 128 with a cap 22 us dQ, 18 us dK and dV;
-// 1,923 tokens in four, 16 heads of 64 with a cap 41 and 46 us (the cap's arithmetic: 24,560 tiles of some 2,000 cycles
-// over 1,024 SIMDs are 20 us).
+// the latency of a wave's few tiles (the remainders' products cost 707 tokens 4%, 4,096 16%): 707 tokens in six rows,
+// 12 / 2 heads of 128 with a cap 21 us dQ, 20 us dK and dV; 1,923 tokens in four, 16 heads of 64 with a cap 46 and 50 us
+// (the cap's arithmetic: 24,560 tiles of some 2,000 cycles over 1,024 SIMDs are 20 us each).
 // ---------------------------------------------------------------------------------------------
 // Of the dQ blocks: two tiles a wave (then the sums), a word and the waves' parts of r, the dO tile.
 template <int HD>
