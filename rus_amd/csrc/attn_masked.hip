@@ -655,7 +655,8 @@ __device__ __forceinline__ void bwd_dq(const MaskedArgs& a, int blk, int head, c
   const uint64_t again = __ballot(valid && !(all_finite(dq, a.scale) && fabsf(rest) <= 3.402823466e38f));
   uint32_t cols = static_cast<uint32_t>(again) | static_cast<uint32_t>(again >> 32);
   const bool keep = valid && !((cols >> col) & 1);
-  store_row<T, L::kDims>(static_cast<T*>(a.out) + (t * a.h_q + head) * HD, dq, a.scale, h, keep);
+  // (a single key's P is 1 whatever its score: its dQ is 0, not what the roundings leave)
+  store_row<T, L::kDims>(static_cast<T*>(a.out) + (t * a.h_q + head) * HD, dq, vis > 1 ? a.scale : 0.0f, h, keep);
   if (h == 0 && keep) a.dsum[head * a.n_q + t] = vis > 0 ? dsum + rest : 0.0f;
   for (; cols; cols &= cols - 1) plain_dq_row<T, HD, CAP, BIAS>(a, r, iw + __builtin_ctz(cols), head);
 }
@@ -964,7 +965,9 @@ __device__ __forceinline__ void narrow_dq(const MaskedArgs& a, int blk, int head
 #pragma unroll
     for (int q = 0; q < ND; ++q) {  // four registers: head dims 32 d + 8 (e / 4) + 4 h .. + 4
       const int e = wave * 4 * ND + 4 * q;
-      const float o[4] = {x[4 * q], x[4 * q + 1], x[4 * q + 2], x[4 * q + 3]};
+      float o[4];
+#pragma unroll
+      for (int y = 0; y < 4; ++y) o[y] = vis > 1 ? x[4 * q + y] : 0.0f;  // (a single key's P is 1: its dQ is 0)
       store_from_f32<T, 4>(row + 32 * (e >> 4) + acc_row(e & 15, h), o);
     }
   }

@@ -276,6 +276,19 @@ def test_operands_that_look_contiguous_but_are_not_addressable():
             assert torch.equal(a, b), f.__name__
 
 
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("ql", [[1], [1, 1, 40, 1], [1] * 70 + [700] * 12], ids=["one", "few", "blocks_of_128"])
+def test_a_single_key_has_no_score_gradient(dtype, ql):
+    """The P of a query that sees one key is 1 whatever the score: its dq, and what it adds to dk, are 0."""
+    q, k, v, dout = _inputs(ql, ql, 8, 4, 64, dtype, seed=33)
+    for kw in ({}, dict(softcap=5.0, slopes=_slopes(8))):
+        got = _run(q, k, v, dout, ql, ql, **kw)
+        starts = torch.tensor(_cu(ql)[:-1])
+        alone = starts[torch.tensor(ql) == 1]
+        assert not bool(got["dq"].cpu()[starts].any())
+        assert not bool(got["dk"].cpu()[alone].any())
+
+
 def test_gradients_against_differences():
     """(f(x + h e) - f(x - h e)) / 2 h of the definition in float64 along random directions, with the operator's
     gradients from the same inputs."""
