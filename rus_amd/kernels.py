@@ -2748,7 +2748,6 @@ class RopeAxes:
         turns = array.array("d", [f / (2.0 * math.pi) for f in freq])
         table = torch.frombuffer(bytearray(turns.tobytes() + bytes(axis)), dtype=torch.uint8).to(device)  # one copy
         self.turns, self.axis = table[: 8 * self.pairs].view(torch.float64), table[8 * self.pairs :]
-        self.tables = self.axis.data_ptr(), self.turns.data_ptr()
 
     @classmethod
     def sections(cls, sections, theta: float, head_dim: int, device="cuda", order: str = "blocks",
@@ -2822,7 +2821,7 @@ def _rope_axes(fn: str, q: torch.Tensor, k: torch.Tensor | None, pos: torch.Tens
                                      6.0 * n * (hq + hk) * axes.pairs),
                q, "rus_rope_axes", q.data_ptr(), q_st, q_sh, hq, q_out.data_ptr(), _ptr(k), k_st, k_sh, hk,
                _ptr(k_out), n, d, axes.pairs, axes.adjacent, pos.data_ptr(), pos_type, ld_pos, axes.n_axes,
-               *axes.tables, inverse, code)
+               axes.axis.data_ptr(), axes.turns.data_ptr(), inverse, code)
     return q_out, k_out
 
 

@@ -7,7 +7,9 @@ at most goes to 32 bits; sine and cosine are then good to 2^-23, and two product
 
 from __future__ import annotations
 
+import copy
 import math
+import pickle
 
 import pytest
 import torch
@@ -135,3 +137,17 @@ def test_no_tokens():
     axes, q, k, pos, *_ = _case(1, 2, 1, 16, (3, 5), torch.float16)
     a, b = K.rope_axes_fwd(q[:0].to(DEV), k[:0].to(DEV), pos[:, :0].to(DEV), axes)
     assert a.shape == (0, 2, 16) and b.shape == (0, 1, 16)
+
+
+def test_a_copied_handle_reads_its_own_tables():
+    """A model that is deep-copied or pickled takes its handle along; the first one's memory may be gone."""
+    axes = K.RopeAxes.sections((5, 7, 4), 1e4, 32, DEV)
+    q = torch.randn(9, 2, 32, device=DEV)
+    pos = torch.arange(27, device=DEV).view(3, 9)
+    want, _ = K.rope_axes_fwd(q, None, pos, axes)
+    for twin in (copy.deepcopy(axes), pickle.loads(pickle.dumps(axes))):
+        assert twin.axis.data_ptr() != axes.axis.data_ptr()
+        axes.turns.zero_()  # (the first handle's memory in other hands)
+        got, _ = K.rope_axes_fwd(q, None, pos, twin)
+        axes.turns.copy_(twin.turns)
+        assert torch.equal(got, want)
